@@ -17,6 +17,9 @@ from .api import (  # noqa: F401
     MatmulParams,
     CastParams,
     CausalMaskParams,
+    KvPageMapParams,
+    KvPageStoreParams,
+    MhaPagedParams,
     GraphMhaMatch,
     OperatorRegistry,
     Stream,

@@ -57,6 +57,30 @@ class CastParams(ctypes.Structure):
     _fields_ = [("src_dtype", c_int), ("dst_dtype", c_int), ("numel", c_int64)]
 
 
+class KvPageMapParams(ctypes.Structure):
+    """kv_page_map_params_t (include/paged_ops.h)."""
+
+    _fields_ = [(n, c_int64) for n in ("batch_size", "num_tokens", "page_size", "num_pages", "max_pages", "ring_size")]
+
+
+class KvPageStoreParams(ctypes.Structure):
+    """kv_page_store_params_t (include/paged_ops.h); strides of 0 are the dense layout's."""
+
+    _fields_ = [(n, c_int64) for n in ("num_tokens", "num_heads", "num_kv_heads", "head_dim", "page_size",
+                                       "num_pages")] + [("rope_base", c_float)] + \
+               [(n, c_int64) for n in ("q_stride", "kv_stride", "q_out_stride", "page_stride", "row_stride",
+                                       "head_stride")]
+
+
+class MhaPagedParams(ctypes.Structure):
+    """mha_paged_params_t (include/paged_ops.h); strides of 0 are the dense layout's."""
+
+    _fields_ = [(n, c_int64) for n in ("batch_size", "num_tokens", "num_heads", "num_kv_heads", "head_dim")] + \
+               [("scale", c_float)] + \
+               [(n, c_int64) for n in ("page_size", "num_pages", "max_pages", "max_new", "q_stride", "page_stride",
+                                       "row_stride", "head_stride")]
+
+
 ONNX_FLOAT, ONNX_FLOAT16, ONNX_INT64 = 1, 10, 7
 
 

@@ -363,6 +363,64 @@ typedef struct {
 } cf_rope_decode_args_t;
 int cf_launch_rope_decode(const cf_rope_decode_args_t* a, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * Paged KV cache (paged_kv.hip, paged_attn.hip; operators in paged_ops.h).
+ * ------------------------------------------------------------------------------- */
+typedef struct {
+    const int32_t* cache_lens;
+    const int32_t* new_lens;
+    const int32_t* counters;
+    int32_t*       table;
+    int32_t*       ring;
+    int32_t*       seq_lens;
+    int32_t*       q_start;
+    int32_t*       positions;
+    int32_t*       slots;
+    int32_t*       counters_out;
+    int32_t*       info;        /* workspace: cf_page_map_info_ints(B) (the two-launch form) */
+    int32_t        B, T, page_size, num_pages, max_pages, ring_size;
+} cf_page_map_args_t;
+/* Ints of workspace a launch of this size needs (0: it runs as one workgroup). */
+size_t cf_page_map_info_ints(int32_t B, int32_t T);
+int    cf_launch_page_map(const cf_page_map_args_t* a, void* stream);
+
+#define CF_PAGE_ROPE_MAX_DIM 256
+typedef struct {
+    const void*    k;
+    const void*    v;
+    const void*    q;           /* NULL: no Q */
+    const int32_t* slots;
+    const int32_t* positions;   /* read with rope */
+    void*          k_pages;
+    void*          v_pages;
+    void*          q_out;
+    int64_t        T, q_stride, kv_stride, q_out_stride;
+    int64_t        page_stride, row_stride, head_stride;
+    int32_t        H_q, H_kv, d, page_size;
+    int32_t        num_slots;   /* num_pages * page_size */
+    int32_t        rope;
+    int32_t        elem;
+    double         turns[CF_PAGE_ROPE_MAX_DIM / 2];   /* rope: base^(-2i/d) / (2 pi) */
+} cf_page_store_args_t;
+int cf_launch_page_store(const cf_page_store_args_t* a, void* stream);
+
+typedef struct {
+    const void*    q;
+    const void*    k;
+    const void*    v;
+    void*          o;
+    const int32_t* table;
+    const int32_t* seq_lens;
+    const int32_t* q_start;
+    int64_t        q_stride, page_stride, row_stride, head_stride;
+    int32_t        B, T, H_q, H_kv, d;
+    int32_t        page_size, num_pages, max_pages;
+    int32_t        max_new;     /* most rows of one sequence; T where unknown */
+    float          scale;
+    int32_t        elem;
+} cf_paged_attn_args_t;
+int cf_launch_paged_attn(const cf_paged_attn_args_t* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,333 @@
+// paged_kv.hip — the pages of a step and the write of new K and V rows into them (gfx950).
+//
+// page_map: with c_b positions held and n_b tokens new, sequence b takes
+// need_b = ceil((c_b + n_b) / P) - ceil(c_b / P) pages, the ones at places
+// head + E_b .. of the ring with E_b the sum of need before b; token i of b is at position
+// c_b + i and its slot is page * P + (c_b + i) % P.  Everything but the prefix sums is
+// independent per token and per page.
+//
+// page_store: pages[slot[t]] = row t of K and V, with Q and K turned by their positions.
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "kernels.h"
+#include "cdna4.h"
+
+namespace {
+
+using namespace cdna4;
+
+// ------------------------------------------------------------------ map ---
+
+constexpr int kMapThreads = 1024;
+constexpr int kMapOneSeqs = 1024;    // the one-workgroup form: one sequence per thread
+constexpr int kMapOneTokens = 4096;
+
+enum { kNotServed = -1, kEnded = -2 };
+
+// What the tokens and pages of one sequence need to know.
+struct SeqPages {
+    int c;         // positions held
+    int n;         // new tokens (0 for an ended sequence)
+    int first;     // place of its first new page behind the ring's head, kNotServed or kEnded
+    int give;      // ended: place of its first page behind the free ones
+};
+
+struct MapDivs { FastDiv page, ring; };
+
+// The counters as they are used: any content gives a place in the ring.
+struct RingState { int head, avail, tail; };
+__device__ __forceinline__ RingState ring_state(const int32_t* counters, int R, FastDiv by_ring) {
+    RingState r;
+    const int h = max(counters[0], 0);
+    r.head = h - fastdiv(h, by_ring) * R;
+    r.avail = min(max(counters[1], 0), R);
+    r.tail = r.head + r.avail;                     // R <= 2^30
+    if (r.tail >= R) r.tail -= R;
+    return r;
+}
+
+__device__ __forceinline__ int ceil_pages(int x, int P, FastDiv by_page) {
+    const int q = fastdiv(x, by_page);
+    return q + (q * P < x ? 1 : 0);
+}
+
+// The page at place x behind the ring's head (x < avail), or -1 where the ring holds no page.
+__device__ __forceinline__ int ring_page(const cf_page_map_args_t& a, int head, int x, FastDiv by_ring) {
+    const int at = head + x;                       // < 2 R
+    const int page = a.ring[at - fastdiv(at, by_ring) * a.ring_size];
+    return (unsigned)page < (unsigned)a.num_pages ? page : -1;
+}
+
+__device__ __forceinline__ void write_token(const cf_page_map_args_t& a, const RingState& r, const MapDivs& dv, int b,
+                                            const SeqPages& s, int i, int row) {
+    const int pos = s.c + i;
+    const int idx = fastdiv(pos, dv.page);
+    int page = -1;
+    if (s.first >= 0) {
+        const int before = ceil_pages(s.c, a.page_size, dv.page);
+        page = idx < before ? a.table[(size_t)b * a.max_pages + idx] : ring_page(a, r.head, s.first + idx - before, dv.ring);
+        if ((unsigned)page >= (unsigned)a.num_pages) page = -1;
+    }
+    a.positions[row] = pos;
+    a.slots[row] = page < 0 ? -1 : page * a.page_size + (pos - idx * a.page_size);
+}
+
+// Page j that changes hands with sequence b: into its table, or out of it into the ring.
+__device__ __forceinline__ void move_page(const cf_page_map_args_t& a, const RingState& r, const MapDivs& dv, int b,
+                                          const SeqPages& s, int j) {
+    int32_t* const row = a.table + (size_t)b * a.max_pages;
+    if (s.first == kEnded) {
+        a.ring[(uint32_t)(r.tail + s.give + j) % (uint32_t)a.ring_size] = row[j];
+        return;
+    }
+    row[ceil_pages(s.c, a.page_size, dv.page) + j] = s.first >= 0 ? ring_page(a, r.head, s.first + j, dv.ring) : -1;
+}
+
+// The last entry of start[0 .. n) that is not above x (start[0] <= x).
+__device__ __forceinline__ int last_not_above(const int* start, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (start[mid] <= x) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// One workgroup: the prefix sums, a sequence per thread and 1024 sequences at a time.  ONE
+// (up to 1024 sequences): it then writes the tokens and pages too, each found by its
+// number in the sums in LDS; else it leaves SeqPages per sequence in a.info for page_map_fill.
+template <bool ONE>
+__global__ __launch_bounds__(kMapThreads)
+void page_map_scan(cf_page_map_args_t a, MapDivs dv) {
+    constexpr int kWaves = kMapThreads / 64;
+    __shared__ int part[4][kWaves];
+    __shared__ int taken_s, refused_s;
+    __shared__ SeqPages seq[ONE ? kMapOneSeqs : 1];
+    __shared__ int row0[ONE ? kMapOneSeqs : 1], move0[ONE ? kMapOneSeqs : 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int P = a.page_size, cap = a.max_pages * P;
+    const RingState r = ring_state(a.counters, a.ring_size, dv.ring);
+    if (tid == 0) taken_s = refused_s = 0;
+    int carry[4] = {0, 0, 0, 0};                   // rows, pages needed, taken back, moved
+    for (int base = 0; base < a.B; base += kMapThreads) {
+        const int b = base + tid;
+        const bool live = b < a.B;
+        const int n0 = live ? a.new_lens[b] : 0;
+        SeqPages s;
+        s.c = live ? min(max(a.cache_lens[b], 0), cap) : 0;
+        s.n = max(n0, 0);
+        const bool ended = n0 < 0;
+        const uint32_t len = (uint32_t)s.c + (uint32_t)s.n;
+        const bool fits = !ended && len <= (uint32_t)cap;
+        const int before = ceil_pages(s.c, P, dv.page);
+        int v[4];
+        v[0] = s.n;
+        v[1] = fits ? ceil_pages((int)len, P, dv.page) - before : 0;
+        v[2] = ended ? before : 0;
+        v[3] = ended ? before : fits ? v[1] : live ? a.max_pages - before : 0;
+        int ex[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            ex[k] = wave_excl_sum(v[k], lane);
+            if (lane == 63) part[k][wave] = ex[k] + v[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            int sum = 0;
+            for (int w = 0; w < kWaves; w++) {
+                if (w == wave) ex[k] += carry[k] + sum;
+                sum += part[k][w];
+            }
+            carry[k] += sum;
+        }
+        const bool served = fits && (v[1] == 0 || ex[1] + v[1] <= r.avail);
+        s.first = ended ? kEnded : served ? ex[1] : kNotServed;
+        s.give = ex[2];
+        if (live) {
+            a.seq_lens[b] = ended ? 0 : (int)min(len, 0x7fffffffu);
+            a.q_start[b] = ex[0];
+            if (served && v[1] > 0) atomicMax(&taken_s, ex[1] + v[1]);
+            if (!served && !ended) atomicAdd(&refused_s, 1);
+            if constexpr (ONE) {
+                seq[b] = s;
+                row0[b] = ex[0];
+                move0[b] = ex[3];
+            } else {
+                ((int4*)a.info)[b] = int4{s.c, s.n, s.first, s.give};
+            }
+        }
+        __syncthreads();
+    }
+    if (tid == 0) {
+        a.q_start[a.B] = carry[0];
+        if constexpr (!ONE) {                      // counters_out may be counters
+            a.info[4 * (size_t)a.B] = r.head;
+            a.info[4 * (size_t)a.B + 1] = r.avail;
+        }
+        const int head = r.head + taken_s;         // < 2 R
+        a.counters_out[0] = head - fastdiv(head, dv.ring) * a.ring_size;
+        a.counters_out[1] = (int)min((uint32_t)(r.avail - taken_s) + (uint32_t)carry[2], (uint32_t)a.ring_size);
+        a.counters_out[2] = refused_s;
+    }
+    if constexpr (ONE) {
+        for (int t = tid; t < a.T; t += kMapThreads) {
+            if ((uint32_t)t >= (uint32_t)carry[0]) {
+                a.positions[t] = a.slots[t] = -1;
+                continue;
+            }
+            const int b = last_not_above(row0, a.B, t);
+            write_token(a, r, dv, b, seq[b], t - row0[b], t);
+        }
+        for (int i = tid; i < carry[3]; i += kMapThreads) {
+            const int b = last_not_above(move0, a.B, i);
+            move_page(a, r, dv, b, seq[b], i - move0[b]);
+        }
+    }
+}
+
+// Workgroups (b, part): sequence b's tokens and pages, shared by its gridDim.y parts;
+// b = B: the rows behind the last token.
+constexpr int kFillThreads = 256;
+__global__ __launch_bounds__(kFillThreads)
+void page_map_fill(cf_page_map_args_t a, MapDivs dv) {
+    const int b = blockIdx.x;
+    const int i0 = blockIdx.y * kFillThreads + threadIdx.x, step = gridDim.y * kFillThreads;
+    const uint32_t row0 = (uint32_t)a.q_start[b];
+    if (b == a.B) {
+        for (uint32_t t = row0 + (uint32_t)i0; t < (uint32_t)a.T; t += (uint32_t)step) a.positions[t] = a.slots[t] = -1;
+        return;
+    }
+    const RingState r = ring_state((const int32_t*)a.info + 4 * (size_t)a.B, a.ring_size, dv.ring);
+    const int4 v = ((const int4*)a.info)[b];
+    const SeqPages s = {v.x, v.y, v.z, v.w};
+    for (int i = i0; i < s.n && row0 + (uint32_t)i < (uint32_t)a.T; i += step)
+        write_token(a, r, dv, b, s, i, (int)(row0 + (uint32_t)i));
+    const int before = ceil_pages(s.c, a.page_size, dv.page);
+    const uint32_t len = (uint32_t)s.c + (uint32_t)s.n;
+    const int moves = s.first == kEnded ? before
+                    : (len <= (uint32_t)(a.max_pages * a.page_size) ? ceil_pages((int)len, a.page_size, dv.page)
+                                                                    : a.max_pages) - before;
+    for (int j = i0; j < moves; j += step) move_page(a, r, dv, b, s, j);
+}
+
+// ------------------------------------------------------------------ store ---
+
+template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T e[N]; };
+
+// One workgroup per row t: the cosines and sines of its position into LDS, then its K, V
+// and Q rows in pieces of VEC elements: 16 bytes, or, where something is not 16-byte
+// aligned, 2 (a pair to turn) or 1 (no rotation, any head size).
+constexpr int kStoreThreads = 256;
+template <typename T, int VEC>
+__global__ __launch_bounds__(kStoreThreads)
+void page_store(cf_page_store_args_t a, FastDiv by_page, FastDiv by_pieces) {
+    constexpr bool WIDE = VEC * sizeof(T) == 16;
+    __shared__ float2 turn[CF_PAGE_ROPE_MAX_DIM / 2];
+    const int64_t t = blockIdx.x;
+    const int slot = a.slots[t];
+    const int pos = a.rope ? a.positions[t] : 0;
+    if (a.rope) {
+        for (int i = threadIdx.x; i < a.d / 2; i += kStoreThreads) {
+            // The angle in turns: whole ones dropped in 64 bits.
+            double w = (double)pos * a.turns[i];
+            w -= rint(w);
+            float s, c;
+            sincospif(2.0f * (float)w, &s, &c);
+            turn[i] = float2{c, s};
+        }
+        __syncthreads();
+    }
+    const int pieces = a.d / VEC;                  // per head
+    auto move = [&](const T* src, T* dst, bool turned, int piece) {
+        Pack<T, VEC> x;
+        if constexpr (WIDE) x = *(const Pack<T, VEC>*)src;
+        else
+#pragma unroll
+            for (int e = 0; e < VEC; e++) x.e[e] = src[e];
+        if constexpr (VEC > 1)
+            if (turned)
+#pragma unroll
+                for (int e = 0; e < VEC; e += 2) {
+                    const float2 cs = turn[(piece * VEC + e) / 2];
+                    const float u = (float)x.e[e], v = (float)x.e[e + 1];
+                    x.e[e] = (T)(u * cs.x - v * cs.y);
+                    x.e[e + 1] = (T)(u * cs.y + v * cs.x);
+                }
+        if constexpr (WIDE) *(Pack<T, VEC>*)dst = x;
+        else
+#pragma unroll
+            for (int e = 0; e < VEC; e++) dst[e] = x.e[e];
+    };
+    const int nkv = a.H_kv * pieces;
+    if ((unsigned)slot < (unsigned)a.num_slots) {
+        const int page = fastdiv(slot, by_page);
+        const int64_t at = (int64_t)page * a.page_stride + (int64_t)(slot - page * a.page_size) * a.row_stride;
+        const T* const k = (const T*)a.k + t * a.kv_stride;
+        const T* const v = (const T*)a.v + t * a.kv_stride;
+        for (int i = threadIdx.x; i < 2 * nkv; i += kStoreThreads) {
+            const int which = i >= nkv, j = which ? i - nkv : i;
+            const int h = fastdiv(j, by_pieces), piece = j - h * pieces;
+            const int64_t to = at + (int64_t)h * a.head_stride + piece * VEC;
+            move((which ? v : k) + (int64_t)j * VEC, (which ? (T*)a.v_pages : (T*)a.k_pages) + to, a.rope && !which, piece);
+        }
+    }
+    if (a.q && pos >= 0) {
+        const T* const q = (const T*)a.q + t * a.q_stride;
+        T* const o = (T*)a.q_out + t * a.q_out_stride;
+        for (int i = threadIdx.x; i < a.H_q * pieces; i += kStoreThreads) {
+            const int h = fastdiv(i, by_pieces);
+            move(q + (int64_t)i * VEC, o + (int64_t)i * VEC, true, i - h * pieces);
+        }
+    }
+}
+
+template <typename T>
+int launch_store(const cf_page_store_args_t& a, hipStream_t st) {
+    constexpr int kWide = 16 / sizeof(T);
+    const uint64_t ptrs = (uint64_t)(uintptr_t)a.k | (uint64_t)(uintptr_t)a.v | (uint64_t)(uintptr_t)a.k_pages |
+                          (uint64_t)(uintptr_t)a.v_pages | (uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.q_out;
+    const uint64_t steps = (uint64_t)a.kv_stride | (uint64_t)a.q_stride | (uint64_t)a.q_out_stride |
+                           (uint64_t)a.page_stride | (uint64_t)a.row_stride | (uint64_t)a.head_stride | (uint64_t)a.d;
+    const bool wide = ptrs % 16 == 0 && steps % kWide == 0;
+    const dim3 grid((unsigned)a.T), block(kStoreThreads);
+    const FastDiv by_page = fastdiv_make(a.page_size);
+    if (wide) hipLaunchKernelGGL((page_store<T, kWide>), grid, block, 0, st, a, by_page, fastdiv_make(a.d / kWide));
+    else if (a.rope) hipLaunchKernelGGL((page_store<T, 2>), grid, block, 0, st, a, by_page, fastdiv_make(a.d / 2));
+    else hipLaunchKernelGGL((page_store<T, 1>), grid, block, 0, st, a, by_page, fastdiv_make(a.d));
+    return (int)hipGetLastError();
+}
+
+}  // namespace
+
+// Two launches need, per sequence, SeqPages, and once the ring's counters as they were.
+extern "C" size_t cf_page_map_info_ints(int32_t B, int32_t T) {
+    return B <= kMapOneSeqs && T <= kMapOneTokens ? 0 : 4 * (size_t)B + 2;
+}
+
+extern "C" int cf_launch_page_map(const cf_page_map_args_t* a, void* stream) {
+    hipStream_t st = (hipStream_t)stream;
+    if (a->B <= 0 || a->T < 0 || a->page_size <= 0 || a->ring_size <= 0 || a->ring_size > (1 << 30))
+        return (int)hipErrorInvalidValue;
+    const MapDivs dv = {fastdiv_make(a->page_size), fastdiv_make(a->ring_size)};
+    if (cf_page_map_info_ints(a->B, a->T) == 0) {
+        hipLaunchKernelGGL(page_map_scan<true>, dim3(1), dim3(kMapThreads), 0, st, *a, dv);
+        return (int)hipGetLastError();
+    }
+    if (!a->info) return (int)hipErrorInvalidValue;
+    hipLaunchKernelGGL(page_map_scan<false>, dim3(1), dim3(kMapThreads), 0, st, *a, dv);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+    // Long chunks of few sequences are shared by several workgroups.
+    const unsigned parts = (unsigned)(a->T / 2048 < 1 ? 1 : a->T / 2048 > 2048 / a->B ? (2048 / a->B < 1 ? 1 : 2048 / a->B) : a->T / 2048);
+    hipLaunchKernelGGL(page_map_fill, dim3((unsigned)a->B + 1, parts), dim3(kFillThreads), 0, st, *a, dv);
+    return (int)hipGetLastError();
+}
+
+extern "C" int cf_launch_page_store(const cf_page_store_args_t* a, void* stream) {
+    if (a->T <= 0 || a->d <= 0 || a->H_kv <= 0) return (int)hipErrorInvalidValue;
+    return a->elem == CF_ELEM_F16 ? launch_store<_Float16>(*a, (hipStream_t)stream)
+                                  : launch_store<float>(*a, (hipStream_t)stream);
+}

@@ -4,6 +4,7 @@
 #include "mha_ops.h"
 #include "rope_ops.h"
 #include "layer_ops.h"
+#include "paged_ops.h"
 
 int operator_init_all(void) {
     int ret = 0;
