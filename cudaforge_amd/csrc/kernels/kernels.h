@@ -418,7 +418,9 @@ typedef struct {
     int32_t        max_new;     /* most rows of one sequence; T where unknown */
     float          scale;
     int32_t        elem;
+    float*         records;     /* workspace of cf_paged_attn_bytes */
 } cf_paged_attn_args_t;
+size_t cf_paged_attn_bytes(const cf_paged_attn_args_t* a);
 int cf_launch_paged_attn(const cf_paged_attn_args_t* a, void* stream);
 
 #ifdef __cplusplus

@@ -167,7 +167,10 @@ static int paged_attn_op(int elem, const void* inputs[], void* outputs[], const 
     a.max_new = p->max_new > 0 && p->max_new < p->num_tokens ? (int32_t)p->max_new : a.T;
     a.scale = p->scale;
     a.elem = elem;
-    return cf_launch_paged_attn(&a, cf_stream_of(stream));
+    void* st = cf_stream_of(stream);
+    const size_t bytes = cf_paged_attn_bytes(&a);
+    if (bytes > 0 && !(a.records = (float*)gpu_workspace_get_stream(st, bytes))) return -1;
+    return cf_launch_paged_attn(&a, st);
 }
 
 int mha_paged_attn_f32_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream) {
