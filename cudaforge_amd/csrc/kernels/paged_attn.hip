@@ -18,6 +18,16 @@ using namespace cdna4;
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// f(std::integral_constant<int, i>) for i = 0 .. N - 1, unrolled.
+template <typename F, int... S>
+__device__ __forceinline__ void static_for_seq(F& f, std::integer_sequence<int, S...>) {
+    (f(std::integral_constant<int, S>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+    static_for_seq(f, std::make_integer_sequence<int, N>{});
+}
+
 // The rows of sequence b: q_start and seq_lens hold anything, rows stay within 0 .. T and
 // the length within the table.
 struct SeqRows {
@@ -44,13 +54,20 @@ __device__ __forceinline__ SeqRows seq_rows(const cf_paged_attn_args_t& a, int b
 // in one range is finished by its unit; else the units leave m, l and the unnormalised sum
 // per row, and paged_merge joins them.  More than one range needs blocks_b > C, so
 // ns_b < 2 blocks_b / C and there are at most 2 ranges + 1 such units per KV head.
+//
+// Three kernels share this:
+//   paged_heads  up to 16 rows per tile, a wave per unit (decode steps of many sequences);
+//   paged_split  up to 16 rows, the waves of a workgroup share the positions of a unit (few);
+//   paged_wide   64 rows and more; its tiles of up to 16 rows go as in paged_split, so a
+//                batch may mix prompt chunks and decode steps.
 
 struct PagedPlan {
     float*  records;       // of the units of cut tiles
     int32_t max_records;   // per KV head
     int32_t ranges;        // key ranges (per KV head) that fill the chip
     int32_t min_blocks;    // no range is cut shorter
-    int32_t waves;         // units in flight: the step of the unit loop
+    int32_t one_blocks;    // tiles of up to this many blocks are not cut
+    int32_t step;          // of the unit loop
     int32_t merge_groups;  // workgroups that share the rows of a tile's merge
     FastDiv by_page, by_group;
 };
@@ -62,8 +79,8 @@ struct Unit {
 };
 
 // The tiles' geometry, one sequence per lane and 64 at a time.  TM rows per tile, BK
-// positions per key block.
-template <int TM, int BK>
+// positions per key block; a tile of up to 16 rows costs 1 / NARROW of a full one's block.
+template <int TM, int BK, int NARROW>
 struct Geometry {
     const cf_paged_attn_args_t& a;
     const PagedPlan& pl;
@@ -73,18 +90,24 @@ struct Geometry {
     __device__ __forceinline__ SeqRows rows(int b) const { return b < a.B ? seq_rows(a, b) : SeqRows{0, 0, 0}; }
     __device__ __forceinline__ int tiles(const SeqRows& s) const { return (int)(((int64_t)s.n * G + TM - 1) / TM); }
     __device__ __forceinline__ int blocks(const SeqRows& s) const { return (s.len + BK - 1) / BK; }
+    __device__ __forceinline__ bool narrow(const SeqRows& s) const { return NARROW > 1 && s.n * G <= 16; }
+    __device__ __forceinline__ float cost(const SeqRows& s) const {
+        const float w = (float)tiles(s) * (float)blocks(s);
+        return narrow(s) ? w * (1.0f / NARROW) : w;
+    }
+    __device__ __forceinline__ int ranges(const SeqRows& s) const {
+        const int n = blocks(s), c = narrow(s) ? NARROW * C : C;
+        return n <= pl.one_blocks ? 1 : (n + c - 1) / c;
+    }
 
     __device__ __forceinline__ Geometry(const cf_paged_attn_args_t& a_, const PagedPlan& pl_) : a(a_), pl(pl_) {
         lane = threadIdx.x & 63;
         G = a.H_q / a.H_kv;
         first = rows(lane);
-        float w = (float)tiles(first) * (float)blocks(first);
-        for (int b = 64; b < a.B; b += 64) {
-            const SeqRows s = rows(b + lane);
-            w += (float)tiles(s) * (float)blocks(s);
-        }
+        float w = cost(first);
+        for (int b = 64; b < a.B; b += 64) w += cost(rows(b + lane));
         w = ceilf(wave_sum(w) / (float)pl.ranges);
-        C = __builtin_amdgcn_readfirstlane((int)fminf(fmaxf(w, (float)pl.min_blocks), 1e9f));
+        C = __builtin_amdgcn_readfirstlane((int)fminf(fmaxf(w, (float)pl.min_blocks), 1e8f));
     }
     // Item u of all units (MERGE: of all cut tiles); false where there is none.
     template <bool MERGE>
@@ -93,7 +116,7 @@ struct Geometry {
         SeqRows s = first;
         for (int base = 0; base < a.B; base += 64) {
             if (base > 0) s = rows(base + lane);
-            const int t = tiles(s), ns = max((blocks(s) + C - 1) / C, 1);
+            const int t = tiles(s), ns = ranges(s);
             const int items = MERGE ? (ns > 1 ? t : 0) : t * ns;
             const int before = items0 + wave_excl_sum(items, lane);
             const int rec = ns > 1 ? t * ns : 0;
@@ -121,8 +144,64 @@ struct Geometry {
     }
 };
 
+// What a unit computes: rows R0 .. R0 + n_rows - 1 of the sequence's list over positions
+// [key0, key1).  Row R sees positions below base + R / G.
+struct Work {
+    int R0, n_rows, base, key0, key1;
+};
+template <int TM, int BK>
+__device__ __forceinline__ Work unit_work(const cf_paged_attn_args_t& a, const PagedPlan& pl, const Unit& un) {
+    Work w;
+    const int G = a.H_q / a.H_kv;
+    w.R0 = un.tile * TM;
+    w.n_rows = min(un.s.n * G - w.R0, TM);
+    w.base = un.s.len - un.s.n + 1;
+    const int limit = min(max(w.base + fastdiv(w.R0 + w.n_rows - 1, pl.by_group), 0), un.s.len);
+    const int blocks = (limit + BK - 1) / BK;
+    const int per = (blocks + un.n_ranges - 1) / un.n_ranges;
+    const int b0 = min(un.range * per, blocks), b1 = min(b0 + per, blocks);
+    w.key0 = b0 * BK;
+    w.key1 = min(b1 * BK, limit);
+    return w;
+}
+
 // Record of one unit: [m (TM)] [l (TM)] [sum (TM, D)], m in the log2 domain.
 template <int TM, int D> constexpr size_t record_floats() { return (size_t)TM * (D + 2); }
+template <int TM, int D>
+__device__ __forceinline__ float* record_of(const cf_paged_attn_args_t& a, const PagedPlan& pl, const Unit& un, int kvh) {
+    return pl.records + ((size_t)(un.record + un.range) * a.H_kv + kvh) * record_floats<TM, D>();
+}
+
+// Row R of a sequence's list for KV head kvh: its place in Q or O, in rows of heads.
+struct RowAt { int tok, h; };
+__device__ __forceinline__ RowAt row_at(const PagedPlan& pl, int G, int kvh, int R) {
+    const int tok = fastdiv(R, pl.by_group);
+    return {tok, kvh * G + (R - tok * G)};
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, f4_t x) {
+    typedef T four_t __attribute__((ext_vector_type(4)));
+    *(four_t*)p = four_t{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+}
+
+// Table entries through the scalar cache: an ordinary load would make its wait drain the ring.
+typedef const int32_t __attribute__((address_space(4)))* table_t;
+__device__ __forceinline__ table_t table_of(const cf_paged_attn_args_t& a, int b) {
+    return (table_t)(uintptr_t)(a.table + (size_t)b * a.max_pages);
+}
+__device__ __forceinline__ int page_of(const cf_paged_attn_args_t& a, const PagedPlan& pl, table_t table, int key) {
+    return table[min(fastdiv(key, pl.by_page), a.max_pages - 1)];
+}
+// The group of 16 positions from `key` on `page`: where it starts in the cache (elements; page
+// 0 stands in for one that is none), and which of its positions count (below key1, a real page).
+struct Group { int64_t at; uint32_t mask; };
+__device__ __forceinline__ Group group_of(const cf_paged_attn_args_t& a, const PagedPlan& pl, int page, int key, int key1) {
+    const bool valid = (unsigned)page < (unsigned)a.num_pages;
+    const int count = valid ? min(max(key1 - key, 0), 16) : 0;
+    const int in_page = key - fastdiv(key, pl.by_page) * a.page_size;
+    return {(int64_t)(valid ? page : 0) * a.page_stride + (int64_t)in_page * a.row_stride, (1u << count) - 1u};
+}
 
 // LDS rows are swizzled in 16-byte chunks: K (and Q) rows are read 16 rows at one chunk, V
 // rows transposed (fp16, ds_read_b64_tr_b16) or 4 rows of 16 floats (fp32).
@@ -133,371 +212,916 @@ template <typename T, int D> __device__ __forceinline__ int vswz(int row) {
     return sizeof(T) == 4 ? row & 15 : D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3);
 }
 
-// SHARED: a workgroup of 4 waves, 16 NJ rows each, through one ring of 64-position blocks
-// (wave w loads positions 16 w .. 16 w + 15 of each).  Else a wave per unit, up to 16 rows,
-// with a ring of its own and no barrier: the units of neighbouring KV heads in one workgroup,
-// which read the same cache rows at about the same time.
-template <typename T, int D, int NJ, bool SHARED> struct Shape {
+// How rows of D elements lie in LDS and in lanes.
+template <typename T, int D> struct Rows {
     static constexpr bool F16 = sizeof(T) == 2;
-    static constexpr int WAVES = 4;
-    static constexpr int TM = SHARED ? 64 * NJ : 16;
-    static constexpr int BK = SHARED ? 64 : F16 ? 32 : 16;
-    static constexpr int NG = BK / 16;                        // 16-position groups of a block
-    static constexpr int TILE = BK * D;                       // elements of K (or V) per stage
-    static constexpr int NS = SHARED && F16 && D == 64 ? 3 : 2;
-    static constexpr int RINGS = SHARED ? 1 : WAVES;
-    static constexpr int LDS_ELEMS = RINGS * NS * 2 * TILE;
-    // Workgroups per CU by LDS (160 KB), which is waves per SIMD.
-    static constexpr int PER_CU = 160 * 1024 / (LDS_ELEMS * (int)sizeof(T)) > 2 && NJ == 2 ? 2
-                                : 160 * 1024 / (LDS_ELEMS * (int)sizeof(T));
+    static constexpr int CE = 16 / sizeof(T);          // elements per 16-byte chunk
+    static constexpr int CPR = D / CE;                 // chunks per row
+    static constexpr int RPI = 64 / CPR;               // rows per DMA instruction (1 KB)
+    static constexpr int NI = 16 / RPI;                // DMA instructions per 16 rows
+    static constexpr int NF = F16 ? D / 32 : D / 16;   // chunks of a K row a lane takes
+    static constexpr int UT = D / 16;                  // 16-dim tiles of O^T
+    static constexpr int VR = F16 ? UT : 4;            // V read offsets a lane keeps
+    typedef T chunk_t __attribute__((ext_vector_type(CE)));
+    // DMA: lane L of instruction u writes physical chunk L % CPR of row RPI u + L / CPR of a
+    // 16-row group, which holds logical chunk (L % CPR) ^ swizzle.
+    static __device__ __forceinline__ int drow() { return (threadIdx.x & 63) / CPR; }
+    static __device__ __forceinline__ int dch() { return (threadIdx.x & 63) % CPR; }
+    // LDS read offsets (elements) of the lane's K chunks inside 16 rows: fp16 lane (lr, lq)
+    // takes row lr, dims 32 f + 8 lq .. + 7; fp32 dims D / 4 lq + 4 f .. + 3 (k-slot lq of MFMA
+    // step s is dim D / 4 lq + s).
+    static __device__ __forceinline__ void k_offsets(int (&rd)[NF]) {
+        const int lr = threadIdx.x & 15, lq = (threadIdx.x >> 4) & 3;
+#pragma unroll
+        for (int f = 0; f < NF; f++) rd[f] = lr * D + CE * ((F16 ? 4 * f + lq : NF * lq + f) ^ kswz<T, D>(lr));
+    }
+    // ... of its V: fp16 (ds_read_tr4) key 4 lq + lr / 4, dims 16 u + 4 (lr % 4) .. + 3; fp32 row
+    // 4 lq + kk, whose chunk the read adds.
+    static __device__ __forceinline__ void v_offsets(int (&rd)[VR]) {
+        const int lr = threadIdx.x & 15, lq = (threadIdx.x >> 4) & 3;
+#pragma unroll
+        for (int u = 0; u < VR; u++) {
+            if constexpr (F16) {
+                const int row = 4 * lq + (lr >> 2), col = 16 * u + 4 * (lr & 3);
+                rd[u] = row * D + 8 * ((col >> 3) ^ vswz<T, D>(row)) + (col & 7);
+            } else {
+                rd[u] = (4 * lq + u) * D + (lr & 3);
+            }
+        }
+    }
+    // fp32: V of key 16 t + 4 lq + kk, dim 16 u + lr (base: the stage's V).
+    static __device__ __forceinline__ float v_at(const float* base, const int (&rd)[VR], int t, int kk, int u) {
+        const int lr = threadIdx.x & 15, lq = (threadIdx.x >> 4) & 3;
+        return base[rd[kk] + 16 * t * D + 4 * ((4 * u + (lr >> 2)) ^ vswz<T, D>(4 * lq + kk))];
+    }
 };
 
-template <typename T, int D, int NJ, bool SHARED>
-__global__ __launch_bounds__(256, (Shape<T, D, NJ, SHARED>::PER_CU))
-void paged_tiles(cf_paged_attn_args_t a, PagedPlan pl) {
-    using S = Shape<T, D, NJ, SHARED>;
-    constexpr bool F16 = S::F16;
-    constexpr int TM = S::TM, BK = S::BK, NG = S::NG, TILE = S::TILE, NS = S::NS;
-    constexpr int CE = 16 / sizeof(T);            // elements per 16-byte chunk
-    constexpr int CPR = D / CE;                   // chunks per row
-    constexpr int RPI = 64 / CPR;                 // rows per DMA instruction (1 KB)
-    constexpr int NI = 16 / RPI;                  // DMA instructions per 16 rows
-    constexpr int MYG = SHARED ? 1 : NG;          // groups this wave loads
-    constexpr int NL = 2 * MYG * NI;              // DMA instructions per wave and block
-    constexpr int NF = F16 ? D / 32 : D / 16;     // chunks of a K row a lane takes
-    constexpr int UT = D / 16;                    // 16-dim tiles of O^T
-    constexpr uint64_t FULL = BK == 64 ? ~0ull : (1ull << (BK & 63)) - 1;
-    static_assert((NS - 1) * NL < 64, "vmcnt range");
-    __shared__ __attribute__((aligned(16))) T ring_all[S::LDS_ELEMS];
+// The maximum moves only when a block exceeds it by more than 2^kLazy: until then p is at
+// most 2^kLazy, which fp16 holds as exactly as 1, and the sums are not rescaled.
+constexpr float kLazy = 8.0f;
+__device__ __forceinline__ bool move_max(float mloc, float& m, float& alpha) {
+    if (!__builtin_amdgcn_ballot_w64(mloc > m + kLazy)) return false;
+    const float m_new = mloc > m + kLazy ? mloc : m;
+    alpha = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));   // 0 on the first move
+    m = m_new;
+    return true;
+}
 
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int lr = lane & 15, lq = lane >> 4;
-    T* const ring = ring_all + (SHARED ? 0 : wave * NS * 2 * TILE);
+// Scores of a lane's row in a block: key 16 t + 4 lq + i of it counts where its bit of `mk` is
+// set and it is one of the first `seen`.
+template <int NG>
+__device__ __forceinline__ void hide(f4_t (&sc)[NG], uint64_t mk, int seen) {
+    const int at = 4 * ((threadIdx.x >> 4) & 3);
+    const uint64_t bits = mk >> at;
+    seen -= at;
+#pragma unroll
+    for (int t = 0; t < NG; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (!((bits >> (16 * t + i)) & 1) || 16 * t + i >= seen) sc[t][i] = -INFINITY;
+}
+
+// ---- Up to 16 rows, one wave with a ring of its own: no barrier. ----
+template <typename T, int D, int BK_> struct Narrow {
+    static constexpr int BK = BK_, NS = 2;
+    static constexpr int TILE = BK * D;
+    static constexpr int RING = NS * 2 * TILE;               // elements
+};
+
+// Positions [key0, key1) (key0 a multiple of 16) of (b, kvh) for the unit's rows: leaves m and
+// the lane's share of l, and lane (lr, lq) with dims 16 u + 4 lq .. + 3 of row lr.
+template <typename T, int D, int BK>
+__device__ __forceinline__ void narrow_range(const cf_paged_attn_args_t& a, const PagedPlan& pl, T* ring, const SeqRows& s,
+                                             int b, int kvh, const Work& w, int key0, int key1,
+                                             f4_t (&acc)[D / 16], float& m_run, float& l_run) {
+    using R = Rows<T, D>;
+    using N = Narrow<T, D, BK>;
+    typedef typename R::chunk_t chunk_t;
+    constexpr bool F16 = R::F16;
+    constexpr int NG = BK / 16, NS = N::NS, TILE = N::TILE, NI = R::NI, NL = 2 * NG * NI, UT = R::UT, CE = R::CE;
+    constexpr uint64_t FULL = (1ull << BK) - 1;
+    static_assert(NS * NL < 64, "vmcnt range");
+    const int lane = threadIdx.x & 63, lr = lane & 15;
     const int G = a.H_q / a.H_kv;
-    const Geometry<TM, BK> geo(a, pl);
+    const int drow = R::drow(), dch = R::dch();
+#pragma unroll
+    for (int u = 0; u < UT; u++) acc[u] = f4_t{0.f, 0.f, 0.f, 0.f};
+    m_run = -INFINITY;
+    l_run = 0.0f;
+    const int nblk = key1 > key0 ? (key1 - key0 + BK - 1) / BK : 0;
+    if (nblk == 0) return;
     const float c = a.scale * kLog2e;
+    const int seen = min(w.base + fastdiv(w.R0 + min(lr, w.n_rows - 1), pl.by_group), s.len);
+    const int seen_all = min(w.base + fastdiv(w.R0, pl.by_group), s.len);
 
-    // DMA offsets: lane L of instruction u writes physical chunk L % CPR of row RPI u + L / CPR
-    // of a 16-row group, which holds logical chunk (L % CPR) ^ swizzle.
-    const int drow = lane / CPR, dch = lane % CPR;
     uint32_t koff[NI], voff[NI];
 #pragma unroll
     for (int u = 0; u < NI; u++) {
-        const int row = RPI * u + drow;
-        koff[u] = (uint32_t)(row * (uint32_t)a.row_stride + CE * (dch ^ kswz<T, D>(row))) * (uint32_t)sizeof(T);
-        voff[u] = (uint32_t)(row * (uint32_t)a.row_stride + CE * (dch ^ vswz<T, D>(row))) * (uint32_t)sizeof(T);
+        const int row = R::RPI * u + drow;
+        koff[u] = ((uint32_t)row * (uint32_t)a.row_stride + CE * (dch ^ kswz<T, D>(row))) * (uint32_t)sizeof(T);
+        voff[u] = ((uint32_t)row * (uint32_t)a.row_stride + CE * (dch ^ vswz<T, D>(row))) * (uint32_t)sizeof(T);
     }
+    int k_rd[R::NF], v_rd[R::VR];
+    R::k_offsets(k_rd);
+    R::v_offsets(v_rd);
     const uint32_t ring_base = __builtin_amdgcn_readfirstlane(lds_offset(ring));
-    // LDS read offsets (elements) inside a stage.
-    int k_rd[NF];                                 // + 16 t D for key tile t
+    const table_t table = table_of(a, b);
+    const T* const kp = (const T*)a.k + (int64_t)kvh * a.head_stride;
+    const T* const vp = (const T*)a.v + (int64_t)kvh * a.head_stride;
+
+    int pages[NG];                                            // of the next block to issue
+    auto fetch = [&](int blk) {
 #pragma unroll
-    for (int f = 0; f < NF; f++) k_rd[f] = lr * D + CE * ((F16 ? 4 * f + lq : NF * lq + f) ^ kswz<T, D>(lr));
-    int v_rd[F16 ? UT : 4];
-    if constexpr (F16) {
-        // ds_read_tr4: lane addresses key 4 lq + lr / 4, dims 16 u + 4 (lr % 4) .. + 3.
+        for (int g = 0; g < NG; g++) pages[g] = page_of(a, pl, table, key0 + blk * BK + 16 * g);
+    };
+    uint64_t mask[NS];                                        // per stage: positions that count
+    auto issue = [&](int blk, auto stage_c) {
+        constexpr int stage = decltype(stage_c)::value;
+        uint64_t mk = 0;
 #pragma unroll
-        for (int u = 0; u < UT; u++) {
-            const int row = 4 * lq + (lr >> 2), col = 16 * u + 4 * (lr & 3);
-            v_rd[u] = TILE + row * D + 8 * ((col >> 3) ^ vswz<T, D>(row)) + (col & 7);
+        for (int g = 0; g < NG; g++) {
+            const Group gr = group_of(a, pl, pages[g], key0 + blk * BK + 16 * g, key1);
+            mk |= (uint64_t)gr.mask << (16 * g);
+            const uint32_t lds = ring_base + (uint32_t)((stage * 2 * TILE + 16 * g * D) * sizeof(T));
+#pragma unroll
+            for (int u = 0; u < NI; u++) {
+                lds_dma16_s(koff[u], kp + gr.at, lds + u * 1024u);
+                lds_dma16_s(voff[u], vp + gr.at, lds + (uint32_t)(TILE * sizeof(T)) + u * 1024u);
+            }
         }
-    } else {
+        mask[stage] = mk;
+    };
+
+    wait_lds_reads();                                         // what the ring held before
+    fetch(0);
+    // Q rows by DMA into the last stage, which the first blocks leave free.
+    {
+        const uint32_t qlds = ring_base + (uint32_t)((NS - 1) * 2 * TILE * sizeof(T));
 #pragma unroll
-        for (int kk = 0; kk < 4; kk++) v_rd[kk] = TILE + (4 * lq + kk) * D + (lr & 3);
+        for (int u = 0; u < NI; u++) {
+            const int row = R::RPI * u + drow;
+            const RowAt at = row_at(pl, G, kvh, w.R0 + min(row, w.n_rows - 1));
+            lds_dma16((const T*)a.q + (int64_t)(s.row0 + at.tok) * a.q_stride + at.h * D + CE * (dch ^ kswz<T, D>(row)),
+                      __builtin_amdgcn_readfirstlane(qlds + u * 1024u));
+        }
     }
-
-    for (int unit = SHARED ? (int)blockIdx.x : (int)blockIdx.x * S::WAVES + wave;; unit += pl.waves) {
-        const int range_id = unit / a.H_kv, kvh = unit - range_id * a.H_kv;
-        Unit un;
-        if (!geo.template find<false>(range_id, un)) break;
-        const int n_rows = min(un.s.n * G - un.tile * TM, TM);
-        const int R0 = un.tile * TM;
-        // Row R sees positions below base + R / G; the tile's last row the most.
-        const int base = un.s.len - un.s.n + 1;
-        const int limit = min(max(base + fastdiv(R0 + n_rows - 1, pl.by_group), 0), un.s.len);
-        const int all_blocks = (limit + BK - 1) / BK;
-        const int per = (all_blocks + un.n_ranges - 1) / un.n_ranges;
-        const int kb0 = min(un.range * per, all_blocks), nblk = min(kb0 + per, all_blocks) - kb0;
-
-        const int wrow = SHARED ? 16 * NJ * wave : 0;             // this wave's first row of the tile
-        const bool active = wrow < n_rows;
-        int seen[NJ];                                             // positions the lane's row sees
+    issue(0, std::integral_constant<int, 0>{});
+    if (1 < nblk) fetch(1);
+    wait_vm<NL>();
+    chunk_t qf[R::NF];                                        // B operand Q^T
 #pragma unroll
-        for (int j = 0; j < NJ; j++)
-            seen[j] = min(base + fastdiv(R0 + min(wrow + 16 * j + lr, n_rows - 1), pl.by_group), un.s.len);
-        const int seen_all = min(base + fastdiv(R0 + wrow, pl.by_group), un.s.len);   // every row of the wave
+    for (int f = 0; f < R::NF; f++) qf[f] = *(const chunk_t*)(ring + (NS - 1) * 2 * TILE + k_rd[f]);
+    wait_lds_reads();
 
-        typedef const int32_t __attribute__((address_space(4)))* const_i32;
-        const const_i32 table = (const_i32)(uintptr_t)(a.table + (size_t)un.b * a.max_pages);
+    auto step = [&](int bi, auto stage_c) {
+        constexpr int stage = decltype(stage_c)::value;
+        if (bi + NS - 1 < nblk) {
+            wait_lds_reads();                                 // the last reads of that stage
+            issue(bi + NS - 1, std::integral_constant<int, (stage + NS - 1) % NS>{});
+            if (bi + NS < nblk) fetch(bi + NS);
+        }
+        wait_ahead<NL, NS - 1>(min(NS - 1, nblk - 1 - bi));
+        const uint64_t mk = mask[stage];
+        T* const st = ring + stage * 2 * TILE;
+        if (mk != FULL) {
+            // V where nothing counts: 0, as p = 0 times whatever it holds need not be.
+#pragma unroll
+            for (int u = 0; u < NG * NI; u++) {
+                const int row = R::RPI * u + drow;
+                if (!((mk >> row) & 1)) *(uint4*)(st + TILE + row * D + CE * dch) = uint4{};
+            }
+            wait_lds_reads();
+        }
+        const int k0 = key0 + bi * BK;
+        // S^T: sc[t][i] = score(key k0 + 16 t + 4 lq + i, row lr).
+        f4_t sc[NG];
+#pragma unroll
+        for (int t = 0; t < NG; t++) {
+            sc[t] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int f = 0; f < R::NF; f++) {
+                const chunk_t kf = *(const chunk_t*)(st + 16 * t * D + k_rd[f]);
+                if constexpr (F16) {
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[f], sc[t], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[f][e], sc[t], 0, 0, 0);
+                }
+            }
+        }
+        if (mk != FULL || k0 + BK > seen_all) {
+            hide(sc, mk, seen - k0);
+        }
+        float mloc = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+#pragma unroll
+        for (int t = 1; t < NG; t++) mloc = fmaxf(mloc, fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3])));
+        mloc = max_xor32(max_xor16(mloc)) * c;                // -inf if the row sees nothing here
+        float alpha;
+        if (move_max(mloc, m_run, alpha)) {
+            l_run *= alpha;
+#pragma unroll
+            for (int u = 0; u < UT; u++) acc[u] *= alpha;
+        }
+        const float m_use = m_run == -INFINITY ? 0.0f : m_run;
+        _Float16 hi[F16 ? 4 * NG : 1], lo[F16 ? 4 * NG : 1];
+#pragma unroll
+        for (int t = 0; t < NG; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], c, -m_use));
+                l_run += p;
+                if constexpr (F16) {
+                    hi[4 * t + i] = (_Float16)p;
+                    lo[4 * t + i] = (_Float16)(p - (float)hi[4 * t + i]);
+                } else {
+                    sc[t][i] = p;
+                }
+            }
+        // O^T += V^T P^T, the lane's own scores being its B operand.  This wave waits on memory,
+        // not on products: p as the sum of two fp16 numbers, so that its rounding (2^-11 of it,
+        // otherwise as large as the result's own) leaves the result.
+        if constexpr (F16 && NG == 2) {
+            const h8_t pf = {hi[0], hi[1], hi[2], hi[3], hi[4], hi[5], hi[6], hi[7]};
+            const h8_t pr = {lo[0], lo[1], lo[2], lo[3], lo[4], lo[5], lo[6], lo[7]};
+#pragma unroll
+            for (int u = 0; u < UT; u++) {
+                const _Float16* const v = (const _Float16*)st + TILE + v_rd[u];
+                const h8_t vf = cat8(ds_read_tr4(v), ds_read_tr4(v + 16 * D));
+                acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pr, acc[u], 0, 0, 0);
+                acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf, acc[u], 0, 0, 0);
+            }
+        } else if constexpr (F16) {
+            // Both parts of 16 positions in one 32-k MFMA, V twice.
+            const h8_t pf = {hi[0], hi[1], hi[2], hi[3], lo[0], lo[1], lo[2], lo[3]};
+#pragma unroll
+            for (int u = 0; u < UT; u++) {
+                const h4_t v = ds_read_tr4((const _Float16*)st + TILE + v_rd[u]);
+                acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(cat8(v, v), pf, acc[u], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < NG; t++)
+#pragma unroll
+                for (int kk = 0; kk < 4; kk++)
+#pragma unroll
+                    for (int u = 0; u < UT; u++)
+                        acc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::v_at((const float*)st + TILE, v_rd, t, kk, u),
+                                                                      sc[t][kk], acc[u], 0, 0, 0);
+        }
+    };
+    for_each_stage<NS>(nblk, step);
+}
+
+// A wave per unit, the units of neighbouring KV heads in one workgroup: they read the same
+// cache rows at about the same time.
+template <typename T, int D> struct Heads {
+    static constexpr int WAVES = 4, BK = sizeof(T) == 2 ? 32 : 16;
+    static constexpr int RING = Narrow<T, D, BK>::RING;
+    static constexpr int PER_CU = 160 * 1024 / (WAVES * RING * (int)sizeof(T));
+};
+template <typename T, int D>
+__global__ __launch_bounds__(256, (Heads<T, D>::PER_CU))
+void paged_heads(cf_paged_attn_args_t a, PagedPlan pl) {
+    using H = Heads<T, D>;
+    __shared__ __attribute__((aligned(16))) T ring_all[H::WAVES * H::RING];
+    const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int G = a.H_q / a.H_kv;
+    const Geometry<16, H::BK, 1> geo(a, pl);
+    for (int unit = (int)blockIdx.x * H::WAVES + wave;; unit += pl.step) {
+        const int id = unit / a.H_kv, kvh = unit - id * a.H_kv;
+        Unit un;
+        if (!geo.template find<false>(id, un)) break;
+        const Work w = unit_work<16, H::BK>(a, pl, un);
+        f4_t acc[D / 16];
+        float m, l;
+        narrow_range<T, D, H::BK>(a, pl, ring_all + wave * H::RING, un.s, un.b, kvh, w, w.key0, w.key1, acc, m, l);
+        l = add_xor32(add_xor16(l));
+        if (lr < w.n_rows) {
+            if (un.n_ranges > 1) {
+                float* const rec = record_of<16, D>(a, pl, un, kvh);
+#pragma unroll
+                for (int u = 0; u < D / 16; u++) *(f4_t*)(rec + 2 * 16 + lr * D + 16 * u + 4 * lq) = acc[u];
+                if (lq == 0) {
+                    rec[lr] = m;
+                    rec[16 + lr] = l;
+                }
+            } else {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const RowAt at = row_at(pl, G, kvh, w.R0 + lr);
+                T* const o = (T*)a.o + ((int64_t)(un.s.row0 + at.tok) * a.H_q + at.h) * D + 4 * lq;
+#pragma unroll
+                for (int u = 0; u < D / 16; u++) store4(o + 16 * u, acc[u] * inv);
+            }
+        }
+    }
+}
+
+// Up to 16 rows by all waves of a workgroup: each takes a share of the unit's positions, and
+// they join their m, l and sums in LDS (WAVES rings at `lds`, one each).
+template <typename T, int D, int TM, int WAVES>
+__device__ __forceinline__ void narrow_unit(const cf_paged_attn_args_t& a, const PagedPlan& pl, T* lds, const Unit& un,
+                                            int kvh, const Work& w) {
+    constexpr int RING = Narrow<T, D, 16>::RING, LD = D + 4;
+    static_assert(16 * (LD + 2) * 4 <= RING * (int)sizeof(T), "a wave's rows fit its ring");
+    const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    T* const ring = lds + wave * RING;
+    const int groups = w.key1 > w.key0 ? (w.key1 - w.key0 + 15) / 16 : 0;
+    const int per = (groups + WAVES - 1) / WAVES * 16;
+    const int k0 = min(w.key0 + wave * per, w.key1), k1 = min(k0 + per, w.key1);
+    f4_t acc[D / 16];
+    float m, l;
+    narrow_range<T, D, 16>(a, pl, ring, un.s, un.b, kvh, w, k0, k1, acc, m, l);
+    l = add_xor32(add_xor16(l));
+    float* const mine = (float*)ring;                         // [16][LD], m [16], l [16]
+    wait_lds_reads();
+#pragma unroll
+    for (int u = 0; u < D / 16; u++) *(f4_t*)(mine + lr * LD + 16 * u + 4 * lq) = acc[u];
+    if (lq == 0) {
+        mine[16 * LD + lr] = m;
+        mine[16 * LD + 16 + lr] = l;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < w.n_rows * (D / 4); i += 64 * WAVES) {
+        const int row = i / (D / 4), d4 = i % (D / 4);
+        float M = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < WAVES; v++) M = fmaxf(M, ((const float*)(lds + v * RING))[16 * LD + row]);
+        const float m_use = M == -INFINITY ? 0.0f : M;
+        float L = 0.0f;
+        f4_t sum = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int v = 0; v < WAVES; v++) {
+            const float* const p = (const float*)(lds + v * RING);
+            const float x = __builtin_amdgcn_exp2f(p[16 * LD + row] - m_use);
+            L += p[16 * LD + 16 + row] * x;
+            sum += *(const f4_t*)(p + row * LD + 4 * d4) * x;
+        }
+        if (un.n_ranges > 1) {
+            float* const rec = record_of<TM, D>(a, pl, un, kvh);
+            *(f4_t*)(rec + 2 * TM + row * D + 4 * d4) = sum;
+            if (d4 == 0) {
+                rec[row] = M;
+                rec[TM + row] = L;
+            }
+        } else {
+            const RowAt at = row_at(pl, a.H_q / a.H_kv, kvh, w.R0 + row);
+            store4((T*)a.o + ((int64_t)(un.s.row0 + at.tok) * a.H_q + at.h) * D + 4 * d4,
+                   sum * (L == 0.0f ? 0.0f : 1.0f / L));
+        }
+    }
+    __syncthreads();                                          // the rings, before the next unit
+}
+
+template <typename T, int D> struct Split {
+    static constexpr int WAVES = sizeof(T) * D > 256 ? 4 : 8;   // 16 or (fp32, d = 128) 32 KB of LDS each
+};
+template <typename T, int D>
+__global__ __launch_bounds__(64 * (Split<T, D>::WAVES), (Split<T, D>::WAVES) / 4)
+void paged_split(cf_paged_attn_args_t a, PagedPlan pl) {
+    constexpr int WAVES = Split<T, D>::WAVES;
+    __shared__ __attribute__((aligned(16))) T lds[WAVES * Narrow<T, D, 16>::RING];
+    const Geometry<16, 64, 1> geo(a, pl);
+    for (int unit = (int)blockIdx.x;; unit += pl.step) {
+        const int id = unit / a.H_kv, kvh = unit - id * a.H_kv;
+        Unit un;
+        if (!geo.template find<false>(id, un)) break;
+        narrow_unit<T, D, 16, WAVES>(a, pl, lds, un, kvh, unit_work<16, 64>(a, pl, un));
+    }
+}
+
+// The end of a wide tile's wave: NJ blocks of 16 rows from row wrow of the tile.  Lane (lr, lq)
+// holds dims 16 u + 4 lq .. + 3 of row lr of each, and l whole.
+template <typename T, int D, int TM, int NJ>
+__device__ __forceinline__ void wide_store(const cf_paged_attn_args_t& a, const PagedPlan& pl, const Unit& un, int kvh,
+                                           const Work& w, int wrow, const f4_t (&acc)[NJ][D / 16], const float (&m)[NJ],
+                                           const float (&l)[NJ]) {
+    const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
+    float* const rec = un.n_ranges > 1 ? record_of<TM, D>(a, pl, un, kvh) : nullptr;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+        const int row = wrow + 16 * j + lr;
+        if (row >= w.n_rows) continue;
+        if (rec) {
+#pragma unroll
+            for (int u = 0; u < D / 16; u++) *(f4_t*)(rec + 2 * TM + row * D + 16 * u + 4 * lq) = acc[j][u];
+            if (lq == 0) {
+                rec[row] = m[j];
+                rec[TM + row] = l[j];
+            }
+            continue;
+        }
+        const float inv = l[j] == 0.0f ? 0.0f : 1.0f / l[j];
+        const RowAt at = row_at(pl, a.H_q / a.H_kv, kvh, w.R0 + row);
+        T* const o = (T*)a.o + ((int64_t)(un.s.row0 + at.tok) * a.H_q + at.h) * D + 4 * lq;
+#pragma unroll
+        for (int u = 0; u < D / 16; u++) store4(o + 16 * u, acc[j][u] * inv);
+    }
+}
+
+// ---- fp16, wide tiles: 8 waves of 16 NJ rows through one ring of 64-position blocks. ----
+// Scores and sums cost the matrix cores about what softmax costs the vector unit (d = 128, 32
+// rows, 64 positions: 64 MFMAs of 16 clk against ~190 vector instructions of 4 clk and 32
+// exponentials of 16), and a wave does one after the other.  So the two waves of a SIMD, w and
+// w + 4, take turns: with phases cut by barriers, waves 0 .. 3 run products while waves 4 .. 7
+// run softmax, then the other way round.  Products of turn i are S(i) = K_i Q^T and
+// O += V_{i-1} P(i-1), so a stage of the ring is K_i with V_{i-1}; with NS stages, NS - 2 of
+// them are still under way when one is needed.
+template <int D, int NJ> struct Wide16 {
+    static constexpr int TM = 128 * NJ, BK = 64, NS = 4;
+    static constexpr int TILE = BK * D;
+    static constexpr int STAGE = 2 * TILE;
+    static constexpr int LDS = NS * STAGE;                   // 128 KB (d = 128), 64 KB
+    static_assert(TM * D <= 2 * STAGE, "Q fits the last two stages");
+    static_assert(8 * Narrow<_Float16, D, 16>::RING <= LDS, "the rings of narrow tiles fit");
+};
+
+template <int D, int NJ>
+__device__ __forceinline__ void wide16_unit(const cf_paged_attn_args_t& a, const PagedPlan& pl, _Float16* lds, const Unit& un,
+                                            int kvh, const Work& w) {
+    using T = _Float16;
+    using R = Rows<T, D>;
+    using W = Wide16<D, NJ>;
+    constexpr int BK = W::BK, NS = W::NS, TILE = W::TILE, STAGE = W::STAGE, UT = R::UT, NF = R::NF;
+    constexpr int HI = R::NI / 2;                            // DMA instructions per 8 rows
+    constexpr int NL = 2 * HI;                               // ... of a wave per stage
+    static_assert(R::RPI <= 8 && (NS - 1) * NL < 64, "eight rows per wave");
+    const int lane = threadIdx.x & 63, lr = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int G = a.H_q / a.H_kv, drow = R::drow(), dch = R::dch();
+    const float c = a.scale * kLog2e;
+    const int wrow = 16 * NJ * wave;
+    const bool active = wrow < w.n_rows;
+    const int n = w.key1 > w.key0 ? (w.key1 - w.key0 + BK - 1) / BK : 0;
+    f4_t acc[NJ][UT], lsum[NJ];
+    float m_run[NJ];
+    int seen[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+        m_run[j] = -INFINITY;
+        lsum[j] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < UT; u++) acc[j][u] = f4_t{0.f, 0.f, 0.f, 0.f};
+        seen[j] = min(w.base + fastdiv(w.R0 + min(wrow + 16 * j + lr, w.n_rows - 1), pl.by_group), un.s.len);
+    }
+    const int seen_all = min(w.base + fastdiv(w.R0 + min(wrow, w.n_rows - 1), pl.by_group), un.s.len);
+
+    if (n > 0) {
+        // This wave's rows of a block: 8 half + 0 .. 7 of group `grp`.
+        const int grp = wave >> 1, half = wave & 1;
+        uint32_t koff[HI], voff[HI];
+#pragma unroll
+        for (int u = 0; u < HI; u++) {
+            const int row = 8 * half + R::RPI * u + drow;
+            koff[u] = ((uint32_t)row * (uint32_t)a.row_stride + 8 * (dch ^ kswz<T, D>(row))) * 2u;
+            voff[u] = ((uint32_t)row * (uint32_t)a.row_stride + 8 * (dch ^ vswz<T, D>(row))) * 2u;
+        }
+        int k_rd[NF], v_rd[UT];
+        R::k_offsets(k_rd);
+        R::v_offsets(v_rd);
+        const uint32_t lds_base = __builtin_amdgcn_readfirstlane(lds_offset(lds));
+        const uint32_t my_lds = lds_base + (uint32_t)((16 * grp + 8 * half) * D * 2);
+        const table_t table = table_of(a, un.b);
         const T* const kp = (const T*)a.k + (int64_t)kvh * a.head_stride;
         const T* const vp = (const T*)a.v + (int64_t)kvh * a.head_stride;
-        int pages[NG];                                            // of the next block to issue
-        auto fetch = [&](int blk) {
+
+        // Stage i of the ring is issued with the pages of block i (K) and what is kept of block
+        // i - 1 (V).  Blocks outside 0 .. n - 1 load the nearest one, so every stage is NL loads.
+        int pages[4];
+        auto fetch = [&](int i) {
+            const int key = w.key0 + min(i, n - 1) * BK;
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const int key = (kb0 + blk) * BK + 16 * g;
-                pages[g] = table[min(fastdiv(key, pl.by_page), a.max_pages - 1)];
+            for (int g = 0; g < 4; g++) pages[g] = page_of(a, pl, table, key + 16 * g);
+        };
+        int64_t v_at = 0;
+        uint64_t mask[NS];                                    // of blocks i .. i + NS - 1 (i: this turn)
+        auto issue = [&](int i, int slot) -> uint64_t {
+            const int key = w.key0 + min(i, n - 1) * BK;
+            uint64_t mk = 0;
+            int64_t k_at = 0;
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const Group gr = group_of(a, pl, pages[g], key + 16 * g, w.key1);
+                mk |= (uint64_t)gr.mask << (16 * g);
+                if (g == grp) k_at = gr.at;
+            }
+            if (i == 0) v_at = k_at;
+            const uint32_t to = my_lds + (uint32_t)(slot * STAGE * 2);
+#pragma unroll
+            for (int u = 0; u < HI; u++) {
+                lds_dma16_s(koff[u], kp + k_at, to + u * 1024u);
+                lds_dma16_s(voff[u], vp + v_at, to + (uint32_t)(TILE * 2) + u * 1024u);
+            }
+            v_at = k_at;
+            return mk;
+        };
+
+        fetch(0);
+        {
+            const uint32_t qlds = lds_base + (uint32_t)((2 * STAGE + wrow * D) * 2);
+#pragma unroll
+            for (int u = 0; u < 16 * NJ / R::RPI; u++) {
+                const int row = R::RPI * u + drow;
+                const RowAt at = row_at(pl, G, kvh, w.R0 + min(wrow + row, w.n_rows - 1));
+                lds_dma16((const T*)a.q + (int64_t)(un.s.row0 + at.tok) * a.q_stride + at.h * D + 8 * (dch ^ kswz<T, D>(row)),
+                          __builtin_amdgcn_readfirstlane(qlds + u * 1024u));
+            }
+        }
+        mask[0] = issue(0, 0);
+        fetch(1);
+        mask[1] = issue(1, 1);                                // n >= 1: stages 0 and 1 exist
+        fetch(2);
+        wait_vm<2 * NL>();
+        h8_t qf[NJ][NF];
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+#pragma unroll
+            for (int f = 0; f < NF; f++) qf[j][f] = *(const h8_t*)(lds + 2 * STAGE + (wrow + 16 * j) * D + k_rd[f]);
+        wait_lds_reads();
+
+        f4_t sc[NJ][4];
+        h8_t pf[NJ][2];
+        h8_t ones = {1, 1, 1, 1, 1, 1, 1, 1};
+        asm volatile("" : "+v"(ones));                        // kept in registers for the whole loop
+        uint64_t v_mask = ~0ull;                              // of the V of the stage that lands next
+        int slot = 0;                                         // of this turn's stage
+
+        // Before the barrier that starts turn i: its stage has landed, this wave's share of it, and
+        // its V is 0 where nothing counts (p = 0 times whatever it holds need not be).
+        auto landed = [&](int i, int at) {
+            wait_ahead<NL, NS - 2>(min(i == 0 ? 1 : NS - 2, n - i));
+            if (i > 0 && v_mask != ~0ull) {
+#pragma unroll
+                for (int u = 0; u < HI; u++) {
+                    const int row = 16 * grp + 8 * half + R::RPI * u + drow;
+                    if (!((v_mask >> row) & 1)) *(uint4*)(lds + at * STAGE + TILE + row * D + 8 * dch) = uint4{};
+                }
+                wait_lds_reads();
             }
         };
-        uint64_t mask[NS];                                        // per stage: positions that count
-        auto issue = [&](int blk, auto stage_c) {
+        // After it: the stage of turn i - 1 is free.
+        auto refill = [&](int i, int at) {
+            if (i == 0) {
+                if (2 <= n) {
+                    mask[2] = issue(2, 2);
+                    fetch(3);
+                }
+                if (3 <= n) {
+                    mask[3] = issue(3, 3);
+                    fetch(4);
+                }
+            } else if (i + NS - 1 <= n) {
+                mask[NS - 1] = issue(i + NS - 1, at == 0 ? NS - 1 : at - 1);
+                fetch(i + NS);
+            }
+        };
+        // Fragment x of a turn: x < 2 UT is V^T (32-key step x / UT, dims 16 (x % UT)), the rest K
+        // (key tile, then chunk).  They are read kAhead fragments before their products, in
+        // exactly this order: left to itself the compiler reads them all first and spills.
+        constexpr int kAhead = 6, kV = 2 * UT, kAll = kV + 4 * NF;
+        auto products = [&](int at, auto first_c, auto last_c) {   // fragments first .. last - 1
+            constexpr int first = decltype(first_c)::value, last = decltype(last_c)::value;
+            if (!active) return;
+            const T* const st = lds + at * STAGE;
+            h8_t frag[kAhead];
+            auto read = [&](auto x_c) {
+                constexpr int x = decltype(x_c)::value;
+                if constexpr (x < kV) {
+                    const T* const v = st + TILE + v_rd[x % UT] + 32 * (x / UT) * D;
+                    frag[x % kAhead] = cat8(ds_read_tr4(v), ds_read_tr4(v + 16 * D));
+                } else if constexpr (x < kAll) {
+                    frag[x % kAhead] = *(const h8_t*)(st + 16 * ((x - kV) / NF) * D + k_rd[(x - kV) % NF]);
+                }
+            };
+            auto use = [&](auto x_c) {
+                constexpr int x = decltype(x_c)::value;
+                const h8_t f = frag[x % kAhead];
+                // O^T += V^T P^T: in 32-key step s2, k-slot e of lane group lq is key
+                // 32 s2 + 16 (e / 4) + 4 lq + e % 4, the lane's own scores.  l comes out of the matrix
+                // cores too, from the same rounded p that weights V.
+                if constexpr (x < kV) {
+                    if constexpr (x % UT == 0)
+#pragma unroll
+                        for (int j = 0; j < NJ; j++)
+                            lsum[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pf[j][x / UT], lsum[j], 0, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < NJ; j++)
+                        acc[j][x % UT] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, pf[j][x / UT], acc[j][x % UT], 0, 0, 0);
+                } else {
+                    // S^T: sc[j][t][e] = score(key 16 t + 4 lq + e of block i, row j).
+                    constexpr int t = (x - kV) / NF, c0 = (x - kV) % NF;
+#pragma unroll
+                    for (int j = 0; j < NJ; j++)
+                        sc[j][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, qf[j][c0], c0 == 0 ? f4_t{0.f, 0.f, 0.f, 0.f} : sc[j][t],
+                                                                          0, 0, 0);
+                }
+            };
+            __builtin_amdgcn_s_setprio(1);
+            static_for<kAhead - 1>([&](auto k) {
+                constexpr int x = first + decltype(k)::value;
+                if constexpr (x < last) read(std::integral_constant<int, x>{});
+            });
+            __builtin_amdgcn_sched_barrier(0);
+            static_for<last - first>([&](auto k) {
+                constexpr int x = first + decltype(k)::value;
+                if constexpr (x + kAhead - 1 < last) read(std::integral_constant<int, x + kAhead - 1>{});
+                use(std::integral_constant<int, x>{});
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            __builtin_amdgcn_s_setprio(0);
+        };
+        const std::integral_constant<int, 0> from_v;
+        const std::integral_constant<int, kV> to_v;
+        const std::integral_constant<int, kAll> to_k;
+        auto softmax = [&](int i, uint64_t mk) {
+            if (!active) return;
+            const int k0 = w.key0 + i * BK;
+            const bool edge = mk != ~0ull || k0 + BK > seen_all;
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                if (edge) hide(sc[j], mk, seen[j] - k0);
+                // Chains of three-input maxima.
+                float mloc = fmaxf(fmaxf(sc[j][0][0], sc[j][0][1]), sc[j][0][2]);
+#pragma unroll
+                for (int e = 3; e < 15; e += 2)
+                    mloc = fmaxf(fmaxf(mloc, sc[j][e >> 2][e & 3]), sc[j][(e + 1) >> 2][(e + 1) & 3]);
+                mloc = fmaxf(mloc, sc[j][3][3]);
+                mloc = max_xor32(max_xor16(mloc)) * c;        // -inf if the row sees nothing here
+                float alpha;
+                if (move_max(mloc, m_run[j], alpha)) {
+                    lsum[j] *= alpha;
+#pragma unroll
+                    for (int u = 0; u < UT; u++) acc[j][u] *= alpha;
+                }
+                const float m_use = m_run[j] == -INFINITY ? 0.0f : m_run[j];
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        pf[j][t >> 1][(t & 1) * 4 + e] =
+                            (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][t][e], c, -m_use));
+            }
+        };
+        // Turn i's softmax takes the mask of block i; the V of the stage of turn i + 1 is that block's.
+        auto next_turn = [&]() {
+#pragma unroll
+            for (int k = 0; k + 1 < NS; k++) mask[k] = mask[k + 1];
+            slot = slot == NS - 1 ? 0 : slot + 1;
+        };
+
+        landed(0, 0);
+        ring_barrier();
+        refill(0, 0);
+        // Turn i of waves 0 .. 3 takes phases 2 i (products) and 2 i + 1, of the others 2 i + 1 and
+        // 2 i + 2; everybody meets at every barrier, 2 n + 2 of them.
+        auto first_half = [&](int i) {
+            ring_barrier();
+            v_mask = mask[0];
+            softmax(i, v_mask);
+            next_turn();
+            landed(i + 1, slot);
+            ring_barrier();
+            refill(i + 1, slot);
+        };
+        auto second_half = [&](int i) {
+            v_mask = mask[0];
+            const uint64_t mk = v_mask;
+            next_turn();
+            landed(i + 1, slot);
+            ring_barrier();
+            refill(i + 1, slot);
+            softmax(i, mk);
+            ring_barrier();
+        };
+        if (wave < 4) {
+            products(slot, to_v, to_k);
+            first_half(0);
+#pragma clang loop unroll(disable)
+            for (int i = 1; i < n; i++) {
+                products(slot, from_v, to_k);
+                first_half(i);
+            }
+            products(slot, from_v, to_v);
+            ring_barrier();
+        } else {
+            ring_barrier();
+            products(slot, to_v, to_k);
+            second_half(0);
+#pragma clang loop unroll(disable)
+            for (int i = 1; i < n; i++) {
+                products(slot, from_v, to_k);
+                second_half(i);
+            }
+            products(slot, from_v, to_v);
+        }
+    }
+    float l[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; j++) l[j] = lsum[j][0];
+    wide_store<T, D, W::TM, NJ>(a, pl, un, kvh, w, wrow, acc, m_run, l);
+    ring_barrier();                                           // the ring's reads, before the next unit
+}
+
+constexpr int kNarrowCost = 4;
+template <int D, int NJ>
+__global__ __launch_bounds__(512, 2)
+void paged_wide16(cf_paged_attn_args_t a, PagedPlan pl) {
+    using W = Wide16<D, NJ>;
+    __shared__ __attribute__((aligned(16))) _Float16 lds[W::LDS];
+    const Geometry<W::TM, 64, kNarrowCost> geo(a, pl);
+    for (int unit = (int)blockIdx.x;; unit += pl.step) {
+        const int id = unit / a.H_kv, kvh = unit - id * a.H_kv;
+        Unit un;
+        if (!geo.template find<false>(id, un)) break;
+        const Work w = unit_work<W::TM, 64>(a, pl, un);
+        if (w.n_rows <= 16) narrow_unit<_Float16, D, W::TM, 8>(a, pl, lds, un, kvh, w);
+        else wide16_unit<D, NJ>(a, pl, lds, un, kvh, w);
+    }
+}
+
+// ---- fp32, wide tiles: 4 waves of 16 rows, the fp32 MFMA (32 clk each, 128 or 256 of them per
+// 64 positions) bounds it and nothing need be interleaved. ----
+template <int D> struct Wide32 {
+    static constexpr int TM = 64, BK = 64, NS = 2, TILE = BK * D, LDS = NS * 2 * TILE;   // 64 or 128 KB
+    static constexpr int PER_CU = D == 64 ? 2 : 1;
+};
+template <int D>
+__device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const PagedPlan& pl, float* ring, const Unit& un,
+                                            int kvh, const Work& w) {
+    using T = float;
+    using R = Rows<T, D>;
+    using W = Wide32<D>;
+    constexpr int BK = W::BK, NS = W::NS, TILE = W::TILE, NI = R::NI, NL = 2 * NI, UT = R::UT, NF = R::NF;
+    static_assert(NS * NL < 64, "vmcnt range");
+    const int lane = threadIdx.x & 63, lr = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int G = a.H_q / a.H_kv, drow = R::drow(), dch = R::dch();
+    const float c = a.scale * kLog2e;
+    const int wrow = 16 * wave;
+    const bool active = wrow < w.n_rows;
+    const int n = w.key1 > w.key0 ? (w.key1 - w.key0 + BK - 1) / BK : 0;
+    const int seen = min(w.base + fastdiv(w.R0 + min(wrow + lr, w.n_rows - 1), pl.by_group), un.s.len);
+    const int seen_all = min(w.base + fastdiv(w.R0 + min(wrow, w.n_rows - 1), pl.by_group), un.s.len);
+    f4_t acc[1][UT];
+    float m_run = -INFINITY, l_run = 0.0f;
+#pragma unroll
+    for (int u = 0; u < UT; u++) acc[0][u] = f4_t{0.f, 0.f, 0.f, 0.f};
+    if (n > 0) {
+        uint32_t koff[NI], voff[NI];
+#pragma unroll
+        for (int u = 0; u < NI; u++) {
+            const int row = R::RPI * u + drow;
+            koff[u] = ((uint32_t)row * (uint32_t)a.row_stride + 4 * (dch ^ kswz<T, D>(row))) * 4u;
+            voff[u] = ((uint32_t)row * (uint32_t)a.row_stride + 4 * (dch ^ vswz<T, D>(row))) * 4u;
+        }
+        int k_rd[NF], v_rd[R::VR];
+        R::k_offsets(k_rd);
+        R::v_offsets(v_rd);
+        const uint32_t ring_base = __builtin_amdgcn_readfirstlane(lds_offset(ring));
+        const table_t table = table_of(a, un.b);
+        const T* const kp = (const T*)a.k + (int64_t)kvh * a.head_stride;
+        const T* const vp = (const T*)a.v + (int64_t)kvh * a.head_stride;
+        int pages[4];
+        auto fetch = [&](int i) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) pages[g] = page_of(a, pl, table, w.key0 + i * BK + 16 * g);
+        };
+        uint64_t mask[NS];
+        auto issue = [&](int i, auto stage_c) {               // wave w: group w of K and V
             constexpr int stage = decltype(stage_c)::value;
             uint64_t mk = 0;
+            int64_t at = 0;
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const int key = (kb0 + blk) * BK + 16 * g;
-                const bool valid = (unsigned)pages[g] < (unsigned)a.num_pages;
-                const int count = valid ? min(max(limit - key, 0), 16) : 0;
-                mk |= (uint64_t)((1u << count) - 1u) << (16 * g);
-                if (!SHARED || g == wave) {
-                    const int in_page = key - fastdiv(key, pl.by_page) * a.page_size;
-                    const int64_t at = (int64_t)(valid ? pages[g] : 0) * a.page_stride + (int64_t)in_page * a.row_stride;
-                    const uint32_t lds = ring_base + (uint32_t)((stage * 2 * TILE + 16 * g * D) * sizeof(T));
+            for (int g = 0; g < 4; g++) {
+                const Group gr = group_of(a, pl, pages[g], w.key0 + i * BK + 16 * g, w.key1);
+                mk |= (uint64_t)gr.mask << (16 * g);
+                if (g == wave) at = gr.at;
+            }
+            const uint32_t to = ring_base + (uint32_t)((stage * 2 * TILE + wrow * D) * 4);
 #pragma unroll
-                    for (int u = 0; u < NI; u++) {
-                        lds_dma16_s(koff[u], kp + at, lds + u * 1024u);
-                        lds_dma16_s(voff[u], vp + at, lds + (uint32_t)(TILE * sizeof(T)) + u * 1024u);
-                    }
-                }
+            for (int u = 0; u < NI; u++) {
+                lds_dma16_s(koff[u], kp + at, to + u * 1024u);
+                lds_dma16_s(voff[u], vp + at, to + (uint32_t)(TILE * 4) + u * 1024u);
             }
             mask[stage] = mk;
         };
-
-        f4_t acc[NJ][UT];
-        float m_run[NJ], l_run[NJ];
+        fetch(0);
+        {
+            const uint32_t qlds = ring_base + (uint32_t)(((NS - 1) * 2 * TILE + wrow * D) * 4);
 #pragma unroll
-        for (int j = 0; j < NJ; j++) {
-            m_run[j] = -INFINITY;
-            l_run[j] = 0.0f;
-#pragma unroll
-            for (int u = 0; u < UT; u++) acc[j][u] = f4_t{0.f, 0.f, 0.f, 0.f};
-        }
-
-        if (nblk > 0) {
-            // Q rows by DMA into the last stage, which the first blocks leave free.
-            fetch(0);
-            {
-                constexpr int QI = (SHARED ? 16 * NJ : 16) / RPI;
-                const uint32_t qlds = ring_base + (uint32_t)(((NS - 1) * 2 * TILE + wrow * D) * sizeof(T));
-#pragma unroll
-                for (int u = 0; u < QI; u++) {
-                    const int row = min(wrow + RPI * u + drow, n_rows - 1);
-                    const int tok = fastdiv(R0 + row, pl.by_group), h = kvh * G + (R0 + row - tok * G);
-                    lds_dma16((const T*)a.q + (int64_t)(un.s.row0 + tok) * a.q_stride + h * D +
-                                  CE * (dch ^ kswz<T, D>(RPI * u + drow)),
-                              __builtin_amdgcn_readfirstlane(qlds + u * 1024u));
-                }
-            }
-            issue(0, std::integral_constant<int, 0>{});
-            if constexpr (NS > 2)
-                if (1 < nblk) {
-                    fetch(1);
-                    issue(1, std::integral_constant<int, 1>{});
-                }
-            if (nblk >= NS) fetch(NS - 1);
-            if (NS > 2 && nblk >= 2) wait_vm<(NS - 1) * NL>();
-            else wait_vm<NL>();
-            // B operand Q^T: fp16 lane (lr, lq) holds Q[row][32 f + 8 lq .. + 7]; fp32 lane holds
-            // Q[row][D / 4 lq + 4 f .. + 3], k-slot lq of step s being dim D / 4 lq + s.
-            typedef T chunk_t __attribute__((ext_vector_type(CE)));
-            chunk_t qf[NJ][NF];
-            const T* const qs = ring + (NS - 1) * 2 * TILE + wrow * D;
-#pragma unroll
-            for (int j = 0; j < NJ; j++)
-#pragma unroll
-                for (int f = 0; f < NF; f++) qf[j][f] = *(const chunk_t*)(qs + 16 * j * D + k_rd[f]);
-            wait_lds_reads();
-
-            auto step = [&](int bi, auto stage_c) {
-                constexpr int stage = decltype(stage_c)::value;
-                constexpr int next = (stage + NS - 1) % NS;
-                if constexpr (!SHARED) {
-                    if (bi + NS - 1 < nblk) {
-                        wait_lds_reads();                         // the last reads of that stage
-                        issue(bi + NS - 1, std::integral_constant<int, next>{});
-                        if (bi + NS < nblk) fetch(bi + NS);
-                    }
-                    wait_ahead<NL, NS - 1>(min(NS - 1, nblk - 1 - bi));
-                } else {
-                    wait_ahead<NL, NS - 2>(nblk - 1 - bi);
-                }
-                const uint64_t mk = mask[stage];
-                const T* const st = ring + stage * 2 * TILE;
-                if (mk != FULL) {
-                    // V where nothing counts: 0, as p = 0 times whatever it holds need not be.
-#pragma unroll
-                    for (int g = 0; g < NG; g++)
-                        if (!SHARED || g == wave)
-#pragma unroll
-                            for (int u = 0; u < NI; u++) {
-                                const int row = 16 * g + RPI * u + drow;
-                                if (!((mk >> row) & 1)) *(uint4*)(ring + stage * 2 * TILE + TILE + row * D + CE * dch) = uint4{};
-                            }
-                    wait_lds_reads();
-                }
-                if constexpr (SHARED) {
-                    ring_barrier();
-                    if (bi + NS - 1 < nblk) {
-                        issue(bi + NS - 1, std::integral_constant<int, next>{});
-                        if (bi + NS < nblk) fetch(bi + NS);
-                    }
-                }
-                if (!active) return;
-                const int k0 = (kb0 + bi) * BK;
-                // S^T: sc[j][t][i] = score(key k0 + 16 t + 4 lq + i, row j).
-                f4_t sc[NJ][NG];
-#pragma unroll
-                for (int t = 0; t < NG; t++) {
-#pragma unroll
-                    for (int j = 0; j < NJ; j++) sc[j][t] = f4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int f = 0; f < NF; f++) {
-                        const chunk_t kf = *(const chunk_t*)(st + 16 * t * D + k_rd[f]);
-#pragma unroll
-                        for (int j = 0; j < NJ; j++) {
-                            if constexpr (F16) {
-                                sc[j][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[j][f], sc[j][t], 0, 0, 0);
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 4; e++)
-                                    sc[j][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[j][f][e], sc[j][t], 0, 0, 0);
-                            }
-                        }
-                    }
-                }
-                const bool edge = mk != FULL || k0 + BK > seen_all;
-                _Float16 ph[NJ][4 * NG], pl16[SHARED ? 1 : NJ][4 * NG];
-#pragma unroll
-                for (int j = 0; j < NJ; j++) {
-                    if (edge) {
-#pragma unroll
-                        for (int t = 0; t < NG; t++)
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                const int key = 16 * t + 4 * lq + i;
-                                if (!((mk >> key) & 1) || k0 + key >= seen[j]) sc[j][t][i] = -INFINITY;
-                            }
-                    }
-                    float mloc = fmaxf(fmaxf(sc[j][0][0], sc[j][0][1]), fmaxf(sc[j][0][2], sc[j][0][3]));
-#pragma unroll
-                    for (int t = 1; t < NG; t++)
-                        mloc = fmaxf(mloc, fmaxf(fmaxf(sc[j][t][0], sc[j][t][1]), fmaxf(sc[j][t][2], sc[j][t][3])));
-                    mloc = max_xor32(max_xor16(mloc)) * c;        // -inf if the row sees nothing here
-                    // The maximum moves only when a block exceeds it by more than 2^kLazy.
-                    constexpr float kLazy = 8.0f;
-                    if (__builtin_amdgcn_ballot_w64(mloc > m_run[j] + kLazy)) {
-                        const float m_new = mloc > m_run[j] + kLazy ? mloc : m_run[j];
-                        const float alpha = __builtin_amdgcn_exp2f(m_run[j] - (m_new == -INFINITY ? 0.0f : m_new));
-                        m_run[j] = m_new;
-                        l_run[j] *= alpha;
-#pragma unroll
-                        for (int u = 0; u < UT; u++) acc[j][u] *= alpha;
-                    }
-                    const float m_use = m_run[j] == -INFINITY ? 0.0f : m_run[j];
-                    float psum = 0.0f;
-#pragma unroll
-                    for (int t = 0; t < NG; t++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][t][i], c, -m_use));
-                            psum += p;
-                            if constexpr (F16) {
-                                ph[j][4 * t + i] = (_Float16)p;
-                                if constexpr (!SHARED) pl16[j][4 * t + i] = (_Float16)(p - (float)ph[j][4 * t + i]);
-                            } else {
-                                sc[j][t][i] = p;
-                            }
-                        }
-                    l_run[j] += psum;
-                }
-                // O^T += V^T P^T.  fp16: in 32-key step s, k-slot e of lane group lq is key
-                // 32 s + 16 (e / 4) + 4 lq + e % 4; fp32: in step kk of key tile t, key 16 t + 4 lq + kk:
-                // the lane's own scores either way.
-                if constexpr (F16) {
-#pragma unroll
-                    for (int s2 = 0; s2 < NG / 2; s2++) {
-                        h8_t pf[NJ], pr[SHARED ? 1 : NJ];
-#pragma unroll
-                        for (int j = 0; j < NJ; j++)
-#pragma unroll
-                            for (int e = 0; e < 8; e++) {
-                                pf[j][e] = ph[j][8 * s2 + e];
-                                if constexpr (!SHARED) pr[j][e] = pl16[j][8 * s2 + e];
-                            }
-#pragma unroll
-                        for (int u = 0; u < UT; u++) {
-                            const h8_t vf = cat8(ds_read_tr4((const _Float16*)st + v_rd[u] + 32 * s2 * D),
-                                                 ds_read_tr4((const _Float16*)st + v_rd[u] + (32 * s2 + 16) * D));
-#pragma unroll
-                            for (int j = 0; j < NJ; j++) {
-                                // A wave of its own waits on memory, not on products: p as two fp16 numbers.
-                                if constexpr (!SHARED)
-                                    acc[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pr[j], acc[j][u], 0, 0, 0);
-                                acc[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[j], acc[j][u], 0, 0, 0);
-                            }
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int t = 0; t < NG; t++)
-#pragma unroll
-                        for (int kk = 0; kk < 4; kk++)
-#pragma unroll
-                            for (int u = 0; u < UT; u++) {
-                                const float vf = st[v_rd[kk] + 16 * t * D + 4 * ((4 * u + (lr >> 2)) ^ vswz<T, D>(4 * lq + kk))];
-#pragma unroll
-                                for (int j = 0; j < NJ; j++)
-                                    acc[j][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf, sc[j][t][kk], acc[j][u], 0, 0, 0);
-                            }
-                }
-            };
-            for_each_stage<NS>(nblk, step);
-        }
-
-        // Lane (lr, lq) holds dims 16 u + 4 lq .. + 3 of row lr.
-        if (active) {
-            float* const rec = un.n_ranges > 1
-                ? pl.records + ((size_t)(un.record + un.range) * a.H_kv + kvh) * record_floats<TM, D>() : nullptr;
-#pragma unroll
-            for (int j = 0; j < NJ; j++) {
-                const int row = wrow + 16 * j + lr;
-                const float l = add_xor32(add_xor16(l_run[j]));
-                if (row >= n_rows) continue;
-                if (rec) {
-#pragma unroll
-                    for (int u = 0; u < UT; u++) *(f4_t*)(rec + 2 * TM + row * D + 16 * u + 4 * lq) = acc[j][u];
-                    if (lq == 0) {
-                        rec[row] = m_run[j];
-                        rec[TM + row] = l;
-                    }
-                    continue;
-                }
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                const int tok = fastdiv(R0 + row, pl.by_group), h = kvh * G + (R0 + row - tok * G);
-                T* const o = (T*)a.o + ((int64_t)(un.s.row0 + tok) * a.H_q + h) * D + 4 * lq;
-#pragma unroll
-                for (int u = 0; u < UT; u++) {
-                    typedef T four_t __attribute__((ext_vector_type(4)));
-                    *(four_t*)(o + 16 * u) = four_t{(T)(acc[j][u][0] * inv), (T)(acc[j][u][1] * inv), (T)(acc[j][u][2] * inv),
-                                                    (T)(acc[j][u][3] * inv)};
-                }
+            for (int u = 0; u < NI; u++) {
+                const int row = R::RPI * u + drow;
+                const RowAt at = row_at(pl, G, kvh, w.R0 + min(wrow + row, w.n_rows - 1));
+                lds_dma16((const T*)a.q + (int64_t)(un.s.row0 + at.tok) * a.q_stride + at.h * D + 4 * (dch ^ kswz<T, D>(row)),
+                          __builtin_amdgcn_readfirstlane(qlds + u * 1024u));
             }
         }
-        if constexpr (SHARED) ring_barrier();                     // the ring's reads, before the next unit's Q
+        issue(0, std::integral_constant<int, 0>{});
+        if (1 < n) fetch(1);
+        wait_vm<NL>();
+        f4_t qf[NF];
+#pragma unroll
+        for (int f = 0; f < NF; f++) qf[f] = *(const f4_t*)(ring + (NS - 1) * 2 * TILE + wrow * D + k_rd[f]);
+        wait_lds_reads();
+        auto step = [&](int i, auto stage_c) {
+            constexpr int stage = decltype(stage_c)::value;
+            wait_vm<0>();
+            const uint64_t mk = mask[stage];
+            const T* const st = ring + stage * 2 * TILE;
+            if (mk != ~0ull) {
+#pragma unroll
+                for (int u = 0; u < NI; u++) {
+                    const int row = wrow + R::RPI * u + drow;
+                    if (!((mk >> row) & 1)) *(uint4*)(ring + stage * 2 * TILE + TILE + row * D + 4 * dch) = uint4{};
+                }
+                wait_lds_reads();
+            }
+            ring_barrier();
+            if (i + 1 < n) {
+                issue(i + 1, std::integral_constant<int, (stage + 1) % NS>{});
+                if (i + 2 < n) fetch(i + 2);
+            }
+            if (!active) return;
+            const int k0 = w.key0 + i * BK;
+            f4_t sc[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                sc[t] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int f = 0; f < NF; f++) {
+                    const f4_t kf = *(const f4_t*)(st + 16 * t * D + k_rd[f]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[f][e], sc[t], 0, 0, 0);
+                }
+            }
+            if (mk != ~0ull || k0 + BK > seen_all) {
+                hide(sc, mk, seen - k0);
+            }
+            float mloc = sc[0][0];
+#pragma unroll
+            for (int e = 1; e < 16; e++) mloc = fmaxf(mloc, sc[e >> 2][e & 3]);
+            mloc = max_xor32(max_xor16(mloc)) * c;
+            float alpha;
+            if (move_max(mloc, m_run, alpha)) {
+                l_run *= alpha;
+#pragma unroll
+                for (int u = 0; u < UT; u++) acc[0][u] *= alpha;
+            }
+            const float m_use = m_run == -INFINITY ? 0.0f : m_run;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    sc[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][e], c, -m_use));
+                    l_run += sc[t][e];
+                }
+            // In step kk of key tile t, k-slot lq is key 16 t + 4 lq + kk: the lane's own score.
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int kk = 0; kk < 4; kk++)
+#pragma unroll
+                    for (int u = 0; u < UT; u++)
+                        acc[0][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::v_at(st + TILE, v_rd, t, kk, u), sc[t][kk],
+                                                                         acc[0][u], 0, 0, 0);
+        };
+        for_each_stage<NS>(n, step);
+    }
+    const float m[1] = {m_run}, l[1] = {add_xor32(add_xor16(l_run))};
+    wide_store<T, D, W::TM, 1>(a, pl, un, kvh, w, wrow, acc, m, l);
+    ring_barrier();                                           // the ring's reads, before the next unit
+}
+
+template <int D>
+__global__ __launch_bounds__(256, (Wide32<D>::PER_CU))
+void paged_wide32(cf_paged_attn_args_t a, PagedPlan pl) {
+    using W = Wide32<D>;
+    __shared__ __attribute__((aligned(16))) float lds[W::LDS];
+    const Geometry<W::TM, 64, kNarrowCost> geo(a, pl);
+    for (int unit = (int)blockIdx.x;; unit += pl.step) {
+        const int id = unit / a.H_kv, kvh = unit - id * a.H_kv;
+        Unit un;
+        if (!geo.template find<false>(id, un)) break;
+        const Work w = unit_work<W::TM, 64>(a, pl, un);
+        if (w.n_rows <= 16) narrow_unit<float, D, W::TM, 4>(a, pl, lds, un, kvh, w);
+        else wide32_unit<D>(a, pl, lds, un, kvh, w);
     }
 }
 
 // Joins the ranges of cut tiles: O = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s.  A
 // workgroup per (tile, KV head) and ROWS rows: 256 / ROWS threads per row, D / 4 of them side
 // by side over the dims, the rest sharing the ranges.
-template <typename T, int D, int TM, int BK, int ROWS>
+template <typename T, int D, int TM, int BK, int NARROW, int ROWS>
 __global__ __launch_bounds__(256)
 void paged_merge(cf_paged_attn_args_t a, PagedPlan pl) {
     constexpr int DL = D / 4, SUBS = 256 / ROWS / DL;      // lanes over the dims, shares of the ranges
     static_assert(SUBS >= 1, "rows per workgroup");
     __shared__ float ml[2][ROWS][SUBS];
     __shared__ f4_t part[SUBS > 1 ? SUBS * ROWS * DL : 1];
-    const Geometry<TM, BK> geo(a, pl);
+    const Geometry<TM, BK, NARROW> geo(a, pl);
     const int G = a.H_q / a.H_kv;
     const int d4 = threadIdx.x % DL, sub = threadIdx.x / DL % SUBS, r = threadIdx.x / (DL * SUBS);
     for (int unit = blockIdx.x;; unit += gridDim.x) {
@@ -546,10 +1170,8 @@ void paged_merge(cf_paged_attn_args_t a, PagedPlan pl) {
             }
             if (sub == 0 && row < n_rows) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                const int R = un.tile * TM + row, tok = fastdiv(R, pl.by_group), h = kvh * G + (R - tok * G);
-                typedef T four_t __attribute__((ext_vector_type(4)));
-                *(four_t*)((T*)a.o + ((int64_t)(un.s.row0 + tok) * a.H_q + h) * D + 4 * d4) =
-                    four_t{(T)(acc[0] * inv), (T)(acc[1] * inv), (T)(acc[2] * inv), (T)(acc[3] * inv)};
+                const RowAt at = row_at(pl, G, kvh, un.tile * TM + row);
+                store4((T*)a.o + ((int64_t)(un.s.row0 + at.tok) * a.H_q + at.h) * D + 4 * d4, acc * inv);
             }
         }
     }
@@ -620,13 +1242,16 @@ void paged_any(cf_paged_attn_args_t a, FastDiv by_page) {
         if (lane + 64 * i < a.d) o[lane + 64 * i] = (T)(acc[i] * inv);
 }
 
-// The plan of a call on the matrix cores: the kernel's form and how its work is cut.
+// The plan of a call on the matrix cores: the kernel and how its work is cut.
+enum Form { kHeads, kSplit, kWide1, kWide2 };   // kWide2: fp16 tiles of 256 rows
 struct Plan {
     PagedPlan pl;
-    int  nj;              // 0: a wave per unit (16-row tiles), 1 or 2: workgroups of 64 or 128 rows
+    Form form;
     int  wgs, merge_wgs;
     size_t bytes;         // workspace
 };
+
+int64_t g_split_units = 128, g_wide2_units = 192;
 
 bool fast_ok(const cf_paged_attn_args_t& a) {
     const uint64_t ptrs = (uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.k | (uint64_t)(uintptr_t)a.v | (uint64_t)(uintptr_t)a.o;
@@ -637,38 +1262,44 @@ bool fast_ok(const cf_paged_attn_args_t& a) {
            (int64_t)a.T * (a.H_q / a.H_kv) <= (1 << 30) && (uint64_t)a.row_stride * es * 16 < (1ull << 32);
 }
 
+// A divisor of the launches' grids: how many pieces of work (of any length) fill the chip.
 Plan make_plan(const cf_paged_attn_args_t& a) {
     Plan p;
     const int64_t G = a.H_q / a.H_kv, cus = cu_count();
     const bool f16 = a.elem == CF_ELEM_F16;
-    if ((int64_t)a.max_new * G <= 16) p.nj = 0;
-    else p.nj = f16 && ((int64_t)a.T * G + 127) / 128 * a.H_kv >= 2 * cus ? 2 : 1;
-    const int64_t TM = p.nj == 0 ? 16 : 64 * p.nj, BK = p.nj > 0 ? 64 : f16 ? 32 : 16;
-    // Units in flight: a workgroup of four waves takes 128 KB (d = 128) or 64 KB of LDS without
-    // shared tiles; with them 64 KB, 48 KB or (fp32, d = 128) 128 KB.
-    const int64_t per_cu = p.nj == 0 ? (a.d == 128 ? 4 : 8) : (!f16 && a.d == 128) ? 1 : 2;
-    const int64_t slots = cus * per_cu;
-    const int64_t fill = slots / a.H_kv > 0 ? slots / a.H_kv : 1;
-    // Tiles of the call, at most (where max_new holds).
-    int64_t tiles = (int64_t)a.T * G / TM + (a.B < a.T ? a.B : a.T);
-    if ((int64_t)a.max_new * G <= TM && tiles > a.B) tiles = a.B;
+    const int64_t rows = (int64_t)a.max_new * G;              // of a sequence, at most
+    // Tiles of TM rows of the call, at most (where max_new holds).
+    auto tiles_of = [&](int64_t TM) {
+        const int64_t t = (int64_t)a.T * G / TM + (a.B < a.T ? a.B : a.T);
+        return rows <= TM && t > a.B ? (int64_t)a.B : t;
+    };
+    if (rows <= 16) p.form = tiles_of(16) * a.H_kv >= g_split_units ? kHeads : kSplit;
+    else p.form = f16 && (int64_t)a.T * G / 256 * a.H_kv >= g_wide2_units ? kWide2 : kWide1;
+    const int64_t TM = p.form <= kSplit ? 16 : !f16 ? 64 : p.form == kWide2 ? 256 : 128;
+    const int64_t BK = p.form != kHeads ? 64 : f16 ? 32 : 16;
+    const int64_t tiles = tiles_of(TM);
+    // Units in flight, by the LDS a workgroup takes.
+    const int64_t per_cu = p.form == kHeads ? (a.d == 128 ? 4 : 8) : p.form == kSplit ? (f16 && a.d == 64 ? 2 : 1)
+                         : f16 || a.d == 128 ? 1 : 2;
+    const int64_t fill = cus * per_cu > a.H_kv ? cus * per_cu / a.H_kv : 1;
     int64_t ranges = fill;
-    if (p.nj == 0) ranges = tiles <= fill / 2 ? fill - tiles : tiles <= fill ? 2 * fill - tiles : 2 * fill;
+    if (p.form <= kSplit) ranges = tiles <= fill / 2 ? fill - tiles : tiles <= fill ? 2 * fill - tiles : 2 * fill;
     p.pl.ranges = (int32_t)(ranges > 0 ? ranges : 1);
-    p.pl.min_blocks = (int32_t)(256 / BK);
+    p.pl.min_blocks = (int32_t)(p.form == kHeads ? 256 / BK : p.form == kSplit ? 4 : 4);
+    p.pl.one_blocks = (int32_t)((p.form == kSplit ? 1024 : 512) / BK);
     p.pl.max_records = 2 * p.pl.ranges + 8;
     const int64_t most_blocks = ((int64_t)a.max_pages * a.page_size + BK - 1) / BK;
-    const bool cut = most_blocks > p.pl.min_blocks;
+    const bool cut = most_blocks > p.pl.one_blocks;
     p.bytes = cut ? (size_t)p.pl.max_records * a.H_kv * (TM * (a.d + 2)) * sizeof(float) : 0;
     int64_t units = (tiles + (cut ? ranges : 0)) * a.H_kv;
     if (units > (1 << 24)) units = 1 << 24;
-    p.wgs = (int)(p.nj == 0 ? (units + 3) / 4 : units);
-    p.pl.waves = p.nj == 0 ? 4 * p.wgs : p.wgs;
+    p.wgs = (int)(p.form == kHeads ? (units + 3) / 4 : units);
+    p.pl.step = p.form == kHeads ? 4 * p.wgs : p.wgs;
+    const int64_t most_rows = rows < TM ? rows : TM;
+    p.pl.merge_groups = (int32_t)(p.form <= kSplit ? most_rows : (most_rows + 3) / 4);
     const int64_t cut_tiles = tiles < ranges + 4 ? tiles : ranges + 4;
-    const int64_t most_rows = (int64_t)a.max_new * G < TM ? (int64_t)a.max_new * G : TM;
-    p.pl.merge_groups = (int32_t)(p.nj == 0 ? most_rows : (most_rows + 3) / 4);
     const int64_t merge_wgs = cut_tiles * a.H_kv * p.pl.merge_groups;
-    p.merge_wgs = !cut ? 0 : merge_wgs > (1 << 20) ? 1 << 20 : (int)merge_wgs;
+    p.merge_wgs = !cut ? 0 : merge_wgs > 4096 ? 4096 : (int)merge_wgs;
     p.pl.by_page = fastdiv_make(a.page_size);
     p.pl.by_group = fastdiv_make((int)G);
     p.pl.records = nullptr;
@@ -677,19 +1308,23 @@ Plan make_plan(const cf_paged_attn_args_t& a) {
 
 template <typename T, int D>
 int launch_tiles(const cf_paged_attn_args_t& a, const Plan& p, hipStream_t st) {
-    const dim3 grid((unsigned)p.wgs), block(256);
-    if (p.nj == 0) hipLaunchKernelGGL((paged_tiles<T, D, 1, false>), grid, block, 0, st, a, p.pl);
-    else if (p.nj == 1) hipLaunchKernelGGL((paged_tiles<T, D, 1, true>), grid, block, 0, st, a, p.pl);
-    // fp32 products take 16 times as long as fp16's: 16 rows a wave keep the matrix cores busy.
-    else if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((paged_tiles<T, D, 2, true>), grid, block, 0, st, a, p.pl);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.merge_wgs == 0) return (int)e;
-    const dim3 mgrid((unsigned)p.merge_wgs);
-    constexpr int BK0 = Shape<T, D, 1, false>::BK;
-    if (p.nj == 0) hipLaunchKernelGGL((paged_merge<T, D, 16, BK0, 1>), mgrid, block, 0, st, a, p.pl);
-    else if (p.nj == 1) hipLaunchKernelGGL((paged_merge<T, D, 64, 64, 4>), mgrid, block, 0, st, a, p.pl);
-    else if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((paged_merge<T, D, 128, 64, 4>), mgrid, block, 0, st, a, p.pl);
-    return (int)hipGetLastError();
+    constexpr bool F16 = sizeof(T) == 2;
+    const dim3 grid((unsigned)p.wgs), mgrid((unsigned)p.merge_wgs);
+    auto go = [&](auto tiles, int threads, auto merge) {
+        hipLaunchKernelGGL(tiles, grid, dim3(threads), 0, st, a, p.pl);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess || p.merge_wgs == 0) return (int)e;
+        hipLaunchKernelGGL(merge, mgrid, dim3(256), 0, st, a, p.pl);
+        return (int)hipGetLastError();
+    };
+    if (p.form == kHeads) return go(paged_heads<T, D>, 256, paged_merge<T, D, 16, Heads<T, D>::BK, 1, 1>);
+    if (p.form == kSplit) return go(paged_split<T, D>, 64 * Split<T, D>::WAVES, paged_merge<T, D, 16, 64, 1, 1>);
+    if constexpr (F16) {
+        if (p.form == kWide2) return go(paged_wide16<D, 2>, 512, paged_merge<T, D, 256, 64, kNarrowCost, 4>);
+        return go(paged_wide16<D, 1>, 512, paged_merge<T, D, 128, 64, kNarrowCost, 4>);
+    } else {
+        return go(paged_wide32<D>, 256, paged_merge<T, D, 64, 64, kNarrowCost, 4>);
+    }
 }
 
 }  // namespace
