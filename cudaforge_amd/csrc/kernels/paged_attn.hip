@@ -268,17 +268,20 @@ __device__ __forceinline__ bool move_max(float mloc, float& m, float& alpha) {
 }
 
 // Scores of a lane's row in a block: key 16 t + 4 lq + i of it counts where its bit of `mk` is
-// set and it is one of the first `seen`.
+// set and it is one of the first `seen`.  Bit by bit in vector registers: comparisons would
+// take a pair of scalar registers per score.
 template <int NG>
 __device__ __forceinline__ void hide(f4_t (&sc)[NG], uint64_t mk, int seen) {
-    const int at = 4 * ((threadIdx.x >> 4) & 3);
-    const uint64_t bits = mk >> at;
-    seen -= at;
+    const uint64_t low = seen <= 0 ? 0 : seen >= 64 ? ~0ull : (1ull << seen) - 1;
+    const uint64_t bits = (mk & low) >> (4 * ((threadIdx.x >> 4) & 3));
 #pragma unroll
     for (int t = 0; t < NG; t++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (!((bits >> (16 * t + i)) & 1) || 16 * t + i >= seen) sc[t][i] = -INFINITY;
+        for (int i = 0; i < 4; i++) {
+            const uint32_t half = t < 2 ? (uint32_t)bits : (uint32_t)(bits >> 32);
+            const uint32_t keep = (uint32_t)((int32_t)(half << (31 - 16 * (t & 1) - i)) >> 31);
+            sc[t][i] = __uint_as_float((__float_as_uint(sc[t][i]) & keep) | (0xff800000u & ~keep));
+        }
 }
 
 // ---- Up to 16 rows, one wave with a ring of its own: no barrier. ----
@@ -634,13 +637,14 @@ template <int D, int NJ> struct Wide16 {
     static constexpr int TILE = BK * D;
     static constexpr int STAGE = 2 * TILE;
     static constexpr int LDS = NS * STAGE;                   // 128 KB (d = 128), 64 KB
+    static constexpr int MASKS = 2 * NS;                     // blocks whose masks are kept
     static_assert(TM * D <= 2 * STAGE, "Q fits the last two stages");
     static_assert(8 * Narrow<_Float16, D, 16>::RING <= LDS, "the rings of narrow tiles fit");
 };
 
 template <int D, int NJ>
-__device__ __forceinline__ void wide16_unit(const cf_paged_attn_args_t& a, const PagedPlan& pl, _Float16* lds, const Unit& un,
-                                            int kvh, const Work& w) {
+__device__ __forceinline__ void wide16_unit(const cf_paged_attn_args_t& a, const PagedPlan& pl, _Float16* lds,
+                                            uint64_t* masks, const Unit& un, int kvh, const Work& w) {
     using T = _Float16;
     using R = Rows<T, D>;
     using W = Wide16<D, NJ>;
@@ -687,35 +691,25 @@ __device__ __forceinline__ void wide16_unit(const cf_paged_attn_args_t& a, const
         const T* const kp = (const T*)a.k + (int64_t)kvh * a.head_stride;
         const T* const vp = (const T*)a.v + (int64_t)kvh * a.head_stride;
 
-        // Stage i of the ring is issued with the pages of block i (K) and what is kept of block
-        // i - 1 (V).  Blocks outside 0 .. n - 1 load the nearest one, so every stage is NL loads.
-        int pages[4];
-        auto fetch = [&](int i) {
-            const int key = w.key0 + min(i, n - 1) * BK;
-#pragma unroll
-            for (int g = 0; g < 4; g++) pages[g] = page_of(a, pl, table, key + 16 * g);
-        };
+        // Stage i of the ring is issued with the page of block i (K) and what is kept of block i - 1
+        // (V).  Blocks outside 0 .. n - 1 load the nearest one, so every stage is NL loads.  A wave
+        // looks up its own group's page only; which positions of it count goes to the others
+        // through LDS.
+        int page;
         int64_t v_at = 0;
-        uint64_t mask[NS];                                    // of blocks i .. i + NS - 1 (i: this turn)
-        auto issue = [&](int i, int slot) -> uint64_t {
-            const int key = w.key0 + min(i, n - 1) * BK;
-            uint64_t mk = 0;
-            int64_t k_at = 0;
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const Group gr = group_of(a, pl, pages[g], key + 16 * g, w.key1);
-                mk |= (uint64_t)gr.mask << (16 * g);
-                if (g == grp) k_at = gr.at;
-            }
-            if (i == 0) v_at = k_at;
-            const uint32_t to = my_lds + (uint32_t)(slot * STAGE * 2);
+        auto key_of = [&](int i) { return w.key0 + min(i, n - 1) * BK + 16 * grp; };
+        auto fetch = [&](int i) { page = page_of(a, pl, table, key_of(i)); };
+        auto issue = [&](int i, int to_slot) {
+            const Group gr = group_of(a, pl, page, key_of(i), w.key1);
+            if (lane == 0) ((uint16_t*)masks)[4 * (i % W::MASKS) + grp] = (uint16_t)gr.mask;
+            if (i == 0) v_at = gr.at;
+            const uint32_t to = my_lds + (uint32_t)(to_slot * STAGE * 2);
 #pragma unroll
             for (int u = 0; u < HI; u++) {
-                lds_dma16_s(koff[u], kp + k_at, to + u * 1024u);
+                lds_dma16_s(koff[u], kp + gr.at, to + u * 1024u);
                 lds_dma16_s(voff[u], vp + v_at, to + (uint32_t)(TILE * 2) + u * 1024u);
             }
-            v_at = k_at;
-            return mk;
+            v_at = gr.at;
         };
 
         fetch(0);
@@ -729,9 +723,9 @@ __device__ __forceinline__ void wide16_unit(const cf_paged_attn_args_t& a, const
                           __builtin_amdgcn_readfirstlane(qlds + u * 1024u));
             }
         }
-        mask[0] = issue(0, 0);
+        issue(0, 0);
         fetch(1);
-        mask[1] = issue(1, 1);                                // n >= 1: stages 0 and 1 exist
+        issue(1, 1);                                          // n >= 1: stages 0 and 1 exist
         fetch(2);
         wait_vm<2 * NL>();
         h8_t qf[NJ][NF];
@@ -745,46 +739,35 @@ __device__ __forceinline__ void wide16_unit(const cf_paged_attn_args_t& a, const
         h8_t pf[NJ][2];
         h8_t ones = {1, 1, 1, 1, 1, 1, 1, 1};
         asm volatile("" : "+v"(ones));                        // kept in registers for the whole loop
-        uint64_t v_mask = ~0ull;                              // of the V of the stage that lands next
+        uint64_t mk = ~0ull;                                  // positions of this turn's block that count
         int slot = 0;                                         // of this turn's stage
 
         // Before the barrier that starts turn i: its stage has landed, this wave's share of it, and
-        // its V is 0 where nothing counts (p = 0 times whatever it holds need not be).
-        auto landed = [&](int i, int at) {
+        // its V (of block i - 1) is 0 where nothing counts (p = 0 times whatever it holds need not be).
+        auto landed = [&](int i) {
             wait_ahead<NL, NS - 2>(min(i == 0 ? 1 : NS - 2, n - i));
-            if (i > 0 && v_mask != ~0ull) {
+            if (i > 0 && mk != ~0ull) {
 #pragma unroll
                 for (int u = 0; u < HI; u++) {
                     const int row = 16 * grp + 8 * half + R::RPI * u + drow;
-                    if (!((v_mask >> row) & 1)) *(uint4*)(lds + at * STAGE + TILE + row * D + 8 * dch) = uint4{};
+                    if (!((mk >> row) & 1)) *(uint4*)(lds + slot * STAGE + TILE + row * D + 8 * dch) = uint4{};
                 }
-                wait_lds_reads();
             }
+            wait_lds_reads();
         };
         // After it: the stage of turn i - 1 is free.
-        auto refill = [&](int i, int at) {
-            if (i == 0) {
-                if (2 <= n) {
-                    mask[2] = issue(2, 2);
-                    fetch(3);
-                }
-                if (3 <= n) {
-                    mask[3] = issue(3, 3);
-                    fetch(4);
-                }
-            } else if (i + NS - 1 <= n) {
-                mask[NS - 1] = issue(i + NS - 1, at == 0 ? NS - 1 : at - 1);
-                fetch(i + NS);
-            }
+        auto refill = [&](int i) {
+            if (i + NS - 1 <= n) issue(i + NS - 1, slot == 0 ? NS - 1 : slot - 1);
         };
         // Fragment x of a turn: x < 2 UT is V^T (32-key step x / UT, dims 16 (x % UT)), the rest K
         // (key tile, then chunk).  They are read kAhead fragments before their products, in
         // exactly this order: left to itself the compiler reads them all first and spills.
         constexpr int kAhead = 6, kV = 2 * UT, kAll = kV + 4 * NF;
-        auto products = [&](int at, auto first_c, auto last_c) {   // fragments first .. last - 1
+        auto products = [&](int i, auto first_c, auto last_c) {   // fragments first .. last - 1
             constexpr int first = decltype(first_c)::value, last = decltype(last_c)::value;
+            if constexpr (last == kAll) mk = masks[i % W::MASKS];
             if (!active) return;
-            const T* const st = lds + at * STAGE;
+            const T* const st = lds + slot * STAGE;
             h8_t frag[kAhead];
             auto read = [&](auto x_c) {
                 constexpr int x = decltype(x_c)::value;
@@ -835,7 +818,7 @@ __device__ __forceinline__ void wide16_unit(const cf_paged_attn_args_t& a, const
         const std::integral_constant<int, 0> from_v;
         const std::integral_constant<int, kV> to_v;
         const std::integral_constant<int, kAll> to_k;
-        auto softmax = [&](int i, uint64_t mk) {
+        auto softmax = [&](int i) {
             if (!active) return;
             const int k0 = w.key0 + i * BK;
             const bool edge = mk != ~0ull || k0 + BK > seen_all;
@@ -864,57 +847,62 @@ __device__ __forceinline__ void wide16_unit(const cf_paged_attn_args_t& a, const
                             (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][t][e], c, -m_use));
             }
         };
-        // Turn i's softmax takes the mask of block i; the V of the stage of turn i + 1 is that block's.
-        auto next_turn = [&]() {
-#pragma unroll
-            for (int k = 0; k + 1 < NS; k++) mask[k] = mask[k + 1];
-            slot = slot == NS - 1 ? 0 : slot + 1;
+        auto next_turn = [&]() { slot = slot == NS - 1 ? 0 : slot + 1; };
+        auto uniform = [](uint64_t x) {
+            return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
+                   (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
         };
 
-        landed(0, 0);
-        ring_barrier();
-        refill(0, 0);
         // Turn i of waves 0 .. 3 takes phases 2 i (products) and 2 i + 1, of the others 2 i + 1 and
-        // 2 i + 2; everybody meets at every barrier, 2 n + 2 of them.
+        // 2 i + 2; everybody meets at every barrier, 2 n + 2 of them.  A stage's page is looked up
+        // during the softmax before its issue: a load through the scalar cache makes the waits for
+        // LDS reads in order wait for everything.
         auto first_half = [&](int i) {
+            mk = uniform(mk);
             ring_barrier();
-            v_mask = mask[0];
-            softmax(i, v_mask);
+            fetch(i + NS);
+            softmax(i);
             next_turn();
-            landed(i + 1, slot);
+            landed(i + 1);
             ring_barrier();
-            refill(i + 1, slot);
+            refill(i + 1);
         };
         auto second_half = [&](int i) {
-            v_mask = mask[0];
-            const uint64_t mk = v_mask;
+            mk = uniform(mk);
             next_turn();
-            landed(i + 1, slot);
+            landed(i + 1);
             ring_barrier();
-            refill(i + 1, slot);
-            softmax(i, mk);
+            refill(i + 1);
+            fetch(i + NS + 1);
+            softmax(i);
             ring_barrier();
         };
+        landed(0);
+        ring_barrier();
+        if (2 <= n) issue(2, 2);
+        fetch(3);
+        if (3 <= n) issue(3, 3);
+        fetch(4);
         if (wave < 4) {
-            products(slot, to_v, to_k);
+            products(0, to_v, to_k);
             first_half(0);
 #pragma clang loop unroll(disable)
             for (int i = 1; i < n; i++) {
-                products(slot, from_v, to_k);
+                products(i, from_v, to_k);
                 first_half(i);
             }
-            products(slot, from_v, to_v);
+            products(n, from_v, to_v);
             ring_barrier();
         } else {
             ring_barrier();
-            products(slot, to_v, to_k);
+            products(0, to_v, to_k);
             second_half(0);
 #pragma clang loop unroll(disable)
             for (int i = 1; i < n; i++) {
-                products(slot, from_v, to_k);
+                products(i, from_v, to_k);
                 second_half(i);
             }
-            products(slot, from_v, to_v);
+            products(n, from_v, to_v);
         }
     }
     float l[NJ];
@@ -930,6 +918,7 @@ __global__ __launch_bounds__(512, 2)
 void paged_wide16(cf_paged_attn_args_t a, PagedPlan pl) {
     using W = Wide16<D, NJ>;
     __shared__ __attribute__((aligned(16))) _Float16 lds[W::LDS];
+    __shared__ uint64_t masks[W::MASKS];
     const Geometry<W::TM, 64, kNarrowCost> geo(a, pl);
     for (int unit = (int)blockIdx.x;; unit += pl.step) {
         const int id = unit / a.H_kv, kvh = unit - id * a.H_kv;
@@ -937,7 +926,7 @@ void paged_wide16(cf_paged_attn_args_t a, PagedPlan pl) {
         if (!geo.template find<false>(id, un)) break;
         const Work w = unit_work<W::TM, 64>(a, pl, un);
         if (w.n_rows <= 16) narrow_unit<_Float16, D, W::TM, 8>(a, pl, lds, un, kvh, w);
-        else wide16_unit<D, NJ>(a, pl, lds, un, kvh, w);
+        else wide16_unit<D, NJ>(a, pl, lds, masks, un, kvh, w);
     }
 }
 
