@@ -185,7 +185,21 @@ __device__ __forceinline__ void store4(T* p, f4_t x) {
     *(four_t*)p = four_t{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
 }
 
-// Table entries through the scalar cache: an ordinary load would make its wait drain the ring.
+// Table entries for the next 64 pieces of a range, one per lane: piece i starts at position
+// key0 + i * step.  A load a piece would be in the way: an ordinary one's wait drains the ring,
+// and one through the scalar cache makes the waits for LDS reads wait for it.  load() drains
+// the ring once per 64 pieces.
+struct Pages {
+    const int32_t* table;
+    int v;                   // lane: entry of piece base + lane
+    __device__ __forceinline__ void load(const cf_paged_attn_args_t& a, const PagedPlan& pl, int base, int key0, int step) {
+        const int key = min(key0 + (base + (int)(threadIdx.x & 63)) * step, a.max_pages * a.page_size - 1);
+        v = table[fastdiv(key, pl.by_page)];
+        asm volatile("" : "+v"(v));   // it has arrived
+    }
+    __device__ __forceinline__ int page(int i) const { return __builtin_amdgcn_readlane(v, i & 63); }
+};
+// One entry through the scalar cache.
 typedef const int32_t __attribute__((address_space(4)))* table_t;
 __device__ __forceinline__ table_t table_of(const cf_paged_attn_args_t& a, int b) {
     return (table_t)(uintptr_t)(a.table + (size_t)b * a.max_pages);
@@ -328,22 +342,19 @@ __device__ __forceinline__ void narrow_range(const cf_paged_attn_args_t& a, cons
     R::k_offsets(k_rd);
     R::v_offsets(v_rd);
     const uint32_t ring_base = __builtin_amdgcn_readfirstlane(lds_offset(ring));
-    const table_t table = table_of(a, b);
     const T* const kp = (const T*)a.k + (int64_t)kvh * a.head_stride;
     const T* const vp = (const T*)a.v + (int64_t)kvh * a.head_stride;
+    Pages pages = {a.table + (size_t)b * a.max_pages, 0};
+    pages.load(a, pl, 0, key0, 16);
 
-    int pages[NG];                                            // of the next block to issue
-    auto fetch = [&](int blk) {
-#pragma unroll
-        for (int g = 0; g < NG; g++) pages[g] = page_of(a, pl, table, key0 + blk * BK + 16 * g);
-    };
     uint64_t mask[NS];                                        // per stage: positions that count
     auto issue = [&](int blk, auto stage_c) {
         constexpr int stage = decltype(stage_c)::value;
         uint64_t mk = 0;
+        if (blk > 0 && blk % (64 / NG) == 0) pages.load(a, pl, blk * NG, key0, 16);
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            const Group gr = group_of(a, pl, pages[g], key0 + blk * BK + 16 * g, key1);
+            const Group gr = group_of(a, pl, pages.page(blk * NG + g), key0 + blk * BK + 16 * g, key1);
             mk |= (uint64_t)gr.mask << (16 * g);
             const uint32_t lds = ring_base + (uint32_t)((stage * 2 * TILE + 16 * g * D) * sizeof(T));
 #pragma unroll
@@ -356,7 +367,6 @@ __device__ __forceinline__ void narrow_range(const cf_paged_attn_args_t& a, cons
     };
 
     wait_lds_reads();                                         // what the ring held before
-    fetch(0);
     // Q rows by DMA into the last stage, which the first blocks leave free.
     {
         const uint32_t qlds = ring_base + (uint32_t)((NS - 1) * 2 * TILE * sizeof(T));
@@ -369,7 +379,6 @@ __device__ __forceinline__ void narrow_range(const cf_paged_attn_args_t& a, cons
         }
     }
     issue(0, std::integral_constant<int, 0>{});
-    if (1 < nblk) fetch(1);
     wait_vm<NL>();
     chunk_t qf[R::NF];                                        // B operand Q^T
 #pragma unroll
@@ -381,7 +390,6 @@ __device__ __forceinline__ void narrow_range(const cf_paged_attn_args_t& a, cons
         if (bi + NS - 1 < nblk) {
             wait_lds_reads();                                 // the last reads of that stage
             issue(bi + NS - 1, std::integral_constant<int, (stage + NS - 1) % NS>{});
-            if (bi + NS < nblk) fetch(bi + NS);
         }
         wait_ahead<NL, NS - 1>(min(NS - 1, nblk - 1 - bi));
         const uint64_t mk = mask[stage];
@@ -595,33 +603,30 @@ void paged_split(cf_paged_attn_args_t a, PagedPlan pl) {
     }
 }
 
-// The end of a wide tile's wave: NJ blocks of 16 rows from row wrow of the tile.  Lane (lr, lq)
-// holds dims 16 u + 4 lq .. + 3 of row lr of each, and l whole.
-template <typename T, int D, int TM, int NJ>
-__device__ __forceinline__ void wide_store(const cf_paged_attn_args_t& a, const PagedPlan& pl, const Unit& un, int kvh,
-                                           const Work& w, int wrow, const f4_t (&acc)[NJ][D / 16], const float (&m)[NJ],
-                                           const float (&l)[NJ]) {
-    const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
-    float* const rec = un.n_ranges > 1 ? record_of<TM, D>(a, pl, un, kvh) : nullptr;
-#pragma unroll
-    for (int j = 0; j < NJ; j++) {
-        const int row = wrow + 16 * j + lr;
-        if (row >= w.n_rows) continue;
-        if (rec) {
-#pragma unroll
-            for (int u = 0; u < D / 16; u++) *(f4_t*)(rec + 2 * TM + row * D + 16 * u + 4 * lq) = acc[j][u];
-            if (lq == 0) {
-                rec[row] = m[j];
-                rec[TM + row] = l[j];
-            }
-            continue;
+// Dims d0 .. d0 + 3 of row `row` of a wide tile: into the unit's record, or normalised into O.
+struct RowOut {
+    float* rec;       // the row's sum in the record, or null
+    void*  o;         // its row of O
+    float  inv;
+};
+template <typename T, int D, int TM>
+__device__ __forceinline__ RowOut row_out(const cf_paged_attn_args_t& a, const PagedPlan& pl, const Unit& un, int kvh,
+                                          const Work& w, int row, float m, float l, bool first) {
+    if (un.n_ranges > 1) {
+        float* const rec = record_of<TM, D>(a, pl, un, kvh);
+        if (first) {
+            rec[row] = m;
+            rec[TM + row] = l;
         }
-        const float inv = l[j] == 0.0f ? 0.0f : 1.0f / l[j];
-        const RowAt at = row_at(pl, a.H_q / a.H_kv, kvh, w.R0 + row);
-        T* const o = (T*)a.o + ((int64_t)(un.s.row0 + at.tok) * a.H_q + at.h) * D + 4 * lq;
-#pragma unroll
-        for (int u = 0; u < D / 16; u++) store4(o + 16 * u, acc[j][u] * inv);
+        return {rec + 2 * TM + row * D, nullptr, 1.0f};
     }
+    const RowAt at = row_at(pl, a.H_q / a.H_kv, kvh, w.R0 + row);
+    return {nullptr, (T*)a.o + ((int64_t)(un.s.row0 + at.tok) * a.H_q + at.h) * D, l == 0.0f ? 0.0f : 1.0f / l};
+}
+template <typename T>
+__device__ __forceinline__ void put4(const RowOut& out, int d0, f4_t x) {
+    if (out.rec) *(f4_t*)(out.rec + d0) = x;
+    else store4((T*)out.o + d0, x * out.inv);
 }
 
 // ---- fp16, wide tiles: 8 waves of 16 NJ rows through one ring of 64-position blocks. ----
@@ -652,7 +657,7 @@ __device__ __forceinline__ void wide16_unit(const cf_paged_attn_args_t& a, const
     constexpr int HI = R::NI / 2;                            // DMA instructions per 8 rows
     constexpr int NL = 2 * HI;                               // ... of a wave per stage
     static_assert(R::RPI <= 8 && (NS - 1) * NL < 64, "eight rows per wave");
-    const int lane = threadIdx.x & 63, lr = lane & 15;
+    const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int G = a.H_q / a.H_kv, drow = R::drow(), dch = R::dch();
     const float c = a.scale * kLog2e;
@@ -775,7 +780,7 @@ __device__ __forceinline__ void wide16_unit(const cf_paged_attn_args_t& a, const
                     const T* const v = st + TILE + v_rd[x % UT] + 32 * (x / UT) * D;
                     frag[x % kAhead] = cat8(ds_read_tr4(v), ds_read_tr4(v + 16 * D));
                 } else if constexpr (x < kAll) {
-                    frag[x % kAhead] = *(const h8_t*)(st + 16 * ((x - kV) / NF) * D + k_rd[(x - kV) % NF]);
+                    frag[x % kAhead] = *(const h8_t*)(st + 16 * ((x - kV) % 4) * D + k_rd[(x - kV) / 4]);
                 }
             };
             auto use = [&](auto x_c) {
@@ -794,7 +799,7 @@ __device__ __forceinline__ void wide16_unit(const cf_paged_attn_args_t& a, const
                         acc[j][x % UT] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, pf[j][x / UT], acc[j][x % UT], 0, 0, 0);
                 } else {
                     // S^T: sc[j][t][e] = score(key 16 t + 4 lq + e of block i, row j).
-                    constexpr int t = (x - kV) / NF, c0 = (x - kV) % NF;
+                    constexpr int t = (x - kV) % 4, c0 = (x - kV) / 4;
 #pragma unroll
                     for (int j = 0; j < NJ; j++)
                         sc[j][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, qf[j][c0], c0 == 0 ? f4_t{0.f, 0.f, 0.f, 0.f} : sc[j][t],
@@ -905,10 +910,15 @@ __device__ __forceinline__ void wide16_unit(const cf_paged_attn_args_t& a, const
             products(n, from_v, to_v);
         }
     }
-    float l[NJ];
 #pragma unroll
-    for (int j = 0; j < NJ; j++) l[j] = lsum[j][0];
-    wide_store<T, D, W::TM, NJ>(a, pl, un, kvh, w, wrow, acc, m_run, l);
+    for (int j = 0; j < NJ; j++) {
+        const int row = wrow + 16 * j + lr;
+        if (row < w.n_rows) {
+            const RowOut out = row_out<T, D, W::TM>(a, pl, un, kvh, w, row, m_run[j], lsum[j][0], lq == 0);
+#pragma unroll
+            for (int u = 0; u < UT; u++) put4<T>(out, 16 * u + 4 * lq, acc[j][u]);
+        }
+    }
     ring_barrier();                                           // the ring's reads, before the next unit
 }
 
@@ -917,7 +927,7 @@ template <int D, int NJ>
 __global__ __launch_bounds__(512, 2)
 void paged_wide16(cf_paged_attn_args_t a, PagedPlan pl) {
     using W = Wide16<D, NJ>;
-    __shared__ __attribute__((aligned(16))) _Float16 lds[W::LDS];
+    __shared__ __attribute__((aligned(1024))) _Float16 lds[W::LDS];
     __shared__ uint64_t masks[W::MASKS];
     const Geometry<W::TM, 64, kNarrowCost> geo(a, pl);
     for (int unit = (int)blockIdx.x;; unit += pl.step) {
@@ -944,7 +954,7 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
     using W = Wide32<D>;
     constexpr int BK = W::BK, NS = W::NS, TILE = W::TILE, NI = R::NI, NL = 2 * NI, UT = R::UT, NF = R::NF;
     static_assert(NS * NL < 64, "vmcnt range");
-    const int lane = threadIdx.x & 63, lr = lane & 15;
+    const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int G = a.H_q / a.H_kv, drow = R::drow(), dch = R::dch();
     const float c = a.scale * kLog2e;
@@ -953,10 +963,10 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
     const int n = w.key1 > w.key0 ? (w.key1 - w.key0 + BK - 1) / BK : 0;
     const int seen = min(w.base + fastdiv(w.R0 + min(wrow + lr, w.n_rows - 1), pl.by_group), un.s.len);
     const int seen_all = min(w.base + fastdiv(w.R0 + min(wrow, w.n_rows - 1), pl.by_group), un.s.len);
-    f4_t acc[1][UT];
+    f4_t acc[UT];
     float m_run = -INFINITY, l_run = 0.0f;
 #pragma unroll
-    for (int u = 0; u < UT; u++) acc[0][u] = f4_t{0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < UT; u++) acc[u] = f4_t{0.f, 0.f, 0.f, 0.f};
     if (n > 0) {
         uint32_t koff[NI], voff[NI];
 #pragma unroll
@@ -969,22 +979,19 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
         R::k_offsets(k_rd);
         R::v_offsets(v_rd);
         const uint32_t ring_base = __builtin_amdgcn_readfirstlane(lds_offset(ring));
-        const table_t table = table_of(a, un.b);
         const T* const kp = (const T*)a.k + (int64_t)kvh * a.head_stride;
         const T* const vp = (const T*)a.v + (int64_t)kvh * a.head_stride;
-        int pages[4];
-        auto fetch = [&](int i) {
-#pragma unroll
-            for (int g = 0; g < 4; g++) pages[g] = page_of(a, pl, table, w.key0 + i * BK + 16 * g);
-        };
+        Pages pages = {a.table + (size_t)un.b * a.max_pages, 0};
+        pages.load(a, pl, 0, w.key0, 16);
         uint64_t mask[NS];
         auto issue = [&](int i, auto stage_c) {               // wave w: group w of K and V
             constexpr int stage = decltype(stage_c)::value;
             uint64_t mk = 0;
             int64_t at = 0;
+            if (i > 0 && i % 16 == 0) pages.load(a, pl, 4 * i, w.key0, 16);
 #pragma unroll
             for (int g = 0; g < 4; g++) {
-                const Group gr = group_of(a, pl, pages[g], w.key0 + i * BK + 16 * g, w.key1);
+                const Group gr = group_of(a, pl, pages.page(4 * i + g), w.key0 + i * BK + 16 * g, w.key1);
                 mk |= (uint64_t)gr.mask << (16 * g);
                 if (g == wave) at = gr.at;
             }
@@ -996,7 +1003,6 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
             }
             mask[stage] = mk;
         };
-        fetch(0);
         {
             const uint32_t qlds = ring_base + (uint32_t)(((NS - 1) * 2 * TILE + wrow * D) * 4);
 #pragma unroll
@@ -1008,7 +1014,6 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
             }
         }
         issue(0, std::integral_constant<int, 0>{});
-        if (1 < n) fetch(1);
         wait_vm<NL>();
         f4_t qf[NF];
 #pragma unroll
@@ -1028,10 +1033,7 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
                 wait_lds_reads();
             }
             ring_barrier();
-            if (i + 1 < n) {
-                issue(i + 1, std::integral_constant<int, (stage + 1) % NS>{});
-                if (i + 2 < n) fetch(i + 2);
-            }
+            if (i + 1 < n) issue(i + 1, std::integral_constant<int, (stage + 1) % NS>{});
             if (!active) return;
             const int k0 = w.key0 + i * BK;
             f4_t sc[4];
@@ -1057,7 +1059,7 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
             if (move_max(mloc, m_run, alpha)) {
                 l_run *= alpha;
 #pragma unroll
-                for (int u = 0; u < UT; u++) acc[0][u] *= alpha;
+                for (int u = 0; u < UT; u++) acc[u] *= alpha;
             }
             const float m_use = m_run == -INFINITY ? 0.0f : m_run;
 #pragma unroll
@@ -1074,13 +1076,17 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
                 for (int kk = 0; kk < 4; kk++)
 #pragma unroll
                     for (int u = 0; u < UT; u++)
-                        acc[0][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::v_at(st + TILE, v_rd, t, kk, u), sc[t][kk],
-                                                                         acc[0][u], 0, 0, 0);
+                        acc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::v_at(st + TILE, v_rd, t, kk, u), sc[t][kk],
+                                                                      acc[u], 0, 0, 0);
         };
         for_each_stage<NS>(n, step);
     }
-    const float m[1] = {m_run}, l[1] = {add_xor32(add_xor16(l_run))};
-    wide_store<T, D, W::TM, 1>(a, pl, un, kvh, w, wrow, acc, m, l);
+    const float l = add_xor32(add_xor16(l_run));
+    if (wrow + lr < w.n_rows) {
+        const RowOut out = row_out<T, D, W::TM>(a, pl, un, kvh, w, wrow + lr, m_run, l, lq == 0);
+#pragma unroll
+        for (int u = 0; u < UT; u++) put4<T>(out, 16 * u + 4 * lq, acc[u]);
+    }
     ring_barrier();                                           // the ring's reads, before the next unit
 }
 
@@ -1246,9 +1252,10 @@ bool fast_ok(const cf_paged_attn_args_t& a) {
     const uint64_t ptrs = (uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.k | (uint64_t)(uintptr_t)a.v | (uint64_t)(uintptr_t)a.o;
     const uint64_t steps = (uint64_t)a.q_stride | (uint64_t)a.page_stride | (uint64_t)a.row_stride | (uint64_t)a.head_stride;
     const uint64_t es = a.elem == CF_ELEM_F16 ? 2 : 4;
-    // Row numbers times the group stay in 31 bits, offsets inside a group of rows in 32.
+    // Row numbers times the group and positions (with what is read ahead) stay in 31 bits, offsets
+    // inside a group of rows in 32.
     return (a.d == 64 || a.d == 128) && a.page_size % 16 == 0 && ptrs % 16 == 0 && steps * es % 16 == 0 && a.scale > 0.0f &&
-           (int64_t)a.T * (a.H_q / a.H_kv) <= (1 << 30) && (uint64_t)a.row_stride * es * 16 < (1ull << 32);
+           (int64_t)a.T * (a.H_q / a.H_kv) <= (1 << 30) && (int64_t)a.max_pages * a.page_size <= (1 << 30) && (uint64_t)a.row_stride * es * 16 < (1ull << 32);
 }
 
 // A divisor of the launches' grids: how many pieces of work (of any length) fill the chip.
