@@ -77,7 +77,7 @@ class MhaPagedParams(ctypes.Structure):
 
     _fields_ = [(n, c_int64) for n in ("batch_size", "num_tokens", "num_heads", "num_kv_heads", "head_dim")] + \
                [("scale", c_float)] + \
-               [(n, c_int64) for n in ("page_size", "num_pages", "max_pages", "max_new", "q_stride", "page_stride",
+               [(n, c_int64) for n in ("page_size", "num_pages", "max_pages", "max_new", "max_len", "q_stride", "page_stride",
                                        "row_stride", "head_stride")]
 
 

@@ -416,6 +416,7 @@ typedef struct {
     int32_t        B, T, H_q, H_kv, d;
     int32_t        page_size, num_pages, max_pages;
     int32_t        max_new;     /* most rows of one sequence; T where unknown */
+    int32_t        max_len;     /* most positions of one; the table's where unknown */
     float          scale;
     int32_t        elem;
     float*         records;     /* workspace of cf_paged_attn_bytes */

@@ -48,12 +48,12 @@ __device__ __forceinline__ SeqRows seq_rows(const cf_paged_attn_args_t& a, int b
 // The n rows of a sequence times the G query heads of a KV head are one list of n G rows
 // (row R: token R / G, head R % G), cut into tiles; a tile reads each K and V row once for
 // all its rows.  A unit of work is (tile, range of key blocks, KV head).  Lengths are known
-// to the device only, so every wave works out the units from them: with `ranges` the ranges
-// that fill the chip, C = ceil(sum_b tiles_b blocks_b / ranges) is the most blocks of one
-// range and sequence b's tiles are cut into ns_b = ceil(blocks_b / C) ranges each.  A tile
-// in one range is finished by its unit; else the units leave m, l and the unnormalised sum
-// per row, and paged_merge joins them.  More than one range needs blocks_b > C, so
-// ns_b < 2 blocks_b / C and there are at most 2 ranges + 1 such units per KV head.
+// to the device only, so every wave works out the units from them: with R the ranges that
+// fill the chip, C = ceil(sum_b tiles_b blocks_b / R) is the most blocks of one range and
+// sequence b's tiles are cut into ns_b = ceil(blocks_b / C) ranges each.  A tile in one range
+// is finished by its unit; else the units leave m, l and the unnormalised sum per row, and
+// paged_merge joins them.  More than one range needs blocks_b > C, so ns_b < 2 blocks_b / C
+// and there are at most 2 R + 1 such units per KV head; R is at most 2 `fill`.
 //
 // Three kernels share this:
 //   paged_heads  up to 16 rows per tile, a wave per unit (decode steps of many sequences);
@@ -64,7 +64,7 @@ __device__ __forceinline__ SeqRows seq_rows(const cf_paged_attn_args_t& a, int b
 struct PagedPlan {
     float*  records;       // of the units of cut tiles
     int32_t max_records;   // per KV head
-    int32_t ranges;        // key ranges (per KV head) that fill the chip
+    int32_t fill;          // units (per KV head) that fill the chip
     int32_t min_blocks;    // no range is cut shorter
     int32_t one_blocks;    // tiles of up to this many blocks are not cut
     int32_t step;          // of the unit loop
@@ -85,7 +85,8 @@ struct Geometry {
     const cf_paged_attn_args_t& a;
     const PagedPlan& pl;
     int G, lane, C;
-    SeqRows first;                       // lane: sequence `lane`, kept for the second pass
+    SeqRows first;                       // lane: sequence `lane`, kept for the second pass,
+    int* kept;                           // by wide tiles in LDS: their registers are all taken
 
     __device__ __forceinline__ SeqRows rows(int b) const { return b < a.B ? seq_rows(a, b) : SeqRows{0, 0, 0}; }
     __device__ __forceinline__ int tiles(const SeqRows& s) const { return (int)(((int64_t)s.n * G + TM - 1) / TM); }
@@ -100,45 +101,66 @@ struct Geometry {
         return n <= pl.one_blocks ? 1 : (n + c - 1) / c;
     }
 
-    __device__ __forceinline__ Geometry(const cf_paged_attn_args_t& a_, const PagedPlan& pl_) : a(a_), pl(pl_) {
+    __device__ __forceinline__ Geometry(const cf_paged_attn_args_t& a_, const PagedPlan& pl_, int* kept_ = nullptr)
+        : a(a_), pl(pl_), kept(kept_) {
         lane = threadIdx.x & 63;
         G = a.H_q / a.H_kv;
         first = rows(lane);
-        float w = cost(first);
-        for (int b = 64; b < a.B; b += 64) w += cost(rows(b + lane));
-        w = ceilf(wave_sum(w) / (float)pl.ranges);
+        if constexpr (NARROW > 1) {          // every wave writes the same
+            kept[lane] = first.row0;
+            kept[64 + lane] = first.n;
+            kept[128 + lane] = first.len;
+        }
+        float w = cost(first), t = (float)tiles(first);
+        for (int b = 64; b < a.B; b += 64) {
+            const SeqRows s = rows(b + lane);
+            w += cost(s);
+            t += (float)tiles(s);
+        }
+        w = wave_sum(w);
+        t = wave_sum(t);
+        // As many ranges as make, with the tiles' last ones, one or two rounds of units.
+        const float fill = (float)pl.fill;
+        const float n = t <= 0.5f * fill ? fill - t : t <= fill ? 2.0f * fill - t : NARROW > 1 ? fill : 2.0f * fill;
+        w = ceilf(w / fmaxf(n, 1.0f));
         C = __builtin_amdgcn_readfirstlane((int)fminf(fmaxf(w, (float)pl.min_blocks), 1e8f));
     }
     // Item u of all units (MERGE: of all cut tiles); false where there is none.
     template <bool MERGE>
     __device__ __forceinline__ bool find(int u, Unit& out) const {
-        int items0 = 0, records0 = 0;
-        SeqRows s = first;
-        for (int base = 0; base < a.B; base += 64) {
-            if (base > 0) s = rows(base + lane);
-            const int t = tiles(s), ns = ranges(s);
-            const int items = MERGE ? (ns > 1 ? t : 0) : t * ns;
-            const int before = items0 + wave_excl_sum(items, lane);
-            const int rec = ns > 1 ? t * ns : 0;
-            const int rec_before = records0 + wave_excl_sum(rec, lane);
-            const unsigned long long hit = __ballot(before <= u && u < before + items);
-            if (hit) {
-                const int src = __builtin_ctzll(hit);
-                const int at = u - __builtin_amdgcn_readlane(before, src);
-                out.n_ranges = __builtin_amdgcn_readlane(ns, src);
-                const int nt = __builtin_amdgcn_readlane(t, src);
-                const int i = MERGE ? at : at / out.n_ranges;
-                out.range = MERGE ? 0 : at - i * out.n_ranges;
-                out.tile = nt - 1 - i;                         // the longest first
-                out.record = __builtin_amdgcn_readlane(rec_before, src) + out.tile * out.n_ranges;
-                out.b = base + src;
-                out.s.row0 = __builtin_amdgcn_readlane(s.row0, src);
-                out.s.n = __builtin_amdgcn_readlane(s.n, src);
-                out.s.len = __builtin_amdgcn_readlane(s.len, src);
-                return out.n_ranges == 1 || out.record + out.n_ranges <= pl.max_records;
+        int items0 = 0;
+        // Wide tiles: the sequences with the long ranges first, narrow tiles last, so that short
+        // pieces fill the end.
+        constexpr int CLASSES = !MERGE && NARROW > 1 ? 3 : 1;
+        for (int cls = 0; cls < CLASSES; cls++) {
+            int records0 = 0;
+            for (int base = 0; base < a.B; base += 64) {
+                const SeqRows s = base > 0 ? rows(base + lane)
+                                : NARROW > 1 ? SeqRows{kept[lane], kept[64 + lane], kept[128 + lane]} : first;
+                const int t = tiles(s), ns = ranges(s), rec = ns > 1 ? t * ns : 0;
+                int items = MERGE ? (ns > 1 ? t : 0) : t * ns;
+                if (CLASSES > 1 && (narrow(s) ? 2 : 2 * blocks(s) > C * ns ? 0 : 1) != cls) items = 0;
+                const int before = items0 + wave_excl_sum(items, lane);
+                const int rec_before = records0 + wave_excl_sum(rec, lane);
+                const unsigned long long hit = __ballot(before <= u && u < before + items);
+                if (hit) {
+                    const int src = __builtin_ctzll(hit);
+                    const int at = u - __builtin_amdgcn_readlane(before, src);
+                    out.n_ranges = __builtin_amdgcn_readlane(ns, src);
+                    const int nt = __builtin_amdgcn_readlane(t, src);
+                    const int i = MERGE ? at : at / out.n_ranges;
+                    out.range = MERGE ? 0 : at - i * out.n_ranges;
+                    out.tile = nt - 1 - i;                     // the longest first
+                    out.record = __builtin_amdgcn_readlane(rec_before, src) + out.tile * out.n_ranges;
+                    out.b = base + src;
+                    out.s.row0 = __builtin_amdgcn_readlane(s.row0, src);
+                    out.s.n = __builtin_amdgcn_readlane(s.n, src);
+                    out.s.len = __builtin_amdgcn_readlane(s.len, src);
+                    return out.n_ranges == 1 || out.record + out.n_ranges <= pl.max_records;
+                }
+                items0 = __builtin_amdgcn_readlane(before + items, 63);
+                records0 = __builtin_amdgcn_readlane(rec_before + rec, 63);
             }
-            items0 = __builtin_amdgcn_readlane(before + items, 63);
-            records0 = __builtin_amdgcn_readlane(rec_before + rec, 63);
         }
         return false;
     }
@@ -767,7 +789,7 @@ __device__ __forceinline__ void wide16_unit(const cf_paged_attn_args_t& a, const
         // Fragment x of a turn: x < 2 UT is V^T (32-key step x / UT, dims 16 (x % UT)), the rest K
         // (key tile, then chunk).  They are read kAhead fragments before their products, in
         // exactly this order: left to itself the compiler reads them all first and spills.
-        constexpr int kAhead = 6, kV = 2 * UT, kAll = kV + 4 * NF;
+        constexpr int kAhead = 8, kV = 2 * UT, kAll = kV + 4 * NF;
         auto products = [&](int i, auto first_c, auto last_c) {   // fragments first .. last - 1
             constexpr int first = decltype(first_c)::value, last = decltype(last_c)::value;
             if constexpr (last == kAll) mk = masks[i % W::MASKS];
@@ -929,7 +951,8 @@ void paged_wide16(cf_paged_attn_args_t a, PagedPlan pl) {
     using W = Wide16<D, NJ>;
     __shared__ __attribute__((aligned(1024))) _Float16 lds[W::LDS];
     __shared__ uint64_t masks[W::MASKS];
-    const Geometry<W::TM, 64, kNarrowCost> geo(a, pl);
+    __shared__ int kept[3 * 64];
+    const Geometry<W::TM, 64, kNarrowCost> geo(a, pl, kept);
     for (int unit = (int)blockIdx.x;; unit += pl.step) {
         const int id = unit / a.H_kv, kvh = unit - id * a.H_kv;
         Unit un;
@@ -1036,18 +1059,23 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
             if (i + 1 < n) issue(i + 1, std::integral_constant<int, (stage + 1) % NS>{});
             if (!active) return;
             const int k0 = w.key0 + i * BK;
-            f4_t sc[4];
+            // Fragments are read kAhead before their products, in this order (four chains of sums).
+            constexpr int kAhead = 4;
+            f4_t sc[4], kf[kAhead];
+            auto read_k = [&](auto x_c) {
+                constexpr int x = decltype(x_c)::value;
+                kf[x % kAhead] = *(const f4_t*)(st + 16 * (x % 4) * D + k_rd[x / 4]);
+            };
+            static_for<kAhead - 1>(read_k);
+            static_for<4 * NF>([&](auto x_c) {
+                constexpr int x = decltype(x_c)::value, t = x % 4, f = x / 4;
+                if constexpr (x + kAhead - 1 < 4 * NF) read_k(std::integral_constant<int, x + kAhead - 1>{});
+                if constexpr (f == 0) sc[t] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                sc[t] = f4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int f = 0; f < NF; f++) {
-                    const f4_t kf = *(const f4_t*)(st + 16 * t * D + k_rd[f]);
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[f][e], sc[t], 0, 0, 0);
-                }
-            }
+                for (int e = 0; e < 4; e++)
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x % kAhead][e], qf[f][e], sc[t], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            });
             if (mk != ~0ull || k0 + BK > seen_all) {
                 hide(sc, mk, seen - k0);
             }
@@ -1070,14 +1098,21 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
                     l_run += sc[t][e];
                 }
             // In step kk of key tile t, k-slot lq is key 16 t + 4 lq + kk: the lane's own score.
+            float vf[2][UT];
+            auto read_v = [&](auto g_c) {
+                constexpr int g = decltype(g_c)::value;
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+                for (int u = 0; u < UT; u++) vf[g % 2][u] = R::v_at(st + TILE, v_rd, g / 4, g % 4, u);
+            };
+            read_v(std::integral_constant<int, 0>{});
+            static_for<16>([&](auto g_c) {
+                constexpr int g = decltype(g_c)::value;
+                if constexpr (g + 1 < 16) read_v(std::integral_constant<int, g + 1>{});
 #pragma unroll
-                for (int kk = 0; kk < 4; kk++)
-#pragma unroll
-                    for (int u = 0; u < UT; u++)
-                        acc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::v_at(st + TILE, v_rd, t, kk, u), sc[t][kk],
-                                                                      acc[u], 0, 0, 0);
+                for (int u = 0; u < UT; u++)
+                    acc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[g % 2][u], sc[g / 4][g % 4], acc[u], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            });
         };
         for_each_stage<NS>(n, step);
     }
@@ -1095,7 +1130,8 @@ __global__ __launch_bounds__(256, (Wide32<D>::PER_CU))
 void paged_wide32(cf_paged_attn_args_t a, PagedPlan pl) {
     using W = Wide32<D>;
     __shared__ __attribute__((aligned(16))) float lds[W::LDS];
-    const Geometry<W::TM, 64, kNarrowCost> geo(a, pl);
+    __shared__ int kept[3 * 64];
+    const Geometry<W::TM, 64, kNarrowCost> geo(a, pl, kept);
     for (int unit = (int)blockIdx.x;; unit += pl.step) {
         const int id = unit / a.H_kv, kvh = unit - id * a.H_kv;
         Unit un;
@@ -1116,7 +1152,8 @@ void paged_merge(cf_paged_attn_args_t a, PagedPlan pl) {
     static_assert(SUBS >= 1, "rows per workgroup");
     __shared__ float ml[2][ROWS][SUBS];
     __shared__ f4_t part[SUBS > 1 ? SUBS * ROWS * DL : 1];
-    const Geometry<TM, BK, NARROW> geo(a, pl);
+    __shared__ int kept[NARROW > 1 ? 3 * 64 : 1];
+    const Geometry<TM, BK, NARROW> geo(a, pl, kept);
     const int G = a.H_q / a.H_kv;
     const int d4 = threadIdx.x % DL, sub = threadIdx.x / DL % SUBS, r = threadIdx.x / (DL * SUBS);
     for (int unit = blockIdx.x;; unit += gridDim.x) {
@@ -1132,14 +1169,33 @@ void paged_merge(cf_paged_attn_args_t a, PagedPlan pl) {
             float m = -INFINITY, l = 0.0f;
             f4_t acc = f4_t{0.f, 0.f, 0.f, 0.f};
             if (row < n_rows)
-                for (int s = sub; s < un.n_ranges; s += SUBS) {
-                    const float ms = rec[s * step + row], ls = rec[s * step + TM + row];
-                    const f4_t as = *(const f4_t*)(rec + s * step + 2 * TM + row * D + 4 * d4);
-                    const float m_new = fmaxf(m, ms), m_use = m_new == -INFINITY ? 0.0f : m_new;
-                    const float wa = __builtin_amdgcn_exp2f(m - m_use), wb = __builtin_amdgcn_exp2f(ms - m_use);
+                for (int s0 = sub; s0 < un.n_ranges; s0 += 4 * SUBS) {
+                    // Four ranges' loads at a time; one behind the last counts for nothing.
+                    float ms[4], ls[4];
+                    f4_t as[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int s = min(s0 + k * SUBS, un.n_ranges - 1);
+                        ms[k] = rec[s * step + row];
+                        ls[k] = rec[s * step + TM + row];
+                        as[k] = *(const f4_t*)(rec + s * step + 2 * TM + row * D + 4 * d4);
+                    }
+                    float m_new = m;
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (s0 + k * SUBS < un.n_ranges) m_new = fmaxf(m_new, ms[k]);
+                    const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+                    const float wa = __builtin_amdgcn_exp2f(m - m_use);
                     m = m_new;
-                    l = l * wa + ls * wb;
-                    acc = acc * wa + as * wb;
+                    l *= wa;
+                    acc *= wa;
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (s0 + k * SUBS < un.n_ranges) {
+                            const float wb = __builtin_amdgcn_exp2f(ms[k] - m_use);
+                            l += ls[k] * wb;
+                            acc += as[k] * wb;
+                        }
                 }
             if constexpr (SUBS > 1) {
                 part[threadIdx.x] = acc;
@@ -1246,7 +1302,7 @@ struct Plan {
     size_t bytes;         // workspace
 };
 
-int64_t g_split_units = 128, g_wide2_units = 192;
+constexpr int64_t g_few_units = 64, g_split_units = 256, g_split_len = 1024, g_wide2_units = 192;
 
 bool fast_ok(const cf_paged_attn_args_t& a) {
     const uint64_t ptrs = (uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.k | (uint64_t)(uintptr_t)a.v | (uint64_t)(uintptr_t)a.o;
@@ -1258,43 +1314,46 @@ bool fast_ok(const cf_paged_attn_args_t& a) {
            (int64_t)a.T * (a.H_q / a.H_kv) <= (1 << 30) && (int64_t)a.max_pages * a.page_size <= (1 << 30) && (uint64_t)a.row_stride * es * 16 < (1ull << 32);
 }
 
-// A divisor of the launches' grids: how many pieces of work (of any length) fill the chip.
+// max_new and max_len only choose: the kernels' loops run until no unit is left, whatever the
+// grid, and a sequence that is longer is computed all the same.
 Plan make_plan(const cf_paged_attn_args_t& a) {
     Plan p;
     const int64_t G = a.H_q / a.H_kv, cus = cu_count();
     const bool f16 = a.elem == CF_ELEM_F16;
     const int64_t rows = (int64_t)a.max_new * G;              // of a sequence, at most
-    // Tiles of TM rows of the call, at most (where max_new holds).
-    auto tiles_of = [&](int64_t TM) {
-        const int64_t t = (int64_t)a.T * G / TM + (a.B < a.T ? a.B : a.T);
-        return rows <= TM && t > a.B ? (int64_t)a.B : t;
+    const int64_t seqs = a.B < a.T ? a.B : a.T;
+    auto tiles_of = [&](int64_t TM) {                         // tiles of the call, at most
+        const int64_t t = ((int64_t)a.T * G + seqs * (TM - 1)) / TM;
+        return rows <= TM && t > seqs ? seqs : t;
     };
-    if (rows <= 16) p.form = tiles_of(16) * a.H_kv >= g_split_units ? kHeads : kSplit;
-    else p.form = f16 && (int64_t)a.T * G / 256 * a.H_kv >= g_wide2_units ? kWide2 : kWide1;
+    if (rows <= 16) {
+        const int64_t units = tiles_of(16) * a.H_kv;
+        p.form = units <= g_few_units || (units <= g_split_units && a.max_len <= g_split_len) ? kSplit : kHeads;
+    } else {
+        p.form = f16 && (int64_t)a.T * G / 256 * a.H_kv >= g_wide2_units ? kWide2 : kWide1;
+    }
     const int64_t TM = p.form <= kSplit ? 16 : !f16 ? 64 : p.form == kWide2 ? 256 : 128;
     const int64_t BK = p.form != kHeads ? 64 : f16 ? 32 : 16;
     const int64_t tiles = tiles_of(TM);
     // Units in flight, by the LDS a workgroup takes.
     const int64_t per_cu = p.form == kHeads ? (a.d == 128 ? 4 : 8) : p.form == kSplit ? (f16 && a.d == 64 ? 2 : 1)
                          : f16 || a.d == 128 ? 1 : 2;
-    const int64_t fill = cus * per_cu > a.H_kv ? cus * per_cu / a.H_kv : 1;
-    int64_t ranges = fill;
-    if (p.form <= kSplit) ranges = tiles <= fill / 2 ? fill - tiles : tiles <= fill ? 2 * fill - tiles : 2 * fill;
-    p.pl.ranges = (int32_t)(ranges > 0 ? ranges : 1);
-    p.pl.min_blocks = (int32_t)(p.form == kHeads ? 256 / BK : p.form == kSplit ? 4 : 4);
-    p.pl.one_blocks = (int32_t)((p.form == kSplit ? 1024 : 512) / BK);
-    p.pl.max_records = 2 * p.pl.ranges + 8;
-    const int64_t most_blocks = ((int64_t)a.max_pages * a.page_size + BK - 1) / BK;
-    const bool cut = most_blocks > p.pl.one_blocks;
+    const int64_t fill = cus * per_cu > a.H_kv ? cus * per_cu / a.H_kv  : 1;
+    p.pl.fill = (int32_t)fill;
+    p.pl.min_blocks = (int32_t)(p.form == kHeads ? 64 / BK : 4);
+    p.pl.one_blocks = (int32_t)((p.form == kHeads ? 128 : p.form == kSplit ? 1024 : 512) / BK);
+    p.pl.max_records = (int32_t)(4 * fill + 8);
+    const bool cut = (a.max_len + BK - 1) / BK > p.pl.one_blocks;
+    if (!cut) p.pl.one_blocks = INT32_MAX;                    // nor is what is longer than max_len
     p.bytes = cut ? (size_t)p.pl.max_records * a.H_kv * (TM * (a.d + 2)) * sizeof(float) : 0;
-    int64_t units = (tiles + (cut ? ranges : 0)) * a.H_kv;
-    if (units > (1 << 24)) units = 1 << 24;
+    int64_t units = (tiles + (cut ? 2 * fill : 0)) * a.H_kv;
+    if (units > (1 << 22)) units = 1 << 22;
     p.wgs = (int)(p.form == kHeads ? (units + 3) / 4 : units);
     p.pl.step = p.form == kHeads ? 4 * p.wgs : p.wgs;
     const int64_t most_rows = rows < TM ? rows : TM;
-    p.pl.merge_groups = (int32_t)(p.form <= kSplit ? most_rows : (most_rows + 3) / 4);
-    const int64_t cut_tiles = tiles < ranges + 4 ? tiles : ranges + 4;
-    const int64_t merge_wgs = cut_tiles * a.H_kv * p.pl.merge_groups;
+    const int64_t merge_rows = p.form <= kSplit ? 1 : 1024 / a.d;   // of a workgroup
+    p.pl.merge_groups = (int32_t)((most_rows + merge_rows - 1) / merge_rows);
+    const int64_t merge_wgs = (tiles < 2 * fill ? tiles : 2 * fill) * a.H_kv * p.pl.merge_groups;
     p.merge_wgs = !cut ? 0 : merge_wgs > 4096 ? 4096 : (int)merge_wgs;
     p.pl.by_page = fastdiv_make(a.page_size);
     p.pl.by_group = fastdiv_make((int)G);
@@ -1316,10 +1375,10 @@ int launch_tiles(const cf_paged_attn_args_t& a, const Plan& p, hipStream_t st) {
     if (p.form == kHeads) return go(paged_heads<T, D>, 256, paged_merge<T, D, 16, Heads<T, D>::BK, 1, 1>);
     if (p.form == kSplit) return go(paged_split<T, D>, 64 * Split<T, D>::WAVES, paged_merge<T, D, 16, 64, 1, 1>);
     if constexpr (F16) {
-        if (p.form == kWide2) return go(paged_wide16<D, 2>, 512, paged_merge<T, D, 256, 64, kNarrowCost, 4>);
-        return go(paged_wide16<D, 1>, 512, paged_merge<T, D, 128, 64, kNarrowCost, 4>);
+        if (p.form == kWide2) return go(paged_wide16<D, 2>, 512, paged_merge<T, D, 256, 64, kNarrowCost, 1024 / D>);
+        return go(paged_wide16<D, 1>, 512, paged_merge<T, D, 128, 64, kNarrowCost, 1024 / D>);
     } else {
-        return go(paged_wide32<D>, 256, paged_merge<T, D, 64, 64, kNarrowCost, 4>);
+        return go(paged_wide32<D>, 256, paged_merge<T, D, 64, 64, kNarrowCost, 1024 / D>);
     }
 }
 

@@ -139,7 +139,7 @@ static int paged_attn_op(int elem, const void* inputs[], void* outputs[], const 
     if (p->batch_size < 0 || p->num_tokens < 0 || H <= 0 || d <= 0 || H % H_kv != 0) return -1;
     if (p->batch_size > INT32_MAX - 1 || p->num_tokens > INT32_MAX || H > 65535 || d > 512) return -1;
     if (!pages_ok(p->page_size, p->num_pages) || p->max_pages <= 0 || !pages_ok(p->page_size, p->max_pages)) return -1;
-    if (p->max_new < 0 || p->q_stride < 0) return -1;
+    if (p->max_new < 0 || p->max_len < 0 || p->q_stride < 0) return -1;
     cache_strides_t cs;
     if (cache_strides(p->page_stride, p->row_stride, p->head_stride, p->page_size, H_kv, d, &cs) != 0) return -1;
     if (p->batch_size == 0 || p->num_tokens == 0) return 0;
@@ -165,6 +165,8 @@ static int paged_attn_op(int elem, const void* inputs[], void* outputs[], const 
     a.num_pages = (int32_t)p->num_pages;
     a.max_pages = (int32_t)p->max_pages;
     a.max_new = p->max_new > 0 && p->max_new < p->num_tokens ? (int32_t)p->max_new : a.T;
+    const int64_t table_len = p->max_pages * p->page_size;
+    a.max_len = (int32_t)(p->max_len > 0 && p->max_len < table_len ? p->max_len : table_len);
     a.scale = p->scale;
     a.elem = elem;
     void* st = cf_stream_of(stream);

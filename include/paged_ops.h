@@ -107,8 +107,9 @@ typedef struct {
     int64_t page_size;
     int64_t num_pages;
     int64_t max_pages;     /* entries of one row of the block table */
-    int64_t max_new;       /* most rows a sequence has in this call, 0 = unknown: chooses the
-                              kernel only, more rows than that are computed all the same */
+    /* Most rows and most positions a sequence has in this call, 0 = unknown (the table's
+     * length).  They choose the kernels only: more than that is computed all the same. */
+    int64_t max_new, max_len;
     int64_t q_stride;      /* elements from row to row of Q; 0 = H_q d */
     int64_t page_stride, row_stride, head_stride;   /* of the cache, as in kv_page_store_params_t */
 } mha_paged_params_t;

@@ -195,7 +195,7 @@ def test_paged_registry_and_layouts(native):
         assert native.operator_find(n.encode()).contents.data_type == t
     assert ctypes.sizeof(cf.KvPageMapParams) == 48
     assert ctypes.sizeof(cf.KvPageStoreParams) == 104
-    assert ctypes.sizeof(cf.MhaPagedParams) == 112
+    assert ctypes.sizeof(cf.MhaPagedParams) == 120
 
 
 MAP_OK = dict(batch_size=2, num_tokens=8, page_size=16, num_pages=64, max_pages=8, ring_size=64)
