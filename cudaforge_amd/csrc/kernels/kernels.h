@@ -419,7 +419,7 @@ typedef struct {
     int32_t        max_len;     /* most positions of one; the table's where unknown */
     float          scale;
     int32_t        elem;
-    float*         records;     /* workspace of cf_paged_attn_bytes */
+    void*          workspace;   /* of cf_paged_attn_bytes */
 } cf_paged_attn_args_t;
 size_t cf_paged_attn_bytes(const cf_paged_attn_args_t* a);
 int cf_launch_paged_attn(const cf_paged_attn_args_t* a, void* stream);

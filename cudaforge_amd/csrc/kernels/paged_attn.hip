@@ -62,6 +62,7 @@ __device__ __forceinline__ SeqRows seq_rows(const cf_paged_attn_args_t& a, int b
 //                batch may mix prompt chunks and decode steps.
 
 struct PagedPlan {
+    int*    cut_tiles;     // their number (per KV head), left by the first workgroup for the merge
     float*  records;       // of the units of cut tiles
     int32_t max_records;   // per KV head
     int32_t fill;          // units (per KV head) that fill the chip
@@ -84,7 +85,7 @@ template <int TM, int BK, int NARROW>
 struct Geometry {
     const cf_paged_attn_args_t& a;
     const PagedPlan& pl;
-    int G, lane, C;
+    int G, lane, C, one;                 // C: most blocks of a range; one: tiles up to it are not cut
     SeqRows first;                       // lane: sequence `lane`, kept for the second pass,
     int* kept;                           // by wide tiles in LDS: their registers are all taken
 
@@ -98,7 +99,7 @@ struct Geometry {
     }
     __device__ __forceinline__ int ranges(const SeqRows& s) const {
         const int n = blocks(s), c = narrow(s) ? NARROW * C : C;
-        return n <= pl.one_blocks ? 1 : (n + c - 1) / c;
+        return n <= one ? 1 : (n + c - 1) / c;
     }
 
     __device__ __forceinline__ Geometry(const cf_paged_attn_args_t& a_, const PagedPlan& pl_, int* kept_ = nullptr)
@@ -123,15 +124,31 @@ struct Geometry {
         const float fill = (float)pl.fill;
         const float n = t <= 0.5f * fill ? fill - t : t <= fill ? 2.0f * fill - t : NARROW > 1 ? fill : 2.0f * fill;
         w = ceilf(w / fmaxf(n, 1.0f));
-        C = __builtin_amdgcn_readfirstlane((int)fminf(fmaxf(w, (float)pl.min_blocks), 1e8f));
+        // Cutting costs wide tiles a merge and records, as much as 5 to 13 blocks: with half the chip
+        // busy or more it pays for long ranges only.
+        const bool few = NARROW > 1 && t <= 0.25f * fill;
+        one = __builtin_amdgcn_readfirstlane(few ? min(pl.one_blocks, 512 / BK) : pl.one_blocks);
+        C = __builtin_amdgcn_readfirstlane((int)fminf(fmaxf(w, (float)(few ? 4 : pl.min_blocks)), 1e8f));
+        if (pl.one_blocks == INT32_MAX) one = INT32_MAX;
+    }
+    // The number of cut tiles, for the merge: most of its workgroups need know no more.
+    __device__ __forceinline__ void leave_cut_tiles() const {
+        if (!pl.cut_tiles || blockIdx.x != 0 || threadIdx.x >= 64) return;
+        int n = ranges(first) > 1 ? tiles(first) : 0;
+        for (int b = 64; b < a.B; b += 64) {
+            const SeqRows s = rows(b + lane);
+            n += ranges(s) > 1 ? tiles(s) : 0;
+        }
+        n += wave_excl_sum(n, lane);
+        if (lane == 63) *pl.cut_tiles = n;
     }
     // Item u of all units (MERGE: of all cut tiles); false where there is none.
     template <bool MERGE>
     __device__ __forceinline__ bool find(int u, Unit& out) const {
         int items0 = 0;
-        // Wide tiles: the sequences with the long ranges first, narrow tiles last, so that short
-        // pieces fill the end.
-        constexpr int CLASSES = !MERGE && NARROW > 1 ? 3 : 1;
+        // Wide tiles: the sequences with the long ranges first, so that short pieces fill the end
+        // (35 sequences, 4 of them chunks: 108 us, in the order of the sequences 131).
+        constexpr int CLASSES = !MERGE && NARROW > 1 ? 2 : 1;
         for (int cls = 0; cls < CLASSES; cls++) {
             int records0 = 0;
             for (int base = 0; base < a.B; base += 64) {
@@ -139,7 +156,7 @@ struct Geometry {
                                 : NARROW > 1 ? SeqRows{kept[lane], kept[64 + lane], kept[128 + lane]} : first;
                 const int t = tiles(s), ns = ranges(s), rec = ns > 1 ? t * ns : 0;
                 int items = MERGE ? (ns > 1 ? t : 0) : t * ns;
-                if (CLASSES > 1 && (narrow(s) ? 2 : 2 * blocks(s) > C * ns ? 0 : 1) != cls) items = 0;
+                if (CLASSES > 1 && (2 * blocks(s) > C * ns ? 0 : 1) != cls) items = 0;
                 const int before = items0 + wave_excl_sum(items, lane);
                 const int rec_before = records0 + wave_excl_sum(rec, lane);
                 const unsigned long long hit = __ballot(before <= u && u < before + items);
@@ -522,6 +539,7 @@ void paged_heads(cf_paged_attn_args_t a, PagedPlan pl) {
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int G = a.H_q / a.H_kv;
     const Geometry<16, H::BK, 1> geo(a, pl);
+    geo.leave_cut_tiles();
     for (int unit = (int)blockIdx.x * H::WAVES + wave;; unit += pl.step) {
         const int id = unit / a.H_kv, kvh = unit - id * a.H_kv;
         Unit un;
@@ -617,6 +635,7 @@ void paged_split(cf_paged_attn_args_t a, PagedPlan pl) {
     constexpr int WAVES = Split<T, D>::WAVES;
     __shared__ __attribute__((aligned(16))) T lds[WAVES * Narrow<T, D, 16>::RING];
     const Geometry<16, 64, 1> geo(a, pl);
+    geo.leave_cut_tiles();
     for (int unit = (int)blockIdx.x;; unit += pl.step) {
         const int id = unit / a.H_kv, kvh = unit - id * a.H_kv;
         Unit un;
@@ -953,6 +972,7 @@ void paged_wide16(cf_paged_attn_args_t a, PagedPlan pl) {
     __shared__ uint64_t masks[W::MASKS];
     __shared__ int kept[3 * 64];
     const Geometry<W::TM, 64, kNarrowCost> geo(a, pl, kept);
+    geo.leave_cut_tiles();
     for (int unit = (int)blockIdx.x;; unit += pl.step) {
         const int id = unit / a.H_kv, kvh = unit - id * a.H_kv;
         Unit un;
@@ -1132,6 +1152,7 @@ void paged_wide32(cf_paged_attn_args_t a, PagedPlan pl) {
     __shared__ __attribute__((aligned(16))) float lds[W::LDS];
     __shared__ int kept[3 * 64];
     const Geometry<W::TM, 64, kNarrowCost> geo(a, pl, kept);
+    geo.leave_cut_tiles();
     for (int unit = (int)blockIdx.x;; unit += pl.step) {
         const int id = unit / a.H_kv, kvh = unit - id * a.H_kv;
         Unit un;
@@ -1152,11 +1173,13 @@ void paged_merge(cf_paged_attn_args_t a, PagedPlan pl) {
     static_assert(SUBS >= 1, "rows per workgroup");
     __shared__ float ml[2][ROWS][SUBS];
     __shared__ f4_t part[SUBS > 1 ? SUBS * ROWS * DL : 1];
+    const int cut_units = *pl.cut_tiles * a.H_kv * pl.merge_groups;
+    if ((int)blockIdx.x >= cut_units) return;
     __shared__ int kept[NARROW > 1 ? 3 * 64 : 1];
     const Geometry<TM, BK, NARROW> geo(a, pl, kept);
     const int G = a.H_q / a.H_kv;
     const int d4 = threadIdx.x % DL, sub = threadIdx.x / DL % SUBS, r = threadIdx.x / (DL * SUBS);
-    for (int unit = blockIdx.x;; unit += gridDim.x) {
+    for (int unit = blockIdx.x; unit < cut_units; unit += gridDim.x) {
         const int th = unit / pl.merge_groups, group = unit - th * pl.merge_groups;
         const int tile_id = th / a.H_kv, kvh = th - tile_id * a.H_kv;
         Unit un;
@@ -1304,6 +1327,8 @@ struct Plan {
 
 constexpr int64_t g_few_units = 64, g_split_units = 256, g_split_len = 1024, g_wide2_units = 192;
 
+constexpr size_t kHeader = 256;   // of the workspace: the number of cut tiles
+
 bool fast_ok(const cf_paged_attn_args_t& a) {
     const uint64_t ptrs = (uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.k | (uint64_t)(uintptr_t)a.v | (uint64_t)(uintptr_t)a.o;
     const uint64_t steps = (uint64_t)a.q_stride | (uint64_t)a.page_stride | (uint64_t)a.row_stride | (uint64_t)a.head_stride;
@@ -1340,12 +1365,13 @@ Plan make_plan(const cf_paged_attn_args_t& a) {
                          : f16 || a.d == 128 ? 1 : 2;
     const int64_t fill = cus * per_cu > a.H_kv ? cus * per_cu / a.H_kv  : 1;
     p.pl.fill = (int32_t)fill;
-    p.pl.min_blocks = (int32_t)(p.form == kHeads ? 64 / BK : 4);
-    p.pl.one_blocks = (int32_t)((p.form == kHeads ? 128 : p.form == kSplit ? 1024 : 512) / BK);
+    const bool wide16 = f16 && p.form > kSplit;
+    p.pl.min_blocks = (int32_t)(p.form == kHeads ? 64 / BK : wide16 ? 12 : 4);
+    p.pl.one_blocks = (int32_t)((p.form == kHeads ? 128 : p.form == kSplit ? 1024 : wide16 ? 1536 : 512) / BK);
     p.pl.max_records = (int32_t)(4 * fill + 8);
-    const bool cut = (a.max_len + BK - 1) / BK > p.pl.one_blocks;
+    const bool cut = (a.max_len + BK - 1) / BK > (wide16 ? 512 / BK : p.pl.one_blocks);
     if (!cut) p.pl.one_blocks = INT32_MAX;                    // nor is what is longer than max_len
-    p.bytes = cut ? (size_t)p.pl.max_records * a.H_kv * (TM * (a.d + 2)) * sizeof(float) : 0;
+    p.bytes = cut ? kHeader + (size_t)p.pl.max_records * a.H_kv * (TM * (a.d + 2)) * sizeof(float) : 0;
     int64_t units = (tiles + (cut ? 2 * fill : 0)) * a.H_kv;
     if (units > (1 << 22)) units = 1 << 22;
     p.wgs = (int)(p.form == kHeads ? (units + 3) / 4 : units);
@@ -1357,6 +1383,7 @@ Plan make_plan(const cf_paged_attn_args_t& a) {
     p.merge_wgs = !cut ? 0 : merge_wgs > 4096 ? 4096 : (int)merge_wgs;
     p.pl.by_page = fastdiv_make(a.page_size);
     p.pl.by_group = fastdiv_make((int)G);
+    p.pl.cut_tiles = nullptr;
     p.pl.records = nullptr;
     return p;
 }
@@ -1392,8 +1419,11 @@ extern "C" int cf_launch_paged_attn(const cf_paged_attn_args_t* a, void* stream)
         return (int)hipErrorInvalidValue;
     if (fast_ok(*a)) {
         Plan p = make_plan(*a);
-        if (p.bytes > 0 && !a->records) return (int)hipErrorInvalidValue;
-        p.pl.records = a->records;
+        if (p.bytes > 0 && !a->workspace) return (int)hipErrorInvalidValue;
+        if (p.bytes > 0) {
+            p.pl.cut_tiles = (int*)a->workspace;
+            p.pl.records = (float*)((char*)a->workspace + kHeader);
+        }
         if (a->elem == CF_ELEM_F16)
             return a->d == 64 ? launch_tiles<_Float16, 64>(*a, p, st) : launch_tiles<_Float16, 128>(*a, p, st);
         return a->d == 64 ? launch_tiles<float, 64>(*a, p, st) : launch_tiles<float, 128>(*a, p, st);
