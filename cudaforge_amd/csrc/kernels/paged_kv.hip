@@ -60,18 +60,13 @@ __device__ __forceinline__ int ring_page(const cf_page_map_args_t& a, int head, 
     return (unsigned)page < (unsigned)a.num_pages ? page : -1;
 }
 
-__device__ __forceinline__ void write_token(const cf_page_map_args_t& a, const RingState& r, const MapDivs& dv, int b,
-                                            const SeqPages& s, int i, int row) {
-    const int pos = s.c + i;
-    const int idx = fastdiv(pos, dv.page);
-    int page = -1;
-    if (s.first >= 0) {
-        const int before = ceil_pages(s.c, a.page_size, dv.page);
-        page = idx < before ? a.table[(size_t)b * a.max_pages + idx] : ring_page(a, r.head, s.first + idx - before, dv.ring);
-        if ((unsigned)page >= (unsigned)a.num_pages) page = -1;
-    }
-    a.positions[row] = pos;
-    a.slots[row] = page < 0 ? -1 : page * a.page_size + (pos - idx * a.page_size);
+// The slot of position pos of sequence b.
+__device__ __forceinline__ int slot_of(const cf_page_map_args_t& a, const RingState& r, const MapDivs& dv, int b,
+                                       const SeqPages& s, int pos) {
+    if (s.first < 0) return -1;
+    const int idx = fastdiv(pos, dv.page), before = ceil_pages(s.c, a.page_size, dv.page);
+    const int page = idx < before ? a.table[(size_t)b * a.max_pages + idx] : ring_page(a, r.head, s.first + idx - before, dv.ring);
+    return (unsigned)page < (unsigned)a.num_pages ? page * a.page_size + (pos - idx * a.page_size) : -1;
 }
 
 // Page j that changes hands with sequence b: into its table, or out of it into the ring.
@@ -85,20 +80,26 @@ __device__ __forceinline__ void move_page(const cf_page_map_args_t& a, const Rin
     row[ceil_pages(s.c, a.page_size, dv.page) + j] = s.first >= 0 ? ring_page(a, r.head, s.first + j, dv.ring) : -1;
 }
 
-// The last entry of start[0 .. n) that is not above x (start[0] <= x).
-__device__ __forceinline__ int last_not_above(const int* start, int n, int x) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (start[mid] <= x) lo = mid; else hi = mid;
+// For N rows at once, so that the LDS reads of one do not wait for another's: the last entry of
+// start[0 .. n) that is not above x[j] (start[0] <= x[j]).
+template <int N>
+__device__ __forceinline__ void last_not_above(const int* start, int n, const int (&x)[N], int (&at)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; j++) at[j] = 0;
+    for (int step = kMapOneSeqs / 2; step > 0; step >>= 1) {
+        if (step >= n) continue;
+        int v[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) v[j] = start[min(at[j] + step, n - 1)];
+#pragma unroll
+        for (int j = 0; j < N; j++) at[j] += at[j] + step < n && v[j] <= x[j] ? step : 0;
     }
-    return lo;
 }
 
-// One workgroup: the prefix sums, a sequence per thread and 1024 sequences at a time.  ONE
-// (up to 1024 sequences): it then writes the tokens and pages too, each found by its
+// One workgroup: the prefix sums, PER neighbouring sequences per thread.  ONE (one per
+// thread, up to 1024 sequences and 4096 tokens): it then writes the tokens and pages too, each found by its
 // number in the sums in LDS; else it leaves SeqPages per sequence in a.info for page_map_fill.
-template <bool ONE>
+template <bool ONE, int PER>
 __global__ __launch_bounds__(kMapThreads)
 void page_map_scan(cf_page_map_args_t a, MapDivs dv) {
     constexpr int kWaves = kMapThreads / 64;
@@ -111,53 +112,71 @@ void page_map_scan(cf_page_map_args_t a, MapDivs dv) {
     const RingState r = ring_state(a.counters, a.ring_size, dv.ring);
     if (tid == 0) taken_s = refused_s = 0;
     int carry[4] = {0, 0, 0, 0};                   // rows, pages needed, taken back, moved
-    for (int base = 0; base < a.B; base += kMapThreads) {
-        const int b = base + tid;
-        const bool live = b < a.B;
-        const int n0 = live ? a.new_lens[b] : 0;
-        SeqPages s;
-        s.c = live ? min(max(a.cache_lens[b], 0), cap) : 0;
-        s.n = max(n0, 0);
-        const bool ended = n0 < 0;
-        const uint32_t len = (uint32_t)s.c + (uint32_t)s.n;
-        const bool fits = !ended && len <= (uint32_t)cap;
-        const int before = ceil_pages(s.c, P, dv.page);
-        int v[4];
-        v[0] = s.n;
-        v[1] = fits ? ceil_pages((int)len, P, dv.page) - before : 0;
-        v[2] = ended ? before : 0;
-        v[3] = ended ? before : fits ? v[1] : live ? a.max_pages - before : 0;
-        int ex[4];
+    for (int base = 0; base < a.B; base += PER * kMapThreads) {
+        SeqPages s[PER];
+        int v[PER][4], sum[4] = {0, 0, 0, 0}, ex[4];
+        bool ended[PER], fits[PER];
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int b = base + PER * tid + j;
+            s[j].c = b < a.B ? a.cache_lens[b] : 0;
+            s[j].n = b < a.B ? a.new_lens[b] : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const bool live = base + PER * tid + j < a.B;
+            ended[j] = s[j].n < 0;
+            s[j].c = min(max(s[j].c, 0), cap);
+            s[j].n = max(s[j].n, 0);
+            const uint32_t len = (uint32_t)s[j].c + (uint32_t)s[j].n;
+            fits[j] = !ended[j] && len <= (uint32_t)cap;
+            const int before = ceil_pages(s[j].c, P, dv.page);
+            v[j][0] = s[j].n;
+            v[j][1] = fits[j] ? ceil_pages((int)len, P, dv.page) - before : 0;
+            v[j][2] = ended[j] ? before : 0;
+            v[j][3] = ended[j] ? before : fits[j] ? v[j][1] : live ? a.max_pages - before : 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) sum[k] += v[j][k];
+        }
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            ex[k] = wave_excl_sum(v[k], lane);
-            if (lane == 63) part[k][wave] = ex[k] + v[k];
+            ex[k] = wave_excl_sum(sum[k], lane);
+            if (lane == 63) part[k][wave] = ex[k] + sum[k];
         }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            int sum = 0;
+            int all = 0;
             for (int w = 0; w < kWaves; w++) {
-                if (w == wave) ex[k] += carry[k] + sum;
-                sum += part[k][w];
+                if (w == wave) ex[k] += carry[k] + all;
+                all += part[k][w];
             }
-            carry[k] += sum;
+            carry[k] += all;
         }
-        const bool served = fits && (v[1] == 0 || ex[1] + v[1] <= r.avail);
-        s.first = ended ? kEnded : served ? ex[1] : kNotServed;
-        s.give = ex[2];
-        if (live) {
-            a.seq_lens[b] = ended ? 0 : (int)min(len, 0x7fffffffu);
-            a.q_start[b] = ex[0];
-            if (served && v[1] > 0) atomicMax(&taken_s, ex[1] + v[1]);
-            if (!served && !ended) atomicAdd(&refused_s, 1);
-            if constexpr (ONE) {
-                seq[b] = s;
-                row0[b] = ex[0];
-                move0[b] = ex[3];
-            } else {
-                ((int4*)a.info)[b] = int4{s.c, s.n, s.first, s.give};
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int b = base + PER * tid + j;
+            const bool served = fits[j] && (v[j][1] == 0 || ex[1] + v[j][1] <= r.avail);
+            s[j].first = ended[j] ? kEnded : served ? ex[1] : kNotServed;
+            s[j].give = ex[2];
+            // Ends of what is taken rise with the sequences: the last one's counts.
+            const uint64_t takes = __builtin_amdgcn_ballot_w64(served && v[j][1] > 0);
+            const uint64_t refused = __builtin_amdgcn_ballot_w64(b < a.B && !served && !ended[j]);
+            if (takes && lane == 63 - __builtin_clzll(takes)) atomicMax(&taken_s, ex[1] + v[j][1]);
+            if (refused && lane == 0) atomicAdd(&refused_s, __builtin_popcountll(refused));
+            if (b < a.B) {
+                a.seq_lens[b] = ended[j] ? 0 : (int)min((uint32_t)s[j].c + (uint32_t)s[j].n, 0x7fffffffu);
+                a.q_start[b] = ex[0];
+                if constexpr (ONE) {
+                    seq[b] = s[j];
+                    row0[b] = ex[0];
+                    move0[b] = ex[3];
+                } else {
+                    ((int4*)a.info)[b] = int4{s[j].c, s[j].n, s[j].first, s[j].give};
+                }
             }
+#pragma unroll
+            for (int k = 0; k < 4; k++) ex[k] += v[j][k];
         }
         __syncthreads();
     }
@@ -173,17 +192,33 @@ void page_map_scan(cf_page_map_args_t a, MapDivs dv) {
         a.counters_out[2] = refused_s;
     }
     if constexpr (ONE) {
-        for (int t = tid; t < a.T; t += kMapThreads) {
-            if ((uint32_t)t >= (uint32_t)carry[0]) {
-                a.positions[t] = a.slots[t] = -1;
-                continue;
+        constexpr int N = kMapOneTokens / kMapThreads;
+        int t[N], b[N], pos[N], slot[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) t[j] = tid + j * kMapThreads;
+        if (tid < a.T) {
+            last_not_above(row0, a.B, t, b);
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                const SeqPages s = seq[b[j]];
+                const uint32_t i = (uint32_t)(t[j] - row0[b[j]]);
+                // Behind the last row; or new_lens whose sum passes 32 bits.
+                const bool none = (uint32_t)t[j] >= (uint32_t)carry[0] || i >= (uint32_t)s.n || t[j] >= a.T;
+                pos[j] = none ? -1 : s.c + (int)i;
+                slot[j] = none ? -1 : slot_of(a, r, dv, b[j], s, pos[j]);
             }
-            const int b = last_not_above(row0, a.B, t);
-            write_token(a, r, dv, b, seq[b], t - row0[b], t);
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if (t[j] < a.T) {
+                    a.positions[t[j]] = pos[j];
+                    a.slots[t[j]] = slot[j];
+                }
         }
         for (int i = tid; i < carry[3]; i += kMapThreads) {
-            const int b = last_not_above(move0, a.B, i);
-            move_page(a, r, dv, b, seq[b], i - move0[b]);
+            const int x[1] = {i};
+            int at[1];
+            last_not_above(move0, a.B, x, at);
+            move_page(a, r, dv, at[0], seq[at[0]], i - move0[at[0]]);
         }
     }
 }
@@ -203,8 +238,11 @@ void page_map_fill(cf_page_map_args_t a, MapDivs dv) {
     const RingState r = ring_state((const int32_t*)a.info + 4 * (size_t)a.B, a.ring_size, dv.ring);
     const int4 v = ((const int4*)a.info)[b];
     const SeqPages s = {v.x, v.y, v.z, v.w};
-    for (int i = i0; i < s.n && row0 + (uint32_t)i < (uint32_t)a.T; i += step)
-        write_token(a, r, dv, b, s, i, (int)(row0 + (uint32_t)i));
+    for (int i = i0; i < s.n && row0 + (uint32_t)i < (uint32_t)a.T; i += step) {
+        const uint32_t t = row0 + (uint32_t)i;
+        a.positions[t] = s.c + i;
+        a.slots[t] = slot_of(a, r, dv, b, s, s.c + i);
+    }
     const int before = ceil_pages(s.c, a.page_size, dv.page);
     const uint32_t len = (uint32_t)s.c + (uint32_t)s.n;
     const int moves = s.first == kEnded ? before
@@ -313,11 +351,14 @@ extern "C" int cf_launch_page_map(const cf_page_map_args_t* a, void* stream) {
         return (int)hipErrorInvalidValue;
     const MapDivs dv = {fastdiv_make(a->page_size), fastdiv_make(a->ring_size)};
     if (cf_page_map_info_ints(a->B, a->T) == 0) {
-        hipLaunchKernelGGL(page_map_scan<true>, dim3(1), dim3(kMapThreads), 0, st, *a, dv);
+        hipLaunchKernelGGL((page_map_scan<true, 1>), dim3(1), dim3(kMapThreads), 0, st, *a, dv);
         return (int)hipGetLastError();
     }
     if (!a->info) return (int)hipErrorInvalidValue;
-    hipLaunchKernelGGL(page_map_scan<false>, dim3(1), dim3(kMapThreads), 0, st, *a, dv);
+    // Four sequences a thread for more than a workgroup has threads: their loads wait together
+    // (3000 sequences: 11.6 us for both launches, one at a time 17; 256: 13 us, one at a time 11).
+    if (a->B <= kMapThreads) hipLaunchKernelGGL((page_map_scan<false, 1>), dim3(1), dim3(kMapThreads), 0, st, *a, dv);
+    else hipLaunchKernelGGL((page_map_scan<false, 4>), dim3(1), dim3(kMapThreads), 0, st, *a, dv);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
     // Long chunks of few sequences are shared by several workgroups.

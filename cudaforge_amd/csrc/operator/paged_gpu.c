@@ -96,9 +96,12 @@ static int page_store_op(int elem, const void* inputs[], void* outputs[], const 
             a.q_stride = p->q_stride > 0 ? p->q_stride : p->num_heads * p->head_dim;
             a.q_out_stride = p->q_out_stride > 0 ? p->q_out_stride : p->num_heads * p->head_dim;
         }
-        /* In turns, so that the kernel reduces an angle by dropping whole numbers. */
-        const double two_pi = 6.283185307179586476925286766559;
-        for (int i = 0; i < a.d / 2; i++) a.turns[i] = pow((double)p->rope_base, -2.0 * i / (double)a.d) / two_pi;
+        /* In turns, so that the kernel reduces an angle by dropping whole numbers; one power and
+         * products of 64 bits of mantissa (128 of them are off by 2^-57), as a power per pair
+         * would take longer than the launch. */
+        const long double step = powl((long double)p->rope_base, -2.0L / (long double)a.d);
+        long double turns = 1.0L / 6.283185307179586476925286766559L;
+        for (int i = 0; i < a.d / 2; i++, turns *= step) a.turns[i] = (double)turns;
     }
     cache_strides_t cs;
     if (cache_strides(p->page_stride, p->row_stride, p->head_stride, p->page_size, p->num_kv_heads, p->head_dim, &cs) != 0)

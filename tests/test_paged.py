@@ -366,6 +366,21 @@ def test_map_edges(gpu, many):
              ref_map(cached, n, table, ring, max(head, 0) % 9, min(max(avail, 0), 9), T, P, num_pages))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("many", [False, True])
+def test_map_of_lengths_whose_sum_passes_32_bits(gpu, many):
+    """Nothing out of range is touched: entries of the table stay pages or -1, slots stay below the
+    last page's end."""
+    P, width, num_pages, T = 16, 4, 64, 50
+    big = 2 ** 31 - 1
+    new = [5, big, big, 3, big, 20] + [1] * (1100 if many else 0)
+    cached = [0] * len(new)
+    table, ring = np.full((len(new), width), -1, I32), np.arange(num_pages, dtype=I32)
+    got = run_map(cached, new, table, ring, 0, num_pages, T, P, num_pages)
+    assert (got["table"] >= -1).all() and (got["table"] < num_pages).all()
+    assert (got["slots"] >= -1).all() and (got["slots"] < num_pages * P).all()
+
+
 # ------------------------------------------------------------------ the store (GPU) ---
 
 @pytest.mark.gpu
