@@ -265,6 +265,86 @@ template <typename T, int D> __device__ __forceinline__ int vswz(int row) {
     return sizeof(T) == 4 ? row & 15 : D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3);
 }
 
+// ---- One row of one head by a wave, 64 positions at a time: lanes are positions for the
+// scores and dims (at most 64 DIMS) for the sum over V. ----
+template <typename T, int DIMS>
+__device__ __forceinline__ void plain_row(const cf_paged_attn_args_t& a, FastDiv by_page, const SeqRows& s, int b, int tok,
+                                          int h, int d) {
+    const int lane = threadIdx.x & 63;
+    const int seen = min(s.len - s.n + tok + 1, s.len);
+    const int32_t* const table = a.table + (size_t)b * a.max_pages;
+    const T* const q = (const T*)a.q + (int64_t)(s.row0 + tok) * a.q_stride + (int64_t)h * d;
+    const T* const k = (const T*)a.k + (int64_t)(h / (a.H_q / a.H_kv)) * a.head_stride;
+    const T* const v = (const T*)a.v + (int64_t)(h / (a.H_q / a.H_kv)) * a.head_stride;
+    const float c = a.scale * kLog2e;
+    float m = -INFINITY, l = 0.0f, acc[DIMS];
+#pragma unroll
+    for (int i = 0; i < DIMS; i++) acc[i] = 0.0f;
+#pragma clang loop unroll(disable)
+    for (int k0 = 0; k0 < seen; k0 += 64) {
+        const int key = k0 + lane;
+        int64_t at = 0;
+        float x = -INFINITY;
+        if (key < seen) {
+            const int idx = fastdiv(key, by_page);
+            const int page = table[idx];
+            if ((unsigned)page < (unsigned)a.num_pages) {
+                at = (int64_t)page * a.page_stride + (int64_t)(key - idx * a.page_size) * a.row_stride;
+                float dot = 0.0f;
+#pragma clang loop unroll(disable)
+                for (int e = 0; e < d; e++) dot = __builtin_fmaf((float)q[e], (float)k[at + e], dot);
+                x = dot * c;
+            }
+        }
+        const float m_new = fmaxf(m, wave_max(x));
+        if (m_new == -INFINITY && !__builtin_amdgcn_ballot_w64(x != x)) continue;
+        const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha = exp2f(m - m_use), p = exp2f(x - m_use);
+        m = m_new;
+        l = l * alpha + wave_sum(p);
+#pragma unroll
+        for (int i = 0; i < DIMS; i++) acc[i] *= alpha;
+#pragma clang loop unroll(disable)
+        for (int j = 0; j < min(64, seen - k0); j++) {
+            const float pj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(p), j));
+            if (pj == 0.0f) continue;          // not attended: its V may hold anything
+            const int64_t row = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(at >> 32), j) << 32) |
+                                          (uint32_t)__builtin_amdgcn_readlane((int)at, j));
+#pragma unroll
+            for (int i = 0; i < DIMS; i++)
+                if (lane + 64 * i < d) acc[i] = __builtin_fmaf(pj, (float)v[row + lane + 64 * i], acc[i]);
+        }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T* const o = (T*)a.o + ((int64_t)(s.row0 + tok) * a.H_q + h) * d;
+#pragma unroll
+    for (int i = 0; i < DIMS; i++)
+        if (lane + 64 * i < d) o[lane + 64 * i] = (T)(acc[i] * inv);
+}
+
+// On the matrix cores a position that another row of the tile sees counts as 0 times its V,
+// which is no 0 where V is infinite or NaN.  A sum that is NaN while l is a number may come from
+// one: such a row is computed again, where only what it sees is touched.
+template <typename T, int D>
+__device__ __forceinline__ void redo_row(const cf_paged_attn_args_t& a, const PagedPlan& pl, const Unit& un, int kvh, int R) {
+    const int G = a.H_q / a.H_kv, tok = fastdiv(R, pl.by_group);
+    plain_row<T, D / 64>(a, pl.by_page, un.s, un.b, tok, kvh * G + (R - tok * G), D);
+}
+template <int N>
+__device__ __forceinline__ bool spoilt(const f4_t (&acc)[N], float l) {
+    f4_t x = acc[0];
+#pragma unroll
+    for (int u = 1; u < N; u++) x += acc[u];
+    const float y = (x[0] + x[1]) + (x[2] + x[3]);
+    return y != y && l == l;
+}
+// Bit r: one of the lanes r, r + 16, r + 32 and r + 48 has `bad` set.
+__device__ __forceinline__ uint32_t rows_of_16(bool bad) {
+    const uint64_t b = __builtin_amdgcn_ballot_w64(bad);
+    const uint32_t x = (uint32_t)b | (uint32_t)(b >> 32);
+    return (x | x >> 16) & 0xffffu;
+}
+
 // How rows of D elements lie in LDS and in lanes.
 template <typename T, int D> struct Rows {
     static constexpr bool F16 = sizeof(T) == 2;
@@ -549,7 +629,8 @@ void paged_heads(cf_paged_attn_args_t a, PagedPlan pl) {
         float m, l;
         narrow_range<T, D, H::BK>(a, pl, ring_all + wave * H::RING, un.s, un.b, kvh, w, w.key0, w.key1, acc, m, l);
         l = add_xor32(add_xor16(l));
-        if (lr < w.n_rows) {
+        uint32_t again = un.n_ranges > 1 ? 0 : rows_of_16(lr < w.n_rows && spoilt(acc, l));
+        if (lr < w.n_rows && !((again >> lr) & 1)) {
             if (un.n_ranges > 1) {
                 float* const rec = record_of<16, D>(a, pl, un, kvh);
 #pragma unroll
@@ -566,13 +647,15 @@ void paged_heads(cf_paged_attn_args_t a, PagedPlan pl) {
                 for (int u = 0; u < D / 16; u++) store4(o + 16 * u, acc[u] * inv);
             }
         }
+        for (; again; again &= again - 1) redo_row<T, D>(a, pl, un, kvh, w.R0 + __builtin_ctz(again));
     }
 }
 
 // Up to 16 rows by all waves of a workgroup: each takes a share of the unit's positions, and
-// they join their m, l and sums in LDS (WAVES rings at `lds`, one each).
+// they join their m, l and sums in LDS (WAVES rings at `lds`, one each).  True where rows that
+// this wave finished have to be computed again.
 template <typename T, int D, int TM, int WAVES>
-__device__ __forceinline__ void narrow_unit(const cf_paged_attn_args_t& a, const PagedPlan& pl, T* lds, const Unit& un,
+__device__ __forceinline__ bool narrow_unit(const cf_paged_attn_args_t& a, const PagedPlan& pl, T* lds, const Unit& un,
                                             int kvh, const Work& w) {
     constexpr int RING = Narrow<T, D, 16>::RING, LD = D + 4;
     static_assert(16 * (LD + 2) * 4 <= RING * (int)sizeof(T), "a wave's rows fit its ring");
@@ -595,6 +678,7 @@ __device__ __forceinline__ void narrow_unit(const cf_paged_attn_args_t& a, const
         mine[16 * LD + 16 + lr] = l;
     }
     __syncthreads();
+    bool again = false;
     for (int i = threadIdx.x; i < w.n_rows * (D / 4); i += 64 * WAVES) {
         const int row = i / (D / 4), d4 = i % (D / 4);
         float M = -INFINITY;
@@ -618,12 +702,25 @@ __device__ __forceinline__ void narrow_unit(const cf_paged_attn_args_t& a, const
                 rec[TM + row] = L;
             }
         } else {
+            const f4_t one[1] = {sum};
+            again |= spoilt(one, L);
             const RowAt at = row_at(pl, a.H_q / a.H_kv, kvh, w.R0 + row);
             store4((T*)a.o + ((int64_t)(un.s.row0 + at.tok) * a.H_q + at.h) * D + 4 * d4,
                    sum * (L == 0.0f ? 0.0f : 1.0f / L));
         }
     }
     __syncthreads();                                          // the rings, before the next unit
+    return __builtin_amdgcn_ballot_w64(again) != 0;
+}
+
+// Those rows of the wave.
+template <typename T, int D, int WAVES>
+__device__ __forceinline__ void redo_narrow(const cf_paged_attn_args_t& a, const PagedPlan& pl, const Unit& un, int kvh,
+                                            const Work& w) {
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    wait_vm<0>();                                             // what it stored is stored
+    for (int r = 0; r < w.n_rows; r++)
+        if (r / (256 / D) % WAVES == wave) redo_row<T, D>(a, pl, un, kvh, w.R0 + r);
 }
 
 template <typename T, int D> struct Split {
@@ -640,7 +737,8 @@ void paged_split(cf_paged_attn_args_t a, PagedPlan pl) {
         const int id = unit / a.H_kv, kvh = unit - id * a.H_kv;
         Unit un;
         if (!geo.template find<false>(id, un)) break;
-        narrow_unit<T, D, 16, WAVES>(a, pl, lds, un, kvh, unit_work<16, 64>(a, pl, un));
+        const Work w = unit_work<16, 64>(a, pl, un);
+        if (narrow_unit<T, D, 16, WAVES>(a, pl, lds, un, kvh, w)) redo_narrow<T, D, WAVES>(a, pl, un, kvh, w);
     }
 }
 
@@ -688,8 +786,9 @@ template <int D, int NJ> struct Wide16 {
     static_assert(8 * Narrow<_Float16, D, 16>::RING <= LDS, "the rings of narrow tiles fit");
 };
 
+// Returns the wave's rows that have to be computed again, a bit each.
 template <int D, int NJ>
-__device__ __forceinline__ void wide16_unit(const cf_paged_attn_args_t& a, const PagedPlan& pl, _Float16* lds,
+__device__ __forceinline__ uint32_t wide16_unit(const cf_paged_attn_args_t& a, const PagedPlan& pl, _Float16* lds,
                                             uint64_t* masks, const Unit& un, int kvh, const Work& w) {
     using T = _Float16;
     using R = Rows<T, D>;
@@ -951,16 +1050,20 @@ __device__ __forceinline__ void wide16_unit(const cf_paged_attn_args_t& a, const
             products(n, from_v, to_v);
         }
     }
+    uint32_t again_all = 0;
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
         const int row = wrow + 16 * j + lr;
-        if (row < w.n_rows) {
+        const uint32_t again = un.n_ranges > 1 ? 0 : rows_of_16(row < w.n_rows && spoilt(acc[j], lsum[j][0]));
+        if (row < w.n_rows && !((again >> lr) & 1)) {
             const RowOut out = row_out<T, D, W::TM>(a, pl, un, kvh, w, row, m_run[j], lsum[j][0], lq == 0);
 #pragma unroll
             for (int u = 0; u < UT; u++) put4<T>(out, 16 * u + 4 * lq, acc[j][u]);
         }
+        again_all |= again << (16 * j);
     }
     ring_barrier();                                           // the ring's reads, before the next unit
+    return again_all;
 }
 
 constexpr int kNarrowCost = 4;
@@ -977,9 +1080,17 @@ void paged_wide16(cf_paged_attn_args_t a, PagedPlan pl) {
         const int id = unit / a.H_kv, kvh = unit - id * a.H_kv;
         Unit un;
         if (!geo.template find<false>(id, un)) break;
-        const Work w = unit_work<W::TM, 64>(a, pl, un);
-        if (w.n_rows <= 16) narrow_unit<_Float16, D, W::TM, 8>(a, pl, lds, un, kvh, w);
-        else wide16_unit<D, NJ>(a, pl, lds, masks, un, kvh, w);
+        Work w = unit_work<W::TM, 64>(a, pl, un);
+        const bool narrow = w.n_rows <= 16;
+        const uint32_t again = narrow ? narrow_unit<_Float16, D, W::TM, 8>(a, pl, lds, un, kvh, w)
+                                      : wide16_unit<D, NJ>(a, pl, lds, masks, un, kvh, w);
+        if (!again) continue;
+        if (!geo.template find<false>(id, un)) break;         // found anew: nothing is kept for this
+        w = unit_work<W::TM, 64>(a, pl, un);
+        if (narrow) redo_narrow<_Float16, D, 8>(a, pl, un, kvh, w);
+        const int row0 = w.R0 + 16 * NJ * __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+        for (uint32_t left = narrow ? 0 : again; left; left &= left - 1)
+            redo_row<_Float16, D>(a, pl, un, kvh, row0 + __builtin_ctz(left));
     }
 }
 
@@ -1137,11 +1248,13 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
         for_each_stage<NS>(n, step);
     }
     const float l = add_xor32(add_xor16(l_run));
-    if (wrow + lr < w.n_rows) {
+    uint32_t again = un.n_ranges > 1 ? 0 : rows_of_16(wrow + lr < w.n_rows && spoilt(acc, l));
+    if (wrow + lr < w.n_rows && !((again >> lr) & 1)) {
         const RowOut out = row_out<T, D, W::TM>(a, pl, un, kvh, w, wrow + lr, m_run, l, lq == 0);
 #pragma unroll
         for (int u = 0; u < UT; u++) put4<T>(out, 16 * u + 4 * lq, acc[u]);
     }
+    for (; again; again &= again - 1) redo_row<T, D>(a, pl, un, kvh, w.R0 + wrow + __builtin_ctz(again));
     ring_barrier();                                           // the ring's reads, before the next unit
 }
 
@@ -1158,8 +1271,8 @@ void paged_wide32(cf_paged_attn_args_t a, PagedPlan pl) {
         Unit un;
         if (!geo.template find<false>(id, un)) break;
         const Work w = unit_work<W::TM, 64>(a, pl, un);
-        if (w.n_rows <= 16) narrow_unit<float, D, W::TM, 4>(a, pl, lds, un, kvh, w);
-        else wide32_unit<D>(a, pl, lds, un, kvh, w);
+        if (w.n_rows > 16) wide32_unit<D>(a, pl, lds, un, kvh, w);
+        else if (narrow_unit<float, D, W::TM, 4>(a, pl, lds, un, kvh, w)) redo_narrow<float, D, 4>(a, pl, un, kvh, w);
     }
 }
 
@@ -1242,22 +1355,29 @@ void paged_merge(cf_paged_attn_args_t a, PagedPlan pl) {
                 }
                 __syncthreads();
             }
-            if (sub == 0 && row < n_rows) {
+            const bool mine = sub == 0 && row < n_rows;
+            const f4_t one[1] = {acc};
+            uint64_t bad = __builtin_amdgcn_ballot_w64(mine && spoilt(one, l));
+            if (mine && bad == 0) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 const RowAt at = row_at(pl, G, kvh, un.tile * TM + row);
                 store4((T*)a.o + ((int64_t)(un.s.row0 + at.tok) * a.H_q + at.h) * D + 4 * d4, acc * inv);
             }
+            if (bad != 0)                                     // this wave's rows, all of them
+                for (uint64_t left = __builtin_amdgcn_ballot_w64(mine); left;) {
+                    const int again = __builtin_amdgcn_readlane(row, __builtin_ctzll(left));
+                    redo_row<T, D>(a, pl, un, kvh, un.tile * TM + again);
+                    left &= ~__builtin_amdgcn_ballot_w64(row == again);
+                }
         }
     }
 }
 
-// ---- Every shape: one wave per row and head, 64 positions at a time.  Lanes are positions
-// for the scores and dims for the sum over V. ----
+// ---- Every shape: a wave per row and head. ----
 constexpr int kAnyDims = 512 / 64;             // dims per lane
 template <typename T>
 __global__ __launch_bounds__(256)
 void paged_any(cf_paged_attn_args_t a, FastDiv by_page) {
-    const int lane = threadIdx.x & 63;
     const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int t = (int)(unit / a.H_q), h = (int)(unit - (int64_t)t * a.H_q);
     if (t >= a.T) return;
@@ -1268,52 +1388,7 @@ void paged_any(cf_paged_attn_args_t a, FastDiv by_page) {
     }
     const SeqRows s = seq_rows(a, lo);
     if (t < s.row0 || t >= s.row0 + s.n) return;
-    const int seen = min(s.len - s.n + (t - s.row0) + 1, s.len);
-    const int32_t* const table = a.table + (size_t)lo * a.max_pages;
-    const T* const q = (const T*)a.q + (int64_t)t * a.q_stride + (int64_t)h * a.d;
-    const T* const k = (const T*)a.k + (int64_t)(h / (a.H_q / a.H_kv)) * a.head_stride;
-    const T* const v = (const T*)a.v + (int64_t)(h / (a.H_q / a.H_kv)) * a.head_stride;
-    const float c = a.scale * kLog2e;
-    float m = -INFINITY, l = 0.0f, acc[kAnyDims];
-#pragma unroll
-    for (int i = 0; i < kAnyDims; i++) acc[i] = 0.0f;
-    for (int k0 = 0; k0 < seen; k0 += 64) {
-        const int key = k0 + lane;
-        int64_t at = 0;
-        float x = -INFINITY;
-        if (key < seen) {
-            const int idx = fastdiv(key, by_page);
-            const int page = table[idx];
-            if ((unsigned)page < (unsigned)a.num_pages) {
-                at = (int64_t)page * a.page_stride + (int64_t)(key - idx * a.page_size) * a.row_stride;
-                float dot = 0.0f;
-                for (int e = 0; e < a.d; e++) dot = __builtin_fmaf((float)q[e], (float)k[at + e], dot);
-                x = dot * c;
-            }
-        }
-        const float m_new = fmaxf(m, wave_max(x));
-        if (m_new == -INFINITY && !__builtin_amdgcn_ballot_w64(x != x)) continue;
-        const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-        const float alpha = exp2f(m - m_use), p = exp2f(x - m_use);
-        m = m_new;
-        l = l * alpha + wave_sum(p);
-#pragma unroll
-        for (int i = 0; i < kAnyDims; i++) acc[i] *= alpha;
-        for (int j = 0; j < min(64, seen - k0); j++) {
-            const float pj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(p), j));
-            if (pj == 0.0f) continue;          // not attended: its V may hold anything
-            const int64_t row = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(at >> 32), j) << 32) |
-                                          (uint32_t)__builtin_amdgcn_readlane((int)at, j));
-#pragma unroll
-            for (int i = 0; i < kAnyDims; i++)
-                if (lane + 64 * i < a.d) acc[i] = __builtin_fmaf(pj, (float)v[row + lane + 64 * i], acc[i]);
-        }
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T* const o = (T*)a.o + ((int64_t)t * a.H_q + h) * a.d;
-#pragma unroll
-    for (int i = 0; i < kAnyDims; i++)
-        if (lane + 64 * i < a.d) o[lane + 64 * i] = (T)(acc[i] * inv);
+    plain_row<T, kAnyDims>(a, by_page, s, lo, t - s.row0, h, a.d);
 }
 
 // The plan of a call on the matrix cores: the kernel and how its work is cut.

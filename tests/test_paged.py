@@ -572,6 +572,98 @@ def test_attention_scales(gpu, f16, scale):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("H,H_kv,d,new,past", [
+    (48, 16, 64, [300, 250, 400, 290], [100, 0, 700, 64]),      # fp16: tiles of 256 rows, not cut
+    (64, 16, 128, [300, 200, 350], [100, 1700, 40]),
+    (128, 64, 64, [384], [2500]),                               # ... and cut
+    (8, 8, 64, [200] * 3 + [1] * 70 + [90], [0, 900, 5000] + [11 * i for i in range(70)] + [2000]),
+])
+def test_attention_wide_tiles(gpu, f16, H, H_kv, d, new, past):
+    c = Paged(new, past, H, H_kv, d, 16, f16, seed=9)
+    c.check(c.run(max_new=max(new)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("new,past", [([1, 1, 1], [5000, 20, 1300]), ([200, 1, 30], [3000, 2500, 10]), ([2] * 40, [1100] * 40)])
+def test_attention_with_hints_that_are_too_small(gpu, f16, new, past):
+    """max_new and max_len choose kernels; what passes them is computed all the same."""
+    for H, H_kv, d in ((8, 2, 128), (16, 16, 64)):
+        c = Paged(new, past, H, H_kv, d, 16, f16, seed=11)
+        for max_new, max_len in ((1, 0), (1, 64), (max(new), 1), (17, 600), (2 ** 40, 2 ** 40)):
+            c.check(c.run(max_new=max_new, max_len=max_len))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("H,H_kv,d,P,new,past", [
+    (8, 2, 64, 16, [12, 2, 8], [100, 30, 0]), (8, 2, 128, 16, [4, 4, 4], [2500, 60, 1500]), (12, 12, 64, 16, [9] * 12, [300] * 12),
+    (8, 4, 128, 32, [150, 40, 90], [33, 0, 200]), (4, 4, 64, 16, [130, 2], [4000, 3000]), (128, 64, 64, 16, [400], [64]),
+    (4, 2, 40, 5, [7, 3], [20, 9]),
+])
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+def test_attention_ignores_what_a_row_does_not_see(gpu, f16, H, H_kv, d, P, new, past, bad):
+    """K and V of one new position of every sequence are infinite or NaN: the rows before it are
+    what they are without, those from it on are not finite in that dim of V."""
+    c = Paged(new, past, H, H_kv, d, P, f16, seed=13)
+    at = [n // 2 for n in new]                      # row of each sequence whose position it is
+    places = [(c.table[b, (past[b] + i) // P], (past[b] + i) % P) for b, i in enumerate(at)]
+    kept = [(c.kp[x].copy(), c.vp[x].copy()) for x in places]
+    for x in places:
+        c.vp[x][:, 3] = bad
+    got = c.run(max_new=max(new))
+    for b, i in enumerate(at):
+        seeing = got[c.start[b] + i:c.start[b + 1], :, 3]
+        assert np.isnan(seeing).all() if np.isnan(bad) else (seeing == np.inf).all()
+    for x in places:
+        c.kp[x] = bad
+    with_k = c.run(max_new=max(new))
+    for x, (k, v) in zip(places, kept):
+        c.kp[x], c.vp[x] = k, v
+    clean = c.run(max_new=max(new))
+    c.check(clean)
+    for o, dims in ((got, np.arange(d) != 3), (with_k, np.zeros(d, bool))):
+        mixed = clean.copy()                        # what cannot be compared is the clean result's
+        for b, i in enumerate(at):
+            rows = slice(c.start[b], c.start[b] + i)
+            mixed[rows] = o[rows]
+            rows = slice(c.start[b] + i, c.start[b + 1])
+            mixed[rows][..., dims] = o[rows][..., dims]
+        c.check(mixed)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("new", [[1] * 3, [60, 1, 200]])
+def test_attention_cut_and_captured(gpu, f16, new):
+    """A captured call whose tiles are cut, replayed at other lengths with eager work in between."""
+    c = Paged(new, [4000, 9, 2500], 16, 4, 128, 16, f16, seed=21)
+    s = cf.Stream()
+    bufs = [dev(x) for x in (c.q, c.kp, c.vp, c.table, c.lens, c.start)]
+    o, full = dev(np.full(c.q.shape, 7.0, c.dt)), c.lens.copy()
+    call = lambda out: cf.call_op(c.op, bufs, [out], c.params(max_new=max(new)), s)
+    assert call(o) == 0
+    s.synchronize()
+    assert gpu.gpu_capture_begin(s.handle) == 0
+    assert call(o) == 0
+    graph = ctypes.c_void_p()
+    assert gpu.gpu_capture_end(s.handle, ctypes.byref(graph)) == 0
+    for drop in (0, 700, 64, 2300, 0):
+        c.lens = np.maximum(full - drop, new).astype(I32)
+        bufs[4].upload(c.lens)
+        assert gpu.gpu_graph_launch(graph, s.handle) == 0
+        s.synchronize()
+        got = o.download()
+        c.check(got)
+        eager = dev(np.full(c.q.shape, 7.0, c.dt))
+        assert call(eager) == 0
+        s.synchronize()
+        assert np.array_equal(eager.download(), got)
+    gpu.gpu_graph_exec_destroy(graph)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f16", [False, True])
 def test_attention_of_a_contiguous_decode_cache(gpu, f16):
     """The cache of MHA_Decode as pages: the same attention as mha_decode_attn."""
     B, H, H_kv, d, cap, P = 5, 32, 8, 128, 512, 32
