@@ -70,7 +70,8 @@ struct PagedPlan {
     int32_t one_blocks;    // tiles of up to this many blocks are not cut
     int32_t step;          // of the unit loop
     int32_t merge_groups;  // workgroups that share the rows of a tile's merge
-    FastDiv by_page, by_group;
+    int32_t G;             // query heads per KV head
+    FastDiv by_page, by_group, by_kv;
 };
 
 // A unit's tile and range, or the tile to merge.
@@ -85,27 +86,27 @@ template <int TM, int BK, int NARROW>
 struct Geometry {
     const cf_paged_attn_args_t& a;
     const PagedPlan& pl;
-    int G, lane, C, one;                 // C: most blocks of a range; one: tiles up to it are not cut
+    int lane, one;                       // tiles of up to `one` blocks are not cut
+    float C, inv_C;                      // most blocks of a range
     SeqRows first;                       // lane: sequence `lane`, kept for the second pass,
     int* kept;                           // by wide tiles in LDS: their registers are all taken
 
     __device__ __forceinline__ SeqRows rows(int b) const { return b < a.B ? seq_rows(a, b) : SeqRows{0, 0, 0}; }
-    __device__ __forceinline__ int tiles(const SeqRows& s) const { return (int)(((int64_t)s.n * G + TM - 1) / TM); }
+    __device__ __forceinline__ int tiles(const SeqRows& s) const { return (int)(((int64_t)s.n * pl.G + TM - 1) / TM); }
     __device__ __forceinline__ int blocks(const SeqRows& s) const { return (s.len + BK - 1) / BK; }
-    __device__ __forceinline__ bool narrow(const SeqRows& s) const { return NARROW > 1 && s.n * G <= 16; }
+    __device__ __forceinline__ bool narrow(const SeqRows& s) const { return NARROW > 1 && s.n * pl.G <= 16; }
     __device__ __forceinline__ float cost(const SeqRows& s) const {
         const float w = (float)tiles(s) * (float)blocks(s);
         return narrow(s) ? w * (1.0f / NARROW) : w;
     }
     __device__ __forceinline__ int ranges(const SeqRows& s) const {
-        const int n = blocks(s), c = narrow(s) ? NARROW * C : C;
-        return n <= one ? 1 : (n + c - 1) / c;
+        const int n = blocks(s);
+        return n <= one ? 1 : (int)((float)(n - 1) * (narrow(s) ? inv_C * (1.0f / NARROW) : inv_C)) + 1;
     }
 
     __device__ __forceinline__ Geometry(const cf_paged_attn_args_t& a_, const PagedPlan& pl_, int* kept_ = nullptr)
         : a(a_), pl(pl_), kept(kept_) {
         lane = threadIdx.x & 63;
-        G = a.H_q / a.H_kv;
         first = rows(lane);
         if constexpr (NARROW > 1) {          // every wave writes the same
             kept[lane] = first.row0;
@@ -128,7 +129,8 @@ struct Geometry {
         // busy or more it pays for long ranges only.
         const bool few = NARROW > 1 && t <= 0.25f * fill;
         one = __builtin_amdgcn_readfirstlane(few ? min(pl.one_blocks, 512 / BK) : pl.one_blocks);
-        C = __builtin_amdgcn_readfirstlane((int)fminf(fmaxf(w, (float)(few ? 4 : pl.min_blocks)), 1e8f));
+        C = fmaxf(w, (float)(few ? 4 : pl.min_blocks));
+        inv_C = 1.0f / C;
         if (pl.one_blocks == INT32_MAX) one = INT32_MAX;
     }
     // The number of cut tiles, for the merge: most of its workgroups need know no more.
@@ -155,17 +157,18 @@ struct Geometry {
                 const SeqRows s = base > 0 ? rows(base + lane)
                                 : NARROW > 1 ? SeqRows{kept[lane], kept[64 + lane], kept[128 + lane]} : first;
                 const int t = tiles(s), ns = ranges(s), rec = ns > 1 ? t * ns : 0;
+                const bool cut = __builtin_amdgcn_ballot_w64(ns > 1) != 0;
                 int items = MERGE ? (ns > 1 ? t : 0) : t * ns;
-                if (CLASSES > 1 && (2 * blocks(s) > C * ns ? 0 : 1) != cls) items = 0;
+                if (CLASSES > 1 && (2.0f * (float)blocks(s) > C * (float)ns ? 0 : 1) != cls) items = 0;
                 const int before = items0 + wave_excl_sum(items, lane);
-                const int rec_before = records0 + wave_excl_sum(rec, lane);
+                const int rec_before = records0 + (cut ? wave_excl_sum(rec, lane) : 0);
                 const unsigned long long hit = __ballot(before <= u && u < before + items);
                 if (hit) {
                     const int src = __builtin_ctzll(hit);
                     const int at = u - __builtin_amdgcn_readlane(before, src);
                     out.n_ranges = __builtin_amdgcn_readlane(ns, src);
                     const int nt = __builtin_amdgcn_readlane(t, src);
-                    const int i = MERGE ? at : at / out.n_ranges;
+                    const int i = MERGE || out.n_ranges == 1 ? at : at / out.n_ranges;
                     out.range = MERGE ? 0 : at - i * out.n_ranges;
                     out.tile = nt - 1 - i;                     // the longest first
                     out.record = __builtin_amdgcn_readlane(rec_before, src) + out.tile * out.n_ranges;
@@ -191,13 +194,12 @@ struct Work {
 template <int TM, int BK>
 __device__ __forceinline__ Work unit_work(const cf_paged_attn_args_t& a, const PagedPlan& pl, const Unit& un) {
     Work w;
-    const int G = a.H_q / a.H_kv;
     w.R0 = un.tile * TM;
-    w.n_rows = min(un.s.n * G - w.R0, TM);
+    w.n_rows = min(un.s.n * pl.G - w.R0, TM);
     w.base = un.s.len - un.s.n + 1;
     const int limit = min(max(w.base + fastdiv(w.R0 + w.n_rows - 1, pl.by_group), 0), un.s.len);
     const int blocks = (limit + BK - 1) / BK;
-    const int per = (blocks + un.n_ranges - 1) / un.n_ranges;
+    const int per = un.n_ranges == 1 ? blocks : (blocks + un.n_ranges - 1) / un.n_ranges;
     const int b0 = min(un.range * per, blocks), b1 = min(b0 + per, blocks);
     w.key0 = b0 * BK;
     w.key1 = min(b1 * BK, limit);
@@ -224,20 +226,6 @@ __device__ __forceinline__ void store4(T* p, f4_t x) {
     *(four_t*)p = four_t{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
 }
 
-// Table entries for the next 64 pieces of a range, one per lane: piece i starts at position
-// key0 + i * step.  A load a piece would be in the way: an ordinary one's wait drains the ring,
-// and one through the scalar cache makes the waits for LDS reads wait for it.  load() drains
-// the ring once per 64 pieces.
-struct Pages {
-    const int32_t* table;
-    int v;                   // lane: entry of piece base + lane
-    __device__ __forceinline__ void load(const cf_paged_attn_args_t& a, const PagedPlan& pl, int base, int key0, int step) {
-        const int key = min(key0 + (base + (int)(threadIdx.x & 63)) * step, a.max_pages * a.page_size - 1);
-        v = table[fastdiv(key, pl.by_page)];
-        asm volatile("" : "+v"(v));   // it has arrived
-    }
-    __device__ __forceinline__ int page(int i) const { return __builtin_amdgcn_readlane(v, i & 63); }
-};
 // One entry through the scalar cache.
 typedef const int32_t __attribute__((address_space(4)))* table_t;
 __device__ __forceinline__ table_t table_of(const cf_paged_attn_args_t& a, int b) {
@@ -255,6 +243,40 @@ __device__ __forceinline__ Group group_of(const cf_paged_attn_args_t& a, const P
     const int in_page = key - fastdiv(key, pl.by_page) * a.page_size;
     return {(int64_t)(valid ? page : 0) * a.page_stride + (int64_t)in_page * a.row_stride, (1u << count) - 1u};
 }
+
+// The next 64 groups of a range, one per lane.  A load of a table entry per group would be in
+// the way: an ordinary one's wait drains the ring, and one through the scalar cache makes the
+// waits for LDS reads wait for it; and a group's place takes some 40 scalar instructions.
+// load() drains the ring once per 64 groups.
+struct Groups {
+    const int32_t* table;
+    int lo, hi, mask;        // lane: Group of base + lane
+    uint64_t whole;          // bit: all 16 positions of it count
+    __device__ __forceinline__ void load(const cf_paged_attn_args_t& a, const PagedPlan& pl, int base, int key0, int key1) {
+        const int key = key0 + (base + (int)(threadIdx.x & 63)) * 16;
+        const Group g = group_of(a, pl, table[fastdiv(min(key, a.max_pages * a.page_size - 1), pl.by_page)], key, key1);
+        lo = (int)g.at;
+        hi = (int)(g.at >> 32);
+        mask = (int)g.mask;
+        asm volatile("" : "+v"(lo), "+v"(hi), "+v"(mask));    // they have arrived
+        whole = __builtin_amdgcn_ballot_w64(mask == 0xffff);
+    }
+    __device__ __forceinline__ int64_t at(int i) const {
+        return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i & 63) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane(lo, i & 63));
+    }
+    // Positions of groups i .. i + N - 1 that count (i a multiple of N).
+    template <int N>
+    __device__ __forceinline__ uint64_t masks(int i) const {
+        constexpr uint64_t all = N == 4 ? ~0ull : (1ull << (16 * N & 63)) - 1;
+        if ((~(whole >> (i & 63)) & ((1u << N) - 1)) == 0) return all;
+        uint64_t mk = 0;
+#pragma unroll
+        for (int g = 0; g < N; g++)
+            mk |= (uint64_t)(uint32_t)__builtin_amdgcn_readlane(mask, (i + g) & 63) << (16 * g);
+        return mk;
+    }
+};
 
 // LDS rows are swizzled in 16-byte chunks: K (and Q) rows are read 16 rows at one chunk, V
 // rows transposed (fp16, ds_read_b64_tr_b16) or 4 rows of 16 floats (fp32).
@@ -327,7 +349,7 @@ __device__ __forceinline__ void plain_row(const cf_paged_attn_args_t& a, FastDiv
 // one: such a row is computed again, where only what it sees is touched.
 template <typename T, int D>
 __device__ __forceinline__ void redo_row(const cf_paged_attn_args_t& a, const PagedPlan& pl, const Unit& un, int kvh, int R) {
-    const int G = a.H_q / a.H_kv, tok = fastdiv(R, pl.by_group);
+    const int G = pl.G, tok = fastdiv(R, pl.by_group);
     plain_row<T, D / 64>(a, pl.by_page, un.s, un.b, tok, kvh * G + (R - tok * G), D);
 }
 template <int N>
@@ -345,6 +367,15 @@ __device__ __forceinline__ uint32_t rows_of_16(bool bad) {
     return (x | x >> 16) & 0xffffu;
 }
 
+// The lane, as a unit's code sees it: what is worked out from it stays inside the unit.  Taken
+// out of the loop over units, all kernels' offsets would be held at once, and wide tiles have
+// no registers for that.
+__device__ __forceinline__ int unit_lane() {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
 // How rows of D elements lie in LDS and in lanes.
 template <typename T, int D> struct Rows {
     static constexpr bool F16 = sizeof(T) == 2;
@@ -358,20 +389,20 @@ template <typename T, int D> struct Rows {
     typedef T chunk_t __attribute__((ext_vector_type(CE)));
     // DMA: lane L of instruction u writes physical chunk L % CPR of row RPI u + L / CPR of a
     // 16-row group, which holds logical chunk (L % CPR) ^ swizzle.
-    static __device__ __forceinline__ int drow() { return (threadIdx.x & 63) / CPR; }
-    static __device__ __forceinline__ int dch() { return (threadIdx.x & 63) % CPR; }
+    static __device__ __forceinline__ int drow(int lane) { return lane / CPR; }
+    static __device__ __forceinline__ int dch(int lane) { return lane % CPR; }
     // LDS read offsets (elements) of the lane's K chunks inside 16 rows: fp16 lane (lr, lq)
     // takes row lr, dims 32 f + 8 lq .. + 7; fp32 dims D / 4 lq + 4 f .. + 3 (k-slot lq of MFMA
     // step s is dim D / 4 lq + s).
-    static __device__ __forceinline__ void k_offsets(int (&rd)[NF]) {
-        const int lr = threadIdx.x & 15, lq = (threadIdx.x >> 4) & 3;
+    static __device__ __forceinline__ void k_offsets(int (&rd)[NF], int lane) {
+        const int lr = lane & 15, lq = lane >> 4;
 #pragma unroll
         for (int f = 0; f < NF; f++) rd[f] = lr * D + CE * ((F16 ? 4 * f + lq : NF * lq + f) ^ kswz<T, D>(lr));
     }
     // ... of its V: fp16 (ds_read_tr4) key 4 lq + lr / 4, dims 16 u + 4 (lr % 4) .. + 3; fp32 row
     // 4 lq + kk, whose chunk the read adds.
-    static __device__ __forceinline__ void v_offsets(int (&rd)[VR]) {
-        const int lr = threadIdx.x & 15, lq = (threadIdx.x >> 4) & 3;
+    static __device__ __forceinline__ void v_offsets(int (&rd)[VR], int lane) {
+        const int lr = lane & 15, lq = lane >> 4;
 #pragma unroll
         for (int u = 0; u < VR; u++) {
             if constexpr (F16) {
@@ -383,8 +414,8 @@ template <typename T, int D> struct Rows {
         }
     }
     // fp32: V of key 16 t + 4 lq + kk, dim 16 u + lr (base: the stage's V).
-    static __device__ __forceinline__ float v_at(const float* base, const int (&rd)[VR], int t, int kk, int u) {
-        const int lr = threadIdx.x & 15, lq = (threadIdx.x >> 4) & 3;
+    static __device__ __forceinline__ float v_at(const float* base, const int (&rd)[VR], int lane, int t, int kk, int u) {
+        const int lr = lane & 15, lq = lane >> 4;
         return base[rd[kk] + 16 * t * D + 4 * ((4 * u + (lr >> 2)) ^ vswz<T, D>(4 * lq + kk))];
     }
 };
@@ -404,9 +435,9 @@ __device__ __forceinline__ bool move_max(float mloc, float& m, float& alpha) {
 // set and it is one of the first `seen`.  Bit by bit in vector registers: comparisons would
 // take a pair of scalar registers per score.
 template <int NG>
-__device__ __forceinline__ void hide(f4_t (&sc)[NG], uint64_t mk, int seen) {
+__device__ __forceinline__ void hide(f4_t (&sc)[NG], uint64_t mk, int seen, int lane) {
     const uint64_t low = seen <= 0 ? 0 : seen >= 64 ? ~0ull : (1ull << seen) - 1;
-    const uint64_t bits = (mk & low) >> (4 * ((threadIdx.x >> 4) & 3));
+    const uint64_t bits = (mk & low) >> (4 * (lane >> 4));
 #pragma unroll
     for (int t = 0; t < NG; t++)
 #pragma unroll
@@ -437,9 +468,9 @@ __device__ __forceinline__ void narrow_range(const cf_paged_attn_args_t& a, cons
     constexpr int NG = BK / 16, NS = N::NS, TILE = N::TILE, NI = R::NI, NL = 2 * NG * NI, UT = R::UT, CE = R::CE;
     constexpr uint64_t FULL = (1ull << BK) - 1;
     static_assert(NS * NL < 64, "vmcnt range");
-    const int lane = threadIdx.x & 63, lr = lane & 15;
-    const int G = a.H_q / a.H_kv;
-    const int drow = R::drow(), dch = R::dch();
+    const int lane = unit_lane(), lr = lane & 15;
+    const int G = pl.G;
+    const int drow = R::drow(lane), dch = R::dch(lane);
 #pragma unroll
     for (int u = 0; u < UT; u++) acc[u] = f4_t{0.f, 0.f, 0.f, 0.f};
     m_run = -INFINITY;
@@ -458,31 +489,29 @@ __device__ __forceinline__ void narrow_range(const cf_paged_attn_args_t& a, cons
         voff[u] = ((uint32_t)row * (uint32_t)a.row_stride + CE * (dch ^ vswz<T, D>(row))) * (uint32_t)sizeof(T);
     }
     int k_rd[R::NF], v_rd[R::VR];
-    R::k_offsets(k_rd);
-    R::v_offsets(v_rd);
+    R::k_offsets(k_rd, lane);
+    R::v_offsets(v_rd, lane);
     const uint32_t ring_base = __builtin_amdgcn_readfirstlane(lds_offset(ring));
     const T* const kp = (const T*)a.k + (int64_t)kvh * a.head_stride;
     const T* const vp = (const T*)a.v + (int64_t)kvh * a.head_stride;
-    Pages pages = {a.table + (size_t)b * a.max_pages, 0};
-    pages.load(a, pl, 0, key0, 16);
+    Groups groups = {a.table + (size_t)b * a.max_pages, 0, 0, 0, 0};
+    groups.load(a, pl, 0, key0, key1);
 
     uint64_t mask[NS];                                        // per stage: positions that count
     auto issue = [&](int blk, auto stage_c) {
         constexpr int stage = decltype(stage_c)::value;
-        uint64_t mk = 0;
-        if (blk > 0 && blk % (64 / NG) == 0) pages.load(a, pl, blk * NG, key0, 16);
+        if (blk > 0 && blk % (64 / NG) == 0) groups.load(a, pl, blk * NG, key0, key1);
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            const Group gr = group_of(a, pl, pages.page(blk * NG + g), key0 + blk * BK + 16 * g, key1);
-            mk |= (uint64_t)gr.mask << (16 * g);
+            const int64_t at = groups.at(blk * NG + g);
             const uint32_t lds = ring_base + (uint32_t)((stage * 2 * TILE + 16 * g * D) * sizeof(T));
 #pragma unroll
             for (int u = 0; u < NI; u++) {
-                lds_dma16_s(koff[u], kp + gr.at, lds + u * 1024u);
-                lds_dma16_s(voff[u], vp + gr.at, lds + (uint32_t)(TILE * sizeof(T)) + u * 1024u);
+                lds_dma16_s(koff[u], kp + at, lds + u * 1024u);
+                lds_dma16_s(voff[u], vp + at, lds + (uint32_t)(TILE * sizeof(T)) + u * 1024u);
             }
         }
-        mask[stage] = mk;
+        mask[stage] = groups.template masks<NG>(blk * NG);
     };
 
     wait_lds_reads();                                         // what the ring held before
@@ -541,7 +570,7 @@ __device__ __forceinline__ void narrow_range(const cf_paged_attn_args_t& a, cons
             }
         }
         if (mk != FULL || k0 + BK > seen_all) {
-            hide(sc, mk, seen - k0);
+            hide(sc, mk, seen - k0, lane);
         }
         float mloc = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
 #pragma unroll
@@ -596,7 +625,7 @@ __device__ __forceinline__ void narrow_range(const cf_paged_attn_args_t& a, cons
                 for (int kk = 0; kk < 4; kk++)
 #pragma unroll
                     for (int u = 0; u < UT; u++)
-                        acc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::v_at((const float*)st + TILE, v_rd, t, kk, u),
+                        acc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::v_at((const float*)st + TILE, v_rd, lane, t, kk, u),
                                                                       sc[t][kk], acc[u], 0, 0, 0);
         }
     };
@@ -615,16 +644,16 @@ __global__ __launch_bounds__(256, (Heads<T, D>::PER_CU))
 void paged_heads(cf_paged_attn_args_t a, PagedPlan pl) {
     using H = Heads<T, D>;
     __shared__ __attribute__((aligned(16))) T ring_all[H::WAVES * H::RING];
-    const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int G = a.H_q / a.H_kv;
+    const int G = pl.G;
     const Geometry<16, H::BK, 1> geo(a, pl);
     geo.leave_cut_tiles();
     for (int unit = (int)blockIdx.x * H::WAVES + wave;; unit += pl.step) {
-        const int id = unit / a.H_kv, kvh = unit - id * a.H_kv;
+        const int id = fastdiv(unit, pl.by_kv), kvh = unit - id * a.H_kv;
         Unit un;
         if (!geo.template find<false>(id, un)) break;
         const Work w = unit_work<16, H::BK>(a, pl, un);
+        const int lane = unit_lane(), lr = lane & 15, lq = lane >> 4;
         f4_t acc[D / 16];
         float m, l;
         narrow_range<T, D, H::BK>(a, pl, ring_all + wave * H::RING, un.s, un.b, kvh, w, w.key0, w.key1, acc, m, l);
@@ -659,7 +688,7 @@ __device__ __forceinline__ bool narrow_unit(const cf_paged_attn_args_t& a, const
                                             int kvh, const Work& w) {
     constexpr int RING = Narrow<T, D, 16>::RING, LD = D + 4;
     static_assert(16 * (LD + 2) * 4 <= RING * (int)sizeof(T), "a wave's rows fit its ring");
-    const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
+    const int lane = unit_lane(), lr = lane & 15, lq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     T* const ring = lds + wave * RING;
     const int groups = w.key1 > w.key0 ? (w.key1 - w.key0 + 15) / 16 : 0;
@@ -704,7 +733,7 @@ __device__ __forceinline__ bool narrow_unit(const cf_paged_attn_args_t& a, const
         } else {
             const f4_t one[1] = {sum};
             again |= spoilt(one, L);
-            const RowAt at = row_at(pl, a.H_q / a.H_kv, kvh, w.R0 + row);
+            const RowAt at = row_at(pl, pl.G, kvh, w.R0 + row);
             store4((T*)a.o + ((int64_t)(un.s.row0 + at.tok) * a.H_q + at.h) * D + 4 * d4,
                    sum * (L == 0.0f ? 0.0f : 1.0f / L));
         }
@@ -734,7 +763,7 @@ void paged_split(cf_paged_attn_args_t a, PagedPlan pl) {
     const Geometry<16, 64, 1> geo(a, pl);
     geo.leave_cut_tiles();
     for (int unit = (int)blockIdx.x;; unit += pl.step) {
-        const int id = unit / a.H_kv, kvh = unit - id * a.H_kv;
+        const int id = fastdiv(unit, pl.by_kv), kvh = unit - id * a.H_kv;
         Unit un;
         if (!geo.template find<false>(id, un)) break;
         const Work w = unit_work<16, 64>(a, pl, un);
@@ -759,7 +788,7 @@ __device__ __forceinline__ RowOut row_out(const cf_paged_attn_args_t& a, const P
         }
         return {rec + 2 * TM + row * D, nullptr, 1.0f};
     }
-    const RowAt at = row_at(pl, a.H_q / a.H_kv, kvh, w.R0 + row);
+    const RowAt at = row_at(pl, pl.G, kvh, w.R0 + row);
     return {nullptr, (T*)a.o + ((int64_t)(un.s.row0 + at.tok) * a.H_q + at.h) * D, l == 0.0f ? 0.0f : 1.0f / l};
 }
 template <typename T>
@@ -797,9 +826,9 @@ __device__ __forceinline__ uint32_t wide16_unit(const cf_paged_attn_args_t& a, c
     constexpr int HI = R::NI / 2;                            // DMA instructions per 8 rows
     constexpr int NL = 2 * HI;                               // ... of a wave per stage
     static_assert(R::RPI <= 8 && (NS - 1) * NL < 64, "eight rows per wave");
-    const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
+    const int lane = unit_lane(), lr = lane & 15, lq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int G = a.H_q / a.H_kv, drow = R::drow(), dch = R::dch();
+    const int G = pl.G, drow = R::drow(lane), dch = R::dch(lane);
     const float c = a.scale * kLog2e;
     const int wrow = 16 * NJ * wave;
     const bool active = wrow < w.n_rows;
@@ -828,8 +857,8 @@ __device__ __forceinline__ uint32_t wide16_unit(const cf_paged_attn_args_t& a, c
             voff[u] = ((uint32_t)row * (uint32_t)a.row_stride + 8 * (dch ^ vswz<T, D>(row))) * 2u;
         }
         int k_rd[NF], v_rd[UT];
-        R::k_offsets(k_rd);
-        R::v_offsets(v_rd);
+        R::k_offsets(k_rd, lane);
+        R::v_offsets(v_rd, lane);
         const uint32_t lds_base = __builtin_amdgcn_readfirstlane(lds_offset(lds));
         const uint32_t my_lds = lds_base + (uint32_t)((16 * grp + 8 * half) * D * 2);
         const table_t table = table_of(a, un.b);
@@ -969,7 +998,7 @@ __device__ __forceinline__ uint32_t wide16_unit(const cf_paged_attn_args_t& a, c
             const bool edge = mk != ~0ull || k0 + BK > seen_all;
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
-                if (edge) hide(sc[j], mk, seen[j] - k0);
+                if (edge) hide(sc[j], mk, seen[j] - k0, lane);
                 // Chains of three-input maxima.
                 float mloc = fmaxf(fmaxf(sc[j][0][0], sc[j][0][1]), sc[j][0][2]);
 #pragma unroll
@@ -1077,7 +1106,7 @@ void paged_wide16(cf_paged_attn_args_t a, PagedPlan pl) {
     const Geometry<W::TM, 64, kNarrowCost> geo(a, pl, kept);
     geo.leave_cut_tiles();
     for (int unit = (int)blockIdx.x;; unit += pl.step) {
-        const int id = unit / a.H_kv, kvh = unit - id * a.H_kv;
+        const int id = fastdiv(unit, pl.by_kv), kvh = unit - id * a.H_kv;
         Unit un;
         if (!geo.template find<false>(id, un)) break;
         Work w = unit_work<W::TM, 64>(a, pl, un);
@@ -1108,9 +1137,9 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
     using W = Wide32<D>;
     constexpr int BK = W::BK, NS = W::NS, TILE = W::TILE, NI = R::NI, NL = 2 * NI, UT = R::UT, NF = R::NF;
     static_assert(NS * NL < 64, "vmcnt range");
-    const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
+    const int lane = unit_lane(), lr = lane & 15, lq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int G = a.H_q / a.H_kv, drow = R::drow(), dch = R::dch();
+    const int G = pl.G, drow = R::drow(lane), dch = R::dch(lane);
     const float c = a.scale * kLog2e;
     const int wrow = 16 * wave;
     const bool active = wrow < w.n_rows;
@@ -1130,32 +1159,25 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
             voff[u] = ((uint32_t)row * (uint32_t)a.row_stride + 4 * (dch ^ vswz<T, D>(row))) * 4u;
         }
         int k_rd[NF], v_rd[R::VR];
-        R::k_offsets(k_rd);
-        R::v_offsets(v_rd);
+        R::k_offsets(k_rd, lane);
+        R::v_offsets(v_rd, lane);
         const uint32_t ring_base = __builtin_amdgcn_readfirstlane(lds_offset(ring));
         const T* const kp = (const T*)a.k + (int64_t)kvh * a.head_stride;
         const T* const vp = (const T*)a.v + (int64_t)kvh * a.head_stride;
-        Pages pages = {a.table + (size_t)un.b * a.max_pages, 0};
-        pages.load(a, pl, 0, w.key0, 16);
+        Groups groups = {a.table + (size_t)un.b * a.max_pages, 0, 0, 0, 0};
+        groups.load(a, pl, 0, w.key0, w.key1);
         uint64_t mask[NS];
         auto issue = [&](int i, auto stage_c) {               // wave w: group w of K and V
             constexpr int stage = decltype(stage_c)::value;
-            uint64_t mk = 0;
-            int64_t at = 0;
-            if (i > 0 && i % 16 == 0) pages.load(a, pl, 4 * i, w.key0, 16);
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const Group gr = group_of(a, pl, pages.page(4 * i + g), w.key0 + i * BK + 16 * g, w.key1);
-                mk |= (uint64_t)gr.mask << (16 * g);
-                if (g == wave) at = gr.at;
-            }
+            if (i > 0 && i % 16 == 0) groups.load(a, pl, 4 * i, w.key0, w.key1);
+            const int64_t at = groups.at(4 * i + wave);
             const uint32_t to = ring_base + (uint32_t)((stage * 2 * TILE + wrow * D) * 4);
 #pragma unroll
             for (int u = 0; u < NI; u++) {
                 lds_dma16_s(koff[u], kp + at, to + u * 1024u);
                 lds_dma16_s(voff[u], vp + at, to + (uint32_t)(TILE * 4) + u * 1024u);
             }
-            mask[stage] = mk;
+            mask[stage] = groups.template masks<4>(4 * i);
         };
         {
             const uint32_t qlds = ring_base + (uint32_t)(((NS - 1) * 2 * TILE + wrow * D) * 4);
@@ -1208,7 +1230,7 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
                 __builtin_amdgcn_sched_barrier(0);
             });
             if (mk != ~0ull || k0 + BK > seen_all) {
-                hide(sc, mk, seen - k0);
+                hide(sc, mk, seen - k0, lane);
             }
             float mloc = sc[0][0];
 #pragma unroll
@@ -1233,7 +1255,7 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
             auto read_v = [&](auto g_c) {
                 constexpr int g = decltype(g_c)::value;
 #pragma unroll
-                for (int u = 0; u < UT; u++) vf[g % 2][u] = R::v_at(st + TILE, v_rd, g / 4, g % 4, u);
+                for (int u = 0; u < UT; u++) vf[g % 2][u] = R::v_at(st + TILE, v_rd, lane, g / 4, g % 4, u);
             };
             read_v(std::integral_constant<int, 0>{});
             static_for<16>([&](auto g_c) {
@@ -1267,7 +1289,7 @@ void paged_wide32(cf_paged_attn_args_t a, PagedPlan pl) {
     const Geometry<W::TM, 64, kNarrowCost> geo(a, pl, kept);
     geo.leave_cut_tiles();
     for (int unit = (int)blockIdx.x;; unit += pl.step) {
-        const int id = unit / a.H_kv, kvh = unit - id * a.H_kv;
+        const int id = fastdiv(unit, pl.by_kv), kvh = unit - id * a.H_kv;
         Unit un;
         if (!geo.template find<false>(id, un)) break;
         const Work w = unit_work<W::TM, 64>(a, pl, un);
@@ -1290,11 +1312,11 @@ void paged_merge(cf_paged_attn_args_t a, PagedPlan pl) {
     if ((int)blockIdx.x >= cut_units) return;
     __shared__ int kept[NARROW > 1 ? 3 * 64 : 1];
     const Geometry<TM, BK, NARROW> geo(a, pl, kept);
-    const int G = a.H_q / a.H_kv;
+    const int G = pl.G;
     const int d4 = threadIdx.x % DL, sub = threadIdx.x / DL % SUBS, r = threadIdx.x / (DL * SUBS);
     for (int unit = blockIdx.x; unit < cut_units; unit += gridDim.x) {
         const int th = unit / pl.merge_groups, group = unit - th * pl.merge_groups;
-        const int tile_id = th / a.H_kv, kvh = th - tile_id * a.H_kv;
+        const int tile_id = fastdiv(th, pl.by_kv), kvh = th - tile_id * a.H_kv;
         Unit un;
         if (!geo.template find<true>(tile_id, un)) break;
         const int n_rows = min(un.s.n * G - un.tile * TM, TM);
@@ -1457,7 +1479,9 @@ Plan make_plan(const cf_paged_attn_args_t& a) {
     const int64_t merge_wgs = (tiles < 2 * fill ? tiles : 2 * fill) * a.H_kv * p.pl.merge_groups;
     p.merge_wgs = !cut ? 0 : merge_wgs > 4096 ? 4096 : (int)merge_wgs;
     p.pl.by_page = fastdiv_make(a.page_size);
+    p.pl.G = (int32_t)G;
     p.pl.by_group = fastdiv_make((int)G);
+    p.pl.by_kv = fastdiv_make(a.H_kv);
     p.pl.cut_tiles = nullptr;
     p.pl.records = nullptr;
     return p;
