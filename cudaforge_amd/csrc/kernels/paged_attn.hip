@@ -683,13 +683,18 @@ void paged_heads(cf_paged_attn_args_t a, PagedPlan pl) {
 // Up to 16 rows by all waves of a workgroup: each takes a share of the unit's positions, and
 // they join their m, l and sums in LDS (WAVES rings at `lds`, one each).  True where rows that
 // this wave finished have to be computed again.
-template <typename T, int D, int TM, int WAVES>
+template <typename T, int D, int TM, int WAVES, int ALL = WAVES>
 __device__ __forceinline__ bool narrow_unit(const cf_paged_attn_args_t& a, const PagedPlan& pl, T* lds, const Unit& un,
                                             int kvh, const Work& w) {
     constexpr int RING = Narrow<T, D, 16>::RING, LD = D + 4;
     static_assert(16 * (LD + 2) * 4 <= RING * (int)sizeof(T), "a wave's rows fit its ring");
     const int lane = unit_lane(), lr = lane & 15, lq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    if (ALL > WAVES && wave >= WAVES) {                       // whose rings the LDS has no room for
+        __syncthreads();
+        __syncthreads();
+        return false;
+    }
     T* const ring = lds + wave * RING;
     const int groups = w.key1 > w.key0 ? (w.key1 - w.key0 + 15) / 16 : 0;
     const int per = (groups + WAVES - 1) / WAVES * 16;
@@ -1123,11 +1128,18 @@ void paged_wide16(cf_paged_attn_args_t a, PagedPlan pl) {
     }
 }
 
-// ---- fp32, wide tiles: 4 waves of 16 rows, the fp32 MFMA (32 clk each, 128 or 256 of them per
-// 64 positions) bounds it and nothing need be interleaved. ----
+// ---- fp32, wide tiles: 4 waves of 16 rows, or (d = 128) 8, which share the positions too. ----
+// The fp32 MFMA (32 clk, 128 or 256 of them per 64 positions and 16 rows) bounds it; the rest of
+// a block (its loads, 64 KB through the L1 in 1000 clk with d = 128, and softmax) has to run
+// beside another wave's products.  d = 64: that of a second workgroup of the CU.  d = 128, whose
+// ring takes the LDS: waves w and w + 4 of a SIMD have the same rows and half of every block's
+// positions each, and join their sums in LDS at the end; w goes first, so that one is in its
+// softmax while the other is in its products (200 rows of 32 heads over 1200: 58 us, with 4
+// waves 63; d = 64 with 8 waves: 1 us more a unit, and no faster a block).
 template <int D> struct Wide32 {
     static constexpr int TM = 64, BK = 64, NS = 2, TILE = BK * D, LDS = NS * 2 * TILE;   // 64 or 128 KB
-    static constexpr int PER_CU = D == 64 ? 2 : 1;
+    static constexpr int KS = D == 128 ? 2 : 1;              // waves that share a row's positions
+    static constexpr int WAVES = 4 * KS, PER_CU = D == 64 ? 2 : 1;
 };
 template <int D>
 __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const PagedPlan& pl, float* ring, const Unit& un,
@@ -1135,13 +1147,14 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
     using T = float;
     using R = Rows<T, D>;
     using W = Wide32<D>;
-    constexpr int BK = W::BK, NS = W::NS, TILE = W::TILE, NI = R::NI, NL = 2 * NI, UT = R::UT, NF = R::NF;
+    constexpr int BK = W::BK, NS = W::NS, TILE = W::TILE, NI = R::NI, HI = NI / W::KS, NL = 2 * HI, UT = R::UT, NF = R::NF;
+    constexpr int NT = 4 / W::KS;                            // tiles of 16 positions of a wave
     static_assert(NS * NL < 64, "vmcnt range");
     const int lane = unit_lane(), lr = lane & 15, lq = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), share = wave >> 2;
     const int G = pl.G, drow = R::drow(lane), dch = R::dch(lane);
     const float c = a.scale * kLog2e;
-    const int wrow = 16 * wave;
+    const int wrow = 16 * (wave & 3);
     const bool active = wrow < w.n_rows;
     const int n = w.key1 > w.key0 ? (w.key1 - w.key0 + BK - 1) / BK : 0;
     const int seen = min(w.base + fastdiv(w.R0 + min(wrow + lr, w.n_rows - 1), pl.by_group), un.s.len);
@@ -1151,10 +1164,12 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
 #pragma unroll
     for (int u = 0; u < UT; u++) acc[u] = f4_t{0.f, 0.f, 0.f, 0.f};
     if (n > 0) {
-        uint32_t koff[NI], voff[NI];
+        // This wave loads 16 / KS rows of a block: `first` and on of group `grp`.
+        const int grp = wave / W::KS, first = 16 / W::KS * (wave % W::KS);
+        uint32_t koff[HI], voff[HI];
 #pragma unroll
-        for (int u = 0; u < NI; u++) {
-            const int row = R::RPI * u + drow;
+        for (int u = 0; u < HI; u++) {
+            const int row = first + R::RPI * u + drow;
             koff[u] = ((uint32_t)row * (uint32_t)a.row_stride + 4 * (dch ^ kswz<T, D>(row))) * 4u;
             voff[u] = ((uint32_t)row * (uint32_t)a.row_stride + 4 * (dch ^ vswz<T, D>(row))) * 4u;
         }
@@ -1167,19 +1182,20 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
         Groups groups = {a.table + (size_t)un.b * a.max_pages, 0, 0, 0, 0};
         groups.load(a, pl, 0, w.key0, w.key1);
         uint64_t mask[NS];
-        auto issue = [&](int i, auto stage_c) {               // wave w: group w of K and V
+        auto issue = [&](int i, auto stage_c) {
             constexpr int stage = decltype(stage_c)::value;
             if (i > 0 && i % 16 == 0) groups.load(a, pl, 4 * i, w.key0, w.key1);
-            const int64_t at = groups.at(4 * i + wave);
-            const uint32_t to = ring_base + (uint32_t)((stage * 2 * TILE + wrow * D) * 4);
+            const int64_t at = groups.at(4 * i + grp);
+            const uint32_t to = ring_base + (uint32_t)((stage * 2 * TILE + (16 * grp + first) * D) * 4);
 #pragma unroll
-            for (int u = 0; u < NI; u++) {
+            for (int u = 0; u < HI; u++) {
                 lds_dma16_s(koff[u], kp + at, to + u * 1024u);
                 lds_dma16_s(voff[u], vp + at, to + (uint32_t)(TILE * 4) + u * 1024u);
             }
             mask[stage] = groups.template masks<4>(4 * i);
         };
         {
+            // (Waves that share rows bring them to the same place.)
             const uint32_t qlds = ring_base + (uint32_t)(((NS - 1) * 2 * TILE + wrow * D) * 4);
 #pragma unroll
             for (int u = 0; u < NI; u++) {
@@ -1195,15 +1211,15 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
 #pragma unroll
         for (int f = 0; f < NF; f++) qf[f] = *(const f4_t*)(ring + (NS - 1) * 2 * TILE + wrow * D + k_rd[f]);
         wait_lds_reads();
+        if (W::KS > 1 && share == 0) __builtin_amdgcn_s_setprio(1);
         auto step = [&](int i, auto stage_c) {
             constexpr int stage = decltype(stage_c)::value;
             wait_vm<0>();
             const uint64_t mk = mask[stage];
-            const T* const st = ring + stage * 2 * TILE;
             if (mk != ~0ull) {
 #pragma unroll
-                for (int u = 0; u < NI; u++) {
-                    const int row = wrow + R::RPI * u + drow;
+                for (int u = 0; u < HI; u++) {
+                    const int row = 16 * grp + first + R::RPI * u + drow;
                     if (!((mk >> row) & 1)) *(uint4*)(ring + stage * 2 * TILE + TILE + row * D + 4 * dch) = uint4{};
                 }
                 wait_lds_reads();
@@ -1211,30 +1227,37 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
             ring_barrier();
             if (i + 1 < n) issue(i + 1, std::integral_constant<int, (stage + 1) % NS>{});
             if (!active) return;
-            const int k0 = w.key0 + i * BK;
-            // Fragments are read kAhead before their products, in this order (four chains of sums).
-            constexpr int kAhead = 4;
-            f4_t sc[4], kf[kAhead];
-            auto read_k = [&](auto x_c) {
-                constexpr int x = decltype(x_c)::value;
-                kf[x % kAhead] = *(const f4_t*)(st + 16 * (x % 4) * D + k_rd[x / 4]);
+            const int k0 = w.key0 + i * BK + 16 * NT * share;
+            const T* const st = ring + stage * 2 * TILE + 16 * NT * share * D;
+            // A dim chunk's fragments are read one or two chunks before their products, in this order;
+            // the tiles' chains of sums go side by side (an MFMA that waits for the one before takes 44).
+            constexpr int kAhead = 1 + 4 / NT;
+            f4_t sc[NT], kf[kAhead][NT];
+            auto read_k = [&](auto f_c) {
+                constexpr int f = decltype(f_c)::value;
+#pragma unroll
+                for (int t = 0; t < NT; t++) kf[f % kAhead][t] = *(const f4_t*)(st + 16 * t * D + k_rd[f]);
             };
             static_for<kAhead - 1>(read_k);
-            static_for<4 * NF>([&](auto x_c) {
-                constexpr int x = decltype(x_c)::value, t = x % 4, f = x / 4;
-                if constexpr (x + kAhead - 1 < 4 * NF) read_k(std::integral_constant<int, x + kAhead - 1>{});
-                if constexpr (f == 0) sc[t] = f4_t{0.f, 0.f, 0.f, 0.f};
+            static_for<NF>([&](auto f_c) {
+                constexpr int f = decltype(f_c)::value;
+                if constexpr (f + kAhead - 1 < NF) read_k(std::integral_constant<int, f + kAhead - 1>{});
+                if constexpr (f == 0)
+#pragma unroll
+                    for (int t = 0; t < NT; t++) sc[t] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x % kAhead][e], qf[f][e], sc[t], 0, 0, 0);
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[f % kAhead][t][e], qf[f][e], sc[t], 0, 0, 0);
                 __builtin_amdgcn_sched_barrier(0);
             });
-            if (mk != ~0ull || k0 + BK > seen_all) {
-                hide(sc, mk, seen - k0, lane);
-            }
-            float mloc = sc[0][0];
+            if (mk != ~0ull || k0 + 16 * NT > seen_all) hide(sc, mk >> (W::KS > 1 ? 32 * share : 0), seen - k0, lane);
+            float mloc = fmaxf(fmaxf(sc[0][0], sc[0][1]), sc[0][2]);
 #pragma unroll
-            for (int e = 1; e < 16; e++) mloc = fmaxf(mloc, sc[e >> 2][e & 3]);
+            for (int e = 3; e < 4 * NT - 1; e += 2)
+                mloc = fmaxf(fmaxf(mloc, sc[e >> 2][e & 3]), sc[(e + 1) >> 2][(e + 1) & 3]);
+            mloc = fmaxf(mloc, sc[NT - 1][3]);
             mloc = max_xor32(max_xor16(mloc)) * c;
             float alpha;
             if (move_max(mloc, m_run, alpha)) {
@@ -1244,7 +1267,7 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
             }
             const float m_use = m_run == -INFINITY ? 0.0f : m_run;
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+            for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     sc[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][e], c, -m_use));
@@ -1258,9 +1281,9 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
                 for (int u = 0; u < UT; u++) vf[g % 2][u] = R::v_at(st + TILE, v_rd, lane, g / 4, g % 4, u);
             };
             read_v(std::integral_constant<int, 0>{});
-            static_for<16>([&](auto g_c) {
+            static_for<4 * NT>([&](auto g_c) {
                 constexpr int g = decltype(g_c)::value;
-                if constexpr (g + 1 < 16) read_v(std::integral_constant<int, g + 1>{});
+                if constexpr (g + 1 < 4 * NT) read_v(std::integral_constant<int, g + 1>{});
 #pragma unroll
                 for (int u = 0; u < UT; u++)
                     acc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[g % 2][u], sc[g / 4][g % 4], acc[u], 0, 0, 0);
@@ -1268,20 +1291,46 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
             });
         };
         for_each_stage<NS>(n, step);
+        if (W::KS > 1) __builtin_amdgcn_s_setprio(0);
     }
-    const float l = add_xor32(add_xor16(l_run));
-    uint32_t again = un.n_ranges > 1 ? 0 : rows_of_16(wrow + lr < w.n_rows && spoilt(acc, l));
-    if (wrow + lr < w.n_rows && !((again >> lr) & 1)) {
-        const RowOut out = row_out<T, D, W::TM>(a, pl, un, kvh, w, wrow + lr, m_run, l, lq == 0);
+    float l = add_xor32(add_xor16(l_run));
+    ring_barrier();                                           // the ring's reads
+    if constexpr (W::KS > 1) {
+        // The second waves' m, l and sums, through the ring.
+        f4_t* const other = (f4_t*)ring + (wave & 3) * (UT + 1) * 64 + lane;
+        static_assert(4 * (UT + 1) * 64 * 4 <= W::LDS, "they fit");
+        if (share == 1) {
 #pragma unroll
-        for (int u = 0; u < UT; u++) put4<T>(out, 16 * u + 4 * lq, acc[u]);
+            for (int u = 0; u < UT; u++) other[64 * u] = acc[u];
+            other[64 * UT] = f4_t{m_run, l, 0.f, 0.f};
+            wait_lds_reads();
+        }
+        ring_barrier();
+        if (share == 0) {
+            const f4_t ml = other[64 * UT];
+            const float M = fmaxf(m_run, ml[0]), m_use = M == -INFINITY ? 0.0f : M;
+            const float x0 = __builtin_amdgcn_exp2f(m_run - m_use), x1 = __builtin_amdgcn_exp2f(ml[0] - m_use);
+            m_run = M;
+            l = l * x0 + ml[1] * x1;
+#pragma unroll
+            for (int u = 0; u < UT; u++) acc[u] = acc[u] * x0 + other[64 * u] * x1;
+        }
+        wait_lds_reads();
+        ring_barrier();                                       // ... before the next unit
     }
-    for (; again; again &= again - 1) redo_row<T, D>(a, pl, un, kvh, w.R0 + wrow + __builtin_ctz(again));
-    ring_barrier();                                           // the ring's reads, before the next unit
+    if (share == 0) {
+        uint32_t again = un.n_ranges > 1 ? 0 : rows_of_16(wrow + lr < w.n_rows && spoilt(acc, l));
+        if (wrow + lr < w.n_rows && !((again >> lr) & 1)) {
+            const RowOut out = row_out<T, D, W::TM>(a, pl, un, kvh, w, wrow + lr, m_run, l, lq == 0);
+#pragma unroll
+            for (int u = 0; u < UT; u++) put4<T>(out, 16 * u + 4 * lq, acc[u]);
+        }
+        for (; again; again &= again - 1) redo_row<T, D>(a, pl, un, kvh, w.R0 + wrow + __builtin_ctz(again));
+    }
 }
 
 template <int D>
-__global__ __launch_bounds__(256, (Wide32<D>::PER_CU))
+__global__ __launch_bounds__(64 * (Wide32<D>::WAVES), (Wide32<D>::PER_CU) * (Wide32<D>::KS))
 void paged_wide32(cf_paged_attn_args_t a, PagedPlan pl) {
     using W = Wide32<D>;
     __shared__ __attribute__((aligned(16))) float lds[W::LDS];
@@ -1294,7 +1343,7 @@ void paged_wide32(cf_paged_attn_args_t a, PagedPlan pl) {
         if (!geo.template find<false>(id, un)) break;
         const Work w = unit_work<W::TM, 64>(a, pl, un);
         if (w.n_rows > 16) wide32_unit<D>(a, pl, lds, un, kvh, w);
-        else if (narrow_unit<float, D, W::TM, 4>(a, pl, lds, un, kvh, w)) redo_narrow<float, D, 4>(a, pl, un, kvh, w);
+        else if (narrow_unit<float, D, W::TM, 4, W::WAVES>(a, pl, lds, un, kvh, w)) redo_narrow<float, D, 4>(a, pl, un, kvh, w);
     }
 }
 
@@ -1504,7 +1553,7 @@ int launch_tiles(const cf_paged_attn_args_t& a, const Plan& p, hipStream_t st) {
         if (p.form == kWide2) return go(paged_wide16<D, 2>, 512, paged_merge<T, D, 256, 64, kNarrowCost, 1024 / D>);
         return go(paged_wide16<D, 1>, 512, paged_merge<T, D, 128, 64, kNarrowCost, 1024 / D>);
     } else {
-        return go(paged_wide32<D>, 256, paged_merge<T, D, 64, 64, kNarrowCost, 1024 / D>);
+        return go(paged_wide32<D>, 64 * Wide32<D>::WAVES, paged_merge<T, D, 64, 64, kNarrowCost, 1024 / D>);
     }
 }
 
