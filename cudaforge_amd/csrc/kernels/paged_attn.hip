@@ -61,10 +61,17 @@ __device__ __forceinline__ SeqRows seq_rows(const cf_paged_attn_args_t& a, int b
 //   paged_wide   64 rows and more; its tiles of up to 16 rows go as in paged_split, so a
 //                batch may mix prompt chunks and decode steps.
 
+struct CutTile {
+    SeqRows s;
+    int b, tile, n_ranges, record;          // record: of its first range
+    int pad;
+};
 struct PagedPlan {
-    int*    cut_tiles;     // their number (per KV head), left by the first workgroup for the merge
+    int*    cut_count;     // cut tiles (per KV head), left by the workgroup behind the units' for
+    CutTile* cut_tiles;    // the merge, which then has no geometry to work out
     float*  records;       // of the units of cut tiles
     int32_t max_records;   // per KV head
+    int32_t unit_wgs;      // workgroups of units
     int32_t fill;          // units (per KV head) that fill the chip
     int32_t min_blocks;    // no range is cut shorter
     int32_t one_blocks;    // tiles of up to this many blocks are not cut
@@ -74,10 +81,10 @@ struct PagedPlan {
     FastDiv by_page, by_group, by_kv;
 };
 
-// A unit's tile and range, or the tile to merge.
+// A unit's tile and range.
 struct Unit {
     SeqRows s;
-    int b, tile, range, n_ranges, record;   // record: of its first range (cut tiles)
+    int b, tile, range, n_ranges, record;   // record: of the tile's first range (cut tiles)
 };
 
 // The tiles' geometry, one sequence per lane and 64 at a time.  TM rows per tile, BK
@@ -133,24 +140,29 @@ struct Geometry {
         inv_C = 1.0f / C;
         if (pl.one_blocks == INT32_MAX) one = INT32_MAX;
     }
-    // The number of cut tiles, for the merge: most of its workgroups need know no more.
-    __device__ __forceinline__ void leave_cut_tiles() const {
-        if (!pl.cut_tiles || blockIdx.x != 0 || threadIdx.x >= 64) return;
-        int n = ranges(first) > 1 ? tiles(first) : 0;
-        for (int b = 64; b < a.B; b += 64) {
-            const SeqRows s = rows(b + lane);
-            n += ranges(s) > 1 ? tiles(s) : 0;
+    // True for the workgroup behind the units', which lists the cut tiles.
+    __device__ __forceinline__ bool lists_cut_tiles() const {
+        if ((int)blockIdx.x != pl.unit_wgs) return false;
+        if (threadIdx.x >= 64) return true;
+        int count = 0, records = 0;
+        for (int base = 0; base < a.B; base += 64) {
+            const SeqRows s = rows(base + lane);
+            const int ns = ranges(s), t = ns > 1 ? tiles(s) : 0;
+            const int at = count + wave_excl_sum(t, lane), rec = records + wave_excl_sum(t * ns, lane);
+            for (int i = 0; i < t && rec + (i + 1) * ns <= pl.max_records; i++)
+                pl.cut_tiles[at + i] = CutTile{s, base + lane, i, ns, rec + i * ns, 0};
+            count = __builtin_amdgcn_readlane(at + t, 63);
+            records = __builtin_amdgcn_readlane(rec + t * ns, 63);
         }
-        n += wave_excl_sum(n, lane);
-        if (lane == 63) *pl.cut_tiles = n;
+        if (lane == 0) *pl.cut_count = min(count, pl.max_records / 2);
+        return true;
     }
-    // Item u of all units (MERGE: of all cut tiles); false where there is none.
-    template <bool MERGE>
+    // Unit u; false where there is none.
     __device__ __forceinline__ bool find(int u, Unit& out) const {
         int items0 = 0;
         // Wide tiles: the sequences with the long ranges first, so that short pieces fill the end
         // (35 sequences, 4 of them chunks: 108 us, in the order of the sequences 131).
-        constexpr int CLASSES = !MERGE && NARROW > 1 ? 2 : 1;
+        constexpr int CLASSES = NARROW > 1 ? 2 : 1;
         for (int cls = 0; cls < CLASSES; cls++) {
             int records0 = 0;
             for (int base = 0; base < a.B; base += 64) {
@@ -158,7 +170,7 @@ struct Geometry {
                                 : NARROW > 1 ? SeqRows{kept[lane], kept[64 + lane], kept[128 + lane]} : first;
                 const int t = tiles(s), ns = ranges(s), rec = ns > 1 ? t * ns : 0;
                 const bool cut = __builtin_amdgcn_ballot_w64(ns > 1) != 0;
-                int items = MERGE ? (ns > 1 ? t : 0) : t * ns;
+                int items = t * ns;
                 if (CLASSES > 1 && (2.0f * (float)blocks(s) > C * (float)ns ? 0 : 1) != cls) items = 0;
                 const int before = items0 + wave_excl_sum(items, lane);
                 const int rec_before = records0 + (cut ? wave_excl_sum(rec, lane) : 0);
@@ -168,8 +180,8 @@ struct Geometry {
                     const int at = u - __builtin_amdgcn_readlane(before, src);
                     out.n_ranges = __builtin_amdgcn_readlane(ns, src);
                     const int nt = __builtin_amdgcn_readlane(t, src);
-                    const int i = MERGE || out.n_ranges == 1 ? at : at / out.n_ranges;
-                    out.range = MERGE ? 0 : at - i * out.n_ranges;
+                    const int i = out.n_ranges == 1 ? at : at / out.n_ranges;
+                    out.range = at - i * out.n_ranges;
                     out.tile = nt - 1 - i;                     // the longest first
                     out.record = __builtin_amdgcn_readlane(rec_before, src) + out.tile * out.n_ranges;
                     out.b = base + src;
@@ -347,8 +359,8 @@ __device__ __forceinline__ void plain_row(const cf_paged_attn_args_t& a, FastDiv
 // On the matrix cores a position that another row of the tile sees counts as 0 times its V,
 // which is no 0 where V is infinite or NaN.  A sum that is NaN while l is a number may come from
 // one: such a row is computed again, where only what it sees is touched.
-template <typename T, int D>
-__device__ __forceinline__ void redo_row(const cf_paged_attn_args_t& a, const PagedPlan& pl, const Unit& un, int kvh, int R) {
+template <typename T, int D, typename Tile>     // Unit or CutTile
+__device__ __forceinline__ void redo_row(const cf_paged_attn_args_t& a, const PagedPlan& pl, const Tile& un, int kvh, int R) {
     const int G = pl.G, tok = fastdiv(R, pl.by_group);
     plain_row<T, D / 64>(a, pl.by_page, un.s, un.b, tok, kvh * G + (R - tok * G), D);
 }
@@ -647,11 +659,11 @@ void paged_heads(cf_paged_attn_args_t a, PagedPlan pl) {
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int G = pl.G;
     const Geometry<16, H::BK, 1> geo(a, pl);
-    geo.leave_cut_tiles();
+    if (geo.lists_cut_tiles()) return;
     for (int unit = (int)blockIdx.x * H::WAVES + wave;; unit += pl.step) {
         const int id = fastdiv(unit, pl.by_kv), kvh = unit - id * a.H_kv;
         Unit un;
-        if (!geo.template find<false>(id, un)) break;
+        if (!geo.find(id, un)) break;
         const Work w = unit_work<16, H::BK>(a, pl, un);
         const int lane = unit_lane(), lr = lane & 15, lq = lane >> 4;
         f4_t acc[D / 16];
@@ -766,11 +778,11 @@ void paged_split(cf_paged_attn_args_t a, PagedPlan pl) {
     constexpr int WAVES = Split<T, D>::WAVES;
     __shared__ __attribute__((aligned(16))) T lds[WAVES * Narrow<T, D, 16>::RING];
     const Geometry<16, 64, 1> geo(a, pl);
-    geo.leave_cut_tiles();
+    if (geo.lists_cut_tiles()) return;
     for (int unit = (int)blockIdx.x;; unit += pl.step) {
         const int id = fastdiv(unit, pl.by_kv), kvh = unit - id * a.H_kv;
         Unit un;
-        if (!geo.template find<false>(id, un)) break;
+        if (!geo.find(id, un)) break;
         const Work w = unit_work<16, 64>(a, pl, un);
         if (narrow_unit<T, D, 16, WAVES>(a, pl, lds, un, kvh, w)) redo_narrow<T, D, WAVES>(a, pl, un, kvh, w);
     }
@@ -1109,17 +1121,17 @@ void paged_wide16(cf_paged_attn_args_t a, PagedPlan pl) {
     __shared__ uint64_t masks[W::MASKS];
     __shared__ int kept[3 * 64];
     const Geometry<W::TM, 64, kNarrowCost> geo(a, pl, kept);
-    geo.leave_cut_tiles();
+    if (geo.lists_cut_tiles()) return;
     for (int unit = (int)blockIdx.x;; unit += pl.step) {
         const int id = fastdiv(unit, pl.by_kv), kvh = unit - id * a.H_kv;
         Unit un;
-        if (!geo.template find<false>(id, un)) break;
+        if (!geo.find(id, un)) break;
         Work w = unit_work<W::TM, 64>(a, pl, un);
         const bool narrow = w.n_rows <= 16;
         const uint32_t again = narrow ? narrow_unit<_Float16, D, W::TM, 8>(a, pl, lds, un, kvh, w)
                                       : wide16_unit<D, NJ>(a, pl, lds, masks, un, kvh, w);
         if (!again) continue;
-        if (!geo.template find<false>(id, un)) break;         // found anew: nothing is kept for this
+        if (!geo.find(id, un)) break;         // found anew: nothing is kept for this
         w = unit_work<W::TM, 64>(a, pl, un);
         if (narrow) redo_narrow<_Float16, D, 8>(a, pl, un, kvh, w);
         const int row0 = w.R0 + 16 * NJ * __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -1336,11 +1348,11 @@ void paged_wide32(cf_paged_attn_args_t a, PagedPlan pl) {
     __shared__ __attribute__((aligned(16))) float lds[W::LDS];
     __shared__ int kept[3 * 64];
     const Geometry<W::TM, 64, kNarrowCost> geo(a, pl, kept);
-    geo.leave_cut_tiles();
+    if (geo.lists_cut_tiles()) return;
     for (int unit = (int)blockIdx.x;; unit += pl.step) {
         const int id = fastdiv(unit, pl.by_kv), kvh = unit - id * a.H_kv;
         Unit un;
-        if (!geo.template find<false>(id, un)) break;
+        if (!geo.find(id, un)) break;
         const Work w = unit_work<W::TM, 64>(a, pl, un);
         if (w.n_rows > 16) wide32_unit<D>(a, pl, lds, un, kvh, w);
         else if (narrow_unit<float, D, W::TM, 4, W::WAVES>(a, pl, lds, un, kvh, w)) redo_narrow<float, D, 4>(a, pl, un, kvh, w);
@@ -1350,24 +1362,20 @@ void paged_wide32(cf_paged_attn_args_t a, PagedPlan pl) {
 // Joins the ranges of cut tiles: O = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s.  A
 // workgroup per (tile, KV head) and ROWS rows: 256 / ROWS threads per row, D / 4 of them side
 // by side over the dims, the rest sharing the ranges.
-template <typename T, int D, int TM, int BK, int NARROW, int ROWS>
+template <typename T, int D, int TM, int ROWS>
 __global__ __launch_bounds__(256)
 void paged_merge(cf_paged_attn_args_t a, PagedPlan pl) {
     constexpr int DL = D / 4, SUBS = 256 / ROWS / DL;      // lanes over the dims, shares of the ranges
     static_assert(SUBS >= 1, "rows per workgroup");
     __shared__ float ml[2][ROWS][SUBS];
     __shared__ f4_t part[SUBS > 1 ? SUBS * ROWS * DL : 1];
-    const int cut_units = *pl.cut_tiles * a.H_kv * pl.merge_groups;
-    if ((int)blockIdx.x >= cut_units) return;
-    __shared__ int kept[NARROW > 1 ? 3 * 64 : 1];
-    const Geometry<TM, BK, NARROW> geo(a, pl, kept);
+    const int cut_units = *pl.cut_count * a.H_kv * pl.merge_groups;
     const int G = pl.G;
     const int d4 = threadIdx.x % DL, sub = threadIdx.x / DL % SUBS, r = threadIdx.x / (DL * SUBS);
     for (int unit = blockIdx.x; unit < cut_units; unit += gridDim.x) {
         const int th = unit / pl.merge_groups, group = unit - th * pl.merge_groups;
         const int tile_id = fastdiv(th, pl.by_kv), kvh = th - tile_id * a.H_kv;
-        Unit un;
-        if (!geo.template find<true>(tile_id, un)) break;
+        const CutTile un = pl.cut_tiles[tile_id];
         const int n_rows = min(un.s.n * G - un.tile * TM, TM);
         const float* const rec = pl.records + ((size_t)un.record * a.H_kv + kvh) * record_floats<TM, D>();
         const size_t step = (size_t)a.H_kv * record_floats<TM, D>();
@@ -1473,7 +1481,8 @@ struct Plan {
 
 constexpr int64_t g_few_units = 64, g_split_units = 256, g_split_len = 1024, g_wide2_units = 192;
 
-constexpr size_t kHeader = 256;   // of the workspace: the number of cut tiles
+// Of the workspace: the number of cut tiles (256 bytes) and the list of them.
+size_t header_bytes(int32_t max_records) { return 256 + ((size_t)max_records / 2 * sizeof(CutTile) + 255) / 256 * 256; }
 
 bool fast_ok(const cf_paged_attn_args_t& a) {
     const uint64_t ptrs = (uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.k | (uint64_t)(uintptr_t)a.v | (uint64_t)(uintptr_t)a.o;
@@ -1517,7 +1526,7 @@ Plan make_plan(const cf_paged_attn_args_t& a) {
     p.pl.max_records = (int32_t)(4 * fill + 8);
     const bool cut = (a.max_len + BK - 1) / BK > (wide16 ? 512 / BK : p.pl.one_blocks);
     if (!cut) p.pl.one_blocks = INT32_MAX;                    // nor is what is longer than max_len
-    p.bytes = cut ? kHeader + (size_t)p.pl.max_records * a.H_kv * (TM * (a.d + 2)) * sizeof(float) : 0;
+    p.bytes = cut ? header_bytes(p.pl.max_records) + (size_t)p.pl.max_records * a.H_kv * (TM * (a.d + 2)) * sizeof(float) : 0;
     int64_t units = (tiles + (cut ? 2 * fill : 0)) * a.H_kv;
     if (units > (1 << 22)) units = 1 << 22;
     p.wgs = (int)(p.form == kHeads ? (units + 3) / 4 : units);
@@ -1531,6 +1540,9 @@ Plan make_plan(const cf_paged_attn_args_t& a) {
     p.pl.G = (int32_t)G;
     p.pl.by_group = fastdiv_make((int)G);
     p.pl.by_kv = fastdiv_make(a.H_kv);
+    p.pl.unit_wgs = p.wgs;
+    if (cut) p.wgs++;
+    p.pl.cut_count = nullptr;
     p.pl.cut_tiles = nullptr;
     p.pl.records = nullptr;
     return p;
@@ -1547,13 +1559,13 @@ int launch_tiles(const cf_paged_attn_args_t& a, const Plan& p, hipStream_t st) {
         hipLaunchKernelGGL(merge, mgrid, dim3(256), 0, st, a, p.pl);
         return (int)hipGetLastError();
     };
-    if (p.form == kHeads) return go(paged_heads<T, D>, 256, paged_merge<T, D, 16, Heads<T, D>::BK, 1, 1>);
-    if (p.form == kSplit) return go(paged_split<T, D>, 64 * Split<T, D>::WAVES, paged_merge<T, D, 16, 64, 1, 1>);
+    if (p.form == kHeads) return go(paged_heads<T, D>, 256, paged_merge<T, D, 16, 1>);
+    if (p.form == kSplit) return go(paged_split<T, D>, 64 * Split<T, D>::WAVES, paged_merge<T, D, 16, 1>);
     if constexpr (F16) {
-        if (p.form == kWide2) return go(paged_wide16<D, 2>, 512, paged_merge<T, D, 256, 64, kNarrowCost, 1024 / D>);
-        return go(paged_wide16<D, 1>, 512, paged_merge<T, D, 128, 64, kNarrowCost, 1024 / D>);
+        if (p.form == kWide2) return go(paged_wide16<D, 2>, 512, paged_merge<T, D, 256, 1024 / D>);
+        return go(paged_wide16<D, 1>, 512, paged_merge<T, D, 128, 1024 / D>);
     } else {
-        return go(paged_wide32<D>, 64 * Wide32<D>::WAVES, paged_merge<T, D, 64, 64, kNarrowCost, 1024 / D>);
+        return go(paged_wide32<D>, 64 * Wide32<D>::WAVES, paged_merge<T, D, 64, 1024 / D>);
     }
 }
 
@@ -1569,8 +1581,9 @@ extern "C" int cf_launch_paged_attn(const cf_paged_attn_args_t* a, void* stream)
         Plan p = make_plan(*a);
         if (p.bytes > 0 && !a->workspace) return (int)hipErrorInvalidValue;
         if (p.bytes > 0) {
-            p.pl.cut_tiles = (int*)a->workspace;
-            p.pl.records = (float*)((char*)a->workspace + kHeader);
+            p.pl.cut_count = (int*)a->workspace;
+            p.pl.cut_tiles = (CutTile*)((char*)a->workspace + 256);
+            p.pl.records = (float*)((char*)a->workspace + header_bytes(p.pl.max_records));
         }
         if (a->elem == CF_ELEM_F16)
             return a->d == 64 ? launch_tiles<_Float16, 64>(*a, p, st) : launch_tiles<_Float16, 128>(*a, p, st);
