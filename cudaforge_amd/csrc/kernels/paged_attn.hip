@@ -57,7 +57,7 @@ __device__ __forceinline__ SeqRows seq_rows(const cf_paged_attn_args_t& a, int b
 //
 // Three kernels share this:
 //   paged_heads  up to 16 rows per tile, a wave per unit (decode steps of many sequences);
-//   paged_split  up to 16 rows, the waves of a workgroup share the positions of a unit (few);
+//   paged_split  up to 16 rows of short sequences, the waves of a workgroup share the positions;
 //   paged_wide   64 rows and more; its tiles of up to 16 rows go as in paged_split, so a
 //                batch may mix prompt chunks and decode steps.
 
@@ -80,6 +80,8 @@ struct PagedPlan {
     int32_t G;             // query heads per KV head
     FastDiv by_page, by_group, by_kv;
 };
+
+constexpr int kFewOne = 512, kFewMin = 4;    // positions of tiles that are not cut; blocks of a range
 
 // A unit's tile and range.
 struct Unit {
@@ -132,11 +134,11 @@ struct Geometry {
         const float fill = (float)pl.fill;
         const float n = t <= 0.5f * fill ? fill - t : t <= fill ? 2.0f * fill - t : NARROW > 1 ? fill : 2.0f * fill;
         w = ceilf(w / fmaxf(n, 1.0f));
-        // Cutting costs wide tiles a merge and records, as much as 5 to 13 blocks: with half the chip
-        // busy or more it pays for long ranges only.
+        // With less than a quarter of the chip busy, fp16 wide tiles are cut sooner than else (150 rows
+        // of 12 heads over 3050: 18.3 us, else 19.8).
         const bool few = NARROW > 1 && t <= 0.25f * fill;
-        one = __builtin_amdgcn_readfirstlane(few ? min(pl.one_blocks, 512 / BK) : pl.one_blocks);
-        C = fmaxf(w, (float)(few ? 4 : pl.min_blocks));
+        one = __builtin_amdgcn_readfirstlane(few ? min(pl.one_blocks, kFewOne / BK) : pl.one_blocks);
+        C = fmaxf(w, (float)(few ? kFewMin : pl.min_blocks));
         inv_C = 1.0f / C;
         if (pl.one_blocks == INT32_MAX) one = INT32_MAX;
     }
@@ -778,7 +780,6 @@ void paged_split(cf_paged_attn_args_t a, PagedPlan pl) {
     constexpr int WAVES = Split<T, D>::WAVES;
     __shared__ __attribute__((aligned(16))) T lds[WAVES * Narrow<T, D, 16>::RING];
     const Geometry<16, 64, 1> geo(a, pl);
-    if (geo.lists_cut_tiles()) return;
     for (int unit = (int)blockIdx.x;; unit += pl.step) {
         const int id = fastdiv(unit, pl.by_kv), kvh = unit - id * a.H_kv;
         Unit un;
@@ -1479,7 +1480,18 @@ struct Plan {
     size_t bytes;         // workspace
 };
 
-constexpr int64_t g_few_units = 64, g_split_units = 256, g_split_len = 1024, g_wide2_units = 192;
+// paged_split for sequences of up to 1024 positions, which it finishes in one range, as long as
+// its units, a workgroup each, go in one round: fp16, 32 heads of 128 over 8, us with paged_split
+// and paged_heads: 1 x 512 9.0 and 11.8, 16 x 512 10.9 and 14.6, 32 x 1024 28.0 and 31.8, 64 x 512
+// both 31.3; longer ones need ranges and a merge in both: 8 x 2048 19.8 and 18.2, 16 x 8192 117
+// and 98, 2 x 30000 52.9 and 51.4.
+constexpr int64_t kSplitUnits = 256, kSplitLen = 1024;
+// Tiles of 256 rows read a block's K and V once for twice the rows, but are twice as long a
+// piece of work.  They pay where they fill three quarters of the chip by themselves (4 x 517 rows
+// over 517: 31.8 us, with 128 rows 34.4; 4 x 1024 over 2048: 135 and 159; 1024 over 1024: 38.9 and
+// 28.0), and where long ranges of one or two long sequences can be cut evenly (517 over 8517: 95
+// and 118; 330 over 2530: 36.8 and 38.4; 230 over 2430, 28 units: 33 and 30.8; 4 x 230: 59 and 56).
+constexpr int64_t kFullUnits = 192, kLongUnits = 32, kLongLen = 2048;
 
 // Of the workspace: the number of cut tiles (256 bytes) and the list of them.
 size_t header_bytes(int32_t max_records) { return 256 + ((size_t)max_records / 2 * sizeof(CutTile) + 255) / 256 * 256; }
@@ -1508,31 +1520,37 @@ Plan make_plan(const cf_paged_attn_args_t& a) {
     };
     if (rows <= 16) {
         const int64_t units = tiles_of(16) * a.H_kv;
-        p.form = units <= g_few_units || (units <= g_split_units && a.max_len <= g_split_len) ? kSplit : kHeads;
+        p.form = units <= kSplitUnits && a.max_len <= kSplitLen ? kSplit : kHeads;
     } else {
-        p.form = f16 && (int64_t)a.T * G / 256 * a.H_kv >= g_wide2_units ? kWide2 : kWide1;
+        const int64_t units = (int64_t)a.T * G / 256 * a.H_kv;
+        const bool few_long = a.max_len > kLongLen && 2 * (int64_t)a.max_new >= a.T && units >= kLongUnits;
+        p.form = f16 && (units >= kFullUnits || few_long) ? kWide2 : kWide1;
     }
     const int64_t TM = p.form <= kSplit ? 16 : !f16 ? 64 : p.form == kWide2 ? 256 : 128;
     const int64_t BK = p.form != kHeads ? 64 : f16 ? 32 : 16;
     const int64_t tiles = tiles_of(TM);
     // Units in flight, by the LDS a workgroup takes.
-    const int64_t per_cu = p.form == kHeads ? (a.d == 128 ? 4 : 8) : p.form == kSplit ? (f16 && a.d == 64 ? 2 : 1)
-                         : f16 || a.d == 128 ? 1 : 2;
-    const int64_t fill = cus * per_cu > a.H_kv ? cus * per_cu / a.H_kv  : 1;
+    const int64_t per_cu = p.form == kHeads ? (a.d == 128 ? 4 : 8) : f16 || a.d == 128 ? 1 : 2;
+    const int64_t fill = cus * per_cu > a.H_kv ? cus * per_cu / a.H_kv : 1;
     p.pl.fill = (int32_t)fill;
+    // What is not worth cutting: a merge and the records cost paged_heads 5 us and a wide tile 10
+    // to 12 (517 rows over 1029: 26.7 us, cut from 8 blocks on into ranges of 4: 35; fp32, 200 rows
+    // over 1200: 57 us, from 24 blocks on into ranges of 12: 66).
     const bool wide16 = f16 && p.form > kSplit;
     p.pl.min_blocks = (int32_t)(p.form == kHeads ? 64 / BK : wide16 ? 12 : 4);
-    p.pl.one_blocks = (int32_t)((p.form == kHeads ? 128 : p.form == kSplit ? 1024 : wide16 ? 1536 : 512) / BK);
+    p.pl.one_blocks = (int32_t)((p.form == kHeads ? 128 : wide16 ? 1536 : 512) / BK);
     p.pl.max_records = (int32_t)(4 * fill + 8);
-    const bool cut = (a.max_len + BK - 1) / BK > (wide16 ? 512 / BK : p.pl.one_blocks);
+    const bool cut = p.form != kSplit && (a.max_len + BK - 1) / BK > (wide16 ? kFewOne / BK : p.pl.one_blocks);
     if (!cut) p.pl.one_blocks = INT32_MAX;                    // nor is what is longer than max_len
     p.bytes = cut ? header_bytes(p.pl.max_records) + (size_t)p.pl.max_records * a.H_kv * (TM * (a.d + 2)) * sizeof(float) : 0;
     int64_t units = (tiles + (cut ? 2 * fill : 0)) * a.H_kv;
     if (units > (1 << 22)) units = 1 << 22;
     p.wgs = (int)(p.form == kHeads ? (units + 3) / 4 : units);
     p.pl.step = p.form == kHeads ? 4 * p.wgs : p.wgs;
+    p.pl.unit_wgs = p.wgs;
+    if (cut) p.wgs++;                                         // lists the cut tiles
     const int64_t most_rows = rows < TM ? rows : TM;
-    const int64_t merge_rows = p.form <= kSplit ? 1 : 1024 / a.d;   // of a workgroup
+    const int64_t merge_rows = p.form == kHeads ? 1 : 1024 / a.d;   // of a workgroup
     p.pl.merge_groups = (int32_t)((most_rows + merge_rows - 1) / merge_rows);
     const int64_t merge_wgs = (tiles < 2 * fill ? tiles : 2 * fill) * a.H_kv * p.pl.merge_groups;
     p.merge_wgs = !cut ? 0 : merge_wgs > 4096 ? 4096 : (int)merge_wgs;
@@ -1540,8 +1558,6 @@ Plan make_plan(const cf_paged_attn_args_t& a) {
     p.pl.G = (int32_t)G;
     p.pl.by_group = fastdiv_make((int)G);
     p.pl.by_kv = fastdiv_make(a.H_kv);
-    p.pl.unit_wgs = p.wgs;
-    if (cut) p.wgs++;
     p.pl.cut_count = nullptr;
     p.pl.cut_tiles = nullptr;
     p.pl.records = nullptr;
@@ -1560,7 +1576,10 @@ int launch_tiles(const cf_paged_attn_args_t& a, const Plan& p, hipStream_t st) {
         return (int)hipGetLastError();
     };
     if (p.form == kHeads) return go(paged_heads<T, D>, 256, paged_merge<T, D, 16, 1>);
-    if (p.form == kSplit) return go(paged_split<T, D>, 64 * Split<T, D>::WAVES, paged_merge<T, D, 16, 1>);
+    if (p.form == kSplit) {                                   // nothing is cut
+        hipLaunchKernelGGL((paged_split<T, D>), grid, dim3(64 * Split<T, D>::WAVES), 0, st, a, p.pl);
+        return (int)hipGetLastError();
+    }
     if constexpr (F16) {
         if (p.form == kWide2) return go(paged_wide16<D, 2>, 512, paged_merge<T, D, 256, 1024 / D>);
         return go(paged_wide16<D, 1>, 512, paged_merge<T, D, 128, 1024 / D>);
