@@ -5,6 +5,9 @@
 // over the positions of valid pages (position j: page table[b][j / P], row j % P).  Softmax
 // in one pass: running maximum m and sum l in FP32, everything rescaled by 2^(m_old - m)
 // when the maximum moves; scores are kept in the log2 domain.
+//
+// Times below are of one call among others on one MI355X; "n rows over m" is n new tokens of
+// a sequence of m positions in all, and heads are 32 of 128 over 8 KV heads where none are named.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -55,21 +58,22 @@ __device__ __forceinline__ SeqRows seq_rows(const cf_paged_attn_args_t& a, int b
 // paged_merge joins them.  More than one range needs blocks_b > C, so ns_b < 2 blocks_b / C
 // and there are at most 2 R + 1 such units per KV head; R is at most 2 `fill`.
 //
-// Three kernels share this:
-//   paged_heads  up to 16 rows per tile, a wave per unit (decode steps of many sequences);
-//   paged_split  up to 16 rows of short sequences, the waves of a workgroup share the positions;
-//   paged_wide   64 rows and more; its tiles of up to 16 rows go as in paged_split, so a
-//                batch may mix prompt chunks and decode steps.
+// The kernels that share this:
+//   paged_heads   up to 16 rows per tile, a wave per unit (decode steps);
+//   paged_split   up to 16 rows of short sequences, the waves of a workgroup share the positions;
+//   paged_wide16, paged_wide32   fp16 and fp32 tiles of 64 to 256 rows; tiles of up to 16 rows go
+//                 as in paged_split there, so a batch may mix prompt chunks and decode steps.
 
+// A cut tile, for the merge, which then has no geometry to work out.
 struct CutTile {
     SeqRows s;
     int b, tile, n_ranges, record;          // record: of its first range
-    int pad;
+    int pad;                                // 32 bytes
 };
 struct PagedPlan {
-    int*    cut_count;     // cut tiles (per KV head), left by the workgroup behind the units' for
-    CutTile* cut_tiles;    // the merge, which then has no geometry to work out
-    float*  records;       // of the units of cut tiles
+    int*     cut_count;    // cut tiles (per KV head) and the list of them, which the workgroup
+    CutTile* cut_tiles;    // behind the units' leaves
+    float*   records;      // of the units of cut tiles
     int32_t max_records;   // per KV head
     int32_t unit_wgs;      // workgroups of units
     int32_t fill;          // units (per KV head) that fill the chip
@@ -647,7 +651,10 @@ __device__ __forceinline__ void narrow_range(const cf_paged_attn_args_t& a, cons
 }
 
 // A wave per unit, the units of neighbouring KV heads in one workgroup: they read the same
-// cache rows at about the same time.
+// cache rows at about the same time.  HBM bounds it: with two blocks of 16 KB under way per
+// wave and four waves a CU it streams 5.7 TB/s over long caches (64 rows over 8192 each, 2.15 GB:
+// 380 us), and 16 sequences of 1778 to 4096 positions (227 MB) take 46 us, 41 of them here, the
+// rest the merge.
 template <typename T, int D> struct Heads {
     static constexpr int WAVES = 4, BK = sizeof(T) == 2 ? 32 : 16;
     static constexpr int RING = Narrow<T, D, BK>::RING;
@@ -694,7 +701,8 @@ void paged_heads(cf_paged_attn_args_t a, PagedPlan pl) {
     }
 }
 
-// Up to 16 rows by all waves of a workgroup: each takes a share of the unit's positions, and
+// Up to 16 rows by all waves of a workgroup (latency bounds it: fp32, a row of 12 heads of 64 over
+// 257, 8.9 us; 16 rows over 512 each 10.9): each takes a share of the unit's positions, and
 // they join their m, l and sums in LDS (WAVES rings at `lds`, one each).  True where rows that
 // this wave finished have to be computed again.
 template <typename T, int D, int TM, int WAVES, int ALL = WAVES>
@@ -823,6 +831,11 @@ __device__ __forceinline__ void put4(const RowOut& out, int d0, f4_t x) {
 // run softmax, then the other way round.  Products of turn i are S(i) = K_i Q^T and
 // O += V_{i-1} P(i-1), so a stage of the ring is K_i with V_{i-1}; with NS stages, NS - 2 of
 // them are still under way when one is needed.
+// NJ = 2: the matrix cores bound it, at what clock they leave (about 2.1 GHz): 2048 rows over 8192,
+// 241 GFLOP in 240 to 260 us (925 to 1000 TFLOP/s; a large library product makes 1097).  NJ = 1
+// halves the tile, not the time of a turn (0.9 us for 1.75): each fragment read from LDS feeds
+// one product, so the LDS bounds it with the turn's latencies.  Waves of 32 rows that share the
+// positions instead take 1.1.
 template <int D, int NJ> struct Wide16 {
     static constexpr int TM = 128 * NJ, BK = 64, NS = 4;
     static constexpr int TILE = BK * D;
@@ -953,7 +966,8 @@ __device__ __forceinline__ uint32_t wide16_unit(const cf_paged_attn_args_t& a, c
         };
         // Fragment x of a turn: x < 2 UT is V^T (32-key step x / UT, dims 16 (x % UT)), the rest K
         // (key tile, then chunk).  They are read kAhead fragments before their products, in
-        // exactly this order: left to itself the compiler reads them all first and spills.
+        // exactly this order: left to itself the compiler reads them all first and spills (so does
+        // 10 ahead: 252 us for 239).
         constexpr int kAhead = 8, kV = 2 * UT, kAll = kV + 4 * NF;
         auto products = [&](int i, auto first_c, auto last_c) {   // fragments first .. last - 1
             constexpr int first = decltype(first_c)::value, last = decltype(last_c)::value;
@@ -1113,7 +1127,7 @@ __device__ __forceinline__ uint32_t wide16_unit(const cf_paged_attn_args_t& a, c
     return again_all;
 }
 
-constexpr int kNarrowCost = 4;
+constexpr int kNarrowCost = 4;    // tiles of 16 rows per wide one, by a block's time: its K and V against its products
 template <int D, int NJ>
 __global__ __launch_bounds__(512, 2)
 void paged_wide16(cf_paged_attn_args_t a, PagedPlan pl) {
@@ -1363,6 +1377,7 @@ void paged_wide32(cf_paged_attn_args_t a, PagedPlan pl) {
 // Joins the ranges of cut tiles: O = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s.  A
 // workgroup per (tile, KV head) and ROWS rows: 256 / ROWS threads per row, D / 4 of them side
 // by side over the dims, the rest sharing the ranges.
+// Latency bounds it: 4 to 5 us, 2 of them any launch's.
 template <typename T, int D, int TM, int ROWS>
 __global__ __launch_bounds__(256)
 void paged_merge(cf_paged_attn_args_t a, PagedPlan pl) {

@@ -120,9 +120,11 @@ typedef struct {
  * sequence b is position p = seq_lens[b] - n + i and attends positions 0 .. p (query head h
  * reads KV head h / (H_q / H_kv)).  A row that sees no position (no page of it is valid, or
  * p < 0) gives 0.  Rows of O outside q_start[0] .. q_start[B] are left as they are; what
- * pages hold past seq_lens[b] is not looked at.  d = 64 and 128 with pages of a multiple of
- * 16 positions, 16-byte aligned pointers and strides and scale > 0 run on the matrix cores,
- * every other call on a plain kernel. */
+ * pages hold past seq_lens[b] is not looked at, and what a row does not see does not touch it,
+ * infinite or NaN either (a row whose tile holds such V is computed a second time, by a slow
+ * loop).  Tables may name a page twice and share pages; O must not overlap an input.  d = 64
+ * and 128 with pages of a multiple of 16 positions, 16-byte aligned pointers and strides and
+ * scale > 0 run on the matrix cores, every other call on a plain kernel. */
 int mha_paged_attn_f32_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
 int mha_paged_attn_f16_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
 
