@@ -104,7 +104,18 @@ struct Geometry {
     SeqRows first;                       // lane: sequence `lane`, kept for the second pass,
     int* kept;                           // by wide tiles in LDS: their registers are all taken
 
-    __device__ __forceinline__ SeqRows rows(int b) const { return b < a.B ? seq_rows(a, b) : SeqRows{0, 0, 0}; }
+    __device__ __forceinline__ SeqRows rows(int b) const {
+        SeqRows s = seq_rows(a, min(b, a.B - 1));
+        if (b >= a.B) s.n = s.len = 0;
+        return s;
+    }
+    // Sequences base + lane, base + 64 + lane, ..: the loads of four wait together (1024 sequences
+    // of 128 positions: 154 us, one at a time 192).
+    static constexpr int kAtOnce = 4;
+    __device__ __forceinline__ void next_rows(int base, SeqRows (&s)[kAtOnce]) const {
+#pragma unroll
+        for (int j = 0; j < kAtOnce; j++) s[j] = rows(base + 64 * j + lane);
+    }
     __device__ __forceinline__ int tiles(const SeqRows& s) const { return (int)(((int64_t)s.n * pl.G + TM - 1) / TM); }
     __device__ __forceinline__ int blocks(const SeqRows& s) const { return (s.len + BK - 1) / BK; }
     __device__ __forceinline__ bool narrow(const SeqRows& s) const { return NARROW > 1 && s.n * pl.G <= 16; }
@@ -120,17 +131,23 @@ struct Geometry {
     __device__ __forceinline__ Geometry(const cf_paged_attn_args_t& a_, const PagedPlan& pl_, int* kept_ = nullptr)
         : a(a_), pl(pl_), kept(kept_) {
         lane = threadIdx.x & 63;
-        first = rows(lane);
+        first = lane < a.B ? seq_rows(a, lane) : SeqRows{0, 0, 0};
         if constexpr (NARROW > 1) {          // every wave writes the same
             kept[lane] = first.row0;
             kept[64 + lane] = first.n;
             kept[128 + lane] = first.len;
         }
         float w = cost(first), t = (float)tiles(first);
-        for (int b = 64; b < a.B; b += 64) {
-            const SeqRows s = rows(b + lane);
-            w += cost(s);
-            t += (float)tiles(s);
+        // (Without cuts and kinds of tiles there is nothing to plan.)
+        const bool plans = NARROW > 1 || pl.one_blocks != INT32_MAX;
+        for (int base = 64; plans && base < a.B; base += 64 * kAtOnce) {
+            SeqRows s[kAtOnce];
+            next_rows(base, s);
+#pragma unroll
+            for (int j = 0; j < kAtOnce; j++) {
+                w += cost(s[j]);
+                t += (float)tiles(s[j]);
+            }
         }
         w = wave_sum(w);
         t = wave_sum(t);
@@ -171,9 +188,7 @@ struct Geometry {
         constexpr int CLASSES = NARROW > 1 ? 2 : 1;
         for (int cls = 0; cls < CLASSES; cls++) {
             int records0 = 0;
-            for (int base = 0; base < a.B; base += 64) {
-                const SeqRows s = base > 0 ? rows(base + lane)
-                                : NARROW > 1 ? SeqRows{kept[lane], kept[64 + lane], kept[128 + lane]} : first;
+            auto scan = [&](const SeqRows& s, int base) {
                 const int t = tiles(s), ns = ranges(s), rec = ns > 1 ? t * ns : 0;
                 const bool cut = __builtin_amdgcn_ballot_w64(ns > 1) != 0;
                 int items = t * ns;
@@ -181,24 +196,34 @@ struct Geometry {
                 const int before = items0 + wave_excl_sum(items, lane);
                 const int rec_before = records0 + (cut ? wave_excl_sum(rec, lane) : 0);
                 const unsigned long long hit = __ballot(before <= u && u < before + items);
-                if (hit) {
-                    const int src = __builtin_ctzll(hit);
-                    const int at = u - __builtin_amdgcn_readlane(before, src);
-                    out.n_ranges = __builtin_amdgcn_readlane(ns, src);
-                    const int nt = __builtin_amdgcn_readlane(t, src);
-                    const int i = out.n_ranges == 1 ? at : at / out.n_ranges;
-                    out.range = at - i * out.n_ranges;
-                    out.tile = nt - 1 - i;                     // the longest first
-                    out.record = __builtin_amdgcn_readlane(rec_before, src) + out.tile * out.n_ranges;
-                    out.b = base + src;
-                    out.s.row0 = __builtin_amdgcn_readlane(s.row0, src);
-                    out.s.n = __builtin_amdgcn_readlane(s.n, src);
-                    out.s.len = __builtin_amdgcn_readlane(s.len, src);
-                    return out.n_ranges == 1 || out.record + out.n_ranges <= pl.max_records;
+                if (!hit) {
+                    items0 = __builtin_amdgcn_readlane(before + items, 63);
+                    records0 = __builtin_amdgcn_readlane(rec_before + rec, 63);
+                    return false;
                 }
-                items0 = __builtin_amdgcn_readlane(before + items, 63);
-                records0 = __builtin_amdgcn_readlane(rec_before + rec, 63);
+                const int src = __builtin_ctzll(hit);
+                const int at = u - __builtin_amdgcn_readlane(before, src);
+                out.n_ranges = __builtin_amdgcn_readlane(ns, src);
+                const int nt = __builtin_amdgcn_readlane(t, src);
+                const int i = out.n_ranges == 1 ? at : at / out.n_ranges;
+                out.range = at - i * out.n_ranges;
+                out.tile = nt - 1 - i;                         // the longest first
+                out.record = __builtin_amdgcn_readlane(rec_before, src) + out.tile * out.n_ranges;
+                out.b = base + src;
+                out.s.row0 = __builtin_amdgcn_readlane(s.row0, src);
+                out.s.n = __builtin_amdgcn_readlane(s.n, src);
+                out.s.len = __builtin_amdgcn_readlane(s.len, src);
+                return true;
+            };
+            bool found = scan(NARROW > 1 ? SeqRows{kept[lane], kept[64 + lane], kept[128 + lane]} : first, 0);
+            for (int base = 64; !found && base < a.B; base += 64 * kAtOnce) {
+                SeqRows s[kAtOnce];
+                next_rows(base, s);
+#pragma unroll
+                for (int j = 0; j < kAtOnce; j++)
+                    if (!found && base + 64 * j < a.B) found = scan(s[j], base + 64 * j);
             }
+            if (found) return out.n_ranges == 1 || out.record + out.n_ranges <= pl.max_records;
         }
         return false;
     }
@@ -1473,17 +1498,16 @@ constexpr int kAnyDims = 512 / 64;             // dims per lane
 template <typename T>
 __global__ __launch_bounds__(256)
 void paged_any(cf_paged_attn_args_t a, FastDiv by_page) {
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int t = (int)(unit / a.H_q), h = (int)(unit - (int64_t)t * a.H_q);
-    if (t >= a.T) return;
-    int lo = 0, hi = a.B;                      // the last sequence that does not start behind t
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.q_start[mid] <= t) lo = mid; else hi = mid;
+    for (int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); unit < (int64_t)a.T * a.H_q; unit += 4 * (int64_t)gridDim.x) {
+        const int t = (int)(unit / a.H_q), h = (int)(unit - (int64_t)t * a.H_q);
+        int lo = 0, hi = a.B;                  // the last sequence that does not start behind t
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (a.q_start[mid] <= t) lo = mid; else hi = mid;
+        }
+        const SeqRows s = seq_rows(a, lo);
+        if (t >= s.row0 && t < s.row0 + s.n) plain_row<T, kAnyDims>(a, by_page, s, lo, t - s.row0, h, a.d);
     }
-    const SeqRows s = seq_rows(a, lo);
-    if (t < s.row0 || t >= s.row0 + s.n) return;
-    plain_row<T, kAnyDims>(a, by_page, s, lo, t - s.row0, h, a.d);
 }
 
 // The plan of a call on the matrix cores: the kernel and how its work is cut.
@@ -1624,8 +1648,8 @@ extern "C" int cf_launch_paged_attn(const cf_paged_attn_args_t* a, void* stream)
         return a->d == 64 ? launch_tiles<float, 64>(*a, p, st) : launch_tiles<float, 128>(*a, p, st);
     }
     const FastDiv by_page = fastdiv_make(a->page_size);
-    const int64_t wgs = ((int64_t)a->T * a->H_q + 3) / 4;
-    if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
+    int64_t wgs = ((int64_t)a->T * a->H_q + 3) / 4;
+    if (wgs > (1 << 22)) wgs = 1 << 22;        // a grid has less than 2^32 threads
     if (a->elem == CF_ELEM_F16) hipLaunchKernelGGL(paged_any<_Float16>, dim3((unsigned)wgs), dim3(256), 0, st, *a, by_page);
     else hipLaunchKernelGGL(paged_any<float>, dim3((unsigned)wgs), dim3(256), 0, st, *a, by_page);
     return (int)hipGetLastError();

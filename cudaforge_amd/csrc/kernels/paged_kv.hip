@@ -233,27 +233,29 @@ void page_map_scan(cf_page_map_args_t a, MapDivs dv) {
 constexpr int kFillThreads = 256;
 __global__ __launch_bounds__(kFillThreads)
 void page_map_fill(cf_page_map_args_t a, MapDivs dv) {
-    const int b = blockIdx.x;
     const int i0 = blockIdx.y * kFillThreads + threadIdx.x, step = gridDim.y * kFillThreads;
-    const uint32_t row0 = (uint32_t)a.q_start[b];
-    if (b == a.B) {
-        for (uint32_t t = row0 + (uint32_t)i0; t < (uint32_t)a.T; t += (uint32_t)step) a.positions[t] = a.slots[t] = -1;
-        return;
-    }
     const RingState r = ring_state((const int32_t*)a.info + 4 * (size_t)a.B, a.ring_size, dv.ring);
-    const int4 v = ((const int4*)a.info)[b];
-    const SeqPages s = {v.x, v.y, v.z, v.w};
-    for (int i = i0; i < s.n && row0 + (uint32_t)i < (uint32_t)a.T; i += step) {
-        const uint32_t t = row0 + (uint32_t)i;
-        a.positions[t] = s.c + i;
-        a.slots[t] = slot_of(a, r, dv, b, s, s.c + i);
+    for (int64_t at = blockIdx.x; at <= a.B; at += gridDim.x) {
+        const int b = (int)at;
+        const uint32_t row0 = (uint32_t)a.q_start[b];
+        if (b == a.B) {
+            for (uint32_t t = row0 + (uint32_t)i0; t < (uint32_t)a.T; t += (uint32_t)step) a.positions[t] = a.slots[t] = -1;
+            return;
+        }
+        const int4 v = ((const int4*)a.info)[b];
+        const SeqPages s = {v.x, v.y, v.z, v.w};
+        for (int i = i0; i < s.n && row0 + (uint32_t)i < (uint32_t)a.T; i += step) {
+            const uint32_t t = row0 + (uint32_t)i;
+            a.positions[t] = s.c + i;
+            a.slots[t] = slot_of(a, r, dv, b, s, s.c + i);
+        }
+        const int before = ceil_pages(s.c, a.page_size, dv.page);
+        const uint32_t len = (uint32_t)s.c + (uint32_t)s.n;
+        const int moves = s.first == kEnded ? before
+                        : (len <= (uint32_t)(a.max_pages * a.page_size) ? ceil_pages((int)len, a.page_size, dv.page)
+                                                                        : a.max_pages) - before;
+        for (int j = i0; j < moves; j += step) move_page(a, r, dv, b, s, j);
     }
-    const int before = ceil_pages(s.c, a.page_size, dv.page);
-    const uint32_t len = (uint32_t)s.c + (uint32_t)s.n;
-    const int moves = s.first == kEnded ? before
-                    : (len <= (uint32_t)(a.max_pages * a.page_size) ? ceil_pages((int)len, a.page_size, dv.page)
-                                                                    : a.max_pages) - before;
-    for (int j = i0; j < moves; j += step) move_page(a, r, dv, b, s, j);
 }
 
 // ------------------------------------------------------------------ store ---
@@ -266,10 +268,10 @@ template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T e[N]; };
 constexpr int kStoreThreads = 256;
 template <typename T, int VEC>
 __global__ __launch_bounds__(kStoreThreads)
-void page_store(cf_page_store_args_t a, FastDiv by_page, FastDiv by_pieces) {
+void page_store(cf_page_store_args_t a, int64_t t0, FastDiv by_page, FastDiv by_pieces) {
     constexpr bool WIDE = VEC * sizeof(T) == 16;
     __shared__ float2 turn[CF_PAGE_ROPE_MAX_DIM / 2];
-    const int64_t t = blockIdx.x;
+    const int64_t t = t0 + blockIdx.x;
     const int slot = a.slots[t];
     const int pos = a.rope ? a.positions[t] : 0;
     if (a.rope) {
@@ -335,12 +337,17 @@ int launch_store(const cf_page_store_args_t& a, hipStream_t st) {
     const uint64_t steps = (uint64_t)a.kv_stride | (uint64_t)a.q_stride | (uint64_t)a.q_out_stride |
                            (uint64_t)a.page_stride | (uint64_t)a.row_stride | (uint64_t)a.head_stride | (uint64_t)a.d;
     const bool wide = ptrs % 16 == 0 && steps % kWide == 0;
-    const dim3 grid((unsigned)a.T), block(kStoreThreads);
     const FastDiv by_page = fastdiv_make(a.page_size);
-    if (wide) hipLaunchKernelGGL((page_store<T, kWide>), grid, block, 0, st, a, by_page, fastdiv_make(a.d / kWide));
-    else if (a.rope) hipLaunchKernelGGL((page_store<T, 2>), grid, block, 0, st, a, by_page, fastdiv_make(a.d / 2));
-    else hipLaunchKernelGGL((page_store<T, 1>), grid, block, 0, st, a, by_page, fastdiv_make(a.d));
-    return (int)hipGetLastError();
+    constexpr int64_t kMost = 1 << 23;             // rows of a launch: a grid has less than 2^32 threads
+    for (int64_t t0 = 0; t0 < a.T; t0 += kMost) {
+        const dim3 grid((unsigned)(a.T - t0 < kMost ? a.T - t0 : kMost)), block(kStoreThreads);
+        if (wide) hipLaunchKernelGGL((page_store<T, kWide>), grid, block, 0, st, a, t0, by_page, fastdiv_make(a.d / kWide));
+        else if (a.rope) hipLaunchKernelGGL((page_store<T, 2>), grid, block, 0, st, a, t0, by_page, fastdiv_make(a.d / 2));
+        else hipLaunchKernelGGL((page_store<T, 1>), grid, block, 0, st, a, t0, by_page, fastdiv_make(a.d));
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return (int)e;
+    }
+    return 0;
 }
 
 }  // namespace
@@ -368,7 +375,7 @@ extern "C" int cf_launch_page_map(const cf_page_map_args_t* a, void* stream) {
     if (e != hipSuccess) return (int)e;
     // Long chunks of few sequences are shared by several workgroups.
     const unsigned parts = (unsigned)(a->T / 2048 < 1 ? 1 : a->T / 2048 > 2048 / a->B ? (2048 / a->B < 1 ? 1 : 2048 / a->B) : a->T / 2048);
-    hipLaunchKernelGGL(page_map_fill, dim3((unsigned)a->B + 1, parts), dim3(kFillThreads), 0, st, *a, dv);
+    hipLaunchKernelGGL(page_map_fill, dim3((unsigned)(a->B < (1 << 20) ? a->B + 1 : 1 << 20), parts), dim3(kFillThreads), 0, st, *a, dv);
     return (int)hipGetLastError();
 }
 

@@ -664,6 +664,59 @@ def test_attention_cut_and_captured(gpu, f16, new):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("new", [[1] * 300, [1] * 259 + [40]])
+def test_attention_of_many_sequences(gpu, f16, new):
+    """More sequences than are looked at together, the last group of them not full, some empty."""
+    past = [(53 * i) % 200 for i in range(len(new))]
+    new = [0 if i % 17 == 5 else n for i, n in enumerate(new)]
+    for H, H_kv, d in ((8, 2, 128), (3, 3, 64)):
+        c = Paged(new, past, H, H_kv, d, 16, f16, seed=15)
+        c.check(c.run(max_new=max(new)))
+        c.check(c.run(max_new=max(new), max_len=max(n + p for n, p in zip(new, past))))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("H,H_kv,d", [(64, 1, 128), (48, 1, 64), (40, 2, 64)])
+def test_attention_of_many_heads_per_group(gpu, f16, H, H_kv, d):
+    """One token's heads alone are more than a narrow tile."""
+    for new, past in (([1, 1], [700, 0]), ([3, 0, 2], [90, 5, 2000])):
+        c = Paged(new, past, H, H_kv, d, 16, f16, seed=17)
+        c.check(c.run(max_new=max(new)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f16", [False, True])
+def test_pages_beyond_32_bits(gpu, f16):
+    """Pages 2^30 bytes apart, the last of them 5 to 6 GB into the buffers: stored there, attended from
+    there, by the matrix cores and by the plain kernel (a stride off the 16-byte grid)."""
+    H, H_kv, d, P, n_pages = 8, 2, 64, 16, 6
+    es = 2 if f16 else 4
+    t = "f16" if f16 else "f32"
+    c = Paged([1, 20], [30, 10], H, H_kv, d, P, f16, seed=19, pad=0, spare=0)
+    assert c.n_pages <= n_pages - 1
+    k, v = (np.concatenate([x[c.table[b, j // P], j % P][None] for b in range(2) for j in range(c.lens[b])])
+            for x in (c.kp, c.vp))
+    for extra in (0, 1):
+        step = (1 << 30) // es + extra
+        caches = [cf.DeviceBuffer(n_pages * (step * es)) for _ in range(2)]
+        far = [5, 4, 3, 2][:c.n_pages]                   # pages from the far end
+        table = np.where(c.table >= 0, np.take(np.array(far + [0], I32), np.maximum(c.table, 0)), -1).astype(I32)
+        slots = np.concatenate([[table[b, j // P] * P + j % P for j in range(c.lens[b])] for b in range(2)]).astype(I32)
+        p = cf.KvPageStoreParams(num_tokens=len(slots), num_heads=0, num_kv_heads=H_kv, head_dim=d, page_size=P,
+                                 num_pages=n_pages, page_stride=step)
+        assert cf.call_op("kv_page_store_%s_cuda" % t, [dev(k), dev(v), dev(slots)], caches, p) == 0
+        c2 = cf.MhaPagedParams(batch_size=2, num_tokens=c.T, num_heads=H, num_kv_heads=H_kv, head_dim=d, scale=c.scale,
+                               page_size=P, num_pages=n_pages, max_pages=c.width, page_stride=step)
+        o = dev(np.full(c.q.shape, 7.0, c.dt))
+        assert cf.call_op(c.op, [dev(c.q)] + caches + [dev(table), dev(c.lens), dev(c.start)], [o], c2) == 0
+        c.check(o.download())
+        for x in caches:
+            x.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f16", [False, True])
 def test_attention_of_a_contiguous_decode_cache(gpu, f16):
     """The cache of MHA_Decode as pages: the same attention as mha_decode_attn."""
     B, H, H_kv, d, cap, P = 5, 32, 8, 128, 512, 32
