@@ -346,8 +346,8 @@ __device__ __forceinline__ void plain_row(const cf_paged_attn_args_t& a, FastDiv
 #pragma unroll
     for (int i = 0; i < DIMS; i++) acc[i] = 0.0f;
 #pragma clang loop unroll(disable)
-    for (int k0 = 0; k0 < seen; k0 += 64) {
-        const int key = k0 + lane;
+    for (uint32_t at0 = 0; at0 < (uint32_t)max(seen, 0); at0 += 64) {    // unsigned: up to 2^31 positions
+        const int k0 = (int)at0, key = k0 + lane;
         int64_t at = 0;
         float x = -INFINITY;
         if (key < seen) {
@@ -1013,8 +1013,10 @@ __device__ __forceinline__ uint32_t wide16_unit(const cf_paged_attn_args_t& a, c
                 constexpr int x = decltype(x_c)::value;
                 const h8_t f = frag[x % kAhead];
                 // O^T += V^T P^T: in 32-key step s2, k-slot e of lane group lq is key
-                // 32 s2 + 16 (e / 4) + 4 lq + e % 4, the lane's own scores.  l comes out of the matrix
-                // cores too, from the same rounded p that weights V.
+                // 32 s2 + 16 (e / 4) + 4 lq + e % 4, the lane's own scores.  p is rounded to fp16, the
+                // type of V and of the product (2^-11 of each weight; together, over many positions, less
+                // than the result's own rounding), and l comes out of the matrix cores too, from the
+                // same rounded p that weights V.
                 if constexpr (x < kV) {
                     if constexpr (x % UT == 0)
 #pragma unroll
@@ -1152,7 +1154,9 @@ __device__ __forceinline__ uint32_t wide16_unit(const cf_paged_attn_args_t& a, c
     return again_all;
 }
 
-constexpr int kNarrowCost = 4;    // tiles of 16 rows per wide one, by a block's time: its K and V against its products
+// Blocks of tiles of up to 16 rows that cost a wide tile's one (31 decode rows beside a chunk of 20
+// rows: 59 us; with 3 or 6: 62 and 65).
+constexpr int kNarrowCost = 4;
 template <int D, int NJ>
 __global__ __launch_bounds__(512, 2)
 void paged_wide16(cf_paged_attn_args_t a, PagedPlan pl) {
