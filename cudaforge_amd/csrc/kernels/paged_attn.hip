@@ -95,7 +95,8 @@ struct Unit {
 
 // The tiles' geometry, one sequence per lane and 64 at a time.  TM rows per tile, BK
 // positions per key block; a tile of up to 16 rows costs 1 / NARROW of a full one's block.
-template <int TM, int BK, int NARROW>
+// CUTS: tiles may be cut.
+template <int TM, int BK, int NARROW, bool CUTS = true>
 struct Geometry {
     const cf_paged_attn_args_t& a;
     const PagedPlan& pl;
@@ -125,7 +126,7 @@ struct Geometry {
     }
     __device__ __forceinline__ int ranges(const SeqRows& s) const {
         const int n = blocks(s);
-        return n <= one ? 1 : (int)((float)(n - 1) * (narrow(s) ? inv_C * (1.0f / NARROW) : inv_C)) + 1;
+        return !CUTS || n <= one ? 1 : (int)((float)(n - 1) * (narrow(s) ? inv_C * (1.0f / NARROW) : inv_C)) + 1;
     }
 
     __device__ __forceinline__ Geometry(const cf_paged_attn_args_t& a_, const PagedPlan& pl_, int* kept_ = nullptr)
@@ -137,6 +138,7 @@ struct Geometry {
             kept[64 + lane] = first.n;
             kept[128 + lane] = first.len;
         }
+        if constexpr (!CUTS) return;
         float w = cost(first), t = (float)tiles(first);
         // (Without cuts and kinds of tiles there is nothing to plan.)
         const bool plans = NARROW > 1 || pl.one_blocks != INT32_MAX;
@@ -727,7 +729,7 @@ void paged_heads(cf_paged_attn_args_t a, PagedPlan pl) {
 }
 
 // Up to 16 rows by all waves of a workgroup (latency bounds it: fp32, a row of 12 heads of 64 over
-// 257, 8.9 us; 16 rows over 512 each 10.9): each takes a share of the unit's positions, and
+// 257, 8.2 us; 16 rows over 512 each 10.3): each takes a share of the unit's positions, and
 // they join their m, l and sums in LDS (WAVES rings at `lds`, one each).  True where rows that
 // this wave finished have to be computed again.
 template <typename T, int D, int TM, int WAVES, int ALL = WAVES>
@@ -812,7 +814,7 @@ __global__ __launch_bounds__(64 * (Split<T, D>::WAVES), (Split<T, D>::WAVES) / 4
 void paged_split(cf_paged_attn_args_t a, PagedPlan pl) {
     constexpr int WAVES = Split<T, D>::WAVES;
     __shared__ __attribute__((aligned(16))) T lds[WAVES * Narrow<T, D, 16>::RING];
-    const Geometry<16, 64, 1> geo(a, pl);
+    const Geometry<16, 64, 1, false> geo(a, pl);
     for (int unit = (int)blockIdx.x;; unit += pl.step) {
         const int id = fastdiv(unit, pl.by_kv), kvh = unit - id * a.H_kv;
         Unit un;
@@ -1014,8 +1016,9 @@ __device__ __forceinline__ uint32_t wide16_unit(const cf_paged_attn_args_t& a, c
                 const h8_t f = frag[x % kAhead];
                 // O^T += V^T P^T: in 32-key step s2, k-slot e of lane group lq is key
                 // 32 s2 + 16 (e / 4) + 4 lq + e % 4, the lane's own scores.  p is rounded to fp16, the
-                // type of V and of the product (2^-11 of each weight; together, over many positions, less
-                // than the result's own rounding), and l comes out of the matrix cores too, from the
+                // type of V and of the product (2^-11 of each weight; over thousands of positions together
+                // about as much as the result's own rounding: 2.9e-4 rms of the values, else 2.1e-4; two
+                // products, as narrow tiles take, would cost a third of the time), and l comes out of the matrix cores too, from the
                 // same rounded p that weights V.
                 if constexpr (x < kV) {
                     if constexpr (x % UT == 0)
@@ -1525,7 +1528,7 @@ struct Plan {
 
 // paged_split for sequences of up to 1024 positions, which it finishes in one range, as long as
 // its units, a workgroup each, go in one round: fp16, 32 heads of 128 over 8, us with paged_split
-// and paged_heads: 1 x 512 9.0 and 11.8, 16 x 512 10.9 and 14.6, 32 x 1024 28.0 and 31.8, 64 x 512
+// and paged_heads: 1 x 512 8.3 and 11.8, 16 x 512 10.3 and 14.6, 32 x 1024 28.0 and 31.8, 64 x 512
 // both 31.3; longer ones need ranges and a merge in both: 8 x 2048 19.8 and 18.2, 16 x 8192 117
 // and 98, 2 x 30000 52.9 and 51.4.
 constexpr int64_t kSplitUnits = 256, kSplitLen = 1024;
