@@ -1016,10 +1016,10 @@ __device__ __forceinline__ uint32_t wide16_unit(const cf_paged_attn_args_t& a, c
                 const h8_t f = frag[x % kAhead];
                 // O^T += V^T P^T: in 32-key step s2, k-slot e of lane group lq is key
                 // 32 s2 + 16 (e / 4) + 4 lq + e % 4, the lane's own scores.  p is rounded to fp16, the
-                // type of V and of the product (2^-11 of each weight; over thousands of positions together
-                // about as much as the result's own rounding: 2.9e-4 rms of the values, else 2.1e-4; two
-                // products, as narrow tiles take, would cost a third of the time), and l comes out of the matrix cores too, from the
-                // same rounded p that weights V.
+                // type of V and of the product: 2^-11 of each weight, over thousands of positions together
+                // about as much as the result's own rounding (2.9e-4 rms of the values, else 2.1e-4;
+                // narrow tiles' second product would be half of all products again).  l comes out of
+                // the matrix cores too, from the same rounded p that weights V.
                 if constexpr (x < kV) {
                     if constexpr (x % UT == 0)
 #pragma unroll
