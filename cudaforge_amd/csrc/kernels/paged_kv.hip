@@ -232,30 +232,28 @@ void page_map_scan(cf_page_map_args_t a, MapDivs dv) {
 // b = B: the rows behind the last token.
 constexpr int kFillThreads = 256;
 __global__ __launch_bounds__(kFillThreads)
-void page_map_fill(cf_page_map_args_t a, MapDivs dv) {
+void page_map_fill(cf_page_map_args_t a, MapDivs dv, int b0) {
+    const int b = b0 + (int)blockIdx.x;
     const int i0 = blockIdx.y * kFillThreads + threadIdx.x, step = gridDim.y * kFillThreads;
-    const RingState r = ring_state((const int32_t*)a.info + 4 * (size_t)a.B, a.ring_size, dv.ring);
-    for (int64_t at = blockIdx.x; at <= a.B; at += gridDim.x) {
-        const int b = (int)at;
-        const uint32_t row0 = (uint32_t)a.q_start[b];
-        if (b == a.B) {
-            for (uint32_t t = row0 + (uint32_t)i0; t < (uint32_t)a.T; t += (uint32_t)step) a.positions[t] = a.slots[t] = -1;
-            return;
-        }
-        const int4 v = ((const int4*)a.info)[b];
-        const SeqPages s = {v.x, v.y, v.z, v.w};
-        for (int i = i0; i < s.n && row0 + (uint32_t)i < (uint32_t)a.T; i += step) {
-            const uint32_t t = row0 + (uint32_t)i;
-            a.positions[t] = s.c + i;
-            a.slots[t] = slot_of(a, r, dv, b, s, s.c + i);
-        }
-        const int before = ceil_pages(s.c, a.page_size, dv.page);
-        const uint32_t len = (uint32_t)s.c + (uint32_t)s.n;
-        const int moves = s.first == kEnded ? before
-                        : (len <= (uint32_t)(a.max_pages * a.page_size) ? ceil_pages((int)len, a.page_size, dv.page)
-                                                                        : a.max_pages) - before;
-        for (int j = i0; j < moves; j += step) move_page(a, r, dv, b, s, j);
+    const uint32_t row0 = (uint32_t)a.q_start[b];
+    if (b == a.B) {
+        for (uint32_t t = row0 + (uint32_t)i0; t < (uint32_t)a.T; t += (uint32_t)step) a.positions[t] = a.slots[t] = -1;
+        return;
     }
+    const RingState r = ring_state((const int32_t*)a.info + 4 * (size_t)a.B, a.ring_size, dv.ring);
+    const int4 v = ((const int4*)a.info)[b];
+    const SeqPages s = {v.x, v.y, v.z, v.w};
+    for (int i = i0; i < s.n && row0 + (uint32_t)i < (uint32_t)a.T; i += step) {
+        const uint32_t t = row0 + (uint32_t)i;
+        a.positions[t] = s.c + i;
+        a.slots[t] = slot_of(a, r, dv, b, s, s.c + i);
+    }
+    const int before = ceil_pages(s.c, a.page_size, dv.page);
+    const uint32_t len = (uint32_t)s.c + (uint32_t)s.n;
+    const int moves = s.first == kEnded ? before
+                    : (len <= (uint32_t)(a.max_pages * a.page_size) ? ceil_pages((int)len, a.page_size, dv.page)
+                                                                    : a.max_pages) - before;
+    for (int j = i0; j < moves; j += step) move_page(a, r, dv, b, s, j);
 }
 
 // ------------------------------------------------------------------ store ---
@@ -375,8 +373,13 @@ extern "C" int cf_launch_page_map(const cf_page_map_args_t* a, void* stream) {
     if (e != hipSuccess) return (int)e;
     // Long chunks of few sequences are shared by several workgroups.
     const unsigned parts = (unsigned)(a->T / 2048 < 1 ? 1 : a->T / 2048 > 2048 / a->B ? (2048 / a->B < 1 ? 1 : 2048 / a->B) : a->T / 2048);
-    hipLaunchKernelGGL(page_map_fill, dim3((unsigned)(a->B < (1 << 20) ? a->B + 1 : 1 << 20), parts), dim3(kFillThreads), 0, st, *a, dv);
-    return (int)hipGetLastError();
+    constexpr int kMost = 1 << 23;                 // sequences of a launch: a grid has less than 2^32 threads
+    for (int64_t b0 = 0; b0 <= a->B; b0 += kMost) {
+        const unsigned n = (unsigned)(a->B + 1 - b0 < kMost ? a->B + 1 - b0 : kMost);
+        hipLaunchKernelGGL(page_map_fill, dim3(n, parts), dim3(kFillThreads), 0, st, *a, dv, (int)b0);
+        if ((e = hipGetLastError()) != hipSuccess) return (int)e;
+    }
+    return 0;
 }
 
 extern "C" int cf_launch_page_store(const cf_page_store_args_t* a, void* stream) {
