@@ -82,7 +82,7 @@ struct PagedPlan {
     int32_t step;          // of the unit loop
     int32_t merge_groups;  // workgroups that share the rows of a tile's merge
     int32_t G;             // query heads per KV head
-    FastDiv by_page, by_group, by_kv;
+    FastDiv by_page, by_group, by_kv, by_groups;
 };
 
 constexpr int kFewOne = 512, kFewMin = 4;    // positions of tiles that are not cut; blocks of a range
@@ -1417,13 +1417,21 @@ void paged_merge(cf_paged_attn_args_t a, PagedPlan pl) {
     static_assert(SUBS >= 1, "rows per workgroup");
     __shared__ float ml[2][ROWS][SUBS];
     __shared__ f4_t part[SUBS > 1 ? SUBS * ROWS * DL : 1];
+    // The first tile's entry comes with the number of them (the list is longer than the grid's tiles).
+    auto place = [&](int unit, int& group, int& kvh) {
+        const int th = fastdiv(unit, pl.by_groups), tile_id = fastdiv(th, pl.by_kv);
+        group = unit - th * pl.merge_groups;
+        kvh = th - tile_id * a.H_kv;
+        return tile_id;
+    };
+    int group, kvh;
+    CutTile un = pl.cut_tiles[place(blockIdx.x, group, kvh)];
     const int cut_units = *pl.cut_count * a.H_kv * pl.merge_groups;
+    asm volatile("" : "+s"(un.record), "+s"(un.n_ranges));
     const int G = pl.G;
     const int d4 = threadIdx.x % DL, sub = threadIdx.x / DL % SUBS, r = threadIdx.x / (DL * SUBS);
     for (int unit = blockIdx.x; unit < cut_units; unit += gridDim.x) {
-        const int th = unit / pl.merge_groups, group = unit - th * pl.merge_groups;
-        const int tile_id = fastdiv(th, pl.by_kv), kvh = th - tile_id * a.H_kv;
-        const CutTile un = pl.cut_tiles[tile_id];
+        if (unit != (int)blockIdx.x) un = pl.cut_tiles[place(unit, group, kvh)];
         const int n_rows = min(un.s.n * G - un.tile * TM, TM);
         const float* const rec = pl.records + ((size_t)un.record * a.H_kv + kvh) * record_floats<TM, D>();
         const size_t step = (size_t)a.H_kv * record_floats<TM, D>();
@@ -1604,6 +1612,7 @@ Plan make_plan(const cf_paged_attn_args_t& a) {
     p.pl.G = (int32_t)G;
     p.pl.by_group = fastdiv_make((int)G);
     p.pl.by_kv = fastdiv_make(a.H_kv);
+    p.pl.by_groups = fastdiv_make(p.pl.merge_groups);
     p.pl.cut_count = nullptr;
     p.pl.cut_tiles = nullptr;
     p.pl.records = nullptr;
