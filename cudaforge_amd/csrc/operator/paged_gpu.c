@@ -146,6 +146,8 @@ static int paged_attn_op(int elem, const void* inputs[], void* outputs[], const 
     cache_strides_t cs;
     if (cache_strides(p->page_stride, p->row_stride, p->head_stride, p->page_size, H_kv, d, &cs) != 0) return -1;
     if (p->batch_size == 0 || p->num_tokens == 0) return 0;
+    /* A row's tile may be read after another's rows are written. */
+    for (int i = 0; i < 3; i++) if (outputs[0] == inputs[i]) return -1;
     cf_paged_attn_args_t a;
     memset(&a, 0, sizeof(a));
     a.q = inputs[0];

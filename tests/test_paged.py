@@ -272,6 +272,13 @@ def test_attn_refuses_missing_arrays(native):
         assert _call(native, op, [DP] * 6, [DP], cf.MhaPagedParams(**dict(ATTN_OK, **{zero: 0}))) == 0
 
 
+@pytest.mark.parametrize("op", ["mha_paged_attn_f16_cuda", "mha_paged_attn_f32_cuda"])
+@pytest.mark.parametrize("same", [0, 1, 2])
+def test_attn_refuses_a_result_over_an_input(native, op, same):
+    ins = [DP + 16 * i for i in range(6)]
+    assert _call(native, op, ins, [ins[same]], cf.MhaPagedParams(**ATTN_OK)) == -1
+
+
 def test_references_agree_on_a_plain_case():
     """The oracle of attention against a softmax written out for one row, and its error bounds
     against a planted mistake: one of 200 positions left out is seen."""
