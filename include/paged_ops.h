@@ -122,9 +122,10 @@ typedef struct {
  * p < 0) gives 0.  Rows of O outside q_start[0] .. q_start[B] are left as they are; what
  * pages hold past seq_lens[b] is not looked at, and what a row does not see does not touch it,
  * infinite or NaN either (a row whose tile holds such V is computed a second time, by a slow
- * loop).  Tables may name a page twice and share pages; O must not overlap an input (-1 where it is Q or a cache).  d = 64
- * and 128 with pages of a multiple of 16 positions, 16-byte aligned pointers and strides and
- * scale > 0 run on the matrix cores, every other call on a plain kernel. */
+ * loop).  Tables may name a page twice and share pages; O must not overlap an input (-1 where
+ * it is Q or a cache).  d = 64 and 128 with pages of a multiple of 16 positions, 16-byte
+ * aligned pointers and strides and scale > 0 run on the matrix cores, every other call on a
+ * plain kernel. */
 int mha_paged_attn_f32_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
 int mha_paged_attn_f16_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
 
