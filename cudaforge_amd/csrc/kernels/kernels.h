@@ -377,7 +377,7 @@ typedef struct {
     int32_t*       positions;
     int32_t*       slots;
     int32_t*       counters_out;
-    int32_t*       info;        /* workspace: cf_page_map_info_ints(B) (the two-launch form) */
+    int32_t*       info;        /* workspace: cf_page_map_info_ints(B, T) (the forms of several launches) */
     int32_t        B, T, page_size, num_pages, max_pages, ring_size;
 } cf_page_map_args_t;
 /* Ints of workspace a launch of this size needs (0: it runs as one workgroup). */

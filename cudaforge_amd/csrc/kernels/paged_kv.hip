@@ -4,8 +4,10 @@
 // need_b = ceil((c_b + n_b) / P) - ceil(c_b / P) pages, the ones at places
 // head + E_b .. of the ring with E_b the sum of need before b; token i of b is at position
 // c_b + i and its slot is page * P + (c_b + i) % P.  Everything but the prefix sums is
-// independent per token and per page.  Launch and latency bound it: 16 sequences 6.4 us, 256
-// with 65000 tokens 9.7, 3000 with 63000 tokens 10.5.
+// independent per token and per page.  A sequence that was not served and whose length counts the
+// tokens all the same (in place) is known by its last entry, which is -1: it gets nothing, and
+// when it ends, what it gives back are the entries that are pages.  Launch and latency bound it: 16 sequences 6.6 us, 256
+// with 65000 tokens 9.5, 3000 with 63000 tokens 14.5.
 //
 // page_store: pages[slot[t]] = row t of K and V, with Q and K turned by their positions.  HBM
 // bounds it: 8192 rows of 32 + 2 x 8 heads of 128 fp16, 201 MB, 41 to 43 us (4.8 TB/s; a large
@@ -29,13 +31,14 @@ constexpr int kMapThreads = 1024;
 constexpr int kMapOneSeqs = 1024;
 constexpr int kMapOneTokens = 4096;
 
-enum { kNotServed = -1, kEnded = -2 };
+enum { kNotServed = -1, kEnded = -2, kEndedGaps = -3 };
 
 // What the tokens and pages of one sequence need to know.
 struct SeqPages {
     int c;         // positions held
     int n;         // new tokens (0 for an ended sequence)
-    int first;     // place of its first new page behind the ring's head, kNotServed or kEnded
+    int first;     // place of its first new page behind the ring's head, kNotServed, kEnded or, where
+                   // some of its entries are no pages, kEndedGaps
     int give;      // ended: place of its first page behind the free ones
 };
 
@@ -58,6 +61,12 @@ __device__ __forceinline__ int ceil_pages(int x, int P, FastDiv by_page) {
     return q + (q * P < x ? 1 : 0);
 }
 
+// Entries of a row of the table that a sequence of len positions needs, the whole row where that is
+// more than it has.
+__device__ __forceinline__ int last_entry(const cf_page_map_args_t& a, FastDiv by_page, uint32_t len) {
+    return len <= (uint32_t)(a.max_pages * a.page_size) ? ceil_pages((int)len, a.page_size, by_page) : a.max_pages;
+}
+
 // The page at place x behind the ring's head (x < avail), or -1 where the ring holds no page.
 __device__ __forceinline__ int ring_page(const cf_page_map_args_t& a, int head, int x, FastDiv by_ring) {
     const int at = head + x;                       // < 2 R
@@ -74,15 +83,59 @@ __device__ __forceinline__ int slot_of(const cf_page_map_args_t& a, const RingSt
     return (unsigned)page < (unsigned)a.num_pages ? page * a.page_size + (pos - idx * a.page_size) : -1;
 }
 
+// A page behind the free ones, at place x of those that this call takes back.  Those that the ring
+// has no place for are left out, as every place holds a free page then.
+__device__ __forceinline__ void give_back(const cf_page_map_args_t& a, const RingState& r, int x, int page) {
+    if (x >= a.ring_size - r.avail) return;
+    const int at = r.tail + x;                     // < 2 R
+    a.ring[at >= a.ring_size ? at - a.ring_size : at] = page;
+}
+
+// The pages among the first n entries of row b of the table, whose sequence has ended (kEndedGaps):
+// by a wave, in their order.
+__device__ __forceinline__ void give_back_gaps(const cf_page_map_args_t& a, const RingState& r, int b, const SeqPages& s,
+                                               int n, int lane) {
+    constexpr int kAtOnce = 4;
+    const int32_t* const row = a.table + (size_t)b * a.max_pages;
+    int place = s.give;
+    for (uint32_t at = 0; at < (uint32_t)n; at += 64 * kAtOnce) {
+        int page[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; k++) page[k] = at + 64 * k + lane < (uint32_t)n ? row[at + 64 * k + lane] : -1;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; k++) {
+            const bool real = (unsigned)page[k] < (unsigned)a.num_pages;
+            const uint64_t all = __builtin_amdgcn_ballot_w64(real);
+            if (real) give_back(a, r, place + __builtin_popcountll(all & ((1ull << lane) - 1)), page[k]);
+            place += __builtin_popcountll(all);
+        }
+    }
+}
+
 // Page j that changes hands with sequence b: into its table, or out of it into the ring.
 __device__ __forceinline__ void move_page(const cf_page_map_args_t& a, const RingState& r, const MapDivs& dv, int b,
                                           const SeqPages& s, int j) {
     int32_t* const row = a.table + (size_t)b * a.max_pages;
     if (s.first == kEnded) {
-        a.ring[(uint32_t)(r.tail + s.give + j) % (uint32_t)a.ring_size] = row[j];
+        give_back(a, r, s.give + j, row[j]);
         return;
     }
     row[ceil_pages(s.c, a.page_size, dv.page) + j] = s.first >= 0 ? ring_page(a, r.head, s.first + j, dv.ring) : -1;
+}
+
+// How many of the first n entries of a row of the table are pages: by a wave, 512 entries at a time.
+__device__ __forceinline__ int count_pages(const cf_page_map_args_t& a, const int32_t* row, int n, int lane) {
+    constexpr int kAtOnce = 8;
+    int count = 0;
+    for (uint32_t at = 0; at < (uint32_t)n; at += 64 * kAtOnce) {
+        int page[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; k++) page[k] = at + 64 * k + lane < (uint32_t)n ? row[at + 64 * k + lane] : -1;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; k++)
+            count += __builtin_popcountll(__builtin_amdgcn_ballot_w64((unsigned)page[k] < (unsigned)a.num_pages));
+    }
+    return count;
 }
 
 // For N rows at once, so that the LDS reads of one do not wait for another's: the last entry of
@@ -101,45 +154,120 @@ __device__ __forceinline__ void last_not_above(const int* start, int n, const in
     }
 }
 
+// What a sequence asks for and gives back.
+struct Asked {
+    int c, n;      // positions held; new tokens, negative for an ended sequence
+    int need;      // new pages, kNotServed where its length passes the table, kStuck where it was not
+                   // served before
+    int back;      // ended: entries of its row that are pages
+};
+enum { kStuck = -2 };
+
+// Those of sequences b0 .. b0 + PER - 1 of each thread of a workgroup of WAVES waves.  The rows of
+// ended sequences are read by all its waves.
+template <int PER, int WAVES> struct EndedList { int n; int2 row[PER * WAVES * 64]; };   // sequence and entries, then pages
+template <int PER, int WAVES>
+__device__ __forceinline__ void ask(const cf_page_map_args_t& a, FastDiv by_page, int b0, Asked (&s)[PER], EndedList<PER, WAVES>& ended) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int P = a.page_size, cap = a.max_pages * P;
+    int raw[PER], last[PER], before[PER], place[PER];
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        raw[j] = b0 + j < a.B ? a.cache_lens[b0 + j] : 0;
+        s[j].n = b0 + j < a.B ? a.new_lens[b0 + j] : 0;
+        s[j].back = 0;
+    }
+    if (tid == 0) ended.n = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        s[j].c = min(max(raw[j], 0), cap);
+        before[j] = ceil_pages(s[j].c, P, by_page);
+        last[j] = 0;
+        if (before[j] > 0) {
+            if (s[j].n >= 0) last[j] = a.table[(size_t)(b0 + j) * a.max_pages + before[j] - 1];
+            else ended.row[place[j] = atomicAdd(&ended.n, 1)] = {b0 + j, before[j]};
+        }
+    }
+    __syncthreads();
+    const int n = ended.n;
+    if (n > 0) {
+        for (int i = wave; i < n; i += WAVES) {
+            const int2 e = ended.row[i];
+            const int got = count_pages(a, a.table + (size_t)e.x * a.max_pages, e.y, lane);
+            if (lane == 0) ended.row[i].y = got;
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        if (s[j].n < 0) {
+            s[j].need = 0;
+            if (before[j] > 0) s[j].back = ended.row[place[j]].y;
+            continue;
+        }
+        const uint32_t len = (uint32_t)s[j].c + (uint32_t)s[j].n;
+        s[j].need = last[j] < 0 || raw[j] > cap ? kStuck : len > (uint32_t)cap ? kNotServed
+                  : ceil_pages((int)len, P, by_page) - before[j];
+    }
+}
+
+// Many sequences: their entries lie on as many lines of memory (3000 sequences: 14.5 us for the three
+// launches; with page_map_scan reading the lines, in two launches, 16.7).
+constexpr int kAskThreads = 64;
+__global__ __launch_bounds__(kAskThreads)
+void page_map_ask(cf_page_map_args_t a, FastDiv by_page) {
+    __shared__ EndedList<1, kAskThreads / 64> ended;
+    const int b = (int)blockIdx.x * kAskThreads + (int)threadIdx.x;
+    Asked s[1];
+    ask(a, by_page, b, s, ended);
+    if (b < a.B) ((int4*)a.info)[b] = int4{s[0].c, s[0].n, s[0].need, s[0].back};
+}
+
 // One workgroup: the prefix sums, PER neighbouring sequences per thread.  ONE (one per
 // thread, up to 1024 sequences and 4096 tokens): it then writes the tokens and pages too, each found by its
 // number in the sums in LDS; else it leaves SeqPages per sequence in a.info for page_map_fill.
-template <bool ONE, int PER>
+// ASKED: a.info holds what page_map_ask left.
+template <bool ONE, int PER, bool ASKED>
 __global__ __launch_bounds__(kMapThreads)
 void page_map_scan(cf_page_map_args_t a, MapDivs dv) {
     constexpr int kWaves = kMapThreads / 64;
     __shared__ int part[4][kWaves];
-    __shared__ int taken_s, refused_s;
+    __shared__ int taken_s, refused_s, gaps_s;
     __shared__ SeqPages seq[ONE ? kMapOneSeqs : 1];
     __shared__ int row0[ONE ? kMapOneSeqs : 1], move0[ONE ? kMapOneSeqs : 1];
+    __shared__ EndedList<ASKED ? 1 : PER, ASKED ? 1 : kWaves> ended_rows;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int P = a.page_size, cap = a.max_pages * P;
+    const int P = a.page_size;
     const RingState r = ring_state(a.counters, a.ring_size, dv.ring);
-    if (tid == 0) taken_s = refused_s = 0;
+    if (tid == 0) taken_s = refused_s = gaps_s = 0;
     int carry[4] = {0, 0, 0, 0};                   // rows, pages needed, taken back, moved
     for (int base = 0; base < a.B; base += PER * kMapThreads) {
-        SeqPages s[PER];
+        Asked ak[PER];
         int v[PER][4], sum[4] = {0, 0, 0, 0}, ex[4];
-        bool ended[PER], fits[PER];
+        bool gaps[PER];
+        if constexpr (ASKED) {
 #pragma unroll
-        for (int j = 0; j < PER; j++) {
-            const int b = base + PER * tid + j;
-            s[j].c = b < a.B ? a.cache_lens[b] : 0;
-            s[j].n = b < a.B ? a.new_lens[b] : 0;
+            for (int j = 0; j < PER; j++) {
+                const int b = base + PER * tid + j;
+                const int4 x = b < a.B ? ((const int4*)a.info)[b] : int4{0, 0, 0, 0};
+                ak[j] = {x.x, x.y, x.z, x.w};
+            }
+        } else {
+            ask(a, dv.page, base + PER * tid, ak, ended_rows);
         }
 #pragma unroll
         for (int j = 0; j < PER; j++) {
-            const bool live = base + PER * tid + j < a.B;
-            ended[j] = s[j].n < 0;
-            s[j].c = min(max(s[j].c, 0), cap);
-            s[j].n = max(s[j].n, 0);
-            const uint32_t len = (uint32_t)s[j].c + (uint32_t)s[j].n;
-            fits[j] = !ended[j] && len <= (uint32_t)cap;
-            const int before = ceil_pages(s[j].c, P, dv.page);
-            v[j][0] = s[j].n;
-            v[j][1] = fits[j] ? ceil_pages((int)len, P, dv.page) - before : 0;
-            v[j][2] = ended[j] ? before : 0;
-            v[j][3] = ended[j] ? before : fits[j] ? v[j][1] : live ? a.max_pages - before : 0;
+            const int before = ceil_pages(ak[j].c, P, dv.page);
+            const uint32_t len = (uint32_t)ak[j].c + (uint32_t)max(ak[j].n, 0);
+            v[j][0] = max(ak[j].n, 0);
+            v[j][1] = max(ak[j].need, 0);
+            v[j][2] = ak[j].back;
+            gaps[j] = ak[j].n < 0 && ak[j].back < before;
+            if constexpr (ONE)
+                v[j][3] = gaps[j] ? 0 : ak[j].n < 0 ? before : base + PER * tid + j < a.B ? last_entry(a, dv.page, len) - before : 0;
+            else
+                v[j][3] = 0;
 #pragma unroll
             for (int k = 0; k < 4; k++) sum[k] += v[j][k];
         }
@@ -161,23 +289,24 @@ void page_map_scan(cf_page_map_args_t a, MapDivs dv) {
 #pragma unroll
         for (int j = 0; j < PER; j++) {
             const int b = base + PER * tid + j;
-            const bool served = fits[j] && (v[j][1] == 0 || ex[1] + v[j][1] <= r.avail);
-            s[j].first = ended[j] ? kEnded : served ? ex[1] : kNotServed;
-            s[j].give = ex[2];
+            const bool ended = ak[j].n < 0;
+            const bool served = !ended && (ak[j].need == 0 || (ak[j].need > 0 && ex[1] + ak[j].need <= r.avail));
+            const SeqPages s = {ak[j].c, max(ak[j].n, 0), gaps[j] ? kEndedGaps : ended ? kEnded : served ? ex[1] : kNotServed, ex[2]};
             // Ends of what is taken rise with the sequences: the last one's counts.
             const uint64_t takes = __builtin_amdgcn_ballot_w64(served && v[j][1] > 0);
-            const uint64_t refused = __builtin_amdgcn_ballot_w64(b < a.B && !served && !ended[j]);
+            const uint64_t refused = __builtin_amdgcn_ballot_w64(b < a.B && !served && !ended);
             if (takes && lane == 63 - __builtin_clzll(takes)) atomicMax(&taken_s, ex[1] + v[j][1]);
             if (refused && lane == 0) atomicAdd(&refused_s, __builtin_popcountll(refused));
+            if (ONE && gaps[j]) gaps_s = 1;
             if (b < a.B) {
-                a.seq_lens[b] = ended[j] ? 0 : (int)min((uint32_t)s[j].c + (uint32_t)s[j].n, 0x7fffffffu);
+                a.seq_lens[b] = ended ? 0 : ak[j].need == kStuck ? a.cache_lens[b] : (int)min((uint32_t)s.c + (uint32_t)s.n, 0x7fffffffu);
                 a.q_start[b] = ex[0];
                 if constexpr (ONE) {
-                    seq[b] = s[j];
+                    seq[b] = s;
                     row0[b] = ex[0];
                     move0[b] = ex[3];
                 } else {
-                    ((int4*)a.info)[b] = int4{s[j].c, s[j].n, s[j].first, s[j].give};
+                    ((int4*)a.info)[b] = int4{s.c, s.n, s.first, s.give};
                 }
             }
 #pragma unroll
@@ -193,7 +322,7 @@ void page_map_scan(cf_page_map_args_t a, MapDivs dv) {
         }
         const int head = r.head + taken_s;         // < 2 R
         a.counters_out[0] = head - fastdiv(head, dv.ring) * a.ring_size;
-        a.counters_out[1] = (int)min((uint32_t)(r.avail - taken_s) + (uint32_t)carry[2], (uint32_t)a.ring_size);
+        a.counters_out[1] = r.avail - taken_s + min(carry[2], a.ring_size - r.avail);
         a.counters_out[2] = refused_s;
     }
     if constexpr (ONE) {
@@ -225,6 +354,8 @@ void page_map_scan(cf_page_map_args_t a, MapDivs dv) {
             last_not_above(move0, a.B, x, at);
             move_page(a, r, dv, at[0], seq[at[0]], i - move0[at[0]]);
         }
+        for (int b = gaps_s ? wave : a.B; b < a.B; b += kWaves)
+            if (seq[b].first == kEndedGaps) give_back_gaps(a, r, b, seq[b], ceil_pages(seq[b].c, P, dv.page), lane);
     }
 }
 
@@ -249,10 +380,11 @@ void page_map_fill(cf_page_map_args_t a, MapDivs dv, int b0) {
         a.slots[t] = slot_of(a, r, dv, b, s, s.c + i);
     }
     const int before = ceil_pages(s.c, a.page_size, dv.page);
-    const uint32_t len = (uint32_t)s.c + (uint32_t)s.n;
-    const int moves = s.first == kEnded ? before
-                    : (len <= (uint32_t)(a.max_pages * a.page_size) ? ceil_pages((int)len, a.page_size, dv.page)
-                                                                    : a.max_pages) - before;
+    if (s.first == kEndedGaps) {
+        if (blockIdx.y == 0 && threadIdx.x < 64) give_back_gaps(a, r, b, s, before, threadIdx.x);
+        return;
+    }
+    const int moves = s.first == kEnded ? before : last_entry(a, dv.page, (uint32_t)s.c + (uint32_t)s.n) - before;
     for (int j = i0; j < moves; j += step) move_page(a, r, dv, b, s, j);
 }
 
@@ -350,7 +482,7 @@ int launch_store(const cf_page_store_args_t& a, hipStream_t st) {
 
 }  // namespace
 
-// Two launches need, per sequence, SeqPages, and once the ring's counters as they were.
+// Several launches need, per sequence, Asked or SeqPages, and once the ring's counters as they were.
 extern "C" size_t cf_page_map_info_ints(int32_t B, int32_t T) {
     return B <= kMapOneSeqs && T <= kMapOneTokens ? 0 : 4 * (size_t)B + 2;
 }
@@ -361,16 +493,20 @@ extern "C" int cf_launch_page_map(const cf_page_map_args_t* a, void* stream) {
         return (int)hipErrorInvalidValue;
     const MapDivs dv = {fastdiv_make(a->page_size), fastdiv_make(a->ring_size)};
     if (cf_page_map_info_ints(a->B, a->T) == 0) {
-        hipLaunchKernelGGL((page_map_scan<true, 1>), dim3(1), dim3(kMapThreads), 0, st, *a, dv);
+        hipLaunchKernelGGL((page_map_scan<true, 1, false>), dim3(1), dim3(kMapThreads), 0, st, *a, dv);
         return (int)hipGetLastError();
     }
     if (!a->info) return (int)hipErrorInvalidValue;
-    // Four sequences a thread for more than a workgroup has threads: their loads wait together
-    // (3000 sequences: 11.6 us for both launches, one at a time 17; 256: 13 us, one at a time 11).
-    if (a->B <= kMapThreads) hipLaunchKernelGGL((page_map_scan<false, 1>), dim3(1), dim3(kMapThreads), 0, st, *a, dv);
-    else hipLaunchKernelGGL((page_map_scan<false, 4>), dim3(1), dim3(kMapThreads), 0, st, *a, dv);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return (int)e;
+    // Four sequences a thread for more than a workgroup has threads: their loads wait together.
+    hipError_t e;
+    if (a->B <= kMapThreads) {
+        hipLaunchKernelGGL((page_map_scan<false, 1, false>), dim3(1), dim3(kMapThreads), 0, st, *a, dv);
+    } else {
+        hipLaunchKernelGGL(page_map_ask, dim3((unsigned)((a->B - 1) / kAskThreads + 1)), dim3(kAskThreads), 0, st, *a, dv.page);
+        if ((e = hipGetLastError()) != hipSuccess) return (int)e;
+        hipLaunchKernelGGL((page_map_scan<false, 4, true>), dim3(1), dim3(kMapThreads), 0, st, *a, dv);
+    }
+    if ((e = hipGetLastError()) != hipSuccess) return (int)e;
     // Long chunks of few sequences are shared by several workgroups.
     const unsigned parts = (unsigned)(a->T / 2048 < 1 ? 1 : a->T / 2048 > 2048 / a->B ? (2048 / a->B < 1 ? 1 : 2048 / a->B) : a->T / 2048);
     constexpr int kMost = 1 << 23;                 // sequences of a launch: a grid has less than 2^32 threads

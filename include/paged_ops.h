@@ -58,8 +58,15 @@ typedef struct {
  * served when the pages asked for up to and with it outnumber the free ones (pages that
  * this call takes back count from the next call on), or when its length passes the table:
  * it then takes none, its table entries from the first new page on (to the end of the row
- * where the length passes it) and its slots are -1, and a later call with the same
- * cache_len tries again.  The others are not affected. */
+ * where the length passes it) and its slots are -1.  The others are not affected.  A later
+ * call with the same cache_len tries again (new_lens 0 for those that were served).
+ * seq_lens counts the tokens of a sequence that is not served too.  Where it is cache_lens,
+ * the entry is therefore no longer what the sequence holds; the caller sets it back before
+ * it tries again.  Until then the sequence is known by what it lacks (the entry of its last
+ * position is negative, or its length passes the table): each call counts it as not served,
+ * asks no page for it and leaves its length.  In either state it can be ended: an ended
+ * sequence gives back those of its ceil(cache_len / page_size) entries that are pages, as
+ * far as the ring has places.  No other sequence may hold them. */
 int kv_page_map_i32_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
 
 /* ---- new rows into the pages ---- */
