@@ -348,11 +348,11 @@ void page_map_scan(cf_page_map_args_t a, MapDivs dv) {
                     a.slots[t[j]] = slot[j];
                 }
         }
-        for (int i = tid; i < carry[3]; i += kMapThreads) {
-            const int x[1] = {i};
+        for (uint32_t i = tid; i < (uint32_t)carry[3]; i += kMapThreads) {   // unsigned: up to 2^31 - 1 of them
+            const int x[1] = {(int)i};
             int at[1];
             last_not_above(move0, a.B, x, at);
-            move_page(a, r, dv, at[0], seq[at[0]], i - move0[at[0]]);
+            move_page(a, r, dv, at[0], seq[at[0]], (int)i - move0[at[0]]);
         }
         for (int b = gaps_s ? wave : a.B; b < a.B; b += kWaves)
             if (seq[b].first == kEndedGaps) give_back_gaps(a, r, b, seq[b], ceil_pages(seq[b].c, P, dv.page), lane);
@@ -365,19 +365,19 @@ constexpr int kFillThreads = 256;
 __global__ __launch_bounds__(kFillThreads)
 void page_map_fill(cf_page_map_args_t a, MapDivs dv, int b0) {
     const int b = b0 + (int)blockIdx.x;
-    const int i0 = blockIdx.y * kFillThreads + threadIdx.x, step = gridDim.y * kFillThreads;
+    const uint32_t i0 = blockIdx.y * kFillThreads + threadIdx.x, step = gridDim.y * kFillThreads;
     const uint32_t row0 = (uint32_t)a.q_start[b];
     if (b == a.B) {
-        for (uint32_t t = row0 + (uint32_t)i0; t < (uint32_t)a.T; t += (uint32_t)step) a.positions[t] = a.slots[t] = -1;
+        for (uint32_t t = row0 + i0; t < (uint32_t)a.T; t += step) a.positions[t] = a.slots[t] = -1;
         return;
     }
     const RingState r = ring_state((const int32_t*)a.info + 4 * (size_t)a.B, a.ring_size, dv.ring);
     const int4 v = ((const int4*)a.info)[b];
     const SeqPages s = {v.x, v.y, v.z, v.w};
-    for (int i = i0; i < s.n && row0 + (uint32_t)i < (uint32_t)a.T; i += step) {
-        const uint32_t t = row0 + (uint32_t)i;
-        a.positions[t] = s.c + i;
-        a.slots[t] = slot_of(a, r, dv, b, s, s.c + i);
+    for (uint32_t i = i0; i < (uint32_t)s.n && row0 + i < (uint32_t)a.T; i += step) {
+        const uint32_t t = row0 + i;
+        a.positions[t] = s.c + (int)i;
+        a.slots[t] = slot_of(a, r, dv, b, s, s.c + (int)i);
     }
     const int before = ceil_pages(s.c, a.page_size, dv.page);
     if (s.first == kEndedGaps) {
@@ -385,7 +385,7 @@ void page_map_fill(cf_page_map_args_t a, MapDivs dv, int b0) {
         return;
     }
     const int moves = s.first == kEnded ? before : last_entry(a, dv.page, (uint32_t)s.c + (uint32_t)s.n) - before;
-    for (int j = i0; j < moves; j += step) move_page(a, r, dv, b, s, j);
+    for (uint32_t j = i0; j < (uint32_t)moves; j += step) move_page(a, r, dv, b, s, (int)j);
 }
 
 // ------------------------------------------------------------------ store ---

@@ -249,3 +249,29 @@ def test_many_steps_with_too_few_pages(gpu, T, B):
         seen += len(s.step([int(x) for x in new], run))
     assert seen > 10
     end()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", FORMS)
+def test_a_row_of_almost_2_to_the_31_entries(gpu, T):
+    """The longest row there can be, all of whose entries a request that is not served takes away
+    (8 GiB): up to its end and not past it."""
+    width, tail = 2 ** 31 - 1, 4096
+    table = cf.DeviceBuffer(4 * (width + tail), I32)
+    table.fill_zero()
+    counters, ring, lens, new = (dev(np.array(x, I32)) for x in ([0, 3, 0], [5, 6, 7, 8], [1], [width]))
+    start, pos, slots = (dev(np.full(k, 77, I32)) for k in (2, T, T))
+    p = cf.KvPageMapParams(batch_size=1, num_tokens=T, page_size=1, num_pages=9, max_pages=width, ring_size=4)
+    assert cf.call_op("kv_page_map_i32_cuda", [lens, new, counters], [table, ring, lens, start, pos, slots, counters], p) == 0
+    assert list(counters.download()) == [0, 3, 1] and list(lens.download()) == [width]
+    assert (slots.download() == -1).all() and (pos.download() == 1 + np.arange(T)).all()
+
+    def entries(first, n):
+        out = np.empty(n, I32)
+        assert gpu.gpu_memcpy_d2h(out.ctypes.data, table.ptr + 4 * first, 4 * n, None) == 0
+        return out
+    assert entries(0, 1)[0] == 0
+    for first in (1, 2 ** 30 - 2048, 2 ** 31 - 1 - 4096):
+        assert (entries(first, 4096) == -1).all()
+    assert (entries(width, tail) == 0).all()
+    table.free()
