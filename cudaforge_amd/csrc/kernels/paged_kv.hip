@@ -26,8 +26,11 @@ using namespace cdna4;
 // ------------------------------------------------------------------ map ---
 
 constexpr int kMapThreads = 1024;
-// The one-workgroup form: one sequence and four rows per thread (6.4 to 7.7 us over that range; by
-// two launches 9.4 to 9.6).
+// The one-workgroup form: one sequence and four rows per thread (6.5 to 8 us over that range; by
+// two launches 9.5 to 11.5).  It moves the pages of ended sequences too, at about 1 us per thousand
+// more than two launches (64 requests of 512 pages ending at once: 31 and 11.5 us; 1024 of them 530
+// and 83).  Pages come back as fast as tokens fill them, at most 4096 / page_size a step in the
+// long run, so that costs less than the second launch for every step would.
 constexpr int kMapOneSeqs = 1024;
 constexpr int kMapOneTokens = 4096;
 
