@@ -75,6 +75,8 @@ static int page_store_op(int elem, const void* inputs[], void* outputs[], const 
     const kv_page_store_params_t* p = (const kv_page_store_params_t*)params;
     if (p->num_tokens < 0 || p->num_kv_heads <= 0 || p->head_dim <= 0 || !pages_ok(p->page_size, p->num_pages)) return -1;
     if (p->num_tokens > INT32_MAX || p->num_kv_heads > 65535 || p->head_dim > 65535) return -1;
+    /* The kernel counts the pieces of a K and a V row together in 32 bits. */
+    if (p->num_kv_heads * p->head_dim > (1 << 29)) return -1;
     if (!(p->rope_base >= 0.0f) || isinf(p->rope_base)) return -1;
     if (p->q_stride < 0 || p->kv_stride < 0 || p->q_out_stride < 0) return -1;
     cf_page_store_args_t a;

@@ -75,7 +75,7 @@ typedef struct {
     int64_t num_tokens;    /* T */
     int64_t num_heads;     /* H_q (read with a Q only) */
     int64_t num_kv_heads;  /* H_kv */
-    int64_t head_dim;      /* d; with RoPE even and at most 256 */
+    int64_t head_dim;      /* d; with RoPE even and at most 256; H_kv d at most 2^29 */
     int64_t page_size;
     int64_t num_pages;
     float   rope_base;     /* > 0: Q and K are rotated; 0: rows are stored as they are */
