@@ -97,6 +97,7 @@ static int page_store_op(int elem, const void* inputs[], void* outputs[], const 
             a.H_q = (int32_t)p->num_heads;
             a.q_stride = p->q_stride > 0 ? p->q_stride : p->num_heads * p->head_dim;
             a.q_out_stride = p->q_out_stride > 0 ? p->q_out_stride : p->num_heads * p->head_dim;
+            if (a.q_out == a.q && a.q_out_stride != a.q_stride) return -1;
         }
         /* In turns, so that the kernel reduces an angle by dropping whole numbers; one power and
          * products of 64 bits of mantissa (128 of them are off by 2^-57), as a power per pair

@@ -90,7 +90,7 @@ typedef struct {
 } kv_page_store_params_t;
 
 /* inputs  [K_new (T, H_kv, d), V_new (T, H_kv, d), slots (T), positions (T) (RoPE), Q (T, H_q, d) (RoPE)]
- * outputs [K_pages, V_pages, Q_rotated (T, H_q, d), may be Q]
+ * outputs [K_pages, V_pages, Q_rotated (T, H_q, d), may be Q (with one stride, else -1)]
  * With rope_base = 0 the last two inputs and the last output are not looked at (the arrays may
  * end before them); with RoPE either Q and Q_rotated are both given or both NULL.  Pairs
  * (2i, 2i + 1) turn by position * base^(-2i / d), the angle reduced in 64 bits and the
