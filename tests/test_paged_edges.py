@@ -1,0 +1,78 @@
+"""mha_paged_attn_{f16,f32}_cuda at the edges of what its arrays may hold, against the 64-bit oracle and
+the tolerances of test_paged.py (GPU)."""
+
+import math
+
+import numpy as np
+import pytest
+
+import cudaforge_amd as cf
+from helpers import dev
+from test_paged import I32, Paged, ref_attn
+
+SHAPES = [(8, 2, 64, 16), (8, 2, 128, 32), (16, 1, 64, 16), (5, 5, 33, 7)]     # the last: the plain kernel
+
+
+def fill(c, seed=99):
+    """Finite values where Paged leaves NaN: every position of every page."""
+    rng = np.random.default_rng(seed)
+    for x in (c.kp, c.vp):
+        x[np.isnan(x)] = rng.standard_normal(int(np.isnan(x).sum())).astype(c.dt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("H,H_kv,d,P", SHAPES)
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 1, 2], [40, 1, 33]])
+def test_lengths_past_the_table(gpu, f16, H, H_kv, d, P, new):
+    """A length past its table's row is the row's: its rows are the last positions of it."""
+    c = Paged(new, [90, 300, 20], H, H_kv, d, P, f16, seed=23)
+    fill(c)
+    rng = np.random.default_rng(5)
+    held = c.table >= 0
+    c.table[~held] = rng.integers(0, c.n_pages, int((~held).sum()))           # pages of others: shared
+    full = c.width * P
+    for past in (full + 1, 2 ** 30, 2 ** 31 - 1):
+        c.lens[:] = [past, full, min(past, full + 7)]
+        got = c.run(max_new=max(new))
+        assert not np.isnan(ref_attn(c.q, c.kp, c.vp, c.table, c.lens, c.start, c.scale)[0][:c.start[-1]]).any()
+        c.check(got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("H,H_kv,d,P", SHAPES)
+@pytest.mark.parametrize("wide", [False, True])
+def test_offsets_past_the_rows(gpu, f16, H, H_kv, d, P, wide):
+    """Offsets below 0 and behind the last row are clamped: a sequence has the rows between."""
+    c = Paged([4, 40 if wide else 4, 3, 2], [90, 150, 60, 33], H, H_kv, d, P, f16, seed=25, pad=0)
+    fill(c)
+    for start in ([-4, 4, c.T - 5, 10 ** 6, 2 ** 31 - 1], [-2 ** 31, -7, 5, c.T, c.T + 9], [0, 0, c.T, c.T, c.T],
+                  [3, 4, 6, 6, c.T - 2]):
+        c.start = np.array(start, I32)
+        c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("H,H_kv,d,P", SHAPES)
+@pytest.mark.parametrize("n", [4, 40])
+def test_offsets_out_of_order(gpu, f16, H, H_kv, d, P, n):
+    """Offsets that fall: the sequence that ends before it starts has no rows, the next one has the
+    rows from its offset on.  Rows of one sequence only are that sequence's, rows of none are left."""
+    c = Paged([n, 3, n, 2], [90, 40, 60, 33], H, H_kv, d, P, f16, seed=27)
+    fill(c)
+    a, b = c.start[1], c.start[1] - 2
+    c.start = np.array([0, a, b, b + n, b + n + 2], I32)                      # rows b .. a - 1: two sequences'
+    got = c.run(max_new=n)
+    want, e32, e16 = ref_attn(c.q, c.kp, c.vp, c.table, c.lens, c.start, c.scale)
+    first = c.start.copy()
+    first[2:] = [a] * 3                                                       # the first sequence alone
+    other = ref_attn(c.q, c.kp, c.vp, c.table, c.lens, first, c.scale)[0]
+    tol = e16 + 2.0 ** -11 * np.abs(want) + 2.0 ** -25 if f16 else e32 + 2.0 ** -24 * np.abs(want)
+    alone = np.r_[0:b, a:b + n + 2]
+    assert (np.abs(got[alone] - want[alone]) <= tol[alone]).all()
+    both = got[b:a].astype(np.float64)
+    near = lambda x: np.abs(both - x) <= 4 * tol[b:a] + 2.0 ** -9 * np.abs(x)
+    assert (near(want[b:a]) | near(other[b:a])).all()
+    assert (got[b + n + 2:] == 7.0).all()
