@@ -76,3 +76,22 @@ def test_offsets_out_of_order(gpu, f16, H, H_kv, d, P, n):
     near = lambda x: np.abs(both - x) <= 4 * tol[b:a] + 2.0 ** -9 * np.abs(x)
     assert (near(want[b:a]) | near(other[b:a])).all()
     assert (got[b + n + 2:] == 7.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f16", [True])
+@pytest.mark.parametrize("H,H_kv,d,P", SHAPES[:3])
+@pytest.mark.parametrize("n", [1, 9, 100])
+@pytest.mark.parametrize("far", [9.0, 14.0, 17.6, 20.0])
+def test_many_small_weights_beside_a_large_one(gpu, f16, H, H_kv, d, P, n, far):
+    """One position scores `far` above some ten thousand equal ones: each of them weighs e^-far of it,
+    below what fp16 holds beside 1 (2^-25 = e^-17.3), all together as much as the tolerance many times."""
+    c = Paged([n], [12000 - n], H, H_kv, d, P, f16, seed=31, pad=0)
+    rng = np.random.default_rng(3)
+    c.q[:] = 1
+    c.kp[:] = 0
+    c.vp[:] = (1 + rng.random(c.vp.shape) / 4).astype(c.dt)
+    c.kp[c.table[0, 0], 0] = far / (c.scale * d)
+    c.vp[c.table[0, 0], 0] = 0
+    for hint in (0, 1):                                  # the positions shared out, and in one range
+        c.check(c.run(max_new=n, max_len=hint))
