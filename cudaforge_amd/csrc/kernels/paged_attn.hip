@@ -480,6 +480,19 @@ __device__ __forceinline__ bool move_max(float mloc, float& m, float& alpha) {
     return true;
 }
 
+// A sum of many terms with what its roundings drop (x + y = s + e exactly): l of a long context whose
+// positions weigh too little, each for itself, to be seen beside one that weighs more.
+struct LongSum {
+    float s = 0.0f, e = 0.0f;
+    __device__ __forceinline__ void add(float x) {
+        const float t = s + x, y = t - s;
+        e += (s - (t - y)) + (x - y);
+        s = t;
+    }
+    __device__ __forceinline__ void scale(float x) { s *= x; e *= x; }
+    __device__ __forceinline__ float sum() const { return s + e; }
+};
+
 // Scores of a lane's row in a block: key 16 t + 4 lq + i of it counts where its bit of `mk` is
 // set and it is one of the first `seen`.  Bit by bit in vector registers: comparisons would
 // take a pair of scalar registers per score.
@@ -524,6 +537,7 @@ __device__ __forceinline__ void narrow_range(const cf_paged_attn_args_t& a, cons
     for (int u = 0; u < UT; u++) acc[u] = f4_t{0.f, 0.f, 0.f, 0.f};
     m_run = -INFINITY;
     l_run = 0.0f;
+    LongSum l;
     const int nblk = key1 > key0 ? (key1 - key0 + BK - 1) / BK : 0;
     if (nblk == 0) return;
     const float c = a.scale * kLog2e;
@@ -627,18 +641,19 @@ __device__ __forceinline__ void narrow_range(const cf_paged_attn_args_t& a, cons
         mloc = low_max(max_xor32(max_xor16(mloc)), c);         // -inf if the row sees nothing here
         float alpha;
         if (move_max(mloc, m_run, alpha)) {
-            l_run *= alpha;
+            l.scale(alpha);
 #pragma unroll
             for (int u = 0; u < UT; u++) acc[u] *= alpha;
         }
         const float m_use = m_run == -INFINITY ? 0.0f : m_run;
         _Float16 hi[F16 ? 4 * NG : 1], lo[F16 ? 4 * NG : 1];
+        float l_blk = 0.0f;
 #pragma unroll
         for (int t = 0; t < NG; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], c, -m_use));
-                l_run += p;
+                l_blk += p;
                 if constexpr (F16) {
                     hi[4 * t + i] = (_Float16)p;
                     lo[4 * t + i] = (_Float16)(p - (float)hi[4 * t + i]);
@@ -646,6 +661,7 @@ __device__ __forceinline__ void narrow_range(const cf_paged_attn_args_t& a, cons
                     sc[t][i] = p;
                 }
             }
+        l.add(l_blk);
         // O^T += V^T P^T, the lane's own scores being its B operand.  This wave waits on memory,
         // not on products: p as the sum of two fp16 numbers, so that its rounding (2^-11 of it,
         // otherwise as large as the result's own) leaves the result.
@@ -679,6 +695,7 @@ __device__ __forceinline__ void narrow_range(const cf_paged_attn_args_t& a, cons
         }
     };
     for_each_stage<NS>(nblk, step);
+    l_run = l.sum();
 }
 
 // A wave per unit, the units of neighbouring KV heads in one workgroup: they read the same
@@ -1223,7 +1240,8 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
     const int seen = min(w.base + fastdiv(w.R0 + min(wrow + lr, w.n_rows - 1), pl.by_group), un.s.len);
     const int seen_all = min(w.base + fastdiv(w.R0 + min(wrow, w.n_rows - 1), pl.by_group), un.s.len);
     f4_t acc[UT];
-    float m_run = -INFINITY, l_run = 0.0f;
+    float m_run = -INFINITY;
+    LongSum l_run;
 #pragma unroll
     for (int u = 0; u < UT; u++) acc[u] = f4_t{0.f, 0.f, 0.f, 0.f};
     if (n > 0) {
@@ -1324,18 +1342,20 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
             mloc = low_max(max_xor32(max_xor16(mloc)), c);
             float alpha;
             if (move_max(mloc, m_run, alpha)) {
-                l_run *= alpha;
+                l_run.scale(alpha);
 #pragma unroll
                 for (int u = 0; u < UT; u++) acc[u] *= alpha;
             }
             const float m_use = m_run == -INFINITY ? 0.0f : m_run;
+            float l_blk = 0.0f;
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     sc[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][e], c, -m_use));
-                    l_run += sc[t][e];
+                    l_blk += sc[t][e];
                 }
+            l_run.add(l_blk);
             // In step kk of key tile t, k-slot lq is key 16 t + 4 lq + kk: the lane's own score.
             float vf[2][UT];
             auto read_v = [&](auto g_c) {
@@ -1356,7 +1376,7 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
         for_each_stage<NS>(n, step);
         if (W::KS > 1) __builtin_amdgcn_s_setprio(0);
     }
-    float l = add_xor32(add_xor16(l_run));
+    float l = add_xor32(add_xor16(l_run.sum()));
     ring_barrier();                                           // the ring's reads
     if constexpr (W::KS > 1) {
         // The second waves' m, l and sums, through the ring.

@@ -79,8 +79,8 @@ def test_offsets_out_of_order(gpu, f16, H, H_kv, d, P, n):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("f16", [True])
-@pytest.mark.parametrize("H,H_kv,d,P", SHAPES[:3])
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("H,H_kv,d,P", SHAPES)
 @pytest.mark.parametrize("n", [1, 9, 100])
 @pytest.mark.parametrize("far", [9.0, 14.0, 17.6, 20.0])
 def test_many_small_weights_beside_a_large_one(gpu, f16, H, H_kv, d, P, n, far):
