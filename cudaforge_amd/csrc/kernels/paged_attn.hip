@@ -333,12 +333,14 @@ template <typename T, int D> __device__ __forceinline__ int vswz(int row) {
 }
 
 // ---- One row of one head by a wave, 64 positions at a time: lanes are positions for the
-// scores and dims (at most 64 DIMS) for the sum over V. ----
+// scores and dims (at most 64 DIMS) for the sum over V.  Of positions [key0, key1); into O, or into a
+// record whose m, l and sum for this row start at rec, rec + tm and rec_sum. ----
 template <typename T, int DIMS>
 __device__ __forceinline__ void plain_row(const cf_paged_attn_args_t& a, FastDiv by_page, const SeqRows& s, int b, int tok,
-                                          int h, int d) {
+                                          int h, int d, int key0 = 0, int key1 = INT32_MAX, float* rec = nullptr, int tm = 0,
+                                          float* rec_sum = nullptr) {
     const int lane = threadIdx.x & 63;
-    const int seen = min(s.len - s.n + tok + 1, s.len);
+    const int seen = min(min(s.len - s.n + tok + 1, s.len), key1);
     const int32_t* const table = a.table + (size_t)b * a.max_pages;
     const T* const q = (const T*)a.q + (int64_t)(s.row0 + tok) * a.q_stride + (int64_t)h * d;
     const T* const k = (const T*)a.k + (int64_t)(h / (a.H_q / a.H_kv)) * a.head_stride;
@@ -348,7 +350,7 @@ __device__ __forceinline__ void plain_row(const cf_paged_attn_args_t& a, FastDiv
 #pragma unroll
     for (int i = 0; i < DIMS; i++) acc[i] = 0.0f;
 #pragma clang loop unroll(disable)
-    for (uint32_t at0 = 0; at0 < (uint32_t)max(seen, 0); at0 += 64) {    // unsigned: up to 2^31 positions
+    for (uint32_t at0 = (uint32_t)key0; at0 < (uint32_t)max(seen, 0); at0 += 64) {    // unsigned: up to 2^31 positions
         const int k0 = (int)at0, key = k0 + lane;
         int64_t at = 0;
         float x = -INFINITY;
@@ -382,6 +384,16 @@ __device__ __forceinline__ void plain_row(const cf_paged_attn_args_t& a, FastDiv
                 if (lane + 64 * i < d) acc[i] = __builtin_fmaf(pj, (float)v[row + lane + 64 * i], acc[i]);
         }
     }
+    if (rec) {
+        if (lane == 0) {
+            rec[0] = m;
+            rec[tm] = l;
+        }
+#pragma unroll
+        for (int i = 0; i < DIMS; i++)
+            if (lane + 64 * i < d) rec_sum[lane + 64 * i] = acc[i];
+        return;
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T* const o = (T*)a.o + ((int64_t)(s.row0 + tok) * a.H_q + h) * d;
 #pragma unroll
@@ -389,14 +401,9 @@ __device__ __forceinline__ void plain_row(const cf_paged_attn_args_t& a, FastDiv
         if (lane + 64 * i < d) o[lane + 64 * i] = (T)(acc[i] * inv);
 }
 
-// On the matrix cores a position that another row of the tile sees counts as 0 times its V,
-// which is no 0 where V is infinite or NaN.  A sum that is NaN while l is a number may come from
-// one: such a row is computed again, where only what it sees is touched.
-template <typename T, int D, typename Tile>     // Unit or CutTile
-__device__ __forceinline__ void redo_row(const cf_paged_attn_args_t& a, const PagedPlan& pl, const Tile& un, int kvh, int R) {
-    const int G = pl.G, tok = fastdiv(R, pl.by_group);
-    plain_row<T, D / 64>(a, pl.by_page, un.s, un.b, tok, kvh * G + (R - tok * G), D);
-}
+// On the matrix cores a position that another row of the tile sees counts as 0 times its V, which is
+// no 0 where V is infinite or NaN; and one that the row sees as a weight in two parts, whose products
+// with an infinite V add up to NaN.  Where a sum is NaN while l is a number, mend_rows looks.
 template <int N>
 __device__ __forceinline__ bool spoilt(const f4_t (&acc)[N], float l) {
     f4_t x = acc[0];
@@ -464,6 +471,105 @@ template <typename T, int D> struct Rows {
         return base[rd[kk] + 16 * t * D + 4 * ((4 * u + (lr >> 2)) ^ vswz<T, D>(4 * lq + kk))];
     }
 };
+
+// Which of some V are infinite (up, down) or NaN: a bit for each element of the lane's chunk.
+struct Odd {
+    uint32_t up = 0, down = 0, nan = 0;
+    __device__ __forceinline__ uint32_t any() const { return up | down | nan; }
+};
+template <typename T, int D>
+__device__ __forceinline__ void find_odd(const cf_paged_attn_args_t& a, FastDiv by_page, int b, int kvh, int from, int to, Odd& odd) {
+    using R = Rows<T, D>;
+    constexpr int U = 8;                                     // rows under way per lane
+    constexpr uint32_t kExp = R::F16 ? 0x7c007c00u : 0x7f800000u, kOne = R::F16 ? 0x04000400u : 0x00800000u;
+    constexpr uint32_t kCarry = R::F16 ? 0x80008000u : 0x80000000u;      // an exponent of ones carries into the sign
+    const int lane = threadIdx.x & 63, sub = lane / R::CPR;
+    const int32_t* const table = a.table + (size_t)b * a.max_pages;
+    const T* const v = (const T*)a.v + (int64_t)kvh * a.head_stride + R::CE * (lane % R::CPR);
+    Odd mine;
+#pragma clang loop unroll(disable)
+    for (int p0 = from; p0 < to; p0 += 64) {
+        const int key = min(p0 + lane, to - 1), idx = fastdiv(key, by_page), page = table[idx];
+        const bool valid = (unsigned)page < (unsigned)a.num_pages;
+        const int64_t at = valid ? (int64_t)page * a.page_stride + (int64_t)(key - idx * a.page_size) * a.row_stride : -1;
+        auto chunk = [&](int r) {
+            const int64_t row = (int64_t)((uint64_t)(uint32_t)__shfl((int)(at >> 32), r) << 32 | (uint32_t)__shfl((int)at, r));
+            return row < 0 ? uint4{} : *(const uint4*)(v + row);
+        };
+#pragma clang loop unroll(disable)
+        for (int r0 = sub; r0 < 64; r0 += U * R::RPI) {
+            uint4 x[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) x[u] = chunk(r0 + u * R::RPI);
+            uint32_t hit = 0;
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                hit |= ((x[u].x & kExp) + kOne) | ((x[u].y & kExp) + kOne) | ((x[u].z & kExp) + kOne) | ((x[u].w & kExp) + kOne);
+            if (!__builtin_amdgcn_ballot_w64((hit & kCarry) != 0)) continue;
+#pragma clang loop unroll(disable)
+            for (int u = 0; u < U; u++) {
+                const typename R::chunk_t c = __builtin_bit_cast(typename R::chunk_t, chunk(r0 + u * R::RPI));
+#pragma unroll
+                for (int e = 0; e < R::CE; e++) {
+                    const float f = (float)c[e];
+                    mine.nan |= f != f ? 1u << e : 0u;
+                    mine.up |= f == INFINITY ? 1u << e : 0u;
+                    mine.down |= f == -INFINITY ? 1u << e : 0u;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int step = R::CPR; step < 64; step *= 2) {
+        mine.up |= __shfl_xor(mine.up, step);
+        mine.down |= __shfl_xor(mine.down, step);
+        mine.nan |= __shfl_xor(mine.nan, step);
+    }
+    odd.up |= mine.up;
+    odd.down |= mine.down;
+    odd.nan |= mine.nan;
+}
+
+// Rows row0 + bit of a unit (a bit of `rows` each), computed and stored by this wave, where they are
+// spoilt.  An element is what the V that its row sees make of it: infinite or NaN.  Where these are
+// finite and only a hidden one is not, the row is computed again by the plain loop; hidden positions
+// are a tile's own tokens, so that ends with the call that brings such V.  The V are read once for all
+// rows, but for the tile's tokens (512 rows over 2048, a NaN among the cached V: 225 us, without it 51,
+// with every such row by the plain loop 20000; 16 decode rows over 4000 each 105, 50 and 2070).
+template <typename T, int D, int TM>
+__device__ __forceinline__ void mend_rows(const cf_paged_attn_args_t& a, const PagedPlan& pl, const Unit& un, int kvh,
+                                          const Work& w, int row0, uint32_t rows) {
+    using R = Rows<T, D>;
+    const int lane = threadIdx.x & 63;
+    wait_vm<0>();                                             // what it stored is stored
+    Odd seen;
+    int upto = w.key0;
+    for (; rows; rows &= rows - 1) {
+        const int row = row0 + __builtin_ctz(rows);
+        const RowAt at = row_at(pl, pl.G, kvh, w.R0 + row);
+        const int sees = max(min(min(w.base + at.tok, un.s.len), w.key1), upto);     // rises with the rows
+        find_odd<T, D>(a, pl.by_page, un.b, kvh, upto, sees, seen);
+        upto = sees;
+        Odd hidden;
+        find_odd<T, D>(a, pl.by_page, un.b, kvh, sees, w.key1, hidden);
+        float* const rec = un.n_ranges > 1 ? record_of<TM, D>(a, pl, un, kvh) : nullptr;
+        T* const o = (T*)a.o + ((int64_t)(un.s.row0 + at.tok) * a.H_q + at.h) * D;
+        if (__builtin_amdgcn_ballot_w64((hidden.any() & ~seen.any()) != 0)) {
+            plain_row<T, D / 64>(a, pl.by_page, un.s, un.b, at.tok, at.h, D, w.key0, w.key1, rec ? rec + row : nullptr, TM,
+                                 rec + 2 * TM + row * D);
+            continue;
+        }
+        if (lane >= R::CPR) continue;
+#pragma unroll
+        for (int e = 0; e < R::CE; e++) {
+            if (!((seen.any() >> e) & 1)) continue;
+            const bool up = (seen.up >> e) & 1, down = (seen.down >> e) & 1;
+            const float x = ((seen.nan >> e) & 1) || (up && down) ? NAN : up ? INFINITY : -INFINITY;
+            if (rec) rec[2 * TM + row * D + R::CE * lane + e] = x;
+            else o[R::CE * lane + e] = (T)x;
+        }
+    }
+}
 
 // m is what p = 2^(score - m) is taken against: 2^kStart below a maximum.  It moves only when a block
 // exceeds it by more than 2^kLazy; until then p is at most 2^15, which fp16 holds as exactly as 1,
@@ -727,8 +833,8 @@ void paged_heads(cf_paged_attn_args_t a, PagedPlan pl) {
         float m, l;
         narrow_range<T, D, H::BK>(a, pl, ring_all + wave * H::RING, un.s, un.b, kvh, w, w.key0, w.key1, acc, m, l);
         l = add_xor32(add_xor16(l));
-        uint32_t again = un.n_ranges > 1 ? 0 : rows_of_16(lr < w.n_rows && spoilt(acc, l));
-        if (lr < w.n_rows && !((again >> lr) & 1)) {
+        const uint32_t again = rows_of_16(lr < w.n_rows && spoilt(acc, l));
+        if (lr < w.n_rows) {
             if (un.n_ranges > 1) {
                 float* const rec = record_of<16, D>(a, pl, un, kvh);
 #pragma unroll
@@ -745,14 +851,14 @@ void paged_heads(cf_paged_attn_args_t a, PagedPlan pl) {
                 for (int u = 0; u < D / 16; u++) store4(o + 16 * u, acc[u] * inv);
             }
         }
-        for (; again; again &= again - 1) redo_row<T, D>(a, pl, un, kvh, w.R0 + __builtin_ctz(again));
+        if (again) mend_rows<T, D, 16>(a, pl, un, kvh, w, 0, again);
     }
 }
 
 // Up to 16 rows by all waves of a workgroup (latency bounds it: fp32, a row of 12 heads of 64 over
 // 257, 8.2 us; 16 rows over 512 each 10.3): each takes a share of the unit's positions, and
 // they join their m, l and sums in LDS (WAVES rings at `lds`, one each).  True where rows that
-// this wave finished have to be computed again.
+// this wave stored are spoilt.
 template <typename T, int D, int TM, int WAVES, int ALL = WAVES>
 __device__ __forceinline__ bool narrow_unit(const cf_paged_attn_args_t& a, const PagedPlan& pl, T* lds, const Unit& un,
                                             int kvh, const Work& w) {
@@ -798,6 +904,8 @@ __device__ __forceinline__ bool narrow_unit(const cf_paged_attn_args_t& a, const
             L += p[16 * LD + 16 + row] * x;
             sum += *(const f4_t*)(p + row * LD + 4 * d4) * x;
         }
+        const f4_t one[1] = {sum};
+        again |= spoilt(one, L);
         if (un.n_ranges > 1) {
             float* const rec = record_of<TM, D>(a, pl, un, kvh);
             *(f4_t*)(rec + 2 * TM + row * D + 4 * d4) = sum;
@@ -806,8 +914,6 @@ __device__ __forceinline__ bool narrow_unit(const cf_paged_attn_args_t& a, const
                 rec[TM + row] = L;
             }
         } else {
-            const f4_t one[1] = {sum};
-            again |= spoilt(one, L);
             const RowAt at = row_at(pl, pl.G, kvh, w.R0 + row);
             store4((T*)a.o + ((int64_t)(un.s.row0 + at.tok) * a.H_q + at.h) * D + 4 * d4,
                    sum * (L == 0.0f ? 0.0f : 1.0f / L));
@@ -817,14 +923,15 @@ __device__ __forceinline__ bool narrow_unit(const cf_paged_attn_args_t& a, const
     return __builtin_amdgcn_ballot_w64(again) != 0;
 }
 
-// Those rows of the wave.
-template <typename T, int D, int WAVES>
-__device__ __forceinline__ void redo_narrow(const cf_paged_attn_args_t& a, const PagedPlan& pl, const Unit& un, int kvh,
+// The rows that the wave stored there.
+template <typename T, int D, int TM, int WAVES>
+__device__ __forceinline__ void mend_narrow(const cf_paged_attn_args_t& a, const PagedPlan& pl, const Unit& un, int kvh,
                                             const Work& w) {
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    wait_vm<0>();                                             // what it stored is stored
+    uint32_t rows = 0;
     for (int r = 0; r < w.n_rows; r++)
-        if (r / (256 / D) % WAVES == wave) redo_row<T, D>(a, pl, un, kvh, w.R0 + r);
+        if (r / (256 / D) % WAVES == wave) rows |= 1u << r;
+    mend_rows<T, D, TM>(a, pl, un, kvh, w, 0, rows);
 }
 
 template <typename T, int D> struct Split {
@@ -841,7 +948,7 @@ void paged_split(cf_paged_attn_args_t a, PagedPlan pl) {
         Unit un;
         if (!geo.find(id, un)) break;
         const Work w = unit_work<16, 64>(a, pl, un);
-        if (narrow_unit<T, D, 16, WAVES>(a, pl, lds, un, kvh, w)) redo_narrow<T, D, WAVES>(a, pl, un, kvh, w);
+        if (narrow_unit<T, D, 16, WAVES>(a, pl, lds, un, kvh, w)) mend_narrow<T, D, 16, WAVES>(a, pl, un, kvh, w);
     }
 }
 
@@ -894,7 +1001,7 @@ template <int D, int NJ> struct Wide16 {
     static_assert(8 * Narrow<_Float16, D, 16>::RING <= LDS, "the rings of narrow tiles fit");
 };
 
-// Returns the wave's rows that have to be computed again, a bit each.
+// Returns the wave's rows that are spoilt, a bit each.
 template <int D, int NJ>
 __device__ __forceinline__ uint32_t wide16_unit(const cf_paged_attn_args_t& a, const PagedPlan& pl, _Float16* lds,
                                             uint64_t* masks, const Unit& un, int kvh, const Work& w) {
@@ -1166,8 +1273,8 @@ __device__ __forceinline__ uint32_t wide16_unit(const cf_paged_attn_args_t& a, c
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
         const int row = wrow + 16 * j + lr;
-        const uint32_t again = un.n_ranges > 1 ? 0 : rows_of_16(row < w.n_rows && spoilt(acc[j], lsum[j][0]));
-        if (row < w.n_rows && !((again >> lr) & 1)) {
+        const uint32_t again = rows_of_16(row < w.n_rows && spoilt(acc[j], lsum[j][0]));
+        if (row < w.n_rows) {
             const RowOut out = row_out<T, D, W::TM>(a, pl, un, kvh, w, row, m_run[j], lsum[j][0], lq == 0);
 #pragma unroll
             for (int u = 0; u < UT; u++) put4<T>(out, 16 * u + 4 * lq, acc[j][u]);
@@ -1201,10 +1308,8 @@ void paged_wide16(cf_paged_attn_args_t a, PagedPlan pl) {
         if (!again) continue;
         if (!geo.find(id, un)) break;         // found anew: nothing is kept for this
         w = unit_work<W::TM, 64>(a, pl, un);
-        if (narrow) redo_narrow<_Float16, D, 8>(a, pl, un, kvh, w);
-        const int row0 = w.R0 + 16 * NJ * __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-        for (uint32_t left = narrow ? 0 : again; left; left &= left - 1)
-            redo_row<_Float16, D>(a, pl, un, kvh, row0 + __builtin_ctz(left));
+        if (narrow) mend_narrow<_Float16, D, W::TM, 8>(a, pl, un, kvh, w);
+        else mend_rows<_Float16, D, W::TM>(a, pl, un, kvh, w, 16 * NJ * __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), again);
     }
 }
 
@@ -1402,13 +1507,13 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
         ring_barrier();                                       // ... before the next unit
     }
     if (share == 0) {
-        uint32_t again = un.n_ranges > 1 ? 0 : rows_of_16(wrow + lr < w.n_rows && spoilt(acc, l));
-        if (wrow + lr < w.n_rows && !((again >> lr) & 1)) {
+        const uint32_t again = rows_of_16(wrow + lr < w.n_rows && spoilt(acc, l));
+        if (wrow + lr < w.n_rows) {
             const RowOut out = row_out<T, D, W::TM>(a, pl, un, kvh, w, wrow + lr, m_run, l, lq == 0);
 #pragma unroll
             for (int u = 0; u < UT; u++) put4<T>(out, 16 * u + 4 * lq, acc[u]);
         }
-        for (; again; again &= again - 1) redo_row<T, D>(a, pl, un, kvh, w.R0 + wrow + __builtin_ctz(again));
+        if (again) mend_rows<T, D, W::TM>(a, pl, un, kvh, w, wrow, again);
     }
 }
 
@@ -1426,7 +1531,7 @@ void paged_wide32(cf_paged_attn_args_t a, PagedPlan pl) {
         if (!geo.find(id, un)) break;
         const Work w = unit_work<W::TM, 64>(a, pl, un);
         if (w.n_rows > 16) wide32_unit<D>(a, pl, lds, un, kvh, w);
-        else if (narrow_unit<float, D, W::TM, 4, W::WAVES>(a, pl, lds, un, kvh, w)) redo_narrow<float, D, 4>(a, pl, un, kvh, w);
+        else if (narrow_unit<float, D, W::TM, 4, W::WAVES>(a, pl, lds, un, kvh, w)) mend_narrow<float, D, W::TM, 4>(a, pl, un, kvh, w);
     }
 }
 
@@ -1514,20 +1619,11 @@ void paged_merge(cf_paged_attn_args_t a, PagedPlan pl) {
                 }
                 __syncthreads();
             }
-            const bool mine = sub == 0 && row < n_rows;
-            const f4_t one[1] = {acc};
-            uint64_t bad = __builtin_amdgcn_ballot_w64(mine && spoilt(one, l));
-            if (mine && bad == 0) {
+            if (sub == 0 && row < n_rows) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 const RowAt at = row_at(pl, G, kvh, un.tile * TM + row);
                 store4((T*)a.o + ((int64_t)(un.s.row0 + at.tok) * a.H_q + at.h) * D + 4 * d4, acc * inv);
             }
-            if (bad != 0)                                     // this wave's rows, all of them
-                for (uint64_t left = __builtin_amdgcn_ballot_w64(mine); left;) {
-                    const int again = __builtin_amdgcn_readlane(row, __builtin_ctzll(left));
-                    redo_row<T, D>(a, pl, un, kvh, un.tile * TM + again);
-                    left &= ~__builtin_amdgcn_ballot_w64(row == again);
-                }
         }
     }
 }

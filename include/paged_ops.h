@@ -128,8 +128,9 @@ typedef struct {
  * reads KV head h / (H_q / H_kv)).  A row that sees no position (no page of it is valid, or
  * p < 0) gives 0.  Rows of O outside q_start[0] .. q_start[B] are left as they are; what
  * pages hold past seq_lens[b] is not looked at, and what a row does not see does not touch it,
- * infinite or NaN either (a row whose tile holds such V is computed a second time, by a slow
- * loop).  Tables may name a page twice and share pages; O must not overlap an input (-1 where
+ * infinite or NaN either.  Such V cost time: a tile that holds them reads its V a second time, and
+ * rows that do not see them, though a later token of the same call does, are computed again by a
+ * slow loop.  Tables may name a page twice and share pages; O must not overlap an input (-1 where
  * it is Q or a cache).  d = 64 and 128 with pages of a multiple of 16 positions, 16-byte
  * aligned pointers and strides and scale > 0 run on the matrix cores, every other call on a
  * plain kernel. */

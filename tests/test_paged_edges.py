@@ -95,3 +95,42 @@ def test_many_small_weights_beside_a_large_one(gpu, f16, H, H_kv, d, P, n, far):
     c.vp[c.table[0, 0], 0] = 0
     for hint in (0, 1):                                  # the positions shared out, and in one range
         c.check(c.run(max_new=n, max_len=hint))
+
+
+ODD_CASES = [
+    (8, 2, 64, 16, [12, 2, 8], [100, 30, 7]), (8, 2, 128, 16, [4, 4, 4], [2500, 60, 1500]), (32, 8, 128, 16, [1] * 5, [4000, 300, 90, 2222, 17]),
+    (12, 12, 64, 16, [1, 1], [700, 333]), (12, 12, 64, 16, [9] * 12, [300] * 12), (8, 4, 128, 32, [150, 40, 90, 1], [33, 9, 200, 600]),
+    (4, 4, 64, 16, [130, 2], [4000, 3000]), (128, 64, 64, 16, [400], [64]), (4, 2, 40, 5, [7, 3], [20, 9]),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("H,H_kv,d,P,new,past", ODD_CASES)
+def test_infinite_and_nan_v_among_the_cached(gpu, f16, H, H_kv, d, P, new, past):
+    """Infinite and NaN V of cached positions, which every row sees, in dims of their own; in three of
+    these and one more a new token has another that only rows from it on see."""
+    c = Paged(new, past, H, H_kv, d, P, f16, seed=33)
+    clean = c.vp.copy()
+    inf, nan = np.inf, np.nan
+    at = lambda b, pos: (c.table[b, pos // P], pos % P)
+    want = np.zeros(c.q.shape)                           # inf, -inf or NaN; 0: as without them
+    for b, (n, p) in enumerate(zip(new, past)):
+        r = np.arange(c.start[b], c.start[b + 1])
+        for dim, pos, x in ((3, p // 2, nan), (5, 0, inf), (d - 1, p - 1, -inf), (7, p // 3, inf), (7, p // 2, -inf), (20, p // 4, inf)):
+            c.vp[at(b, pos)][:, dim] = x
+            want[r, :, dim] = nan if want[r[0], 0, dim] == -x else x
+        h = n // 2
+        new_at = at(b, p + h)
+        c.vp[new_at][:, 5], c.vp[new_at][:, 20], c.vp[new_at][:, 3], c.vp[new_at][:, 11] = -inf, inf, inf, nan
+        want[r[h:], :, 5], want[r[h:], :, 11] = nan, nan
+    odd = want != 0
+    dirty = c.vp
+    for hint in (0, 1):
+        c.vp = dirty
+        got = c.run(max_new=max(new), max_len=hint)
+        assert np.array_equal(got[odd].astype(np.float64), want[odd], equal_nan=True)
+        c.vp = clean
+        plain = c.run(max_new=max(new), max_len=hint)
+        got[odd] = plain[odd]
+        c.check(got)
