@@ -420,6 +420,7 @@ typedef struct {
     float          scale;
     int32_t        elem;
     void*          workspace;   /* of cf_paged_attn_bytes */
+    int32_t        uncut;       /* 1: no workspace; long contexts are not shared out */
 } cf_paged_attn_args_t;
 size_t cf_paged_attn_bytes(const cf_paged_attn_args_t* a);
 int cf_launch_paged_attn(const cf_paged_attn_args_t* a, void* stream);

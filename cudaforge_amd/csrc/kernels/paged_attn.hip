@@ -1714,7 +1714,7 @@ Plan make_plan(const cf_paged_attn_args_t& a) {
     p.pl.min_blocks = (int32_t)(p.form == kHeads ? 64 / BK : wide16 ? 12 : 4);
     p.pl.one_blocks = (int32_t)((p.form == kHeads ? 128 : wide16 ? 1536 : 512) / BK);
     p.pl.max_records = (int32_t)(4 * fill + 8);
-    const bool cut = p.form != kSplit && (a.max_len + BK - 1) / BK > (wide16 ? kFewOne / BK : p.pl.one_blocks);
+    const bool cut = !a.uncut && p.form != kSplit && (a.max_len + BK - 1) / BK > (wide16 ? kFewOne / BK : p.pl.one_blocks);
     if (!cut) p.pl.one_blocks = INT32_MAX;                    // nor is what is longer than max_len
     p.bytes = cut ? header_bytes(p.pl.max_records) + (size_t)p.pl.max_records * a.H_kv * (TM * (a.d + 2)) * sizeof(float) : 0;
     int64_t units = (tiles + (cut ? 2 * fill : 0)) * a.H_kv;

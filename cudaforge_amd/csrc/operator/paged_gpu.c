@@ -179,7 +179,11 @@ static int paged_attn_op(int elem, const void* inputs[], void* outputs[], const 
     a.elem = elem;
     void* st = cf_stream_of(stream);
     const size_t bytes = cf_paged_attn_bytes(&a);
-    if (bytes > 0 && !(a.workspace = gpu_workspace_get_stream(st, bytes))) return -1;
+    /* Without a buffer (no memory, or a recording on a stream that has none of that size) no tile
+     * is cut. */
+    if (bytes > 0 && !(a.workspace = gpu_workspace_try_stream(st, bytes)) &&
+        !(a.workspace = gpu_workspace_get_stream(st, bytes)))
+        a.uncut = 1;
     return cf_launch_paged_attn(&a, st);
 }
 

@@ -1,7 +1,8 @@
 """mha_paged_attn_{f16,f32}_cuda at the edges of what its arrays may hold, against the 64-bit oracle and
 the tolerances of test_paged.py (GPU)."""
 
-import math
+import ctypes
+from ctypes import c_void_p
 
 import numpy as np
 import pytest
@@ -134,3 +135,42 @@ def test_infinite_and_nan_v_among_the_cached(gpu, f16, H, H_kv, d, P, new, past)
         plain = c.run(max_new=max(new), max_len=hint)
         got[odd] = plain[odd]
         c.check(got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("new,past", [([1, 1, 1], [5000, 40, 1700]), ([70, 1, 30], [3000, 900, 10])])
+def test_without_memory_for_a_workspace(gpu, f16, new, past):
+    """No buffer to be had, or a recording on a stream that has none: the tiles are not cut, and the call
+    succeeds.  What the stream had before is used again afterwards."""
+    c = Paged(new, past, 8, 2, 128, 16, f16, seed=35)
+    bufs = [dev(x) for x in (c.q, c.kp, c.vp, c.table, c.lens, c.start)]
+    st = cf.Stream()
+    o = dev(np.full(c.q.shape, 7.0, c.dt))
+    gpu.gpu_inject_alloc_failures(1000)
+    try:
+        rc = cf.call_op(c.op, bufs, [o], c.params(max_new=max(new)), st)
+    finally:
+        gpu.gpu_inject_alloc_failures(0)
+    assert rc == 0
+    st.synchronize()
+    c.check(o.download())
+
+    st = cf.Stream()
+    o = dev(np.full(c.q.shape, 7.0, c.dt))
+    ex = c_void_p()
+    held = gpu.gpu_workspace_size()
+    assert gpu.gpu_capture_begin(st.handle) == 0
+    rc = cf.call_op(c.op, bufs, [o], c.params(max_new=max(new)), st)
+    assert gpu.gpu_capture_end(st.handle, ctypes.byref(ex)) == 0
+    assert rc == 0 and gpu.gpu_workspace_size() == held
+    for drop in (0, 500, 0):
+        lens = c.lens.copy()
+        c.lens = np.maximum(lens - drop, new).astype(I32)
+        bufs[4].upload(c.lens)
+        assert gpu.gpu_graph_launch(ex, st.handle) == 0
+        st.synchronize()
+        c.check(o.download())
+        c.lens = lens
+        c.check(c.run(max_new=max(new)))                 # eager, with a buffer
+    gpu.gpu_graph_exec_destroy(ex)
