@@ -1670,6 +1670,12 @@ constexpr int64_t kFullUnits = 192, kLongUnits = 32, kLongLen = 2048;
 // Of the workspace: the number of cut tiles (256 bytes) and the list of them.
 size_t header_bytes(int32_t max_records) { return 256 + ((size_t)max_records / 2 * sizeof(CutTile) + 255) / 256 * 256; }
 
+// A unit looks for its sequence among all of them, so that the time of the tiles rises with the square
+// of their number, that of the plain kernel with the positions (decode rows of 8 heads of 64 over 2,
+// tiles and plain kernel: 1024 sequences of 16 positions 17 and 39 us, 16384 of 128 2.0 and 3.4 ms, 32768 of 16 7.5
+// and 1.4 and of 128 7.8 and 6.6, 65536 of 128 31 and 13).  More than this many take the plain kernel.
+constexpr int kMostSeqs = 32768;
+
 bool fast_ok(const cf_paged_attn_args_t& a) {
     const uint64_t ptrs = (uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.k | (uint64_t)(uintptr_t)a.v | (uint64_t)(uintptr_t)a.o;
     const uint64_t steps = (uint64_t)a.q_stride | (uint64_t)a.page_stride | (uint64_t)a.row_stride | (uint64_t)a.head_stride;
@@ -1677,7 +1683,8 @@ bool fast_ok(const cf_paged_attn_args_t& a) {
     // Row numbers times the group and positions (with what is read ahead) stay in 31 bits, offsets
     // inside a group of rows in 32.
     return (a.d == 64 || a.d == 128) && a.page_size % 16 == 0 && ptrs % 16 == 0 && steps * es % 16 == 0 && a.scale > 0.0f &&
-           (int64_t)a.T * (a.H_q / a.H_kv) <= (1 << 30) && (int64_t)a.max_pages * a.page_size <= (1 << 30) && (uint64_t)a.row_stride * es * 16 < (1ull << 32);
+           a.B <= kMostSeqs && (int64_t)a.T * (a.H_q / a.H_kv) <= (1 << 30) && (int64_t)a.max_pages * a.page_size <= (1 << 30) &&
+           (uint64_t)a.row_stride * es * 16 < (1ull << 32);
 }
 
 // max_new and max_len only choose: the kernels' loops run until no unit is left, whatever the

@@ -132,8 +132,8 @@ typedef struct {
  * rows that do not see them, though a later token of the same call does, are computed again by a
  * slow loop.  Tables may name a page twice and share pages; O must not overlap an input (-1 where
  * it is Q or a cache).  d = 64 and 128 with pages of a multiple of 16 positions, 16-byte
- * aligned pointers and strides and scale > 0 run on the matrix cores, every other call on a
- * plain kernel. */
+ * aligned pointers and strides, scale > 0 and at most 32768 sequences run on the matrix cores,
+ * every other call on a plain kernel. */
 int mha_paged_attn_f32_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
 int mha_paged_attn_f16_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
 
