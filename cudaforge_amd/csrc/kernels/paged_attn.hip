@@ -571,13 +571,16 @@ __device__ __forceinline__ void mend_rows(const cf_paged_attn_args_t& a, const P
     }
 }
 
-// m is what p = 2^(score - m) is taken against: 2^kStart below a maximum.  It moves only when a block
-// exceeds it by more than 2^kLazy; until then p is at most 2^15, which fp16 holds as exactly as 1,
-// and the sums are not rescaled.  Staying below the maximum leaves weights of down to 2^-32 of the
-// largest in fp16's range, whose smallest number is 2^-24: taken against the maximum itself, the many
-// positions of a long context that weigh less than 2^-25 each would all count as 0.
-constexpr float kLazy = 8.0f, kStart = 7.0f;
-__device__ __forceinline__ float low_max(float x, float c) { return __builtin_fmaf(x, c, -kStart); }   // of the row's scores
+// m is what p = 2^(score - m) is taken against, low_max of a block's scores.  It moves only when a
+// block's exceeds it by more than 2^kLazy; until then the sums are not rescaled.
+// fp16: 2^7 below the maximum, so that p is at most 2^15, which fp16 holds as exactly as 1, and weights
+// of down to 2^-32 of the largest are in fp16's range, whose smallest number is 2^-24: taken against
+// the maximum itself, the many positions of a long context that weigh less than 2^-25 each would
+// all count as 0.  fp32: 2^8 above it, so that p is at most 1 and sums do not overflow before V's would.
+constexpr float kLazy = 8.0f;
+template <typename T> __device__ __forceinline__ float low_max(float x, float c) {
+    return __builtin_fmaf(x, c, sizeof(T) == 2 ? -7.0f : kLazy);
+}
 __device__ __forceinline__ bool move_max(float mloc, float& m, float& alpha) {
     if (!__builtin_amdgcn_ballot_w64(mloc > m + kLazy)) return false;
     const float m_new = mloc > m + kLazy ? mloc : m;
@@ -744,7 +747,7 @@ __device__ __forceinline__ void narrow_range(const cf_paged_attn_args_t& a, cons
         float mloc = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
 #pragma unroll
         for (int t = 1; t < NG; t++) mloc = fmaxf(mloc, fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3])));
-        mloc = low_max(max_xor32(max_xor16(mloc)), c);         // -inf if the row sees nothing here
+        mloc = low_max<T>(max_xor32(max_xor16(mloc)), c);         // -inf if the row sees nothing here
         float alpha;
         if (move_max(mloc, m_run, alpha)) {
             l.scale(alpha);
@@ -1195,7 +1198,7 @@ __device__ __forceinline__ uint32_t wide16_unit(const cf_paged_attn_args_t& a, c
                 for (int e = 3; e < 15; e += 2)
                     mloc = fmaxf(fmaxf(mloc, sc[j][e >> 2][e & 3]), sc[j][(e + 1) >> 2][(e + 1) & 3]);
                 mloc = fmaxf(mloc, sc[j][3][3]);
-                mloc = low_max(max_xor32(max_xor16(mloc)), c);  // -inf if the row sees nothing here
+                mloc = low_max<T>(max_xor32(max_xor16(mloc)), c);  // -inf if the row sees nothing here
                 float alpha;
                 if (move_max(mloc, m_run[j], alpha)) {
                     lsum[j] *= alpha;
@@ -1444,7 +1447,7 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
             for (int e = 3; e < 4 * NT - 1; e += 2)
                 mloc = fmaxf(fmaxf(mloc, sc[e >> 2][e & 3]), sc[(e + 1) >> 2][(e + 1) & 3]);
             mloc = fmaxf(mloc, sc[NT - 1][3]);
-            mloc = low_max(max_xor32(max_xor16(mloc)), c);
+            mloc = low_max<T>(max_xor32(max_xor16(mloc)), c);
             float alpha;
             if (move_max(mloc, m_run, alpha)) {
                 l_run.scale(alpha);

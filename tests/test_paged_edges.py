@@ -174,3 +174,17 @@ def test_without_memory_for_a_workspace(gpu, f16, new, past):
         c.lens = lens
         c.check(c.run(max_new=max(new)))                 # eager, with a buffer
     gpu.gpu_graph_exec_destroy(ex)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,H_kv,d,P", SHAPES)
+@pytest.mark.parametrize("n", [1, 9, 100])
+def test_large_fp32_values(gpu, H, H_kv, d, P, n):
+    """V of up to 2^120: weights of at most 1 of 150 positions leave their sum below FP32's 2^128."""
+    c = Paged([n], [150 - n], H, H_kv, d, P, False, seed=37)
+    c.vp[:] *= np.float32(2.0 ** 118)
+    for std in (0, 1, 5):
+        x = Paged([n], [150 - n], H, H_kv, d, P, False, seed=37, k_std=std)
+        x.vp = c.vp
+        for hint in (0, 1):
+            x.check(x.run(max_new=n, max_len=hint))
