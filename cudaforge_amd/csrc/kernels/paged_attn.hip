@@ -991,9 +991,9 @@ __device__ __forceinline__ void put4(const RowOut& out, int d0, f4_t x) {
 // them are still under way when one is needed.
 // NJ = 2: the matrix cores bound it, at what clock they leave (about 2.1 GHz): 2048 rows over 8192,
 // 241 GFLOP in 240 to 260 us (925 to 1000 TFLOP/s; a large library product makes 1097).  NJ = 1
-// halves the tile, not the time of a turn (0.9 us for 1.75): each fragment read from LDS feeds
-// one product, so the LDS bounds it with the turn's latencies.  Waves of 32 rows that share the
-// positions instead take 1.1.
+// halves the tile, and a turn takes two thirds of the time (a tile on every CU, over 8192 positions:
+// 1.52 us a block for 2.23): each fragment read from LDS feeds one product, so the LDS bounds it with
+// the turn's latencies.  Waves of 32 rows that share the positions instead take a fifth longer.
 template <int D, int NJ> struct Wide16 {
     static constexpr int TM = 128 * NJ, BK = 64, NS = 4;
     static constexpr int TILE = BK * D;
@@ -1662,13 +1662,13 @@ struct Plan {
 // and paged_heads: 1 x 512 8.3 and 11.8, 16 x 512 10.3 and 14.6, 32 x 1024 28.0 and 31.8, 64 x 512
 // both 31.3; longer ones need ranges and a merge in both: 8 x 2048 19.8 and 18.2, 16 x 8192 117
 // and 98, 2 x 30000 52.9 and 51.4.
-constexpr int64_t kSplitUnits = 256, kSplitLen = 1024;
+constexpr int64_t kSplitLen = 1024;
 // Tiles of 256 rows read a block's K and V once for twice the rows, but are twice as long a
 // piece of work.  They pay where they fill three quarters of the chip by themselves (4 x 517 rows
 // over 517: 31.8 us, with 128 rows 34.4; 4 x 1024 over 2048: 135 and 159; 1024 over 1024: 38.9 and
 // 28.0), and where long ranges of one or two long sequences can be cut evenly (517 over 8517: 95
 // and 118; 330 over 2530: 36.8 and 38.4; 230 over 2430, 28 units: 33 and 30.8; 4 x 230: 59 and 56).
-constexpr int64_t kFullUnits = 192, kLongUnits = 32, kLongLen = 2048;
+constexpr int64_t kLongLen = 2048;
 
 // Of the workspace: the number of cut tiles (256 bytes) and the list of them.
 size_t header_bytes(int32_t max_records) { return 256 + ((size_t)max_records / 2 * sizeof(CutTile) + 255) / 256 * 256; }
@@ -1704,11 +1704,11 @@ Plan make_plan(const cf_paged_attn_args_t& a) {
     };
     if (rows <= 16) {
         const int64_t units = tiles_of(16) * a.H_kv;
-        p.form = units <= kSplitUnits && a.max_len <= kSplitLen ? kSplit : kHeads;
+        p.form = units <= cus && a.max_len <= kSplitLen ? kSplit : kHeads;
     } else {
         const int64_t units = (int64_t)a.T * G / 256 * a.H_kv;
-        const bool few_long = a.max_len > kLongLen && 2 * (int64_t)a.max_new >= a.T && units >= kLongUnits;
-        p.form = f16 && (units >= kFullUnits || few_long) ? kWide2 : kWide1;
+        const bool few_long = a.max_len > kLongLen && 2 * (int64_t)a.max_new >= a.T && units >= cus / 8;
+        p.form = f16 && (4 * units >= 3 * cus || few_long) ? kWide2 : kWide1;
     }
     const int64_t TM = p.form <= kSplit ? 16 : !f16 ? 64 : p.form == kWide2 ? 256 : 128;
     const int64_t BK = p.form != kHeads ? 64 : f16 ? 32 : 16;
@@ -1718,7 +1718,7 @@ Plan make_plan(const cf_paged_attn_args_t& a) {
     const int64_t fill = cus * per_cu > a.H_kv ? cus * per_cu / a.H_kv : 1;
     p.pl.fill = (int32_t)fill;
     // What is not worth cutting: a merge and the records cost paged_heads 5 us and a wide tile 10
-    // to 12 (517 rows over 1029: 26.7 us, cut from 8 blocks on into ranges of 4: 35; fp32, 200 rows
+    // to 12 (four chunks of 517 rows over 1029 each: 26.7 us, cut from 8 blocks on into ranges of 4: 35; fp32, 200 rows
     // over 1200: 57 us, from 24 blocks on into ranges of 12: 66).
     const bool wide16 = f16 && p.form > kSplit;
     p.pl.min_blocks = (int32_t)(p.form == kHeads ? 64 / BK : wide16 ? 12 : 4);
