@@ -573,17 +573,19 @@ __device__ __forceinline__ void mend_rows(const cf_paged_attn_args_t& a, const P
 
 // m is what p = 2^(score - m) is taken against, low_max of a block's scores.  It moves only when a
 // block's exceeds it by more than 2^kLazy; until then the sums are not rescaled.
-// fp16: 2^7 below the maximum, so that p is at most 2^15, which fp16 holds as exactly as 1, and weights
-// of down to 2^-32 of the largest are in fp16's range, whose smallest number is 2^-24: taken against
+// fp16: 2^7 below the maximum, and p at most 2^15, which fp16 holds as exactly as 1, so that weights of
+// down to 2^-32 of the largest are in fp16's range, whose smallest number is 2^-24: taken against
 // the maximum itself, the many positions of a long context that weigh less than 2^-25 each would
-// all count as 0.  fp32: 2^8 above it, so that p is at most 1 and sums do not overflow before V's would.
-constexpr float kLazy = 8.0f;
+// all count as 0.
+// fp32: the maximum, and p at most 2: sums do not overflow before V's own would, and score - m, whose
+// rounding is p's, stays small (2^8 above the maximum a row of 257 positions was off by 3.5e-7, so 2.8e-7).
+template <typename T> constexpr float kLazy = sizeof(T) == 2 ? 8.0f : 1.0f;
 template <typename T> __device__ __forceinline__ float low_max(float x, float c) {
-    return __builtin_fmaf(x, c, sizeof(T) == 2 ? -7.0f : kLazy);
+    return sizeof(T) == 2 ? __builtin_fmaf(x, c, -7.0f) : x * c;
 }
-__device__ __forceinline__ bool move_max(float mloc, float& m, float& alpha) {
-    if (!__builtin_amdgcn_ballot_w64(mloc > m + kLazy)) return false;
-    const float m_new = mloc > m + kLazy ? mloc : m;
+template <typename T> __device__ __forceinline__ bool move_max(float mloc, float& m, float& alpha) {
+    if (!__builtin_amdgcn_ballot_w64(mloc > m + kLazy<T>)) return false;
+    const float m_new = mloc > m + kLazy<T> ? mloc : m;
     alpha = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));   // 0 on the first move
     m = m_new;
     return true;
@@ -749,7 +751,7 @@ __device__ __forceinline__ void narrow_range(const cf_paged_attn_args_t& a, cons
         for (int t = 1; t < NG; t++) mloc = fmaxf(mloc, fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3])));
         mloc = low_max<T>(max_xor32(max_xor16(mloc)), c);         // -inf if the row sees nothing here
         float alpha;
-        if (move_max(mloc, m_run, alpha)) {
+        if (move_max<T>(mloc, m_run, alpha)) {
             l.scale(alpha);
 #pragma unroll
             for (int u = 0; u < UT; u++) acc[u] *= alpha;
@@ -1200,7 +1202,7 @@ __device__ __forceinline__ uint32_t wide16_unit(const cf_paged_attn_args_t& a, c
                 mloc = fmaxf(mloc, sc[j][3][3]);
                 mloc = low_max<T>(max_xor32(max_xor16(mloc)), c);  // -inf if the row sees nothing here
                 float alpha;
-                if (move_max(mloc, m_run[j], alpha)) {
+                if (move_max<T>(mloc, m_run[j], alpha)) {
                     lsum[j] *= alpha;
 #pragma unroll
                     for (int u = 0; u < UT; u++) acc[j][u] *= alpha;
@@ -1449,7 +1451,7 @@ __device__ __forceinline__ void wide32_unit(const cf_paged_attn_args_t& a, const
             mloc = fmaxf(mloc, sc[NT - 1][3]);
             mloc = low_max<T>(max_xor32(max_xor16(mloc)), c);
             float alpha;
-            if (move_max(mloc, m_run, alpha)) {
+            if (move_max<T>(mloc, m_run, alpha)) {
                 l_run.scale(alpha);
 #pragma unroll
                 for (int u = 0; u < UT; u++) acc[u] *= alpha;
