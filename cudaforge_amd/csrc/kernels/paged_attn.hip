@@ -861,7 +861,7 @@ void paged_heads(cf_paged_attn_args_t a, PagedPlan pl) {
 }
 
 // Up to 16 rows by all waves of a workgroup (latency bounds it: fp32, a row of 12 heads of 64 over
-// 257, 8.2 us; 16 rows over 512 each 10.3): each takes a share of the unit's positions, and
+// 257, 8.6 us; fp16, 16 rows over 512 each 10.1): each takes a share of the unit's positions, and
 // they join their m, l and sums in LDS (WAVES rings at `lds`, one each).  True where rows that
 // this wave stored are spoilt.
 template <typename T, int D, int TM, int WAVES, int ALL = WAVES>
@@ -1667,9 +1667,9 @@ struct Plan {
 constexpr int64_t kSplitLen = 1024;
 // Tiles of 256 rows read a block's K and V once for twice the rows, but are twice as long a
 // piece of work.  They pay where they fill three quarters of the chip by themselves (4 x 517 rows
-// over 517: 31.8 us, with 128 rows 34.4; 4 x 1024 over 2048: 135 and 159; 1024 over 1024: 38.9 and
-// 28.0), and where long ranges of one or two long sequences can be cut evenly (517 over 8517: 95
-// and 118; 330 over 2530: 36.8 and 38.4; 230 over 2430, 28 units: 33 and 30.8; 4 x 230: 59 and 56).
+// over 517: 34.8 us, with 128 rows 38.0; 4 x 1024 over 2048: 139 and 160; 1024 over 1024: 40.1 and
+// 28.7), and where long ranges of one or two long sequences can be cut evenly (517 over 8517: 93 and
+// 115; 330 over 2530: 37.7 and 37.9; 230 over 2430, 28 units: 31.5 and 30.8; 4 x 230: 77 and 58.5).
 constexpr int64_t kLongLen = 2048;
 
 // Of the workspace: the number of cut tiles (256 bytes) and the list of them.
@@ -1720,8 +1720,8 @@ Plan make_plan(const cf_paged_attn_args_t& a) {
     const int64_t fill = cus * per_cu > a.H_kv ? cus * per_cu / a.H_kv : 1;
     p.pl.fill = (int32_t)fill;
     // What is not worth cutting: a merge and the records cost paged_heads 5 us and a wide tile 10
-    // to 12 (four chunks of 517 rows over 1029 each: 26.7 us, cut from 8 blocks on into ranges of 4: 35; fp32, 200 rows
-    // over 1200: 57 us, from 24 blocks on into ranges of 12: 66).
+    // to 12 (517 rows over 1029: 28.5 us, cut from 8 blocks on into ranges of 4: 35.1; fp32, 200 rows
+    // over 1200: 57.5 us, from 24 blocks on into ranges of 12: 90).
     const bool wide16 = f16 && p.form > kSplit;
     p.pl.min_blocks = (int32_t)(p.form == kHeads ? 64 / BK : wide16 ? 12 : 4);
     p.pl.one_blocks = (int32_t)((p.form == kHeads ? 128 : wide16 ? 1536 : 512) / BK);
