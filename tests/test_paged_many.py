@@ -1,6 +1,6 @@
 """The paged operators with more sequences and rows than a launch or a plan takes in one piece (GPU).
 Sequences of one position, whose attention is that position's V, and rows stored as they are, so
-that results are known exactly."""
+that results are known without a sum."""
 
 import numpy as np
 import pytest
@@ -30,7 +30,10 @@ def test_attention_of_very_many_sequences(gpu, f16, B, H, H_kv, d):
                       [dev(q), dev(k), dev(v), dev(page.reshape(B, 1)), dev(lens), dev(np.arange(B + 1, dtype=I32))], [o], p) == 0
     got = o.download()
     want = np.concatenate((v[:, 0], np.zeros((1, H_kv, d), dt)))[page]
-    assert np.array_equal(got, np.repeat(want, H // H_kv, 1))
+    want = np.repeat(want, H // H_kv, 1).astype(np.float64)
+    # O = (p v) (1 / l) with l = p, whatever p is: three roundings of at most 2^-24, of which fp16's one
+    # rounding at the end, of at least 2^-11 v or none, leaves nothing (v is an fp16 number itself).
+    assert (np.abs(got - want) <= (0.0 if f16 else 3.01 * 2.0 ** -24) * np.abs(want)).all()
 
 
 @pytest.mark.gpu
