@@ -812,7 +812,7 @@ __device__ __forceinline__ void narrow_range(const cf_paged_attn_args_t& a, cons
 // A wave per unit, the units of neighbouring KV heads in one workgroup: they read the same
 // cache rows at about the same time.  HBM bounds it: with two blocks of 16 KB under way per
 // wave and four waves a CU it streams 5.7 TB/s over long caches (64 rows over 8192 each, 2.15 GB:
-// 380 us), and 16 sequences of 1778 to 4096 positions (227 MB) take 46 us, 41 of them here, the
+// 380 us), and 16 sequences of 1778 to 4096 positions (227 MB) take 46 us, 42 of them here, the
 // rest the merge.
 template <typename T, int D> struct Heads {
     static constexpr int WAVES = 4, BK = sizeof(T) == 2 ? 32 : 16;
