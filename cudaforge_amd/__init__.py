@@ -20,6 +20,9 @@ from .api import (  # noqa: F401
     KvPageMapParams,
     KvPageStoreParams,
     MhaPagedParams,
+    QkNormRopeParams,
+    KvPageStoreQ8Params,
+    MhaPagedQ8Params,
     GraphMhaMatch,
     OperatorRegistry,
     Stream,

@@ -183,7 +183,8 @@ def _proto(lib):
                  "causal_mask_f32_cuda", "rope_f32_cuda", "rope_f16_cuda", "mha_decode_rope_f32_cuda",
                  "mha_decode_rope_f16_cuda", "mha_decode_attn_f16_noalloc", "kv_page_map_i32_cuda",
                  "kv_page_store_f32_cuda", "kv_page_store_f16_cuda", "mha_paged_attn_f32_cuda",
-                 "mha_paged_attn_f16_cuda"):
+                 "mha_paged_attn_f16_cuda", "qk_norm_rope_f32_cuda", "qk_norm_rope_f16_cuda", "kv_page_store_q8_f32_cuda",
+                 "kv_page_store_q8_f16_cuda", "mha_paged_attn_q8_f32_cuda", "mha_paged_attn_q8_f16_cuda"):
         fn = getattr(lib, name)
         fn.restype = c_int
         fn.argtypes = [POINTER(c_void_p), POINTER(c_void_p), c_void_p, c_void_p]

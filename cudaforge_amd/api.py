@@ -81,6 +81,32 @@ class MhaPagedParams(ctypes.Structure):
                                        "row_stride", "head_stride")]
 
 
+class QkNormRopeParams(ctypes.Structure):
+    """qk_norm_rope_params_t (include/rope_ops.h); strides of 0 are the dense layout's."""
+
+    _fields_ = [(n, c_int64) for n in ("num_tokens", "num_heads", "num_kv_heads", "head_dim", "rotary_dim")] + \
+               [("halves", ctypes.c_int32), ("norm", ctypes.c_int32), ("eps", c_float), ("rope_base", c_float),
+                ("scaling", ctypes.c_int32)] + \
+               [(n, c_float) for n in ("factor", "original_len", "low", "high", "amplitude")] + \
+               [(n, c_int64) for n in ("q_stride", "k_stride", "q_out_stride", "k_out_stride")]
+
+
+class KvPageStoreQ8Params(ctypes.Structure):
+    """kv_page_store_q8_params_t (include/paged_ops.h); strides of 0 are the dense layout's."""
+
+    _fields_ = [(n, c_int64) for n in ("num_tokens", "num_kv_heads", "head_dim", "page_size", "num_pages", "block_size",
+                                       "kv_stride", "page_stride", "row_stride", "head_stride")]
+
+
+class MhaPagedQ8Params(ctypes.Structure):
+    """mha_paged_q8_params_t (include/paged_ops.h); strides of 0 are the dense layout's."""
+
+    _fields_ = [(n, c_int64) for n in ("batch_size", "num_tokens", "num_heads", "num_kv_heads", "head_dim")] + \
+               [("scale", c_float)] + \
+               [(n, c_int64) for n in ("page_size", "num_pages", "max_pages", "block_size", "max_new", "max_len", "q_stride",
+                                       "page_stride", "row_stride", "head_stride")]
+
+
 ONNX_FLOAT, ONNX_FLOAT16, ONNX_INT64 = 1, 10, 7
 
 

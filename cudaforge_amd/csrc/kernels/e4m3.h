@@ -1,0 +1,45 @@
+// e4m3.h — numbers of 8 bits (one sign, four exponent, three mantissa bits) with a power of two that
+// a block of them shares: value = code * 2^(power - 127), power 255 is NaN.  gfx950 converts
+// code times power in one instruction, two codes at a time; it takes the power from the exponent
+// bits of an FP32 number, 0 as 2^-127 and 255 as NaN too.
+#ifndef CF_E4M3_H_
+#define CF_E4M3_H_
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "cdna4.h"
+
+namespace cdna4 {
+
+typedef float f2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+
+// The power as the conversions take it.
+__device__ __forceinline__ float power_bits(int power) { return __uint_as_float((uint32_t)power << 23); }
+
+// Codes 0 and 1 (HI: 2 and 3) of a word.
+template <bool HI> __device__ __forceinline__ f2_t codes_f32(uint32_t w, float power) {
+    return __builtin_bit_cast(f2_t, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8((int)w, power, HI));
+}
+template <bool HI> __device__ __forceinline__ h2_t codes_f16(uint32_t w, float power) {
+    return __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, power, HI));
+}
+template <bool HI> __device__ __forceinline__ b2_t codes_bf16(uint32_t w, float power) {
+    return __builtin_bit_cast(b2_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, power, HI));
+}
+// Two values of at most 448 in size to the nearest codes, ties to even, into the low (HI: high) half of w.
+template <bool HI> __device__ __forceinline__ uint32_t codes_of(uint32_t w, float a, float b) {
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, (int)w, HI);
+}
+
+// The least power whose 448 folds are not below x >= 0 (448 = 1.75 * 2^8); x = 0 and what is too small
+// for any power: 0.
+__device__ __forceinline__ int power_for(float x) {
+    const uint32_t bits = __float_as_uint(x);
+    return max((int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), 0);
+}
+
+}  // namespace cdna4
+
+#endif  // CF_E4M3_H_

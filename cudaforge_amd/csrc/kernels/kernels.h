@@ -425,6 +425,58 @@ typedef struct {
 size_t cf_paged_attn_bytes(const cf_paged_attn_args_t* a);
 int cf_launch_paged_attn(const cf_paged_attn_args_t* a, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * Norms and rotation of Q and K (qk_norm.hip; operators in rope_ops.h).
+ * ------------------------------------------------------------------------------- */
+#define CF_QK_ROPE_MAX_DIM 256
+typedef struct {
+    const void*    x;           /* NULL: no such rows */
+    void*          y;
+    const void*    gain;        /* NULL: ones */
+    const void*    bias;        /* NULL: zeros */
+    int64_t        stride, out_stride;
+    int32_t        heads;
+} cf_qk_rows_t;
+typedef struct {
+    cf_qk_rows_t   rows[2];     /* Q, K */
+    const int32_t* positions;   /* NULL: no rotation */
+    int64_t        T;
+    int32_t        d, r;        /* values of a head, and how many are turned */
+    int32_t        halves, norm, elem;
+    float          eps, amplitude;
+    double         turns[CF_QK_ROPE_MAX_DIM / 2];   /* of each pair, per position */
+} cf_qk_norm_args_t;
+int cf_launch_qk_norm(const cf_qk_norm_args_t* a, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * The paged cache in 8 bits (paged_kv_q8.hip, paged_attn_q8.hip; operators in paged_ops.h).
+ * ------------------------------------------------------------------------------- */
+#define CF_Q8_MAX_BLOCK 64
+typedef struct {
+    const void*    k;
+    const void*    v;
+    const int32_t* slots;
+    uint8_t*       k_pages;
+    uint8_t*       v_pages;
+    uint8_t*       k_scales;
+    uint8_t*       v_scales;
+    int64_t        T, kv_stride;
+    int64_t        page_stride, row_stride, head_stride;   /* bytes */
+    int32_t        H_kv, d, page_size, block;
+    int32_t        num_slots;   /* num_pages * page_size */
+    int32_t        elem;
+} cf_page_store_q8_args_t;
+int cf_launch_page_store_q8(const cf_page_store_q8_args_t* a, void* stream);
+
+typedef struct {
+    cf_paged_attn_args_t at;    /* k and v: bytes, as are the strides of the cache */
+    const uint8_t* k_scales;
+    const uint8_t* v_scales;
+    int32_t        block;
+} cf_paged_q8_args_t;
+size_t cf_paged_attn_q8_bytes(const cf_paged_q8_args_t* a);
+int cf_launch_paged_attn_q8(const cf_paged_q8_args_t* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,204 @@
+// paged_kv_q8.hip — the write of new K and V rows into pages of 8-bit numbers (gfx950).
+//
+// Rows of one block (block positions of a page, one KV head) follow each other in a call: a run.  A
+// wave takes a run of one head of K or V: the largest finite size A of it, the power p = the least
+// with A <= 448 * 2^(p - 127), or the block's own where that is larger and the block was begun by an
+// earlier call, then code = x * 2^(127 - p) to the nearest.  Where the power of a begun block grows,
+// its other codes are rounded to the new one: a division by a power of two, so no mantissa changes
+// but of numbers that leave the normal range.
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "kernels.h"
+#include "cdna4.h"
+#include "e4m3.h"
+
+namespace {
+
+using namespace cdna4;
+
+struct StoreDivs { FastDiv block, blocks; };       // positions of a block, blocks of a page
+
+template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T e[N]; };
+
+// The largest number that the type's own values can be read back as (fp16 61440: 65504 would be
+// rounded to 65536).
+template <typename T> constexpr float kMostStored = sizeof(T) == 2 ? 61440.0f : 0x1.ep127f;
+
+// x at its power.
+__device__ __forceinline__ float to_code(float x, int shift, float most) {
+    const float y = __builtin_amdgcn_fmed3f(ldexpf(x, shift), -most, most);
+    return __builtin_fabsf(x) < INFINITY ? y : NAN;
+}
+__device__ __forceinline__ float finite_size(float x) {
+    const float s = __builtin_fabsf(x);
+    return s < INFINITY ? s : 0.0f;
+}
+
+// A wave's run: rows t .. t + len - 1, whose slots the lanes first .. first + len - 1 hold.
+struct Run {
+    int64_t t;
+    int first, len;
+    uint8_t* cells;        // the block's first position
+    int slot0;             // ... and its slot
+};
+
+// VEC elements of 16 bytes a lane, d / VEC = 2^k lanes a row; VEC = 1: any shape, all lanes on one row.
+template <typename T, int VEC>
+__device__ __forceinline__ void store_run(const cf_page_store_q8_args_t& a, const Run& run, int slot, const T* rows,
+                                          uint8_t* power) {
+    constexpr bool WIDE = VEC > 1;
+    constexpr int KEEP = WIDE ? 8 : 1;             // steps whose rows stay in registers
+    const int lane = threadIdx.x & 63;
+    const int per_row = WIDE ? a.d / VEC : 64, at_once = 64 / per_row;
+    const int sub = WIDE ? lane / per_row : 0, e0 = (lane % per_row) * VEC, step_e = WIDE ? a.d : 64;
+    typedef Pack<T, VEC> pack_t;
+    const int old = *power;
+    auto load = [&](int r, int e) { return *(const pack_t*)(rows + (run.t + min(r, run.len - 1)) * a.kv_stride + e); };
+    auto most_of = [&](const pack_t& x) {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VEC; i++) m = fmaxf(m, finite_size((float)x.e[i]));
+        return m;
+    };
+    pack_t kept[KEEP];
+    float most = 0.0f;
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int s = 0; s < KEEP; s++)
+            if (s * at_once < run.len) kept[s] = load(s * at_once + sub, e0);
+#pragma unroll
+        for (int s = 0; s < KEEP; s++)
+            if (s * at_once < run.len) most = fmaxf(most, most_of(kept[s]));
+    }
+    for (int r = WIDE ? KEEP * at_once : 0; r < run.len; r += at_once)
+        for (int e = e0; e < a.d; e += step_e) most = fmaxf(most, most_of(load(r + sub, e)));
+    const int need = power_for(wave_max(most));
+    const bool mine = lane >= run.first && lane < run.first + run.len;
+    const bool begun = __builtin_amdgcn_ballot_w64(mine && slot == run.slot0) != 0;
+    const int now = begun ? need : max(old, need);
+    if (lane == 0) *power = (uint8_t)now;
+    if (now > old && !begun) {
+        // Positions that the run writes: a bit each.
+        uint32_t lo = mine && slot - run.slot0 < 32 ? 1u << (slot - run.slot0) : 0u;
+        uint32_t hi = mine && slot - run.slot0 >= 32 ? 1u << (slot - run.slot0 - 32) : 0u;
+#pragma unroll
+        for (int m = 1; m < 64; m *= 2) {
+            lo |= __shfl_xor(lo, m);
+            hi |= __shfl_xor(hi, m);
+        }
+        const uint64_t written = (uint64_t)hi << 32 | lo;
+        const float by = power_bits(max(127 + old - now, 1));     // 448 * 2^-126 is no code any more
+        for (int r = sub; r < a.block; r += at_once) {
+            if ((written >> r) & 1) continue;
+            for (int e = e0; e < a.d; e += step_e) {
+                uint8_t* const cell = run.cells + (int64_t)r * a.row_stride + e;
+                if constexpr (WIDE) {
+                    Pack<uint32_t, VEC / 4> c = *(const Pack<uint32_t, VEC / 4>*)cell;
+#pragma unroll
+                    for (int i = 0; i < VEC / 4; i++) {
+                        const f2_t x = codes_f32<false>(c.e[i], by), y = codes_f32<true>(c.e[i], by);
+                        c.e[i] = codes_of<true>(codes_of<false>(0, x[0], x[1]), y[0], y[1]);
+                    }
+                    *(Pack<uint32_t, VEC / 4>*)cell = c;
+                } else {
+                    *cell = (uint8_t)codes_of<false>(0, codes_f32<false>(*cell, by)[0], 0.0f);
+                }
+            }
+        }
+    }
+    const float limit = fminf(448.0f, ldexpf(kMostStored<T>, 127 - now));
+    auto place = [&](int r) { return run.cells + (int64_t)(__shfl(slot, run.first + min(r, run.len - 1)) - run.slot0) * a.row_stride; };
+    auto put = [&](int r, uint8_t* cell, const pack_t& x) {
+        if (r >= run.len) return;
+        if constexpr (WIDE) {
+            Pack<uint32_t, VEC / 4> c;
+#pragma unroll
+            for (int i = 0; i < VEC / 4; i++) {
+                float y[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) y[j] = to_code((float)x.e[4 * i + j], 127 - now, limit);
+                c.e[i] = codes_of<true>(codes_of<false>(0, y[0], y[1]), y[2], y[3]);
+            }
+            *(Pack<uint32_t, VEC / 4>*)cell = c;
+        } else {
+            *cell = (uint8_t)codes_of<false>(0, to_code((float)x.e[0], 127 - now, limit), 0.0f);
+        }
+    };
+    if constexpr (WIDE)
+#pragma unroll
+        for (int s = 0; s < KEEP; s++)
+            if (s * at_once < run.len) put(s * at_once + sub, place(s * at_once + sub) + e0, kept[s]);
+    for (int r = WIDE ? KEEP * at_once : 0; r < run.len; r += at_once) {
+        uint8_t* const cell = place(r + sub);      // (by all lanes)
+        for (int e = e0; e < a.d; e += step_e) put(r + sub, cell + e, load(r + sub, e));
+    }
+}
+
+// Workgroup (x, y): the runs that begin in rows R x .. R x + R - 1, of heads 4 y .. 4 y + 3 of K's
+// and V's, a wave each.  R + block <= 64: the lanes hold the slots of those runs.
+constexpr int kStoreWaves = 4;
+template <typename T, int VEC>
+__global__ __launch_bounds__(64 * kStoreWaves)
+void page_store_q8(cf_page_store_q8_args_t a, StoreDivs dv, int R, int64_t row0) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int unit = (int)blockIdx.y * kStoreWaves + wave;
+    if (unit >= 2 * a.H_kv) return;
+    const int which = unit >= a.H_kv, h = unit - (which ? a.H_kv : 0);
+    const int64_t t0 = row0 + (int64_t)blockIdx.x * R;
+    const int slot = t0 + lane < a.T ? a.slots[t0 + lane] : -1;
+    const int last = t0 > 0 ? a.slots[t0 - 1] : -1;
+    auto block_of = [&](int s) { return (unsigned)s < (unsigned)a.num_slots ? fastdiv(s, dv.block) : -1; };
+    const int block = block_of(slot);
+    const int up = __shfl_up(block, 1), before = lane == 0 ? block_of(last) : up;
+    uint64_t heads = __builtin_amdgcn_ballot_w64(lane < R && block >= 0 && block != before);
+    const T* const rows = (const T*)(which ? a.v : a.k) + (int64_t)h * a.d;
+    uint8_t* const pages = which ? a.v_pages : a.k_pages;
+    uint8_t* const powers = which ? a.v_scales : a.k_scales;
+    for (; heads; heads &= heads - 1) {
+        Run run;
+        run.first = __builtin_ctzll(heads);
+        const int b = __builtin_amdgcn_readlane(block, run.first);
+        const uint64_t same = __builtin_amdgcn_ballot_w64(block == b) >> run.first;
+        run.len = ~same ? __builtin_ctzll(~same) : 64;
+        run.t = t0 + run.first;
+        run.slot0 = b * a.block;
+        const int page = fastdiv(b, dv.blocks);
+        run.cells = pages + (int64_t)page * a.page_stride + (int64_t)(run.slot0 - page * a.page_size) * a.row_stride +
+                    (int64_t)h * a.head_stride;
+        store_run<T, VEC>(a, run, slot, rows, powers + (int64_t)b * a.H_kv + h);
+    }
+}
+
+template <typename T>
+int launch_store(const cf_page_store_q8_args_t& a, hipStream_t st) {
+    constexpr int kWide = 16 / sizeof(T);
+    const uint64_t in = (uint64_t)(uintptr_t)a.k | (uint64_t)(uintptr_t)a.v | (uint64_t)a.kv_stride * sizeof(T);
+    const uint64_t out = (uint64_t)(uintptr_t)a.k_pages | (uint64_t)(uintptr_t)a.v_pages | (uint64_t)a.page_stride |
+                         (uint64_t)a.row_stride | (uint64_t)a.head_stride;
+    const int per_row = a.d / kWide;
+    const bool wide = in % 16 == 0 && out % kWide == 0 && a.d % kWide == 0 && per_row <= 64 && (per_row & (per_row - 1)) == 0;
+    const StoreDivs dv = {fastdiv_make(a.block), fastdiv_make(a.page_size / a.block)};
+    const int R = a.T >= 2048 && a.block <= 48 ? 16 : 1;
+    const unsigned parts = (unsigned)((2 * (int64_t)a.H_kv + kStoreWaves - 1) / kStoreWaves);
+    constexpr int64_t kMost = 1 << 23;             // rows of a launch: a grid has less than 2^32 threads
+    for (int64_t t0 = 0; t0 < a.T; t0 += kMost * R) {
+        const int64_t n = (a.T - t0 + R - 1) / R;
+        const dim3 grid((unsigned)(n < kMost ? n : kMost), parts), block(64 * kStoreWaves);
+        if (wide) hipLaunchKernelGGL((page_store_q8<T, kWide>), grid, block, 0, st, a, dv, R, t0);
+        else hipLaunchKernelGGL((page_store_q8<T, 1>), grid, block, 0, st, a, dv, R, t0);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return (int)e;
+    }
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int cf_launch_page_store_q8(const cf_page_store_q8_args_t* a, void* stream) {
+    if (a->T <= 0 || a->d <= 0 || a->H_kv <= 0 || a->block <= 0 || a->block > CF_Q8_MAX_BLOCK || a->page_size % a->block != 0)
+        return (int)hipErrorInvalidValue;
+    return a->elem == CF_ELEM_F16 ? launch_store<_Float16>(*a, (hipStream_t)stream)
+                                  : launch_store<float>(*a, (hipStream_t)stream);
+}

@@ -135,12 +135,11 @@ int kv_page_store_f16_cuda(const void* inputs[], void* outputs[], const operator
 
 /* ------------------------------------------------------------------ attention --- */
 
-static int paged_attn_op(int elem, const void* inputs[], void* outputs[], const operator_params_t* params,
-                         stream_t* stream) {
-    if (!inputs || !outputs || !params) return -1;
+/* 1: `a` (all zeros before) holds the call; 0: there is nothing to do; -1: refused. */
+static int paged_attn_args(const mha_paged_params_t* p, int elem, const void* inputs[], void* outputs[],
+                           cf_paged_attn_args_t* to) {
     for (int i = 0; i < 6; i++) if (!inputs[i]) return -1;
     if (!outputs[0]) return -1;
-    const mha_paged_params_t* p = (const mha_paged_params_t*)params;
     const int64_t H = p->num_heads, H_kv = p->num_kv_heads > 0 ? p->num_kv_heads : H, d = p->head_dim;
     if (p->batch_size < 0 || p->num_tokens < 0 || H <= 0 || d <= 0 || H % H_kv != 0) return -1;
     if (p->batch_size > INT32_MAX - 1 || p->num_tokens > INT32_MAX || H > 65535 || d > 512) return -1;
@@ -151,8 +150,7 @@ static int paged_attn_op(int elem, const void* inputs[], void* outputs[], const 
     if (p->batch_size == 0 || p->num_tokens == 0) return 0;
     /* A row's tile may be read after another's rows are written. */
     for (int i = 0; i < 3; i++) if (outputs[0] == inputs[i]) return -1;
-    cf_paged_attn_args_t a;
-    memset(&a, 0, sizeof(a));
+    cf_paged_attn_args_t a = *to;
     a.q = inputs[0];
     a.k = inputs[1];
     a.v = inputs[2];
@@ -177,13 +175,27 @@ static int paged_attn_op(int elem, const void* inputs[], void* outputs[], const 
     a.max_len = (int32_t)(p->max_len > 0 && p->max_len < table_len ? p->max_len : table_len);
     a.scale = p->scale;
     a.elem = elem;
+    *to = a;
+    return 1;
+}
+
+/* Without a buffer (no memory, or a recording on a stream that has none of that size) no tile
+ * is cut. */
+static void paged_attn_workspace(cf_paged_attn_args_t* a, size_t bytes, void* st) {
+    if (bytes > 0 && !(a->workspace = gpu_workspace_try_stream(st, bytes)) &&
+        !(a->workspace = gpu_workspace_get_stream(st, bytes)))
+        a->uncut = 1;
+}
+
+static int paged_attn_op(int elem, const void* inputs[], void* outputs[], const operator_params_t* params,
+                         stream_t* stream) {
+    if (!inputs || !outputs || !params) return -1;
+    cf_paged_attn_args_t a;
+    memset(&a, 0, sizeof(a));
+    const int rc = paged_attn_args((const mha_paged_params_t*)params, elem, inputs, outputs, &a);
+    if (rc != 1) return rc;
     void* st = cf_stream_of(stream);
-    const size_t bytes = cf_paged_attn_bytes(&a);
-    /* Without a buffer (no memory, or a recording on a stream that has none of that size) no tile
-     * is cut. */
-    if (bytes > 0 && !(a.workspace = gpu_workspace_try_stream(st, bytes)) &&
-        !(a.workspace = gpu_workspace_get_stream(st, bytes)))
-        a.uncut = 1;
+    paged_attn_workspace(&a, cf_paged_attn_bytes(&a), st);
     return cf_launch_paged_attn(&a, st);
 }
 
@@ -193,6 +205,91 @@ int mha_paged_attn_f32_cuda(const void* inputs[], void* outputs[], const operato
 
 int mha_paged_attn_f16_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream) {
     return paged_attn_op(CF_ELEM_F16, inputs, outputs, params, stream);
+}
+
+/* ------------------------------------------------------------------ the same in 8 bits --- */
+
+/* Positions of a block, 0 where they are not allowed. */
+static int64_t block_of(int64_t block, int64_t page_size) {
+    if (block == 0) block = 16;
+    return block > 0 && block <= CF_Q8_MAX_BLOCK && page_size % block == 0 ? block : 0;
+}
+
+static int page_store_q8_op(int elem, const void* inputs[], void* outputs[], const operator_params_t* params,
+                            stream_t* stream) {
+    if (!inputs || !outputs || !params) return -1;
+    for (int i = 0; i < 3; i++) if (!inputs[i]) return -1;
+    for (int i = 0; i < 4; i++) if (!outputs[i]) return -1;
+    const kv_page_store_q8_params_t* p = (const kv_page_store_q8_params_t*)params;
+    if (p->num_tokens < 0 || p->num_kv_heads <= 0 || p->head_dim <= 0 || !pages_ok(p->page_size, p->num_pages)) return -1;
+    if (p->num_tokens > INT32_MAX || p->num_kv_heads > 65535 || p->head_dim > 65535) return -1;
+    if (p->num_kv_heads * p->head_dim > (1 << 29) || p->kv_stride < 0) return -1;
+    const int64_t block = block_of(p->block_size, p->page_size);
+    if (block == 0) return -1;
+    cache_strides_t cs;
+    if (cache_strides(p->page_stride, p->row_stride, p->head_stride, p->page_size, p->num_kv_heads, p->head_dim, &cs) != 0)
+        return -1;
+    if (p->num_tokens == 0) return 0;
+    cf_page_store_q8_args_t a;
+    memset(&a, 0, sizeof(a));
+    a.k = inputs[0];
+    a.v = inputs[1];
+    a.slots = (const int32_t*)inputs[2];
+    a.k_pages = (uint8_t*)outputs[0];
+    a.v_pages = (uint8_t*)outputs[1];
+    a.k_scales = (uint8_t*)outputs[2];
+    a.v_scales = (uint8_t*)outputs[3];
+    a.T = p->num_tokens;
+    a.kv_stride = p->kv_stride > 0 ? p->kv_stride : p->num_kv_heads * p->head_dim;
+    a.page_stride = cs.page;
+    a.row_stride = cs.row;
+    a.head_stride = cs.head;
+    a.H_kv = (int32_t)p->num_kv_heads;
+    a.d = (int32_t)p->head_dim;
+    a.page_size = (int32_t)p->page_size;
+    a.block = (int32_t)block;
+    a.num_slots = (int32_t)(p->num_pages * p->page_size);
+    a.elem = elem;
+    return cf_launch_page_store_q8(&a, cf_stream_of(stream));
+}
+
+int kv_page_store_q8_f32_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream) {
+    return page_store_q8_op(CF_ELEM_F32, inputs, outputs, params, stream);
+}
+
+int kv_page_store_q8_f16_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream) {
+    return page_store_q8_op(CF_ELEM_F16, inputs, outputs, params, stream);
+}
+
+static int paged_attn_q8_op(int elem, const void* inputs[], void* outputs[], const operator_params_t* params,
+                            stream_t* stream) {
+    if (!inputs || !outputs || !params) return -1;
+    for (int i = 0; i < 8; i++) if (!inputs[i]) return -1;
+    const mha_paged_q8_params_t* p = (const mha_paged_q8_params_t*)params;
+    const mha_paged_params_t same = {
+        .batch_size = p->batch_size, .num_tokens = p->num_tokens, .num_heads = p->num_heads, .num_kv_heads = p->num_kv_heads,
+        .head_dim = p->head_dim, .scale = p->scale, .page_size = p->page_size, .num_pages = p->num_pages,
+        .max_pages = p->max_pages, .max_new = p->max_new, .max_len = p->max_len, .q_stride = p->q_stride,
+        .page_stride = p->page_stride, .row_stride = p->row_stride, .head_stride = p->head_stride};
+    cf_paged_q8_args_t a;
+    memset(&a, 0, sizeof(a));
+    const int rc = paged_attn_args(&same, elem, inputs, outputs, &a.at);
+    if (rc < 0 || (a.block = (int32_t)block_of(p->block_size, p->page_size)) == 0) return -1;
+    if (rc == 0) return 0;
+    for (int i = 6; i < 8; i++) if (outputs[0] == inputs[i]) return -1;
+    a.k_scales = (const uint8_t*)inputs[6];
+    a.v_scales = (const uint8_t*)inputs[7];
+    void* st = cf_stream_of(stream);
+    paged_attn_workspace(&a.at, cf_paged_attn_q8_bytes(&a), st);
+    return cf_launch_paged_attn_q8(&a, st);
+}
+
+int mha_paged_attn_q8_f32_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream) {
+    return paged_attn_q8_op(CF_ELEM_F32, inputs, outputs, params, stream);
+}
+
+int mha_paged_attn_q8_f16_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream) {
+    return paged_attn_q8_op(CF_ELEM_F16, inputs, outputs, params, stream);
 }
 
 /* ------------------------------------------------------------------ registrations --- */
@@ -219,5 +316,25 @@ int register_mha_paged_attn_f32_cuda(void) {
 
 int register_mha_paged_attn_f16_cuda(void) {
     static const operator_registry_t reg = {"mha_paged_attn_f16_cuda", "f16", mha_paged_attn_f16_cuda, 1, OP_FLAG_NONE};
+    return operator_register(&reg);
+}
+
+int register_kv_page_store_q8_f32_cuda(void) {
+    static const operator_registry_t reg = {"kv_page_store_q8_f32_cuda", "f32", kv_page_store_q8_f32_cuda, 1, OP_FLAG_ALLOW_ALIAS};
+    return operator_register(&reg);
+}
+
+int register_kv_page_store_q8_f16_cuda(void) {
+    static const operator_registry_t reg = {"kv_page_store_q8_f16_cuda", "f16", kv_page_store_q8_f16_cuda, 1, OP_FLAG_ALLOW_ALIAS};
+    return operator_register(&reg);
+}
+
+int register_mha_paged_attn_q8_f32_cuda(void) {
+    static const operator_registry_t reg = {"mha_paged_attn_q8_f32_cuda", "f32", mha_paged_attn_q8_f32_cuda, 1, OP_FLAG_NONE};
+    return operator_register(&reg);
+}
+
+int register_mha_paged_attn_q8_f16_cuda(void) {
+    static const operator_registry_t reg = {"mha_paged_attn_q8_f16_cuda", "f16", mha_paged_attn_q8_f16_cuda, 1, OP_FLAG_NONE};
     return operator_register(&reg);
 }

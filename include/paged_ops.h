@@ -145,11 +145,71 @@ typedef struct {
 int mha_paged_attn_f32_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
 int mha_paged_attn_f16_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
 
+/* ---- the same cache in 8 bits ----
+ *
+ * A number of the cache is an e4m3 byte (one sign, four exponent and three mantissa bits, bias 7, at
+ * most 448; 0x7f and 0xff are NaN, infinity there is none) times the power of two of its block:
+ * positions s B .. s B + B - 1 of a page, of one KV head, share a byte e that stands for 2^(e - 127)
+ * (255: NaN).  Layouts: K and V pages (num_pages, page_size, H_kv, d) bytes, K and V powers
+ * (num_pages, page_size / B, H_kv) bytes; 1 + 1 / (B d) bytes a value.  The steps, tables, slots
+ * and lengths are those above; kv_page_map serves both.  A power of two instead of any scale: taking
+ * a larger one later changes no number's mantissa, and fp16 and bf16 hold the values exactly. */
+
+typedef struct {
+    int64_t num_tokens;    /* T */
+    int64_t num_kv_heads;  /* H_kv */
+    int64_t head_dim;      /* d; H_kv d at most 2^29 */
+    int64_t page_size;
+    int64_t num_pages;
+    int64_t block_size;    /* B: at most 64, divides page_size; 0: 16 */
+    int64_t kv_stride;     /* elements from row to row of K_new and V_new; 0: H_kv d */
+    int64_t page_stride, row_stride, head_stride;   /* bytes of the cache; 0: the dense layout's */
+} kv_page_store_q8_params_t;
+
+/* inputs  [K_new (T, H_kv, d), V_new (T, H_kv, d), slots (T)]
+ * outputs [K_pages, V_pages, K_powers, V_powers], in place
+ * The power of a block's new rows is the least whose 448 fold no finite value of theirs exceeds (0 where
+ * there is none).  A block whose first position is among them begins with it; else the block takes
+ * the larger of it and the one that it has, and where that grows what the block holds (all its
+ * positions but the new ones) is divided by as much: exact but for numbers that come below 2^-6 of
+ * the power.  Values are rounded to nearest, ties to even; infinite and NaN ones become NaN.  Where a
+ * rounding would pass the type's largest number, as 65504 to 65536, the one below is stored, so that
+ * what is read back stays finite.  A row with an invalid slot is not stored.  Rows for one block follow
+ * each other, in any order, as kv_page_map gives them, and each slot may be given once per
+ * call: otherwise that block's numbers and powers mean nothing. */
+int kv_page_store_q8_f32_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
+int kv_page_store_q8_f16_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
+
+typedef struct {
+    int64_t batch_size, num_tokens, num_heads, num_kv_heads, head_dim;   /* as in mha_paged_params_t */
+    float   scale;
+    int64_t page_size, num_pages, max_pages;
+    int64_t block_size;    /* as in kv_page_store_q8_params_t */
+    int64_t max_new, max_len;
+    int64_t q_stride;      /* elements from row to row of Q; 0 = H_q d */
+    int64_t page_stride, row_stride, head_stride;   /* bytes of the cache; 0: the dense layout's */
+} mha_paged_q8_params_t;
+
+/* inputs  [Q (T, H_q, d), K_pages, V_pages, block_table (B, max_pages), seq_lens (B), q_start (B + 1),
+ *          K_powers, V_powers]
+ * outputs [O (T, H_q, d)]
+ * mha_paged_attn's rules, on the values that the bytes stand for; Q and O are of the operator's type.
+ * f16: values are taken as fp16 (exact for what kv_page_store_q8_f16 stores; past its range infinite,
+ * below it rounded); f32: as bf16, exact down to 2^-133.  d = 64 and 128 with blocks of a multiple of
+ * 16 positions, 16-byte aligned pages, strides, Q and O, scale > 0 and at most 32768 sequences run on
+ * the matrix cores, every other call on a plain kernel. */
+int mha_paged_attn_q8_f32_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
+int mha_paged_attn_q8_f16_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
+
 int register_kv_page_map_i32_cuda(void);
 int register_kv_page_store_f32_cuda(void);
 int register_kv_page_store_f16_cuda(void);
 int register_mha_paged_attn_f32_cuda(void);
 int register_mha_paged_attn_f16_cuda(void);
+int register_kv_page_store_q8_f32_cuda(void);
+int register_kv_page_store_q8_f16_cuda(void);
+int register_mha_paged_attn_q8_f32_cuda(void);
+int register_mha_paged_attn_q8_f16_cuda(void);
 
 #ifdef __cplusplus
 }
