@@ -14,6 +14,8 @@ namespace cdna4 {
 
 typedef float f2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+typedef __attribute__((__vector_size__(8))) int lds_i2_t;
 
 // The power as the conversions take it.
 __device__ __forceinline__ float power_bits(int power) { return __uint_as_float((uint32_t)power << 23); }
@@ -31,6 +33,37 @@ template <bool HI> __device__ __forceinline__ b2_t codes_bf16(uint32_t w, float 
 // Two values of at most 448 in size to the nearest codes, ties to even, into the low (HI: high) half of w.
 template <bool HI> __device__ __forceinline__ uint32_t codes_of(uint32_t w, float a, float b) {
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, (int)w, HI);
+}
+
+// The same as the type that the matrix cores take, 16 bits wide: B, with eight of them (codes of two
+// words, each with its power) as one operand.
+template <typename B> struct Codes;
+template <> struct Codes<_Float16> {
+    typedef h8_t eight_t;
+    static __device__ __forceinline__ eight_t of(uint32_t lo, float plo, uint32_t hi, float phi) {
+        const h2_t a = codes_f16<false>(lo, plo), b = codes_f16<true>(lo, plo), c = codes_f16<false>(hi, phi), d = codes_f16<true>(hi, phi);
+        return eight_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    }
+    static __device__ __forceinline__ f4_t mfma(eight_t a, eight_t b, f4_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <> struct Codes<__bf16> {
+    typedef b8_t eight_t;
+    static __device__ __forceinline__ eight_t of(uint32_t lo, float plo, uint32_t hi, float phi) {
+        const b2_t a = codes_bf16<false>(lo, plo), b = codes_bf16<true>(lo, plo), c = codes_bf16<false>(hi, phi), d = codes_bf16<true>(hi, phi);
+        return eight_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    }
+    static __device__ __forceinline__ f4_t mfma(eight_t a, eight_t b, f4_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+};
+
+// ds_read_b64_tr_b8: in each 16-lane group, lane i receives byte i % 8 of the 8-byte chunks that
+// lanes i / 8, 2 + i / 8, .., 14 + i / 8 address.  With lane j addressing X[row j / 2][8 (j % 2)],
+// lane i gets column i of the eight rows.
+__device__ __forceinline__ lds_i2_t ds_read_tr8(const uint8_t* p) {
+    return __builtin_amdgcn_ds_read_tr8_b64_v2i32((CF_LDS lds_i2_t*)p);
 }
 
 // The least power whose 448 folds are not below x >= 0 (448 = 1.75 * 2^8); x = 0 and what is too small

@@ -96,6 +96,454 @@ __device__ __forceinline__ void plain_row_q8(const cf_paged_q8_args_t& a, const 
         if (lane + 64 * i < d) o[lane + 64 * i] = (T)(acc[i] * inv);
 }
 
+// ---- On the matrix cores: d = 64 or 128, blocks of a multiple of 16 positions ----
+//
+// Codes go to LDS as they are and become 16-bit operands on their way to the matrix cores, one
+// instruction for two, the power of their block with them: exact, so nothing is scaled afterwards.
+// fp16 rows go with fp16 codes.  FP32 rows go with bf16 codes, and Q and the weights of V as sums of
+// three bf16 numbers, whose 24 bits are FP32's own: three products for one, at 8 times the FP32
+// MFMA's rate.
+
+// T rows: what the matrix cores take, and in how many parts Q and the weights.
+template <typename T> struct Parts;
+template <> struct Parts<_Float16> {
+    typedef _Float16 half_t;
+    static constexpr int Q = 1, P = 2;
+};
+template <> struct Parts<float> {
+    typedef __bf16 half_t;
+    static constexpr int Q = 3, P = 3;
+};
+// x as the sum of N numbers of B, part by part into element e of `to`.
+template <int N, typename B, typename V>
+__device__ __forceinline__ void split_into(V (&to)[N], int e, float x) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const B y = (B)x;
+        to[i][e] = y;
+        x -= (float)y;
+    }
+}
+
+// Rows of D codes in LDS and in lanes, in 16-byte chunks.
+template <int D> struct Rows8 {
+    static constexpr int CPR = D / 16;                 // chunks per row
+    static constexpr int RPI = 64 / CPR;               // rows per DMA instruction (1 KB)
+    static constexpr int NI = 16 / RPI;                // DMA instructions per 16 rows
+    static constexpr int KF = D / 64;                  // chunks of a K row a lane takes
+    static constexpr int UT = D / 16;                  // 16-dim tiles of O^T
+    static __device__ __forceinline__ int drow(int lane) { return lane / CPR; }
+    static __device__ __forceinline__ int dch(int lane) { return lane % CPR; }
+    // Chunks are swizzled so that 8 lanes on 8 rows (K) and 16 lanes on 8 rows (V, rows 4 lq .. + 3
+    // of an even group of 16 and of the odd one behind it) touch every bank once.
+    static __device__ __forceinline__ int kswz(int row) { return D == 128 ? row & 7 : (row >> 1) & 3; }
+    static __device__ __forceinline__ int vswz(int row, int odd) { return D == 128 ? (row & 3) | odd << 2 : ((row >> 1) & 1) | odd << 1; }
+    // Lane (lr, lq) takes chunks 4 f + lq of K row lr: dims 64 f + 16 lq .. + 15, the k-slots of MFMA
+    // steps 2 f and 2 f + 1.
+    static __device__ __forceinline__ void k_offsets(int (&rd)[KF], int lane) {
+        const int lr = lane & 15, lq = lane >> 4;
+#pragma unroll
+        for (int f = 0; f < KF; f++) rd[f] = lr * D + 16 * ((4 * f + lq) ^ kswz(lr));
+    }
+    // V (ds_read_tr8): positions 4 lq .. + 3 of two groups of 16, dims 16 u .. + 15.
+    static __device__ __forceinline__ void v_offsets(int (&rd)[UT], int lane) {
+        const int lr = lane & 15, lq = lane >> 4, odd = lr >> 3, row = 4 * lq + ((lr >> 1) & 3);
+#pragma unroll
+        for (int u = 0; u < UT; u++) rd[u] = (16 * odd + row) * D + 16 * (u ^ vswz(row, odd)) + 8 * (lr & 1);
+    }
+};
+
+// The next 64 groups of 16 positions of a range, one per lane: where each starts (bytes), which
+// of its positions count, and the powers of its K and V (those of a group of none are 2^0).
+struct Groups8 {
+    const int32_t* table;
+    int lo, hi, info;        // lane: base + lane; info: positions, power of K << 16, of V << 24
+    __device__ __forceinline__ void load(const cf_paged_q8_args_t& a, const PagedPlan& pl, const Q8Divs& dv, int kvh, int base,
+                                         int key0, int key1) {
+        const int key = key0 + (base + (int)(threadIdx.x & 63)) * 16;
+        const int page = table[fastdiv(min(key, a.at.max_pages * a.at.page_size - 1), pl.by_page)];
+        const Group g = group_of(a.at, pl, page, key, key1);
+        const int in = key - fastdiv(key, pl.by_page) * a.at.page_size;
+        const int64_t p = ((int64_t)(g.mask ? page : 0) * (a.at.page_size / a.block) + fastdiv(in, dv.block)) * a.at.H_kv + kvh;
+        const uint32_t kp = a.k_scales[p], vp = a.v_scales[p];
+        lo = (int)g.at;
+        hi = (int)(g.at >> 32);
+        info = (int)(g.mask ? g.mask | kp << 16 | vp << 24 : 0x7f7f0000u);
+        asm volatile("" : "+v"(lo), "+v"(hi), "+v"(info));    // they have arrived
+    }
+    __device__ __forceinline__ int64_t at(int i) const {
+        return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i & 63) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane(lo, i & 63));
+    }
+    __device__ __forceinline__ uint32_t what(int i) const { return (uint32_t)__builtin_amdgcn_readlane(info, i & 63); }
+};
+__device__ __forceinline__ float k_power(uint32_t info) { return __uint_as_float((info << 7) & 0x7f800000u); }
+__device__ __forceinline__ float v_power(uint32_t info) { return __uint_as_float((info >> 1) & 0x7f800000u); }
+
+// Which of some V are NaN: a bit for each element of the lane's 16-byte chunk.
+template <int D>
+__device__ __forceinline__ uint32_t find_nan(const cf_paged_q8_args_t& a, const Q8Divs& dv, int b, int kvh, int from, int to) {
+    using R = Rows8<D>;
+    const int lane = threadIdx.x & 63, sub = R::drow(lane);
+    const int32_t* const table = a.at.table + (size_t)b * a.at.max_pages;
+    const uint8_t* const v = (const uint8_t*)a.at.v + (int64_t)kvh * a.at.head_stride + 16 * R::dch(lane);
+    uint32_t found = 0;
+#pragma clang loop unroll(disable)
+    for (int p0 = from; p0 < to; p0 += 64) {
+        const int key = min(p0 + lane, to - 1);
+        const Cell cell = cell_of(a, dv, table, key);
+        const bool all = cell.at >= 0 && a.v_scales[cell.power + kvh] == 255;
+#pragma clang loop unroll(disable)
+        for (int r = sub; r < 64; r += R::RPI) {
+            const int64_t row = (int64_t)((uint64_t)(uint32_t)__shfl((int)(cell.at >> 32), r) << 32 | (uint32_t)__shfl((int)cell.at, r));
+            const bool whole = __shfl((int)all, r);
+            if (row < 0) continue;
+            const uint4 x = *(const uint4*)(v + row);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) found |= (whole || ((w[i] >> (8 * e)) & 0x7f) == 0x7f) ? 1u << (4 * i + e) : 0u;
+        }
+    }
+#pragma unroll
+    for (int step = R::CPR; step < 64; step *= 2) found |= __shfl_xor(found, step);
+    return found;
+}
+
+// Rows row0 + bit of a unit (a bit of `rows` each), computed and stored by this wave, where a sum is NaN
+// while l is a number (spoilt).  An element is NaN where a V that its row sees is; where only V are
+// that it does not see, or none is (codes past fp16's range), the plain loop computes the row again.
+template <typename T, int D, int TM>
+__device__ __forceinline__ void mend_rows8(const cf_paged_q8_args_t& a, const PagedPlan& pl, const Q8Divs& dv, const Unit& un,
+                                           int kvh, const Work& w, int row0, uint32_t rows) {
+    using R = Rows8<D>;
+    const int lane = threadIdx.x & 63;
+    wait_vm<0>();                                             // what it stored is stored
+    uint32_t seen = 0;
+    int upto = w.key0;
+    for (; rows; rows &= rows - 1) {
+        const int row = row0 + __builtin_ctz(rows);
+        const RowAt at = row_at(pl, pl.G, kvh, w.R0 + row);
+        const int sees = max(min(min(w.base + at.tok, un.s.len), w.key1), upto);     // rises with the rows
+        seen |= find_nan<D>(a, dv, un.b, kvh, upto, sees);
+        upto = sees;
+        const uint32_t hidden = find_nan<D>(a, dv, un.b, kvh, sees, w.key1);
+        float* const rec = un.n_ranges > 1 ? record_of<TM, D>(a.at, pl, un, kvh) : nullptr;
+        T* const o = (T*)a.at.o + ((int64_t)(un.s.row0 + at.tok) * a.at.H_q + at.h) * D;
+        if (__builtin_amdgcn_ballot_w64((hidden & ~seen) != 0) || !__builtin_amdgcn_ballot_w64(seen != 0)) {
+            plain_row_q8<T, D / 64>(a, dv, un.s, un.b, at.tok, at.h, D, w.key0, w.key1, rec ? rec + row : nullptr, TM,
+                                    rec + 2 * TM + row * D);
+            continue;
+        }
+        if (lane >= R::CPR) continue;
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            if (!((seen >> e) & 1)) continue;
+            if (rec) rec[2 * TM + row * D + 16 * lane + e] = NAN;
+            else o[16 * lane + e] = (T)NAN;
+        }
+    }
+}
+
+// ---- Up to 16 rows, one wave with a ring of its own: no barrier. ----
+template <int D> struct Narrow8 {
+    static constexpr int BK = 32, NS = 2;
+    static constexpr int TILE = BK * D, STAGE = 2 * TILE;    // bytes
+    static constexpr int RING = NS * STAGE;
+};
+
+// Positions [key0, key1) (key0 a multiple of 16) of (b, kvh) for the unit's rows: leaves m and
+// the lane's share of l, and lane (lr, lq) with dims 16 u + 4 lq .. + 3 of row lr.
+template <typename T, int D>
+__device__ __forceinline__ void narrow_range8(const cf_paged_q8_args_t& a, const PagedPlan& pl, const Q8Divs& dv, uint8_t* ring,
+                                              const SeqRows& s, int b, int kvh, const Work& w, int key0, int key1,
+                                              f4_t (&acc)[D / 16], float& m_run, float& l_run) {
+    using R = Rows8<D>;
+    using N = Narrow8<D>;
+    using B = typename Parts<T>::half_t;
+    using C = Codes<B>;
+    typedef typename C::eight_t eight_t;
+    constexpr int BK = N::BK, NG = BK / 16, NS = N::NS, TILE = N::TILE, STAGE = N::STAGE, NI = R::NI, NL = 2 * NG * NI, UT = R::UT;
+    constexpr int QP = Parts<T>::Q, PP = Parts<T>::P, KS = D / 32;
+    // Q: 16-byte chunks per row, rows per DMA instruction, elements per chunk.
+    constexpr int QC = D * (int)sizeof(T) / 16, QR = 64 / QC, QN = 16 / QR, QE = 16 / (int)sizeof(T);
+    static_assert(16 * D * (int)sizeof(T) <= STAGE, "Q fits a stage");
+    static_assert(NS * NL < 64, "vmcnt range");
+    const int lane = unit_lane(), lr = lane & 15, lq = lane >> 4;
+    const int drow = R::drow(lane), dch = R::dch(lane);
+#pragma unroll
+    for (int u = 0; u < UT; u++) acc[u] = f4_t{0.f, 0.f, 0.f, 0.f};
+    m_run = -INFINITY;
+    l_run = 0.0f;
+    LongSum l;
+    const int nblk = key1 > key0 ? (key1 - key0 + BK - 1) / BK : 0;
+    if (nblk == 0) return;
+    const float c = a.at.scale * kLog2e;
+    const int seen = min(w.base + fastdiv(w.R0 + min(lr, w.n_rows - 1), pl.by_group), s.len);
+    const int seen_all = min(w.base + fastdiv(w.R0, pl.by_group), s.len);
+
+    uint32_t koff[NI], voff[NI][2];
+#pragma unroll
+    for (int u = 0; u < NI; u++) {
+        const int row = R::RPI * u + drow;
+        koff[u] = (uint32_t)row * (uint32_t)a.at.row_stride + 16 * (dch ^ R::kswz(row));
+        voff[u][0] = (uint32_t)row * (uint32_t)a.at.row_stride + 16 * (dch ^ R::vswz(row, 0));
+        voff[u][1] = (uint32_t)row * (uint32_t)a.at.row_stride + 16 * (dch ^ R::vswz(row, 1));
+    }
+    int k_rd[R::KF], v_rd[UT];
+    R::k_offsets(k_rd, lane);
+    R::v_offsets(v_rd, lane);
+    const uint32_t ring_base = __builtin_amdgcn_readfirstlane(lds_offset(ring));
+    const uint8_t* const kp = (const uint8_t*)a.at.k + (int64_t)kvh * a.at.head_stride;
+    const uint8_t* const vp = (const uint8_t*)a.at.v + (int64_t)kvh * a.at.head_stride;
+    Groups8 groups = {a.at.table + (size_t)b * a.at.max_pages, 0, 0, 0};
+    groups.load(a, pl, dv, kvh, 0, key0, key1);
+
+    uint32_t info[NS][NG];
+    auto issue = [&](int blk, auto stage_c) {
+        constexpr int stage = decltype(stage_c)::value;
+        if (blk > 0 && blk % (64 / NG) == 0) groups.load(a, pl, dv, kvh, blk * NG, key0, key1);
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            const int64_t at = groups.at(blk * NG + g);
+            const uint32_t lds = ring_base + (uint32_t)(stage * STAGE + 16 * g * D);
+#pragma unroll
+            for (int u = 0; u < NI; u++) {
+                lds_dma16_s(koff[u], kp + at, lds + u * 1024u);
+                lds_dma16_s(voff[u][g & 1], vp + at, lds + (uint32_t)TILE + u * 1024u);
+            }
+            info[stage][g] = groups.what(blk * NG + g);
+        }
+    };
+
+    wait_lds_reads();                                         // what the ring held before
+    // Q rows by DMA into the last stage, which the first blocks leave free; chunks swizzled by the row.
+    {
+        const uint32_t qlds = ring_base + (uint32_t)((NS - 1) * STAGE);
+#pragma unroll
+        for (int u = 0; u < QN; u++) {
+            const int row = QR * u + lane / QC;
+            const RowAt at = row_at(pl, pl.G, kvh, w.R0 + min(row, w.n_rows - 1));
+            lds_dma16((const T*)a.at.q + (int64_t)(s.row0 + at.tok) * a.at.q_stride + at.h * D + QE * ((lane % QC) ^ (row & 7)),
+                      __builtin_amdgcn_readfirstlane(qlds + u * 1024u));
+        }
+    }
+    issue(0, std::integral_constant<int, 0>{});
+    wait_vm<NL>();
+    // B operand Q^T: in step ks lane (lr, lq) holds dims 64 (ks / 2) + 16 lq + 8 (ks % 2) .. + 7 of row lr.
+    eight_t qf[KS][QP];
+    {
+        const T* const q = (const T*)(ring + (NS - 1) * STAGE) + lr * D;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int dim = 64 * (ks / 2) + 16 * lq + 8 * (ks % 2) + e;
+                const T x = q[QE * ((dim / QE) ^ (lr & 7)) + dim % QE];
+                if constexpr (QP == 1) qf[ks][0][e] = x;
+                else split_into<QP, B>(qf[ks], e, (float)x);
+            }
+    }
+    wait_lds_reads();
+
+    auto step = [&](int bi, auto stage_c) {
+        constexpr int stage = decltype(stage_c)::value;
+        if (bi + NS - 1 < nblk) {
+            wait_lds_reads();                                 // the last reads of that stage
+            issue(bi + NS - 1, std::integral_constant<int, (stage + NS - 1) % NS>{});
+        }
+        wait_ahead<NL, NS - 1>(min(NS - 1, nblk - 1 - bi));
+        uint64_t mk = 0;
+        uint32_t all = 0xffff;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            all &= info[stage][g];
+            mk |= (uint64_t)(info[stage][g] & 0xffff) << (16 * g);
+        }
+        const bool full = (all & 0xffff) == 0xffff;
+        uint8_t* const st = ring + stage * STAGE;
+        if (!full) {
+            // V where nothing counts: 0, as p = 0 times whatever it holds need not be.
+#pragma unroll
+            for (int u = 0; u < NG * NI; u++) {
+                const int row = R::RPI * u + drow;
+                if (!((mk >> row) & 1)) *(uint4*)(st + TILE + row * D + 16 * dch) = uint4{};
+            }
+            wait_lds_reads();
+        }
+        const int k0 = key0 + bi * BK;
+        // S^T: sc[t][i] = score(key k0 + 16 t + 4 lq + i, row lr).
+        f4_t sc[NG];
+#pragma unroll
+        for (int t = 0; t < NG; t++) {
+            sc[t] = f4_t{0.f, 0.f, 0.f, 0.f};
+            const float power = k_power(info[stage][t]);
+#pragma unroll
+            for (int f = 0; f < R::KF; f++) {
+                const uint4 x = *(const uint4*)(st + 16 * t * D + k_rd[f]);
+                const eight_t k0f = C::of(x.x, power, x.y, power), k1f = C::of(x.z, power, x.w, power);
+#pragma unroll
+                for (int i = QP - 1; i >= 0; i--) {           // small parts first
+                    sc[t] = C::mfma(k0f, qf[2 * f][i], sc[t]);
+                    sc[t] = C::mfma(k1f, qf[2 * f + 1][i], sc[t]);
+                }
+            }
+        }
+        if (!full || k0 + BK > seen_all) hide(sc, mk, seen - k0, lane);
+        float mloc = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+#pragma unroll
+        for (int t = 1; t < NG; t++) mloc = fmaxf(mloc, fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3])));
+        mloc = low_max<T>(max_xor32(max_xor16(mloc)), c);     // -inf if the row sees nothing here
+        float alpha;
+        if (move_max<T>(mloc, m_run, alpha)) {
+            l.scale(alpha);
+#pragma unroll
+            for (int u = 0; u < UT; u++) acc[u] *= alpha;
+        }
+        const float m_use = m_run == -INFINITY ? 0.0f : m_run;
+        // O^T += V^T P^T, the lane's own scores being its B operand: in 32-key step j, k-slot e of lane
+        // group lq is key 32 j + 16 (e / 4) + 4 lq + e % 4.  The weights in parts, so that their rounding
+        // leaves the result: this wave waits on memory, not on products.
+        float l_blk = 0.0f;
+        eight_t pf[NG / 2][PP];
+#pragma unroll
+        for (int t = 0; t < NG; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], c, -m_use));
+                l_blk += p;
+                split_into<PP, B>(pf[t / 2], 4 * (t & 1) + i, p);
+            }
+        l.add(l_blk);
+#pragma unroll
+        for (int j = 0; j < NG / 2; j++) {
+            const float p0 = v_power(info[stage][2 * j]), p1 = v_power(info[stage][2 * j + 1]);
+#pragma unroll
+            for (int u = 0; u < UT; u++) {
+                const lds_i2_t x = ds_read_tr8(st + TILE + 32 * j * D + v_rd[u]);
+                const eight_t vf = C::of((uint32_t)x[0], p0, (uint32_t)x[1], p1);
+#pragma unroll
+                for (int i = PP - 1; i >= 0; i--) acc[u] = C::mfma(vf, pf[j][i], acc[u]);
+            }
+        }
+    };
+    for_each_stage<NS>(nblk, step);
+    l_run = l.sum();
+}
+
+// A wave per unit, the units of neighbouring KV heads in one workgroup: they read the same
+// cache rows at about the same time.
+template <int D> struct Heads8 {
+    static constexpr int WAVES = 4;
+    static constexpr int PER_CU = 160 * 1024 / (WAVES * Narrow8<D>::RING) < 4 ? 160 * 1024 / (WAVES * Narrow8<D>::RING) : 4;
+};
+template <typename T, int D>
+__global__ __launch_bounds__(256, (Heads8<D>::PER_CU))
+void paged_heads8(cf_paged_q8_args_t a, PagedPlan pl, Q8Divs dv) {
+    using H = Heads8<D>;
+    constexpr int BK = Narrow8<D>::BK, RING = Narrow8<D>::RING;
+    __shared__ __attribute__((aligned(16))) uint8_t ring_all[H::WAVES * RING];
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const Geometry<16, BK, 1> geo(a.at, pl);
+    if (geo.lists_cut_tiles()) return;
+    for (int unit = (int)blockIdx.x * H::WAVES + wave;; unit += pl.step) {
+        const int id = fastdiv(unit, pl.by_kv), kvh = unit - id * a.at.H_kv;
+        Unit un;
+        if (!geo.find(id, un)) break;
+        const Work w = unit_work<16, BK>(a.at, pl, un);
+        const int lane = unit_lane(), lr = lane & 15, lq = lane >> 4;
+        f4_t acc[D / 16];
+        float m, l;
+        narrow_range8<T, D>(a, pl, dv, ring_all + wave * RING, un.s, un.b, kvh, w, w.key0, w.key1, acc, m, l);
+        l = add_xor32(add_xor16(l));
+        const uint32_t again = rows_of_16(lr < w.n_rows && spoilt(acc, l));
+        if (lr < w.n_rows) {
+            const RowOut out = row_out<T, D, 16>(a.at, pl, un, kvh, w, lr, m, l, lq == 0);
+#pragma unroll
+            for (int u = 0; u < D / 16; u++) put4<T>(out, 16 * u + 4 * lq, acc[u]);
+        }
+        if (again) mend_rows8<T, D, 16>(a, pl, dv, un, kvh, w, 0, again);
+    }
+}
+
+// Up to 16 rows by all waves of a workgroup: each takes a share of the unit's positions, and they
+// join their m, l and sums in LDS (WAVES rings at `lds`, one each).  True where rows that this wave
+// stored are spoilt.
+template <typename T, int D, int TM, int WAVES>
+__device__ __forceinline__ bool narrow_unit8(const cf_paged_q8_args_t& a, const PagedPlan& pl, const Q8Divs& dv, uint8_t* lds,
+                                             const Unit& un, int kvh, const Work& w) {
+    constexpr int RING = Narrow8<D>::RING, BK = Narrow8<D>::BK, LD = D + 4;
+    static_assert(16 * (LD + 2) * 4 <= RING, "a wave's rows fit its ring");
+    const int lane = unit_lane(), lr = lane & 15, lq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    uint8_t* const ring = lds + wave * RING;
+    const int blocks = w.key1 > w.key0 ? (w.key1 - w.key0 + BK - 1) / BK : 0;
+    const int per = (blocks + WAVES - 1) / WAVES * BK;
+    const int k0 = min(w.key0 + wave * per, w.key1), k1 = min(k0 + per, w.key1);
+    f4_t acc[D / 16];
+    float m, l;
+    narrow_range8<T, D>(a, pl, dv, ring, un.s, un.b, kvh, w, k0, k1, acc, m, l);
+    l = add_xor32(add_xor16(l));
+    float* const mine = (float*)ring;                         // [16][LD], m [16], l [16]
+    wait_lds_reads();
+#pragma unroll
+    for (int u = 0; u < D / 16; u++) *(f4_t*)(mine + lr * LD + 16 * u + 4 * lq) = acc[u];
+    if (lq == 0) {
+        mine[16 * LD + lr] = m;
+        mine[16 * LD + 16 + lr] = l;
+    }
+    __syncthreads();
+    bool again = false;
+    for (int i = threadIdx.x; i < w.n_rows * (D / 4); i += 64 * WAVES) {
+        const int row = i / (D / 4), d4 = i % (D / 4);
+        float M = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < WAVES; v++) M = fmaxf(M, ((const float*)(lds + v * RING))[16 * LD + row]);
+        const float m_use = M == -INFINITY ? 0.0f : M;
+        float L = 0.0f;
+        f4_t sum = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int v = 0; v < WAVES; v++) {
+            const float* const p = (const float*)(lds + v * RING);
+            const float x = __builtin_amdgcn_exp2f(p[16 * LD + row] - m_use);
+            L += p[16 * LD + 16 + row] * x;
+            sum += *(const f4_t*)(p + row * LD + 4 * d4) * x;
+        }
+        const f4_t one[1] = {sum};
+        again |= spoilt(one, L);
+        put4<T>(row_out<T, D, TM>(a.at, pl, un, kvh, w, row, M, L, d4 == 0), 4 * d4, sum);
+    }
+    __syncthreads();                                          // the rings, before the next unit
+    return __builtin_amdgcn_ballot_w64(again) != 0;
+}
+
+// The rows that the wave stored there.
+template <typename T, int D, int TM, int WAVES>
+__device__ __forceinline__ void mend_narrow8(const cf_paged_q8_args_t& a, const PagedPlan& pl, const Q8Divs& dv, const Unit& un,
+                                             int kvh, const Work& w) {
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    uint32_t rows = 0;
+    for (int r = 0; r < w.n_rows; r++)
+        if (r / (256 / D) % WAVES == wave) rows |= 1u << r;
+    mend_rows8<T, D, TM>(a, pl, dv, un, kvh, w, 0, rows);
+}
+
+constexpr int kSplitWaves = 8;
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kSplitWaves, 2)
+void paged_split8(cf_paged_q8_args_t a, PagedPlan pl, Q8Divs dv) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kSplitWaves * Narrow8<D>::RING];
+    const Geometry<16, 64, 1, false> geo(a.at, pl);
+    for (int unit = (int)blockIdx.x;; unit += pl.step) {
+        const int id = fastdiv(unit, pl.by_kv), kvh = unit - id * a.at.H_kv;
+        Unit un;
+        if (!geo.find(id, un)) break;
+        const Work w = unit_work<16, 64>(a.at, pl, un);
+        if (narrow_unit8<T, D, 16, kSplitWaves>(a, pl, dv, lds, un, kvh, w)) mend_narrow8<T, D, 16, kSplitWaves>(a, pl, dv, un, kvh, w);
+    }
+}
+
 // ---- Every shape: a wave per row and head. ----
 constexpr int kAnyDims = 512 / 64;             // dims per lane
 template <typename T>
@@ -114,9 +562,96 @@ void paged_any_q8(cf_paged_q8_args_t a, Q8Divs dv) {
     }
 }
 
+// The plan of a call on the matrix cores: the kernel and how its work is cut.
+enum Form8 { kHeads8, kSplit8 };
+struct Plan8 {
+    PagedPlan pl;
+    Form8 form;
+    int  wgs, merge_wgs;
+    size_t bytes;         // workspace
+};
+
+constexpr int64_t kSplitLen8 = 1024;
+
+bool fast_ok8(const cf_paged_q8_args_t& q) {
+    const cf_paged_attn_args_t& a = q.at;
+    const uint64_t ptrs = (uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.k | (uint64_t)(uintptr_t)a.v | (uint64_t)(uintptr_t)a.o;
+    const uint64_t steps = (uint64_t)a.page_stride | (uint64_t)a.row_stride | (uint64_t)a.head_stride;
+    const uint64_t es = a.elem == CF_ELEM_F16 ? 2 : 4;
+    // Row numbers times the group and positions (with what is read ahead) stay in 31 bits, offsets
+    // inside a group of rows in 32.
+    return (a.d == 64 || a.d == 128) && q.block % 16 == 0 && ptrs % 16 == 0 && steps % 16 == 0 && a.q_stride * es % 16 == 0 &&
+           a.scale > 0.0f && a.B <= kMostSeqs && (int64_t)a.T * (a.H_q / a.H_kv) <= (1 << 30) &&
+           (int64_t)a.max_pages * a.page_size <= (1 << 30) && (uint64_t)a.row_stride * 16 < (1ull << 32);
+}
+
+// max_new and max_len only choose: the kernels' loops run until no unit is left, whatever the
+// grid, and a sequence that is longer is computed all the same.
+Plan8 make_plan8(const cf_paged_attn_args_t& a) {
+    Plan8 p;
+    const int64_t G = a.H_q / a.H_kv, cus = cu_count();
+    const int64_t rows = (int64_t)a.max_new * G;              // of a sequence, at most
+    const int64_t seqs = a.B < a.T ? a.B : a.T;
+    auto tiles_of = [&](int64_t TM) {                         // tiles of the call, at most
+        const int64_t t = ((int64_t)a.T * G + seqs * (TM - 1)) / TM;
+        return rows <= TM && t > seqs ? seqs : t;
+    };
+    const int64_t units16 = tiles_of(16) * a.H_kv;
+    p.form = units16 <= cus && a.max_len <= kSplitLen8 ? kSplit8 : kHeads8;
+    const int64_t TM = 16, BK = p.form == kHeads8 ? Narrow8<64>::BK : 64;
+    const int64_t tiles = tiles_of(TM);
+    // Units in flight, by the LDS a workgroup takes.
+    const int64_t per_cu = 4 * (a.d == 128 ? Heads8<128>::PER_CU : Heads8<64>::PER_CU);
+    const int64_t fill = cus * per_cu > a.H_kv ? cus * per_cu / a.H_kv : 1;
+    p.pl.fill = (int32_t)fill;
+    p.pl.min_blocks = (int32_t)(64 / BK);
+    p.pl.one_blocks = (int32_t)(128 / BK);
+    p.pl.max_records = (int32_t)(4 * fill + 8);
+    const bool cut = !a.uncut && p.form != kSplit8 && (a.max_len + BK - 1) / BK > p.pl.one_blocks;
+    if (!cut) p.pl.one_blocks = INT32_MAX;                    // nor is what is longer than max_len
+    p.bytes = cut ? header_bytes(p.pl.max_records) + (size_t)p.pl.max_records * a.H_kv * (TM * (a.d + 2)) * sizeof(float) : 0;
+    int64_t units = (tiles + (cut ? 2 * fill : 0)) * a.H_kv;
+    if (units > (1 << 22)) units = 1 << 22;
+    p.wgs = (int)(p.form == kHeads8 ? (units + 3) / 4 : units);
+    p.pl.step = p.form == kHeads8 ? 4 * p.wgs : p.wgs;
+    p.pl.unit_wgs = p.wgs;
+    if (cut) p.wgs++;                                         // lists the cut tiles
+    const int64_t most_rows = rows < TM ? rows : TM;
+    const int64_t merge_rows = p.form == kHeads8 ? 1 : 1024 / a.d;   // of a workgroup
+    p.pl.merge_groups = (int32_t)((most_rows + merge_rows - 1) / merge_rows);
+    const int64_t merge_wgs = (tiles < 2 * fill ? tiles : 2 * fill) * a.H_kv * p.pl.merge_groups;
+    p.merge_wgs = !cut ? 0 : merge_wgs > 4096 ? 4096 : (int)merge_wgs;
+    p.pl.by_page = fastdiv_make(a.page_size);
+    p.pl.G = (int32_t)G;
+    p.pl.by_group = fastdiv_make((int)G);
+    p.pl.by_kv = fastdiv_make(a.H_kv);
+    p.pl.by_groups = fastdiv_make(p.pl.merge_groups);
+    p.pl.cut_count = nullptr;
+    p.pl.cut_tiles = nullptr;
+    p.pl.records = nullptr;
+    return p;
+}
+
+template <typename T, int D>
+int launch_tiles8(const cf_paged_q8_args_t& a, const Plan8& p, const Q8Divs& dv, hipStream_t st) {
+    const dim3 grid((unsigned)p.wgs), mgrid((unsigned)p.merge_wgs);
+    auto go = [&](auto tiles, int threads, auto merge) {
+        hipLaunchKernelGGL(tiles, grid, dim3(threads), 0, st, a, p.pl, dv);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess || p.merge_wgs == 0) return (int)e;
+        hipLaunchKernelGGL(merge, mgrid, dim3(256), 0, st, a.at, p.pl);
+        return (int)hipGetLastError();
+    };
+    if (p.form == kSplit8) {                                  // nothing is cut
+        hipLaunchKernelGGL((paged_split8<T, D>), grid, dim3(64 * kSplitWaves), 0, st, a, p.pl, dv);
+        return (int)hipGetLastError();
+    }
+    return go(paged_heads8<T, D>, 256, paged_merge<T, D, 16, 1>);
+}
+
 }  // namespace
 
-extern "C" size_t cf_paged_attn_q8_bytes(const cf_paged_q8_args_t*) { return 0; }
+extern "C" size_t cf_paged_attn_q8_bytes(const cf_paged_q8_args_t* a) { return fast_ok8(*a) ? make_plan8(a->at).bytes : 0; }
 
 extern "C" int cf_launch_paged_attn_q8(const cf_paged_q8_args_t* a, void* stream) {
     hipStream_t st = (hipStream_t)stream;
@@ -125,6 +660,18 @@ extern "C" int cf_launch_paged_attn_q8(const cf_paged_q8_args_t* a, void* stream
         t.page_size % a->block != 0)
         return (int)hipErrorInvalidValue;
     const Q8Divs dv = {fastdiv_make(t.page_size), fastdiv_make(a->block)};
+    if (fast_ok8(*a)) {
+        Plan8 p = make_plan8(t);
+        if (p.bytes > 0 && !t.workspace) return (int)hipErrorInvalidValue;
+        if (p.bytes > 0) {
+            p.pl.cut_count = (int*)t.workspace;
+            p.pl.cut_tiles = (CutTile*)((char*)t.workspace + 256);
+            p.pl.records = (float*)((char*)t.workspace + header_bytes(p.pl.max_records));
+        }
+        if (t.elem == CF_ELEM_F16)
+            return t.d == 64 ? launch_tiles8<_Float16, 64>(*a, p, dv, st) : launch_tiles8<_Float16, 128>(*a, p, dv, st);
+        return t.d == 64 ? launch_tiles8<float, 64>(*a, p, dv, st) : launch_tiles8<float, 128>(*a, p, dv, st);
+    }
     int64_t wgs = ((int64_t)t.T * t.H_q + 3) / 4;
     if (wgs > (1 << 22)) wgs = 1 << 22;        // a grid has less than 2^32 threads
     if (t.elem == CF_ELEM_F16) hipLaunchKernelGGL(paged_any_q8<_Float16>, dim3((unsigned)wgs), dim3(256), 0, st, *a, dv);
