@@ -544,6 +544,350 @@ void paged_split8(cf_paged_q8_args_t a, PagedPlan pl, Q8Divs dv) {
     }
 }
 
+// ---- Wide tiles: 8 waves of 16 NJ rows through one ring of 64-position blocks. ----
+// A wave loads its eighth of a block's codes into registers a turn ahead, and puts them into the ring
+// as 16-bit numbers: each code is converted once for the tile, and what the products read is as in
+// attention over a 16-bit cache.  The two waves of a SIMD, w and w + 4, take turns: with phases cut by
+// barriers, waves 0 .. 3 run products while waves 4 .. 7 run softmax, then the other way round.
+// Products of turn i are S(i) = K_i Q^T and O += V_{i-1} P(i-1), so a stage of the ring is K_i with
+// V_{i-1}.  Turn i of waves 0 .. 3 takes phases 2 i (products) and 2 i + 1, of the others 2 i + 1 and
+// 2 i + 2.  Stage i, which turn i - 2 has left by the end of phase 2 i - 3, is written during the softmax
+// phases before it, 2 i - 1 of waves 0 .. 3 and 2 i - 2 of the others: two stages do.
+template <typename T, int D, int NJ> struct Wide8 {
+    static constexpr int TM = 128 * NJ, BK = 64, NS = 2;
+    static constexpr int TILE = BK * D, STAGE = 2 * TILE;    // 16-bit numbers
+    static constexpr int QB = TM * D * (int)sizeof(T);       // bytes of Q, behind the stages
+    static constexpr int LDS = NS * STAGE * 2 + QB > 8 * Narrow8<D>::RING ? NS * STAGE * 2 + QB : 8 * Narrow8<D>::RING;
+    static constexpr int MASKS = 4;                          // blocks whose masks are kept
+};
+
+// Returns the wave's rows that are spoilt, a bit each.
+template <typename T, int D, int NJ>
+__device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, const PagedPlan& pl, const Q8Divs& dv, uint8_t* lds,
+                                               uint64_t* masks, const Unit& un, int kvh, const Work& w) {
+    using R = Rows<_Float16, D>;
+    using W = Wide8<T, D, NJ>;
+    using B = typename Parts<T>::half_t;
+    using C = Codes<B>;
+    typedef typename C::eight_t eight_t;
+    constexpr bool F16 = sizeof(T) == 2;
+    constexpr int BK = W::BK, TILE = W::TILE, STAGE = W::STAGE, UT = R::UT, NF = R::NF;
+    constexpr int QP = Parts<T>::Q, PP = F16 ? 1 : Parts<T>::P;
+    constexpr int QC = D * (int)sizeof(T) / 16, QR = 64 / QC, QE = 16 / (int)sizeof(T);
+    constexpr int CB = D / 8;                                // codes of a lane
+    const int lane = unit_lane(), lr = lane & 15, lq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int G = pl.G;
+    const float c = a.at.scale * kLog2e;
+    const int wrow = 16 * NJ * wave;
+    const bool active = wrow < w.n_rows;
+    const int n = w.key1 > w.key0 ? (w.key1 - w.key0 + BK - 1) / BK : 0;
+    f4_t acc[NJ][UT], lsum[NJ];
+    LongSum l_run[F16 ? 1 : NJ];
+    float m_run[NJ];
+    int seen[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+        m_run[j] = -INFINITY;
+        lsum[j] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < UT; u++) acc[j][u] = f4_t{0.f, 0.f, 0.f, 0.f};
+        seen[j] = min(w.base + fastdiv(w.R0 + min(wrow + 16 * j + lr, w.n_rows - 1), pl.by_group), un.s.len);
+    }
+    const int seen_all = min(w.base + fastdiv(w.R0 + min(wrow, w.n_rows - 1), pl.by_group), un.s.len);
+
+    if (n > 0) {
+        // This wave's rows of a block: 8 half + 0 .. 7 of group `grp`, eight lanes a row.
+        const int grp = wave >> 1, row = 8 * (wave & 1) + (lane >> 3), col = lane & 7;
+        const uint32_t off = (uint32_t)row * (uint32_t)a.at.row_stride + CB * col;
+        const int to_k = (16 * grp + row) * D + 8 * ((CB / 8 * col) ^ kswz<_Float16, D>(row));
+        const int to_v = TILE + (16 * grp + row) * D + 8 * ((CB / 8 * col) ^ vswz<_Float16, D>(row));
+        int k_rd[NF], v_rd[UT];
+        R::k_offsets(k_rd, lane);
+        R::v_offsets(v_rd, lane);
+        _Float16* const ring = (_Float16*)lds;
+        uint8_t* const qlds = lds + W::NS * STAGE * 2;
+        const table_t table = table_of(a.at, un.b);
+        const uint8_t* const kp = (const uint8_t*)a.at.k + (int64_t)kvh * a.at.head_stride;
+        const uint8_t* const vp = (const uint8_t*)a.at.v + (int64_t)kvh * a.at.head_stride;
+        const int bpp = a.at.page_size / a.block;
+
+        // Stage i: codes and powers of block i's K and of block i - 1's V.  Blocks outside 0 .. n - 1 load
+        // the nearest one.  A wave looks up its own group's page only; which positions of it count goes
+        // to the others through LDS.
+        typedef uint32_t words_t __attribute__((ext_vector_type(CB / 4)));
+        words_t kcodes, vcodes;
+        int kpower, vpower, page;
+        uint32_t kmask = 0, vmask = 0;                       // positions that count of what is loaded
+        int64_t v_at = 0, v_power = 0;
+        auto key_of = [&](int i) { return w.key0 + min(i, n - 1) * BK + 16 * grp; };
+        auto fetch = [&](int i) { page = page_of(a.at, pl, table, key_of(i)); };
+        auto load = [&](int i) {
+            const int key = key_of(i);
+            const Group gr = group_of(a.at, pl, page, key, w.key1);
+            const int in = key - fastdiv(key, pl.by_page) * a.at.page_size;
+            const int64_t p = ((int64_t)(gr.mask ? page : 0) * bpp + fastdiv(in, dv.block)) * a.at.H_kv + kvh;
+            if (lane == 0) ((uint16_t*)masks)[4 * (i % W::MASKS) + grp] = (uint16_t)gr.mask;
+            if (i == 0) {
+                v_at = gr.at;
+                v_power = p;
+            }
+            kcodes = *(const words_t*)(kp + gr.at + off);
+            vcodes = *(const words_t*)(vp + v_at + off);
+            kpower = a.k_scales[p];
+            vpower = a.v_scales[v_power];
+            vmask = i == 0 ? gr.mask : kmask;
+            kmask = gr.mask;
+            v_at = gr.at;
+            v_power = p;
+        };
+        auto put = [&](int at, words_t x, int power) {
+            const float p = power_bits(power);
+            *(eight_t*)(ring + at) = C::of(x[0], p, x[1], p);
+            if constexpr (CB == 16) *(eight_t*)(ring + (at ^ 8)) = C::of(x[2], p, x[3], p);
+        };
+        // V where nothing counts: 0, as p = 0 times whatever it holds need not be.
+        auto write = [&](int i) {
+            int odd = i & 1;
+            asm volatile("" : "+s"(odd));
+            const int stage = odd * STAGE;
+            if (vmask != 0xffff) {
+                if (!((vmask >> row) & 1)) vcodes = words_t{};
+                if (vmask == 0) vpower = 127;
+            }
+            put(stage + to_k, kcodes, kpower);
+            put(stage + to_v, vcodes, vpower);
+        };
+
+        fetch(0);
+        {
+            const uint32_t to = __builtin_amdgcn_readfirstlane(lds_offset(qlds)) + (uint32_t)(wrow * D * (int)sizeof(T));
+#pragma unroll
+            for (int u = 0; u < 16 * NJ / QR; u++) {
+                const int r = QR * u + lane / QC;
+                const RowAt at = row_at(pl, G, kvh, w.R0 + min(wrow + r, w.n_rows - 1));
+                lds_dma16((const T*)a.at.q + (int64_t)(un.s.row0 + at.tok) * a.at.q_stride + at.h * D + QE * ((lane % QC) ^ (r & 7)),
+                          __builtin_amdgcn_readfirstlane(to + u * 1024u));
+            }
+        }
+        load(0);
+        fetch(1);
+        wait_vm<0>();
+        // B operand Q^T: lane (lr, lq) takes dims 32 f + 8 lq .. + 7 of row lr.
+        eight_t qf[NJ][NF][QP];
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            const T* const q = (const T*)qlds + (wrow + 16 * j + lr) * D;
+#pragma unroll
+            for (int f = 0; f < NF; f++) {
+                if constexpr (QP == 1) {
+                    qf[j][f][0] = *(const eight_t*)(q + 8 * ((4 * f + lq) ^ (lr & 7)));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        split_into<QP, B>(qf[j][f], e, q[4 * ((8 * f + 2 * lq + e / 4) ^ (lr & 7)) + e % 4]);
+                }
+            }
+        }
+        write(0);
+        load(1);                                              // n >= 1: stages 0 and 1 exist
+        fetch(2);
+        wait_lds_reads();
+
+        f4_t sc[NJ][4];
+        eight_t pf[NJ][2][PP];
+        h8_t ones = {1, 1, 1, 1, 1, 1, 1, 1};
+        if constexpr (F16) asm volatile("" : "+v"(ones));     // kept in registers for the whole loop
+        uint64_t mk = ~0ull;                                  // positions of this turn's block that count
+
+        // Fragment x of a turn: x < 2 UT is V^T (32-key step x / UT, dims 16 (x % UT)), the rest K
+        // (key tile, then chunk).  They are read kAhead fragments before their products, in
+        // exactly this order.
+        constexpr int kAhead = 6, kV = 2 * UT, kAll = kV + 4 * NF;
+        auto products = [&](int i, auto first_c, auto last_c) {   // fragments first .. last - 1
+            constexpr int first = decltype(first_c)::value, last = decltype(last_c)::value;
+            if constexpr (last == kAll) mk = masks[i % W::MASKS];
+            if (!active) return;
+            int odd = i & 1;
+            asm volatile("" : "+s"(odd));
+            const _Float16* const st = ring + odd * STAGE;
+            eight_t frag[kAhead];
+            auto read = [&](auto x_c) {
+                constexpr int x = decltype(x_c)::value;
+                if constexpr (x < kV) {
+                    const _Float16* const v = st + TILE + v_rd[x % UT] + 32 * (x / UT) * D;
+                    frag[x % kAhead] = __builtin_bit_cast(eight_t, cat8(ds_read_tr4(v), ds_read_tr4(v + 16 * D)));
+                } else if constexpr (x < kAll) {
+                    frag[x % kAhead] = *(const eight_t*)(st + 16 * ((x - kV) % 4) * D + k_rd[(x - kV) / 4]);
+                }
+            };
+            auto use = [&](auto x_c) {
+                constexpr int x = decltype(x_c)::value;
+                const eight_t f = frag[x % kAhead];
+                // O^T += V^T P^T: in 32-key step s2, k-slot e of lane group lq is key
+                // 32 s2 + 16 (e / 4) + 4 lq + e % 4, the lane's own scores.  fp16: p is rounded to fp16, the
+                // type of V and of the product, and l comes out of the matrix cores too, from the same
+                // rounded p that weights V.  FP32: p in three parts, small ones first.
+                if constexpr (x < kV) {
+                    if constexpr (F16 && x % UT == 0)
+#pragma unroll
+                        for (int j = 0; j < NJ; j++)
+                            lsum[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, __builtin_bit_cast(h8_t, pf[j][x / UT][0]), lsum[j], 0, 0, 0);
+#pragma unroll
+                    for (int q = PP - 1; q >= 0; q--)
+#pragma unroll
+                        for (int j = 0; j < NJ; j++) acc[j][x % UT] = C::mfma(f, pf[j][x / UT][q], acc[j][x % UT]);
+                } else {
+                    // S^T: sc[j][t][e] = score(key 16 t + 4 lq + e of block i, row j).
+                    constexpr int t = (x - kV) % 4, c0 = (x - kV) / 4;
+#pragma unroll
+                    for (int q = QP - 1; q >= 0; q--)
+#pragma unroll
+                        for (int j = 0; j < NJ; j++)
+                            sc[j][t] = C::mfma(f, qf[j][c0][q], c0 == 0 && q == QP - 1 ? f4_t{0.f, 0.f, 0.f, 0.f} : sc[j][t]);
+                }
+            };
+            __builtin_amdgcn_s_setprio(1);
+            static_for<kAhead - 1>([&](auto k) {
+                constexpr int x = first + decltype(k)::value;
+                if constexpr (x < last) read(std::integral_constant<int, x>{});
+            });
+            __builtin_amdgcn_sched_barrier(0);
+            static_for<last - first>([&](auto k) {
+                constexpr int x = first + decltype(k)::value;
+                if constexpr (x + kAhead - 1 < last) read(std::integral_constant<int, x + kAhead - 1>{});
+                use(std::integral_constant<int, x>{});
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            __builtin_amdgcn_s_setprio(0);
+        };
+        const std::integral_constant<int, 0> from_v;
+        const std::integral_constant<int, kV> to_v_end;
+        const std::integral_constant<int, kAll> to_k_end;
+        auto softmax = [&](int i) {
+            if (!active) return;
+            const int k0 = w.key0 + i * BK;
+            const bool edge = mk != ~0ull || k0 + BK > seen_all;
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                if (edge) hide(sc[j], mk, seen[j] - k0, lane);
+                // Chains of three-input maxima.
+                float mloc = fmaxf(fmaxf(sc[j][0][0], sc[j][0][1]), sc[j][0][2]);
+#pragma unroll
+                for (int e = 3; e < 15; e += 2)
+                    mloc = fmaxf(fmaxf(mloc, sc[j][e >> 2][e & 3]), sc[j][(e + 1) >> 2][(e + 1) & 3]);
+                mloc = fmaxf(mloc, sc[j][3][3]);
+                mloc = low_max<T>(max_xor32(max_xor16(mloc)), c);  // -inf if the row sees nothing here
+                float alpha;
+                if (move_max<T>(mloc, m_run[j], alpha)) {
+                    if constexpr (F16) lsum[j] *= alpha;
+                    else l_run[j].scale(alpha);
+#pragma unroll
+                    for (int u = 0; u < UT; u++) acc[j][u] *= alpha;
+                }
+                const float m_use = m_run[j] == -INFINITY ? 0.0f : m_run[j];
+                float l_blk = 0.0f;
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][t][e], c, -m_use));
+                        if constexpr (!F16) l_blk += p;
+                        split_into<PP, B>(pf[j][t >> 1], (t & 1) * 4 + e, p);
+                    }
+                if constexpr (!F16) l_run[j].add(l_blk);
+            }
+        };
+        auto uniform = [](uint64_t x) {
+            return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
+                   (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+        };
+        // Stage i into the ring, the codes of the next one on their way, the page of the one behind it.
+        auto refill = [&](int i) {
+            if (i > n) return;
+            write(i);
+            __builtin_amdgcn_sched_barrier(0);
+            if (i + 1 <= n) load(i + 1);
+            fetch(i + 2);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        // Everybody meets at every barrier, 2 n + 2 of them; each waits for its LDS accesses before.
+        ring_barrier();
+        auto half = [&](int i, int stage) {
+            mk = uniform(mk);
+            ring_barrier();
+            refill(stage);
+            softmax(i);
+            wait_lds_reads();
+            ring_barrier();
+        };
+        if (wave < 4) {
+            products(0, to_v_end, to_k_end);
+            half(0, 1);
+#pragma clang loop unroll(disable)
+            for (int i = 1; i < n; i++) {
+                products(i, from_v, to_k_end);
+                half(i, i + 1);
+            }
+            products(n, from_v, to_v_end);
+            ring_barrier();
+        } else {
+            refill(1);
+            wait_lds_reads();
+            ring_barrier();
+            products(0, to_v_end, to_k_end);
+            half(0, 2);
+#pragma clang loop unroll(disable)
+            for (int i = 1; i < n; i++) {
+                products(i, from_v, to_k_end);
+                half(i, i + 2);
+            }
+            products(n, from_v, to_v_end);
+        }
+    }
+    uint32_t again_all = 0;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+        const int row = wrow + 16 * j + lr;
+        const float l = F16 ? lsum[j][0] : add_xor32(add_xor16(l_run[F16 ? 0 : j].sum()));
+        const uint32_t again = rows_of_16(row < w.n_rows && spoilt(acc[j], l));
+        if (row < w.n_rows) {
+            const RowOut out = row_out<T, D, W::TM>(a.at, pl, un, kvh, w, row, m_run[j], l, lq == 0);
+#pragma unroll
+            for (int u = 0; u < UT; u++) put4<T>(out, 16 * u + 4 * lq, acc[j][u]);
+        }
+        again_all |= again << (16 * j);
+    }
+    ring_barrier();                                           // the ring's reads, before the next unit
+    return again_all;
+}
+
+constexpr int kNarrowCost8 = 4;              // blocks of tiles of up to 16 rows that cost a wide tile's one
+template <typename T, int D, int NJ>
+__global__ __launch_bounds__(512, 2)
+void paged_wide8(cf_paged_q8_args_t a, PagedPlan pl, Q8Divs dv) {
+    using W = Wide8<T, D, NJ>;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[W::LDS];
+    __shared__ uint64_t masks[W::MASKS];
+    __shared__ int kept[3 * 64];
+    const Geometry<W::TM, 64, kNarrowCost8> geo(a.at, pl, kept);
+    if (geo.lists_cut_tiles()) return;
+    for (int unit = (int)blockIdx.x;; unit += pl.step) {
+        const int id = fastdiv(unit, pl.by_kv), kvh = unit - id * a.at.H_kv;
+        Unit un;
+        if (!geo.find(id, un)) break;
+        Work w = unit_work<W::TM, 64>(a.at, pl, un);
+        const bool narrow = w.n_rows <= 16;
+        const uint32_t again = narrow ? narrow_unit8<T, D, W::TM, 8>(a, pl, dv, lds, un, kvh, w)
+                                      : wide8_unit<T, D, NJ>(a, pl, dv, lds, masks, un, kvh, w);
+        if (!again) continue;
+        if (!geo.find(id, un)) break;         // found anew: nothing is kept for this
+        w = unit_work<W::TM, 64>(a.at, pl, un);
+        if (narrow) mend_narrow8<T, D, W::TM, 8>(a, pl, dv, un, kvh, w);
+        else mend_rows8<T, D, W::TM>(a, pl, dv, un, kvh, w, 16 * NJ * __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), again);
+    }
+}
+
 // ---- Every shape: a wave per row and head. ----
 constexpr int kAnyDims = 512 / 64;             // dims per lane
 template <typename T>
@@ -563,7 +907,7 @@ void paged_any_q8(cf_paged_q8_args_t a, Q8Divs dv) {
 }
 
 // The plan of a call on the matrix cores: the kernel and how its work is cut.
-enum Form8 { kHeads8, kSplit8 };
+enum Form8 { kHeads8, kSplit8, kWide1x8, kWide2x8 };   // kWide2x8: tiles of 256 rows, fp16
 struct Plan8 {
     PagedPlan pl;
     Form8 form;
@@ -572,6 +916,7 @@ struct Plan8 {
 };
 
 constexpr int64_t kSplitLen8 = 1024;
+constexpr int64_t kLongLen8 = 2048;
 
 bool fast_ok8(const cf_paged_q8_args_t& q) {
     const cf_paged_attn_args_t& a = q.at;
@@ -596,18 +941,27 @@ Plan8 make_plan8(const cf_paged_attn_args_t& a) {
         const int64_t t = ((int64_t)a.T * G + seqs * (TM - 1)) / TM;
         return rows <= TM && t > seqs ? seqs : t;
     };
-    const int64_t units16 = tiles_of(16) * a.H_kv;
-    p.form = units16 <= cus && a.max_len <= kSplitLen8 ? kSplit8 : kHeads8;
-    const int64_t TM = 16, BK = p.form == kHeads8 ? Narrow8<64>::BK : 64;
+    const bool f16 = a.elem == CF_ELEM_F16;
+    if (rows <= 16) {
+        const int64_t units = tiles_of(16) * a.H_kv;
+        p.form = units <= cus && a.max_len <= kSplitLen8 ? kSplit8 : kHeads8;
+    } else {
+        const int64_t units = (int64_t)a.T * G / 256 * a.H_kv;
+        const bool few_long = a.max_len > kLongLen8 && 2 * (int64_t)a.max_new >= a.T && units >= cus / 8;
+        p.form = f16 && (4 * units >= 3 * cus || few_long) ? kWide2x8 : kWide1x8;
+    }
+    const bool wide = p.form >= kWide1x8;
+    const int64_t TM = !wide ? 16 : p.form == kWide2x8 ? 256 : 128;
+    const int64_t BK = p.form == kHeads8 ? Narrow8<64>::BK : 64;
     const int64_t tiles = tiles_of(TM);
     // Units in flight, by the LDS a workgroup takes.
-    const int64_t per_cu = 4 * (a.d == 128 ? Heads8<128>::PER_CU : Heads8<64>::PER_CU);
+    const int64_t per_cu = wide ? 1 : 4 * (a.d == 128 ? Heads8<128>::PER_CU : Heads8<64>::PER_CU);
     const int64_t fill = cus * per_cu > a.H_kv ? cus * per_cu / a.H_kv : 1;
     p.pl.fill = (int32_t)fill;
-    p.pl.min_blocks = (int32_t)(64 / BK);
-    p.pl.one_blocks = (int32_t)(128 / BK);
+    p.pl.min_blocks = (int32_t)(wide ? 12 : 64 / BK);
+    p.pl.one_blocks = (int32_t)((wide ? 1536 : 128) / BK);
     p.pl.max_records = (int32_t)(4 * fill + 8);
-    const bool cut = !a.uncut && p.form != kSplit8 && (a.max_len + BK - 1) / BK > p.pl.one_blocks;
+    const bool cut = !a.uncut && p.form != kSplit8 && (a.max_len + BK - 1) / BK > (wide ? kFewOne / BK : p.pl.one_blocks);
     if (!cut) p.pl.one_blocks = INT32_MAX;                    // nor is what is longer than max_len
     p.bytes = cut ? header_bytes(p.pl.max_records) + (size_t)p.pl.max_records * a.H_kv * (TM * (a.d + 2)) * sizeof(float) : 0;
     int64_t units = (tiles + (cut ? 2 * fill : 0)) * a.H_kv;
@@ -646,7 +1000,10 @@ int launch_tiles8(const cf_paged_q8_args_t& a, const Plan8& p, const Q8Divs& dv,
         hipLaunchKernelGGL((paged_split8<T, D>), grid, dim3(64 * kSplitWaves), 0, st, a, p.pl, dv);
         return (int)hipGetLastError();
     }
-    return go(paged_heads8<T, D>, 256, paged_merge<T, D, 16, 1>);
+    if (p.form == kHeads8) return go(paged_heads8<T, D>, 256, paged_merge<T, D, 16, 1>);
+    if constexpr (sizeof(T) == 2)
+        if (p.form == kWide2x8) return go(paged_wide8<T, D, 2>, 512, paged_merge<T, D, 256, 1024 / D>);
+    return go(paged_wide8<T, D, 1>, 512, paged_merge<T, D, 128, 1024 / D>);
 }
 
 }  // namespace
