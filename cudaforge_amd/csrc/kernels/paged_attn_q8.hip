@@ -29,7 +29,7 @@ template <typename T, int DIMS>
 __device__ __forceinline__ void plain_row_q8(const cf_paged_q8_args_t& a, const Q8Divs& dv, const SeqRows& s, int b, int tok,
                                              int h, int d, int key0 = 0, int key1 = INT32_MAX, float* rec = nullptr,
                                              int tm = 0, float* rec_sum = nullptr) {
-    const int lane = threadIdx.x & 63;
+    const int lane = unit_lane();
     const int seen = min(min(s.len - s.n + tok + 1, s.len), key1);
     const int kvh = h / (a.at.H_q / a.at.H_kv);
     const int32_t* const table = a.at.table + (size_t)b * a.at.max_pages;
@@ -158,9 +158,7 @@ template <int D> struct Rows8 {
 struct Groups8 {
     const int32_t* table;
     int lo, hi, info;        // lane: base + lane; info: positions, power of K << 16, of V << 24
-    __device__ __forceinline__ void load(const cf_paged_q8_args_t& a, const PagedPlan& pl, const Q8Divs& dv, int kvh, int base,
-                                         int key0, int key1) {
-        const int key = key0 + (base + (int)(threadIdx.x & 63)) * 16;
+    __device__ __forceinline__ void find(const cf_paged_q8_args_t& a, const PagedPlan& pl, const Q8Divs& dv, int kvh, int key, int key1) {
         const int page = table[fastdiv(min(key, a.at.max_pages * a.at.page_size - 1), pl.by_page)];
         const Group g = group_of(a.at, pl, page, key, key1);
         const int in = key - fastdiv(key, pl.by_page) * a.at.page_size;
@@ -169,6 +167,10 @@ struct Groups8 {
         lo = (int)g.at;
         hi = (int)(g.at >> 32);
         info = (int)(g.mask ? g.mask | kp << 16 | vp << 24 : 0x7f7f0000u);
+    }
+    __device__ __forceinline__ void load(const cf_paged_q8_args_t& a, const PagedPlan& pl, const Q8Divs& dv, int kvh, int base,
+                                         int key0, int key1) {
+        find(a, pl, dv, kvh, key0 + (base + unit_lane()) * 16, key1);
         asm volatile("" : "+v"(lo), "+v"(hi), "+v"(info));    // they have arrived
     }
     __device__ __forceinline__ int64_t at(int i) const {
@@ -180,35 +182,48 @@ struct Groups8 {
 __device__ __forceinline__ float k_power(uint32_t info) { return __uint_as_float((info << 7) & 0x7f800000u); }
 __device__ __forceinline__ float v_power(uint32_t info) { return __uint_as_float((info >> 1) & 0x7f800000u); }
 
-// Which of some V are NaN: a bit for each element of the lane's 16-byte chunk.
+// 16 zeros, made where they are used: kept in registers for a whole kernel, wide tiles had no room.
+__device__ __forceinline__ uint4 zeros() {
+    uint32_t z = 0;
+    asm volatile("" : "+v"(z));
+    return uint4{z, z, z, z};
+}
+
+// Which of some V are NaN: bit 7 of the byte of each element of the lane's 16-byte chunk.
+struct Nans {
+    uint32_t w[4] = {0, 0, 0, 0};
+    __device__ __forceinline__ bool any_but(const Nans& x) const {
+        return ((w[0] & ~x.w[0]) | (w[1] & ~x.w[1]) | (w[2] & ~x.w[2]) | (w[3] & ~x.w[3])) != 0;
+    }
+};
 template <int D>
-__device__ __forceinline__ uint32_t find_nan(const cf_paged_q8_args_t& a, const Q8Divs& dv, int b, int kvh, int from, int to) {
+__device__ __forceinline__ void find_nan(const cf_paged_q8_args_t& a, const Q8Divs& dv, int b, int kvh, int from, int to, Nans& found) {
     using R = Rows8<D>;
-    const int lane = threadIdx.x & 63, sub = R::drow(lane);
+    const int lane = unit_lane(), sub = R::drow(lane);
     const int32_t* const table = a.at.table + (size_t)b * a.at.max_pages;
     const uint8_t* const v = (const uint8_t*)a.at.v + (int64_t)kvh * a.at.head_stride + 16 * R::dch(lane);
-    uint32_t found = 0;
+    Nans mine;
 #pragma clang loop unroll(disable)
     for (int p0 = from; p0 < to; p0 += 64) {
         const int key = min(p0 + lane, to - 1);
         const Cell cell = cell_of(a, dv, table, key);
-        const bool all = cell.at >= 0 && a.v_scales[cell.power + kvh] == 255;
+        const int all = cell.at >= 0 && a.v_scales[cell.power + kvh] == 255 ? 0x7f7f7f7f : 0;
 #pragma clang loop unroll(disable)
         for (int r = sub; r < 64; r += R::RPI) {
             const int64_t row = (int64_t)((uint64_t)(uint32_t)__shfl((int)(cell.at >> 32), r) << 32 | (uint32_t)__shfl((int)cell.at, r));
-            const bool whole = __shfl((int)all, r);
-            if (row < 0) continue;
-            const uint4 x = *(const uint4*)(v + row);
+            const uint32_t whole = (uint32_t)__shfl(all, r);
+            const uint4 x = row < 0 ? uint4{} : *(const uint4*)(v + row);
             const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) found |= (whole || ((w[i] >> (8 * e)) & 0x7f) == 0x7f) ? 1u << (4 * i + e) : 0u;
+            for (int i = 0; i < 4; i++) mine.w[i] |= (((w[i] | whole) & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
         }
     }
 #pragma unroll
-    for (int step = R::CPR; step < 64; step *= 2) found |= __shfl_xor(found, step);
-    return found;
+    for (int i = 0; i < 4; i++) {
+#pragma unroll
+        for (int step = R::CPR; step < 64; step *= 2) mine.w[i] |= __shfl_xor(mine.w[i], step);
+        found.w[i] |= mine.w[i];
+    }
 }
 
 // Rows row0 + bit of a unit (a bit of `rows` each), computed and stored by this wave, where a sum is NaN
@@ -218,20 +233,21 @@ template <typename T, int D, int TM>
 __device__ __forceinline__ void mend_rows8(const cf_paged_q8_args_t& a, const PagedPlan& pl, const Q8Divs& dv, const Unit& un,
                                            int kvh, const Work& w, int row0, uint32_t rows) {
     using R = Rows8<D>;
-    const int lane = threadIdx.x & 63;
+    const int lane = unit_lane();
     wait_vm<0>();                                             // what it stored is stored
-    uint32_t seen = 0;
+    Nans seen;
     int upto = w.key0;
     for (; rows; rows &= rows - 1) {
         const int row = row0 + __builtin_ctz(rows);
         const RowAt at = row_at(pl, pl.G, kvh, w.R0 + row);
         const int sees = max(min(min(w.base + at.tok, un.s.len), w.key1), upto);     // rises with the rows
-        seen |= find_nan<D>(a, dv, un.b, kvh, upto, sees);
+        find_nan<D>(a, dv, un.b, kvh, upto, sees, seen);
         upto = sees;
-        const uint32_t hidden = find_nan<D>(a, dv, un.b, kvh, sees, w.key1);
+        Nans hidden;
+        find_nan<D>(a, dv, un.b, kvh, sees, w.key1, hidden);
         float* const rec = un.n_ranges > 1 ? record_of<TM, D>(a.at, pl, un, kvh) : nullptr;
         T* const o = (T*)a.at.o + ((int64_t)(un.s.row0 + at.tok) * a.at.H_q + at.h) * D;
-        if (__builtin_amdgcn_ballot_w64((hidden & ~seen) != 0) || !__builtin_amdgcn_ballot_w64(seen != 0)) {
+        if (__builtin_amdgcn_ballot_w64(hidden.any_but(seen)) || !__builtin_amdgcn_ballot_w64(seen.any_but(Nans{}))) {
             plain_row_q8<T, D / 64>(a, dv, un.s, un.b, at.tok, at.h, D, w.key0, w.key1, rec ? rec + row : nullptr, TM,
                                     rec + 2 * TM + row * D);
             continue;
@@ -239,7 +255,7 @@ __device__ __forceinline__ void mend_rows8(const cf_paged_q8_args_t& a, const Pa
         if (lane >= R::CPR) continue;
 #pragma unroll
         for (int e = 0; e < 16; e++) {
-            if (!((seen >> e) & 1)) continue;
+            if (!((seen.w[e / 4] >> (8 * (e % 4) + 7)) & 1)) continue;
             if (rec) rec[2 * TM + row * D + 16 * lane + e] = NAN;
             else o[16 * lane + e] = (T)NAN;
         }
@@ -368,7 +384,7 @@ __device__ __forceinline__ void narrow_range8(const cf_paged_q8_args_t& a, const
 #pragma unroll
             for (int u = 0; u < NG * NI; u++) {
                 const int row = R::RPI * u + drow;
-                if (!((mk >> row) & 1)) *(uint4*)(st + TILE + row * D + 16 * dch) = uint4{};
+                if (!((mk >> row) & 1)) *(uint4*)(st + TILE + row * D + 16 * dch) = zeros();
             }
             wait_lds_reads();
         }
@@ -495,7 +511,7 @@ __device__ __forceinline__ bool narrow_unit8(const cf_paged_q8_args_t& a, const 
     }
     __syncthreads();
     bool again = false;
-    for (int i = threadIdx.x; i < w.n_rows * (D / 4); i += 64 * WAVES) {
+    for (int i = 64 * wave + lane; i < w.n_rows * (D / 4); i += 64 * WAVES) {
         const int row = i / (D / 4), d4 = i % (D / 4);
         float M = -INFINITY;
 #pragma unroll
@@ -558,13 +574,20 @@ template <typename T, int D, int NJ> struct Wide8 {
     static constexpr int TILE = BK * D, STAGE = 2 * TILE;    // 16-bit numbers
     static constexpr int QB = TM * D * (int)sizeof(T);       // bytes of Q, behind the stages
     static constexpr int LDS = NS * STAGE * 2 + QB > 8 * Narrow8<D>::RING ? NS * STAGE * 2 + QB : 8 * Narrow8<D>::RING;
-    static constexpr int MASKS = 4;                          // blocks whose masks are kept
 };
+
+// An address in scalar registers, which stays there: what a lane adds to it is 32 bits wide.
+__device__ __forceinline__ const CF_GLOBAL uint8_t* uniform_at(const uint8_t* p) {
+    const uint64_t x = (uint64_t)(uintptr_t)p;
+    uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)x), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32));
+    asm volatile("" : "+s"(lo), "+s"(hi));
+    return (const CF_GLOBAL uint8_t*)(uintptr_t)((uint64_t)hi << 32 | lo);
+}
 
 // Returns the wave's rows that are spoilt, a bit each.
 template <typename T, int D, int NJ>
 __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, const PagedPlan& pl, const Q8Divs& dv, uint8_t* lds,
-                                               uint64_t* masks, const Unit& un, int kvh, const Work& w) {
+                                               const Unit& un, int kvh, const Work& w) {
     using R = Rows<_Float16, D>;
     using W = Wide8<T, D, NJ>;
     using B = typename Parts<T>::half_t;
@@ -607,59 +630,57 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
         R::v_offsets(v_rd, lane);
         _Float16* const ring = (_Float16*)lds;
         uint8_t* const qlds = lds + W::NS * STAGE * 2;
-        const table_t table = table_of(a.at, un.b);
         const uint8_t* const kp = (const uint8_t*)a.at.k + (int64_t)kvh * a.at.head_stride;
         const uint8_t* const vp = (const uint8_t*)a.at.v + (int64_t)kvh * a.at.head_stride;
-        const int bpp = a.at.page_size / a.block;
 
-        // Stage i: codes and powers of block i's K and of block i - 1's V.  Blocks outside 0 .. n - 1 load
-        // the nearest one.  A wave looks up its own group's page only; which positions of it count goes
-        // to the others through LDS.
+        // The next 64 blocks, one per lane: this wave's group of each, and which of them count as a whole.
+        Groups8 groups = {a.at.table + (size_t)un.b * a.at.max_pages, 0, 0, 0};
+        uint64_t whole = 0;
+        auto key_of = [&](int i, int g) { return w.key0 + i * BK + 16 * g; };
+        auto mask_of = [&](int i, int g) {                   // positions that count of group g of block i
+            const int key = key_of(i, g);
+            const int page = groups.table[fastdiv(min(key, a.at.max_pages * a.at.page_size - 1), pl.by_page)];
+            return group_of(a.at, pl, page, key, w.key1).mask;
+        };
+        auto look = [&](int i) {
+            groups.find(a, pl, dv, kvh, key_of(i + lane, grp), w.key1);
+            uint32_t m = 0xffff;
+#pragma unroll
+            for (int g = 0; g < 4; g++) m &= mask_of(i + lane, g);
+            asm volatile("" : "+v"(groups.lo), "+v"(groups.hi), "+v"(groups.info));
+            whole = __builtin_amdgcn_ballot_w64(m == 0xffff);
+        };
+        // Stage i: codes and powers of block i's K and of block i - 1's V.  (Block n stands in where there is
+        // none: page 0, and nothing of it counts.)
         typedef uint32_t words_t __attribute__((ext_vector_type(CB / 4)));
         words_t kcodes, vcodes;
-        int kpower, vpower, page;
-        uint32_t kmask = 0, vmask = 0;                       // positions that count of what is loaded
-        int64_t v_at = 0, v_power = 0;
-        auto key_of = [&](int i) { return w.key0 + min(i, n - 1) * BK + 16 * grp; };
-        auto fetch = [&](int i) { page = page_of(a.at, pl, table, key_of(i)); };
+        uint32_t kinfo = 0, vinfo = 0, wholes = 0;           // wholes: a bit for each of the last blocks
+        int64_t v_at = 0;
         auto load = [&](int i) {
-            const int key = key_of(i);
-            const Group gr = group_of(a.at, pl, page, key, w.key1);
-            const int in = key - fastdiv(key, pl.by_page) * a.at.page_size;
-            const int64_t p = ((int64_t)(gr.mask ? page : 0) * bpp + fastdiv(in, dv.block)) * a.at.H_kv + kvh;
-            if (lane == 0) ((uint16_t*)masks)[4 * (i % W::MASKS) + grp] = (uint16_t)gr.mask;
-            if (i == 0) {
-                v_at = gr.at;
-                v_power = p;
-            }
-            kcodes = *(const words_t*)(kp + gr.at + off);
-            vcodes = *(const words_t*)(vp + v_at + off);
-            kpower = a.k_scales[p];
-            vpower = a.v_scales[v_power];
-            vmask = i == 0 ? gr.mask : kmask;
-            kmask = gr.mask;
-            v_at = gr.at;
-            v_power = p;
+            if (i % 64 == 0) look(i);
+            const int64_t at = groups.at(i);
+            if (i == 0) v_at = at;
+            kcodes = *(const CF_GLOBAL words_t*)(uniform_at(kp + at) + off);
+            vcodes = *(const CF_GLOBAL words_t*)(uniform_at(vp + v_at) + off);
+            vinfo = kinfo;
+            kinfo = groups.what(i);
+            v_at = at;
+            wholes = wholes << 1 | (uint32_t)((whole >> (i & 63)) & 1);
         };
-        auto put = [&](int at, words_t x, int power) {
-            const float p = power_bits(power);
-            *(eight_t*)(ring + at) = C::of(x[0], p, x[1], p);
-            if constexpr (CB == 16) *(eight_t*)(ring + (at ^ 8)) = C::of(x[2], p, x[3], p);
+        auto put = [&](int at, words_t x, float power) {
+            *(eight_t*)(ring + at) = C::of(x[0], power, x[1], power);
+            if constexpr (CB == 16) *(eight_t*)(ring + (at ^ 8)) = C::of(x[2], power, x[3], power);
         };
         // V where nothing counts: 0, as p = 0 times whatever it holds need not be.
         auto write = [&](int i) {
             int odd = i & 1;
             asm volatile("" : "+s"(odd));
             const int stage = odd * STAGE;
-            if (vmask != 0xffff) {
-                if (!((vmask >> row) & 1)) vcodes = words_t{};
-                if (vmask == 0) vpower = 127;
-            }
-            put(stage + to_k, kcodes, kpower);
-            put(stage + to_v, vcodes, vpower);
+            if ((vinfo & 0xffff) != 0xffff && !((vinfo >> row) & 1)) vcodes = words_t{};
+            put(stage + to_k, kcodes, k_power(kinfo));
+            put(stage + to_v, vcodes, v_power(vinfo));
         };
 
-        fetch(0);
         {
             const uint32_t to = __builtin_amdgcn_readfirstlane(lds_offset(qlds)) + (uint32_t)(wrow * D * (int)sizeof(T));
 #pragma unroll
@@ -671,7 +692,6 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
             }
         }
         load(0);
-        fetch(1);
         wait_vm<0>();
         // B operand Q^T: lane (lr, lq) takes dims 32 f + 8 lq .. + 7 of row lr.
         eight_t qf[NJ][NF][QP];
@@ -691,14 +711,12 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
         }
         write(0);
         load(1);                                              // n >= 1: stages 0 and 1 exist
-        fetch(2);
         wait_lds_reads();
 
         f4_t sc[NJ][4];
         eight_t pf[NJ][2][PP];
         h8_t ones = {1, 1, 1, 1, 1, 1, 1, 1};
         if constexpr (F16) asm volatile("" : "+v"(ones));     // kept in registers for the whole loop
-        uint64_t mk = ~0ull;                                  // positions of this turn's block that count
 
         // Fragment x of a turn: x < 2 UT is V^T (32-key step x / UT, dims 16 (x % UT)), the rest K
         // (key tile, then chunk).  They are read kAhead fragments before their products, in
@@ -706,7 +724,6 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
         constexpr int kAhead = 6, kV = 2 * UT, kAll = kV + 4 * NF;
         auto products = [&](int i, auto first_c, auto last_c) {   // fragments first .. last - 1
             constexpr int first = decltype(first_c)::value, last = decltype(last_c)::value;
-            if constexpr (last == kAll) mk = masks[i % W::MASKS];
             if (!active) return;
             int odd = i & 1;
             asm volatile("" : "+s"(odd));
@@ -764,10 +781,15 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
         const std::integral_constant<int, 0> from_v;
         const std::integral_constant<int, kV> to_v_end;
         const std::integral_constant<int, kAll> to_k_end;
-        auto softmax = [&](int i) {
+        auto softmax = [&](int i, bool full) {
             if (!active) return;
             const int k0 = w.key0 + i * BK;
-            const bool edge = mk != ~0ull || k0 + BK > seen_all;
+            const bool edge = !full || k0 + BK > seen_all;
+            uint64_t mk = ~0ull;                              // positions that count
+            if (!full) {
+                mk = 0;
+                for (int g = 0; g < 4; g++) mk |= (uint64_t)mask_of(i, g) << (16 * g);
+            }
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
                 if (edge) hide(sc[j], mk, seen[j] - k0, lane);
@@ -798,26 +820,20 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
                 if constexpr (!F16) l_run[j].add(l_blk);
             }
         };
-        auto uniform = [](uint64_t x) {
-            return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
-                   (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
-        };
-        // Stage i into the ring, the codes of the next one on their way, the page of the one behind it.
+        // Stage i into the ring, the codes of the next one on their way.
         auto refill = [&](int i) {
-            if (i > n) return;
-            write(i);
+            if (i <= n) write(i);
             __builtin_amdgcn_sched_barrier(0);
             if (i + 1 <= n) load(i + 1);
-            fetch(i + 2);
+            else wholes <<= 1;
             __builtin_amdgcn_sched_barrier(0);
         };
         // Everybody meets at every barrier, 2 n + 2 of them; each waits for its LDS accesses before.
         ring_barrier();
         auto half = [&](int i, int stage) {
-            mk = uniform(mk);
             ring_barrier();
             refill(stage);
-            softmax(i);
+            softmax(i, (wholes >> (stage + 1 - i)) & 1);
             wait_lds_reads();
             ring_barrier();
         };
@@ -868,7 +884,6 @@ __global__ __launch_bounds__(512, 2)
 void paged_wide8(cf_paged_q8_args_t a, PagedPlan pl, Q8Divs dv) {
     using W = Wide8<T, D, NJ>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[W::LDS];
-    __shared__ uint64_t masks[W::MASKS];
     __shared__ int kept[3 * 64];
     const Geometry<W::TM, 64, kNarrowCost8> geo(a.at, pl, kept);
     if (geo.lists_cut_tiles()) return;
@@ -879,7 +894,7 @@ void paged_wide8(cf_paged_q8_args_t a, PagedPlan pl, Q8Divs dv) {
         Work w = unit_work<W::TM, 64>(a.at, pl, un);
         const bool narrow = w.n_rows <= 16;
         const uint32_t again = narrow ? narrow_unit8<T, D, W::TM, 8>(a, pl, dv, lds, un, kvh, w)
-                                      : wide8_unit<T, D, NJ>(a, pl, dv, lds, masks, un, kvh, w);
+                                      : wide8_unit<T, D, NJ>(a, pl, dv, lds, un, kvh, w);
         if (!again) continue;
         if (!geo.find(id, un)) break;         // found anew: nothing is kept for this
         w = unit_work<W::TM, 64>(a.at, pl, un);
@@ -958,8 +973,8 @@ Plan8 make_plan8(const cf_paged_attn_args_t& a) {
     const int64_t per_cu = wide ? 1 : 4 * (a.d == 128 ? Heads8<128>::PER_CU : Heads8<64>::PER_CU);
     const int64_t fill = cus * per_cu > a.H_kv ? cus * per_cu / a.H_kv : 1;
     p.pl.fill = (int32_t)fill;
-    p.pl.min_blocks = (int32_t)(wide ? 12 : 64 / BK);
-    p.pl.one_blocks = (int32_t)((wide ? 1536 : 128) / BK);
+    p.pl.min_blocks = (int32_t)(wide ? f16 ? 12 : 4 : 64 / BK);
+    p.pl.one_blocks = (int32_t)((wide ? f16 ? 1536 : 512 : 128) / BK);
     p.pl.max_records = (int32_t)(4 * fill + 8);
     const bool cut = !a.uncut && p.form != kSplit8 && (a.max_len + BK - 1) / BK > (wide ? kFewOne / BK : p.pl.one_blocks);
     if (!cut) p.pl.one_blocks = INT32_MAX;                    // nor is what is longer than max_len

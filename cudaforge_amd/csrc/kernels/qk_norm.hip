@@ -74,8 +74,197 @@ void qk_norm_any(cf_qk_norm_args_t a) {
     }
 }
 
+// ---- Rows of 16-byte pieces: two of them per lane, the next power of two of d / 2 pieces lanes a
+// head.  A lane's pieces hold both values of its pairs: with `halves` pieces j and j + r / 2 values,
+// else neighbours; lane j has pairs VEC j .. + VEC - 1 either way, whose cosines and sines the
+// workgroup works out once per row.  HBM bounds it. ----
+constexpr int kThreads = 256;
+template <typename T> struct alignas(16) Piece { T e[16 / sizeof(T)]; };
+
+struct WideQk {
+    int lanes;             // a head's, a power of two
+    int rows;              // of a workgroup
+    int per_row;           // heads of Q and K
+    FastDiv by_heads;
+};
+
+// Sum over the lanes of a head.
+__device__ __forceinline__ float head_sum(float x, int lanes) {
+    if (lanes > 1) x += dpp_f<kDppXor1>(x);
+    if (lanes > 2) x += dpp_f<kDppXor2>(x);
+    if (lanes > 4) x += dpp_f<kDppHalfMirror>(x);
+    if (lanes > 8) x += dpp_f<kDppMirror>(x);
+    if (lanes > 16) x = add_xor16(x);
+    if (lanes > 32) x = add_xor32(x);
+    return x;
+}
+
+constexpr int kRows = 4;
+template <typename T>
+__global__ __launch_bounds__(kThreads)
+void qk_norm_wide(cf_qk_norm_args_t a, WideQk p, int64_t row0) {
+    constexpr int VEC = 16 / sizeof(T);
+    // Two pairs' (cos, sin) together, those of neighbouring lanes beside each other.
+    __shared__ f4_t turns[kRows][VEC / 2][CF_QK_ROPE_MAX_DIM / 2 / VEC + 1];
+    const int tid = threadIdx.x;
+    const int64_t t0 = row0 + (int64_t)blockIdx.x * p.rows;
+    const int n_rows = (int)min((int64_t)p.rows, a.T - t0);
+    // This lane's pieces.
+    const int j = tid & (p.lanes - 1), half = a.r / (2 * VEC);
+    const bool real = 2 * VEC * j < a.d, halves = a.halves && a.r > 0;
+    const int e0 = halves ? (j < half ? VEC * j : 2 * VEC * j) : 2 * VEC * j;
+    const int e1 = halves && j < half ? e0 + a.r / 2 : e0 + VEC;
+    const bool turned0 = e0 < a.r, turned1 = halves ? turned0 : e1 < a.r;
+    typedef Piece<T> piece_t;
+    piece_t gain[2][2], bias[2][2];
+    auto of_head = [&](piece_t (&to)[2], const void* from, float without) {
+        if (from && real) {
+            to[0] = *(const piece_t*)((const T*)from + e0);
+            to[1] = *(const piece_t*)((const T*)from + e1);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; e++) to[0].e[e] = to[1].e[e] = (T)without;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        of_head(gain[i], a.rows[i].gain, 1.0f);
+        of_head(bias[i], a.rows[i].bias, 0.0f);
+    }
+    struct Item { int row, which, h; bool any; piece_t x[2]; };
+    const int items = n_rows * p.per_row, step = kThreads / p.lanes * gridDim.y;
+    auto load = [&](int item) {
+        Item it;
+        it.any = item < items && real;
+        it.row = fastdiv(min(item, items - 1), p.by_heads);
+        const int head = min(item, items - 1) - it.row * p.per_row;
+        it.which = head >= a.rows[0].heads;
+        it.h = head - (it.which ? a.rows[0].heads : 0);
+        const cf_qk_rows_t& rows = a.rows[it.which];
+        const T* const x = (const T*)rows.x + (t0 + it.row) * rows.stride + (int64_t)it.h * a.d;
+        it.x[0] = *(const piece_t*)(x + (it.any ? e0 : 0));
+        it.x[1] = *(const piece_t*)(x + (it.any ? e1 : 0));
+        return it;
+    };
+    int item = blockIdx.y * (kThreads / p.lanes) + tid / p.lanes;
+    Item next = load(item);
+    if (a.positions) {
+        for (int i = tid; i < n_rows * (a.r / 2); i += kThreads) {
+            const int row = i / (a.r / 2), pair = i - row * (a.r / 2);
+            const float2 cs = turn_of(a, a.positions[t0 + row], pair);
+            ((float2*)&turns[row][pair % VEC / 2][pair / VEC])[pair & 1] = cs;
+        }
+        __syncthreads();
+    }
+    for (; item < (items + kThreads / p.lanes - 1) / (kThreads / p.lanes) * (kThreads / p.lanes); item += step) {
+        const Item it = next;
+        next = load(item + step);
+        float u[2][VEC];
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int e = 0; e < VEC; e++) u[k][e] = it.any ? (float)it.x[k].e[e] : 0.0f;
+        if (a.norm) {
+            if (a.norm == 2) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < VEC; e++) sum += u[0][e] + u[1][e];
+                const float mean = head_sum(sum, p.lanes) / (float)a.d;
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) u[k][e] = it.any ? u[k][e] - mean : 0.0f;
+            }
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < VEC; e++) sum = __builtin_fmaf(u[0][e], u[0][e], __builtin_fmaf(u[1][e], u[1][e], sum));
+            const float scale = 1.0f / sqrtf(head_sum(sum, p.lanes) / (float)a.d + a.eps);
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int e = 0; e < VEC; e++)
+                    u[k][e] = u[k][e] * scale * (float)(it.which ? gain[1][k].e[e] : gain[0][k].e[e]);
+            if (a.norm == 2)
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) u[k][e] += (float)(it.which ? bias[1][k].e[e] : bias[0][k].e[e]);
+        }
+        if (a.positions && turned0) {
+            float2 cs[VEC];
+#pragma unroll
+            for (int q = 0; q < VEC / 2; q++) {
+                const f4_t x = turns[it.row][q][j];
+                cs[2 * q] = float2{x[0], x[1]};
+                cs[2 * q + 1] = float2{x[2], x[3]};
+            }
+            auto turn = [](float& x, float& y, float2 c) {
+                const float v = x;
+                x = v * c.x - y * c.y;
+                y = v * c.y + y * c.x;
+            };
+            if (halves) {
+#pragma unroll
+                for (int e = 0; e < VEC; e++) turn(u[0][e], u[1][e], cs[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; e += 2) turn(u[0][e], u[0][e + 1], cs[e / 2]);
+                if (turned1)
+#pragma unroll
+                    for (int e = 0; e < VEC; e += 2) turn(u[1][e], u[1][e + 1], cs[VEC / 2 + e / 2]);
+            }
+        }
+        if (!it.any || (a.positions && a.positions[t0 + it.row] < 0)) continue;
+        const cf_qk_rows_t& rows = a.rows[it.which];
+        T* const y = (T*)rows.y + (t0 + it.row) * rows.out_stride + (int64_t)it.h * a.d;
+        piece_t out[2];
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int e = 0; e < VEC; e++) out[k].e[e] = (T)u[k][e];
+        *(piece_t*)(y + e0) = out[0];
+        *(piece_t*)(y + e1) = out[1];
+    }
+}
+
+template <typename T>
+bool wide_ok(const cf_qk_norm_args_t& a) {
+    constexpr int VEC = 16 / sizeof(T);
+    uint64_t all = 0;
+    for (int i = 0; i < 2; i++) {
+        const cf_qk_rows_t& r = a.rows[i];
+        if (r.heads == 0) continue;
+        all |= (uint64_t)(uintptr_t)r.x | (uint64_t)(uintptr_t)r.y | (uint64_t)(uintptr_t)r.gain | (uint64_t)(uintptr_t)r.bias |
+               (uint64_t)r.stride * sizeof(T) | (uint64_t)r.out_stride * sizeof(T);
+    }
+    return all % 16 == 0 && a.d % (2 * VEC) == 0 && a.d <= 64 * 2 * VEC && (a.halves ? a.r / 2 : a.r) % VEC == 0;
+}
+
+template <typename T>
+int launch_qk_wide(const cf_qk_norm_args_t& a, hipStream_t st) {
+    constexpr int VEC = 16 / sizeof(T);
+    WideQk p;
+    p.lanes = 1;
+    while (2 * VEC * p.lanes < a.d) p.lanes *= 2;
+    p.per_row = a.rows[0].heads + a.rows[1].heads;
+    p.by_heads = fastdiv_make(p.per_row);
+    // Few rows: a workgroup for every 256 lanes' worth of heads.
+    const bool few = a.T < 1024;
+    p.rows = few ? 1 : kRows;
+    const int64_t parts = few ? ((int64_t)p.per_row * p.lanes + kThreads - 1) / kThreads : 1;
+    constexpr int64_t kMost = 1 << 22;             // workgroups of a launch: a grid has less than 2^32 threads
+    for (int64_t t0 = 0; t0 < a.T; t0 += kMost * p.rows) {
+        const int64_t n = (a.T - t0 + p.rows - 1) / p.rows;
+        hipLaunchKernelGGL(qk_norm_wide<T>, dim3((unsigned)(n < kMost ? n : kMost), (unsigned)parts), dim3(kThreads), 0, st, a, p, t0);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return (int)e;
+    }
+    return 0;
+}
+
 template <typename T>
 int launch_qk(const cf_qk_norm_args_t& a, hipStream_t st) {
+    if (wide_ok<T>(a)) return launch_qk_wide<T>(a, st);
     const int heads = a.rows[0].heads + a.rows[1].heads;
     int64_t wgs = (a.T * heads + kAnyWaves - 1) / kAnyWaves;
     if (wgs > (1 << 22)) wgs = 1 << 22;            // a grid has less than 2^32 threads
