@@ -263,28 +263,26 @@ __device__ __forceinline__ void mend_rows8(const cf_paged_q8_args_t& a, const Pa
 }
 
 // ---- Up to 16 rows, one wave with a ring of its own: no barrier. ----
-template <int D> struct Narrow8 {
-    static constexpr int BK = 32, NS = 2;
+template <int D, int STAGES = 2> struct Narrow8 {
+    static constexpr int BK = 32, NS = STAGES;
     static constexpr int TILE = BK * D, STAGE = 2 * TILE;    // bytes
     static constexpr int RING = NS * STAGE;
 };
 
 // Positions [key0, key1) (key0 a multiple of 16) of (b, kvh) for the unit's rows: leaves m and
 // the lane's share of l, and lane (lr, lq) with dims 16 u + 4 lq .. + 3 of row lr.
-template <typename T, int D>
+template <typename T, int D, int STAGES = 2>
 __device__ __forceinline__ void narrow_range8(const cf_paged_q8_args_t& a, const PagedPlan& pl, const Q8Divs& dv, uint8_t* ring,
                                               const SeqRows& s, int b, int kvh, const Work& w, int key0, int key1,
                                               f4_t (&acc)[D / 16], float& m_run, float& l_run) {
     using R = Rows8<D>;
-    using N = Narrow8<D>;
+    using N = Narrow8<D, STAGES>;
     using B = typename Parts<T>::half_t;
     using C = Codes<B>;
     typedef typename C::eight_t eight_t;
+    typedef T q8_t __attribute__((ext_vector_type(8)));
     constexpr int BK = N::BK, NG = BK / 16, NS = N::NS, TILE = N::TILE, STAGE = N::STAGE, NI = R::NI, NL = 2 * NG * NI, UT = R::UT;
     constexpr int QP = Parts<T>::Q, PP = Parts<T>::P, KS = D / 32;
-    // Q: 16-byte chunks per row, rows per DMA instruction, elements per chunk.
-    constexpr int QC = D * (int)sizeof(T) / 16, QR = 64 / QC, QN = 16 / QR, QE = 16 / (int)sizeof(T);
-    static_assert(16 * D * (int)sizeof(T) <= STAGE, "Q fits a stage");
     static_assert(NS * NL < 64, "vmcnt range");
     const int lane = unit_lane(), lr = lane & 15, lq = lane >> 4;
     const int drow = R::drow(lane), dch = R::dch(lane);
@@ -299,6 +297,15 @@ __device__ __forceinline__ void narrow_range8(const cf_paged_q8_args_t& a, const
     const int seen = min(w.base + fastdiv(w.R0 + min(lr, w.n_rows - 1), pl.by_group), s.len);
     const int seen_all = min(w.base + fastdiv(w.R0, pl.by_group), s.len);
 
+    // B operand Q^T: in step ks lane (lr, lq) holds dims 64 (ks / 2) + 16 lq + 8 (ks % 2) .. + 7 of row lr.  Its
+    // loads wait together with those of the table.
+    q8_t q[KS];
+    {
+        const RowAt at = row_at(pl, pl.G, kvh, w.R0 + min(lr, w.n_rows - 1));
+        const T* const from = (const T*)a.at.q + (int64_t)(s.row0 + at.tok) * a.at.q_stride + at.h * D + 16 * lq;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) q[ks] = *(const CF_GLOBAL q8_t*)(from + 64 * (ks / 2) + 8 * (ks % 2));
+    }
     uint32_t koff[NI], voff[NI][2];
 #pragma unroll
     for (int u = 0; u < NI; u++) {
@@ -333,35 +340,18 @@ __device__ __forceinline__ void narrow_range8(const cf_paged_q8_args_t& a, const
         }
     };
 
-    wait_lds_reads();                                         // what the ring held before
-    // Q rows by DMA into the last stage, which the first blocks leave free; chunks swizzled by the row.
-    {
-        const uint32_t qlds = ring_base + (uint32_t)((NS - 1) * STAGE);
-#pragma unroll
-        for (int u = 0; u < QN; u++) {
-            const int row = QR * u + lane / QC;
-            const RowAt at = row_at(pl, pl.G, kvh, w.R0 + min(row, w.n_rows - 1));
-            lds_dma16((const T*)a.at.q + (int64_t)(s.row0 + at.tok) * a.at.q_stride + at.h * D + QE * ((lane % QC) ^ (row & 7)),
-                      __builtin_amdgcn_readfirstlane(qlds + u * 1024u));
-        }
-    }
-    issue(0, std::integral_constant<int, 0>{});
-    wait_vm<NL>();
-    // B operand Q^T: in step ks lane (lr, lq) holds dims 64 (ks / 2) + 16 lq + 8 (ks % 2) .. + 7 of row lr.
     eight_t qf[KS][QP];
-    {
-        const T* const q = (const T*)(ring + (NS - 1) * STAGE) + lr * D;
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++)
+    for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int dim = 64 * (ks / 2) + 16 * lq + 8 * (ks % 2) + e;
-                const T x = q[QE * ((dim / QE) ^ (lr & 7)) + dim % QE];
-                if constexpr (QP == 1) qf[ks][0][e] = x;
-                else split_into<QP, B>(qf[ks], e, (float)x);
-            }
-    }
-    wait_lds_reads();
+        for (int e = 0; e < 8; e++) {
+            if constexpr (QP == 1) qf[ks][0][e] = q[ks][e];
+            else split_into<QP, B>(qf[ks], e, (float)q[ks][e]);
+        }
+    wait_lds_reads();                                         // what the ring held before
+    static_for<NS - 1>([&](auto i) {
+        if (i < nblk) issue(i, i);
+    });
 
     auto step = [&](int bi, auto stage_c) {
         constexpr int stage = decltype(stage_c)::value;
@@ -451,17 +441,18 @@ __device__ __forceinline__ void narrow_range8(const cf_paged_q8_args_t& a, const
 // A wave per unit, the units of neighbouring KV heads in one workgroup: they read the same
 // cache rows at about the same time.
 template <int D> struct Heads8 {
-    static constexpr int WAVES = 4;
-    static constexpr int PER_CU = 160 * 1024 / (WAVES * Narrow8<D>::RING) < 4 ? 160 * 1024 / (WAVES * Narrow8<D>::RING) : 4;
+    static constexpr int WAVES = 4, NS = 2;
+    static constexpr int RING = Narrow8<D, NS>::RING;
+    static constexpr int FIT = 160 * 1024 / (WAVES * RING), PER_CU = FIT < 4 ? FIT : 4;
 };
 template <typename T, int D>
 __global__ __launch_bounds__(256, (Heads8<D>::PER_CU))
 void paged_heads8(cf_paged_q8_args_t a, PagedPlan pl, Q8Divs dv) {
     using H = Heads8<D>;
-    constexpr int BK = Narrow8<D>::BK, RING = Narrow8<D>::RING;
+    constexpr int BK = Narrow8<D>::BK, RING = H::RING;
     __shared__ __attribute__((aligned(16))) uint8_t ring_all[H::WAVES * RING];
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const Geometry<16, BK, 1> geo(a.at, pl);
+    const Geometry<16, BK, 1, true, true> geo(a.at, pl);
     if (geo.lists_cut_tiles()) return;
     for (int unit = (int)blockIdx.x * H::WAVES + wave;; unit += pl.step) {
         const int id = fastdiv(unit, pl.by_kv), kvh = unit - id * a.at.H_kv;
@@ -471,7 +462,7 @@ void paged_heads8(cf_paged_q8_args_t a, PagedPlan pl, Q8Divs dv) {
         const int lane = unit_lane(), lr = lane & 15, lq = lane >> 4;
         f4_t acc[D / 16];
         float m, l;
-        narrow_range8<T, D>(a, pl, dv, ring_all + wave * RING, un.s, un.b, kvh, w, w.key0, w.key1, acc, m, l);
+        narrow_range8<T, D, H::NS>(a, pl, dv, ring_all + wave * RING, un.s, un.b, kvh, w, w.key0, w.key1, acc, m, l);
         l = add_xor32(add_xor16(l));
         const uint32_t again = rows_of_16(lr < w.n_rows && spoilt(acc, l));
         if (lr < w.n_rows) {
@@ -970,7 +961,7 @@ Plan8 make_plan8(const cf_paged_attn_args_t& a) {
     const int64_t BK = p.form == kHeads8 ? Narrow8<64>::BK : 64;
     const int64_t tiles = tiles_of(TM);
     // Units in flight, by the LDS a workgroup takes.
-    const int64_t per_cu = wide ? 1 : 4 * (a.d == 128 ? Heads8<128>::PER_CU : Heads8<64>::PER_CU);
+    const int64_t per_cu = wide ? 1 : a.d == 128 ? 4 : 8;
     const int64_t fill = cus * per_cu > a.H_kv ? cus * per_cu / a.H_kv : 1;
     p.pl.fill = (int32_t)fill;
     p.pl.min_blocks = (int32_t)(wide ? f16 ? 12 : 4 : 64 / BK);
@@ -979,7 +970,7 @@ Plan8 make_plan8(const cf_paged_attn_args_t& a) {
     const bool cut = !a.uncut && p.form != kSplit8 && (a.max_len + BK - 1) / BK > (wide ? kFewOne / BK : p.pl.one_blocks);
     if (!cut) p.pl.one_blocks = INT32_MAX;                    // nor is what is longer than max_len
     p.bytes = cut ? header_bytes(p.pl.max_records) + (size_t)p.pl.max_records * a.H_kv * (TM * (a.d + 2)) * sizeof(float) : 0;
-    int64_t units = (tiles + (cut ? 2 * fill : 0)) * a.H_kv;
+    int64_t units = (p.form == kHeads8 && cut && tiles <= fill ? fill : tiles + (cut ? 2 * fill : 0)) * a.H_kv;
     if (units > (1 << 22)) units = 1 << 22;
     p.wgs = (int)(p.form == kHeads8 ? (units + 3) / 4 : units);
     p.pl.step = p.form == kHeads8 ? 4 * p.wgs : p.wgs;

@@ -26,7 +26,32 @@ template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T e[N]; };
 // rounded to 65536).
 template <typename T> constexpr float kMostStored = sizeof(T) == 2 ? 61440.0f : 0x1.ep127f;
 
-// x at its power.
+// The largest size among a piece's values, by their bits: n of them, and whether all are finite.
+template <int N> __device__ __forceinline__ float largest(const Pack<_Float16, N>& x, bool& finite) {
+    typedef unsigned short us2_t __attribute__((ext_vector_type(2)));
+    us2_t m = {0, 0};
+    if constexpr (N > 1) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const us2_t b = __builtin_bit_cast(us2_t, h2_t{x.e[i], x.e[i + 1]}) & us2_t{0x7fff, 0x7fff};
+            m = __builtin_elementwise_max(m, b);
+        }
+    } else {
+        m[0] = __builtin_bit_cast(unsigned short, x.e[0]) & 0x7fff;
+    }
+    const unsigned short most = m[0] > m[1] ? m[0] : m[1];
+    finite &= most < 0x7c00;
+    return (float)__builtin_bit_cast(_Float16, most);
+}
+template <int N> __device__ __forceinline__ float largest(const Pack<float, N>& x, bool& finite) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) m = max(m, __float_as_uint(x.e[i]) & 0x7fffffffu);
+    finite &= m < 0x7f800000u;
+    return __uint_as_float(m);
+}
+
+// x at its power, in reach of the codes.
 __device__ __forceinline__ float to_code(float x, int shift, float most) {
     const float y = __builtin_amdgcn_fmed3f(ldexpf(x, shift), -most, most);
     return __builtin_fabsf(x) < INFINITY ? y : NAN;
@@ -56,24 +81,29 @@ __device__ __forceinline__ void store_run(const cf_page_store_q8_args_t& a, cons
     typedef Pack<T, VEC> pack_t;
     const int old = *power;
     auto load = [&](int r, int e) { return *(const pack_t*)(rows + (run.t + min(r, run.len - 1)) * a.kv_stride + e); };
-    auto most_of = [&](const pack_t& x) {
-        float m = 0.0f;
-#pragma unroll
-        for (int i = 0; i < VEC; i++) m = fmaxf(m, finite_size((float)x.e[i]));
-        return m;
-    };
     pack_t kept[KEEP];
     float most = 0.0f;
+    bool finite = true;
     if constexpr (WIDE) {
 #pragma unroll
         for (int s = 0; s < KEEP; s++)
             if (s * at_once < run.len) kept[s] = load(s * at_once + sub, e0);
 #pragma unroll
         for (int s = 0; s < KEEP; s++)
-            if (s * at_once < run.len) most = fmaxf(most, most_of(kept[s]));
+            if (s * at_once < run.len) most = fmaxf(most, largest(kept[s], finite));
     }
     for (int r = WIDE ? KEEP * at_once : 0; r < run.len; r += at_once)
-        for (int e = e0; e < a.d; e += step_e) most = fmaxf(most, most_of(load(r + sub, e)));
+        for (int e = e0; e < a.d; e += step_e) most = fmaxf(most, largest(load(r + sub, e), finite));
+    finite = !__builtin_amdgcn_ballot_w64(!finite);
+    if (!finite) {                                 // once more, without what is infinite or NaN
+        most = 0.0f;
+        for (int r = 0; r < run.len; r += at_once)
+            for (int e = e0; e < a.d; e += step_e) {
+                const pack_t x = load(r + sub, e);
+#pragma unroll
+                for (int i = 0; i < VEC; i++) most = fmaxf(most, finite_size((float)x.e[i]));
+            }
+    }
     const int need = power_for(wave_max(most));
     const bool mine = lane >= run.first && lane < run.first + run.len;
     const bool begun = __builtin_amdgcn_ballot_w64(mine && slot == run.slot0) != 0;
@@ -108,7 +138,8 @@ __device__ __forceinline__ void store_run(const cf_page_store_q8_args_t& a, cons
             }
         }
     }
-    const float limit = fminf(448.0f, ldexpf(kMostStored<T>, 127 - now));
+    // Where no code can pass 448 or the type's largest number, as almost always, one instruction does.
+    const float limit = fminf(448.0f, ldexpf(kMostStored<T>, 127 - now)), over = power_bits(now);
     auto place = [&](int r) { return run.cells + (int64_t)(__shfl(slot, run.first + min(r, run.len - 1)) - run.slot0) * a.row_stride; };
     auto put = [&](int r, uint8_t* cell, const pack_t& x) {
         if (r >= run.len) return;
@@ -116,10 +147,16 @@ __device__ __forceinline__ void store_run(const cf_page_store_q8_args_t& a, cons
             Pack<uint32_t, VEC / 4> c;
 #pragma unroll
             for (int i = 0; i < VEC / 4; i++) {
-                float y[4];
+                if (limit == 448.0f) {
+                    typedef T two_t __attribute__((ext_vector_type(2)));
+                    const s2_t w = codes_over<false>(s2_t{0, 0}, two_t{x.e[4 * i], x.e[4 * i + 1]}, over);
+                    c.e[i] = __builtin_bit_cast(uint32_t, codes_over<true>(w, two_t{x.e[4 * i + 2], x.e[4 * i + 3]}, over));
+                } else {
+                    float y[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) y[j] = to_code((float)x.e[4 * i + j], 127 - now, limit);
-                c.e[i] = codes_of<true>(codes_of<false>(0, y[0], y[1]), y[2], y[3]);
+                    for (int j = 0; j < 4; j++) y[j] = to_code((float)x.e[4 * i + j], 127 - now, limit);
+                    c.e[i] = codes_of<true>(codes_of<false>(0, y[0], y[1]), y[2], y[3]);
+                }
             }
             *(Pack<uint32_t, VEC / 4>*)cell = c;
         } else {
@@ -137,7 +174,7 @@ __device__ __forceinline__ void store_run(const cf_page_store_q8_args_t& a, cons
 }
 
 // Workgroup (x, y): the runs that begin in rows R x .. R x + R - 1, of heads 4 y .. 4 y + 3 of K's
-// and V's, a wave each.  R + block <= 64: the lanes hold the slots of those runs.
+// and V's, a wave each, whose lanes hold the slots of 64 rows.
 constexpr int kStoreWaves = 4;
 template <typename T, int VEC>
 __global__ __launch_bounds__(64 * kStoreWaves)
@@ -160,14 +197,20 @@ void page_store_q8(cf_page_store_q8_args_t a, StoreDivs dv, int R, int64_t row0)
         Run run;
         run.first = __builtin_ctzll(heads);
         const int b = __builtin_amdgcn_readlane(block, run.first);
-        const uint64_t same = __builtin_amdgcn_ballot_w64(block == b) >> run.first;
-        run.len = ~same ? __builtin_ctzll(~same) : 64;
         run.t = t0 + run.first;
+        int its_slot = slot;
+        uint64_t same = __builtin_amdgcn_ballot_w64(block == b) >> run.first;
+        if (run.first + a.block > 64) {            // it may go on behind the 64
+            its_slot = run.t + lane < a.T ? a.slots[run.t + lane] : -1;
+            same = __builtin_amdgcn_ballot_w64(block_of(its_slot) == b);
+            run.first = 0;
+        }
+        run.len = ~same ? __builtin_ctzll(~same) : 64;
         run.slot0 = b * a.block;
         const int page = fastdiv(b, dv.blocks);
         run.cells = pages + (int64_t)page * a.page_stride + (int64_t)(run.slot0 - page * a.page_size) * a.row_stride +
                     (int64_t)h * a.head_stride;
-        store_run<T, VEC>(a, run, slot, rows, powers + (int64_t)b * a.H_kv + h);
+        store_run<T, VEC>(a, run, its_slot, rows, powers + (int64_t)b * a.H_kv + h);
     }
 }
 
@@ -180,7 +223,11 @@ int launch_store(const cf_page_store_q8_args_t& a, hipStream_t st) {
     const int per_row = a.d / kWide;
     const bool wide = in % 16 == 0 && out % kWide == 0 && a.d % kWide == 0 && per_row <= 64 && (per_row & (per_row - 1)) == 0;
     const StoreDivs dv = {fastdiv_make(a.block), fastdiv_make(a.page_size / a.block)};
-    const int R = a.T >= 2048 && a.block <= 48 ? 16 : 1;
+    // Few rows of a workgroup cost launches of workgroups that find no run, many cost turns where each is a
+    // run of its own (8 heads of 128 fp16, us with 1, 4, 8 and 16 rows: 256 sequences of one row 6.0, 6.2, 9.8
+    // and 17.1; 840 rows of 3 sequences, blocks of 32, 8.8, 5.9, 6.4 and 6.4; 2048 rows of 2 23.9, 9.5, 6.6
+    // and 6.4; 8192 rows of 4 49.1, 19.9, 13.3 and 11.8).
+    const int R = a.T < 1024 ? 4 : a.T < 4096 ? 8 : 16;
     const unsigned parts = (unsigned)((2 * (int64_t)a.H_kv + kStoreWaves - 1) / kStoreWaves);
     constexpr int64_t kMost = 1 << 23;             // rows of a launch: a grid has less than 2^32 threads
     for (int64_t t0 = 0; t0 < a.T; t0 += kMost * R) {

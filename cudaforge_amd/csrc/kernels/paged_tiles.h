@@ -90,8 +90,8 @@ struct Unit {
 
 // The tiles' geometry, one sequence per lane and 64 at a time.  TM rows per tile, BK
 // positions per key block; a tile of up to 16 rows costs 1 / NARROW of a full one's block.
-// CUTS: tiles may be cut.
-template <int TM, int BK, int NARROW, bool CUTS = true>
+// CUTS: tiles may be cut.  COUNTS: ranges of few sequences are counted, so that they go in one round.
+template <int TM, int BK, int NARROW, bool CUTS = true, bool COUNTS = false>
 struct Geometry {
     const cf_paged_attn_args_t& a;
     const PagedPlan& pl;
@@ -159,6 +159,22 @@ struct Geometry {
         C = fmaxf(w, (float)(few ? kFewMin : pl.min_blocks));
         inv_C = 1.0f / C;
         if (pl.one_blocks == INT32_MAX) one = INT32_MAX;
+        if constexpr (COUNTS) {
+            // The shortest ranges of which there are no more than `fill`, if they are not much longer than
+            // an equal share (else a few long sequences would wait for ranges of their own).
+            if (!plans || a.B > 64 || t > fill) return;
+            const float share = fmaxf(wave_sum(cost(first)) / fill, (float)pl.min_blocks), was = C;
+            C = ceilf(share);
+            for (int i = 0; i < 8; i++) {
+                inv_C = 1.0f / C;
+                const float units = wave_sum((float)(tiles(first) * ranges(first)));
+                if (units <= fill) return;
+                C = fmaxf(C + 1.0f, ceilf(C * (units / fill)));
+                if (C > 1.5f * share + 1.0f) break;
+            }
+            C = was;
+            inv_C = 1.0f / C;
+        }
     }
     // True for the workgroup behind the units', which lists the cut tiles.
     __device__ __forceinline__ bool lists_cut_tiles() const {
