@@ -69,12 +69,12 @@ struct Run {
     int slot0;             // ... and its slot
 };
 
-// VEC elements of 16 bytes a lane, d / VEC = 2^k lanes a row; VEC = 1: any shape, all lanes on one row.
-template <typename T, int VEC>
+// VEC elements of 16 bytes a lane, d / VEC = 2^k lanes a row, KEEP steps of rows in registers; VEC = 1:
+// any shape, all lanes on one row.
+template <typename T, int VEC, int KEEP>
 __device__ __forceinline__ void store_run(const cf_page_store_q8_args_t& a, const Run& run, int slot, const T* rows,
                                           uint8_t* power) {
     constexpr bool WIDE = VEC > 1;
-    constexpr int KEEP = WIDE ? 8 : 1;             // steps whose rows stay in registers
     const int lane = threadIdx.x & 63;
     const int per_row = WIDE ? a.d / VEC : 64, at_once = 64 / per_row;
     const int sub = WIDE ? lane / per_row : 0, e0 = (lane % per_row) * VEC, step_e = WIDE ? a.d : 64;
@@ -176,7 +176,7 @@ __device__ __forceinline__ void store_run(const cf_page_store_q8_args_t& a, cons
 // Workgroup (x, y): the runs that begin in rows R x .. R x + R - 1, of heads 4 y .. 4 y + 3 of K's
 // and V's, a wave each, whose lanes hold the slots of 64 rows.
 constexpr int kStoreWaves = 4;
-template <typename T, int VEC>
+template <typename T, int VEC, int KEEP>
 __global__ __launch_bounds__(64 * kStoreWaves)
 void page_store_q8(cf_page_store_q8_args_t a, StoreDivs dv, int R, int64_t row0) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -210,7 +210,7 @@ void page_store_q8(cf_page_store_q8_args_t a, StoreDivs dv, int R, int64_t row0)
         const int page = fastdiv(b, dv.blocks);
         run.cells = pages + (int64_t)page * a.page_stride + (int64_t)(run.slot0 - page * a.page_size) * a.row_stride +
                     (int64_t)h * a.head_stride;
-        store_run<T, VEC>(a, run, its_slot, rows, powers + (int64_t)b * a.H_kv + h);
+        store_run<T, VEC, KEEP>(a, run, its_slot, rows, powers + (int64_t)b * a.H_kv + h);
     }
 }
 
@@ -233,8 +233,9 @@ int launch_store(const cf_page_store_q8_args_t& a, hipStream_t st) {
     for (int64_t t0 = 0; t0 < a.T; t0 += kMost * R) {
         const int64_t n = (a.T - t0 + R - 1) / R;
         const dim3 grid((unsigned)(n < kMost ? n : kMost), parts), block(64 * kStoreWaves);
-        if (wide) hipLaunchKernelGGL((page_store_q8<T, kWide>), grid, block, 0, st, a, dv, R, t0);
-        else hipLaunchKernelGGL((page_store_q8<T, 1>), grid, block, 0, st, a, dv, R, t0);
+        if (wide && a.block * per_row <= 8 * 64) hipLaunchKernelGGL((page_store_q8<T, kWide, 8>), grid, block, 0, st, a, dv, R, t0);
+        else if (wide) hipLaunchKernelGGL((page_store_q8<T, kWide, 16>), grid, block, 0, st, a, dv, R, t0);
+        else hipLaunchKernelGGL((page_store_q8<T, 1, 1>), grid, block, 0, st, a, dv, R, t0);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return (int)e;
     }

@@ -76,16 +76,16 @@ void qk_norm_any(cf_qk_norm_args_t a) {
 
 // ---- Rows of 16-byte pieces: two of them per lane, the next power of two of d / 2 pieces lanes a
 // head.  A lane's pieces hold both values of its pairs: with `halves` pieces j and j + r / 2 values,
-// else neighbours; lane j has pairs VEC j .. + VEC - 1 either way, whose cosines and sines the
-// workgroup works out once per row.  HBM bounds it. ----
+// else neighbours; lane j has pairs VEC j .. + VEC - 1 either way.  It stays on one row and goes over
+// its heads, so that it keeps their cosines and sines, which the workgroup works out once per row.
+// HBM bounds it. ----
 constexpr int kThreads = 256;
 template <typename T> struct alignas(16) Piece { T e[16 / sizeof(T)]; };
 
 struct WideQk {
     int lanes;             // a head's, a power of two
     int rows;              // of a workgroup
-    int per_row;           // heads of Q and K
-    FastDiv by_heads;
+    int at_once;           // heads of a row: rows * at_once * lanes = kThreads
 };
 
 // Sum over the lanes of a head.
@@ -100,23 +100,38 @@ __device__ __forceinline__ float head_sum(float x, int lanes) {
 }
 
 constexpr int kRows = 4;
-template <typename T>
+template <typename T, int NORM>
 __global__ __launch_bounds__(kThreads)
 void qk_norm_wide(cf_qk_norm_args_t a, WideQk p, int64_t row0) {
     constexpr int VEC = 16 / sizeof(T);
+    typedef Piece<T> piece_t;
     // Two pairs' (cos, sin) together, those of neighbouring lanes beside each other.
     __shared__ f4_t turns[kRows][VEC / 2][CF_QK_ROPE_MAX_DIM / 2 / VEC + 1];
-    const int tid = threadIdx.x;
-    const int64_t t0 = row0 + (int64_t)blockIdx.x * p.rows;
+    const int tid = threadIdx.x, slot = tid / p.lanes, row = slot / p.at_once;
+    const int64_t t0 = row0 + (int64_t)blockIdx.x * p.rows, t = t0 + row;
     const int n_rows = (int)min((int64_t)p.rows, a.T - t0);
+    const int n_q = a.rows[0].heads, heads = n_q + a.rows[1].heads;
     // This lane's pieces.
     const int j = tid & (p.lanes - 1), half = a.r / (2 * VEC);
     const bool real = 2 * VEC * j < a.d, halves = a.halves && a.r > 0;
     const int e0 = halves ? (j < half ? VEC * j : 2 * VEC * j) : 2 * VEC * j;
     const int e1 = halves && j < half ? e0 + a.r / 2 : e0 + VEC;
     const bool turned0 = e0 < a.r, turned1 = halves ? turned0 : e1 < a.r;
-    typedef Piece<T> piece_t;
-    piece_t gain[2][2], bias[2][2];
+    const int step = p.at_once * (int)gridDim.y;
+    int head = slot % p.at_once + p.at_once * (int)blockIdx.y;
+    const int pos = a.positions && row < n_rows ? a.positions[t] : 0;
+    const bool skip = row >= n_rows || pos < 0;
+    auto load = [&](int h, piece_t (&x)[2]) {
+        if (h >= heads || skip || !real) return;
+        const cf_qk_rows_t& rows = a.rows[h >= n_q];
+        const T* const from = (const T*)rows.x + t * rows.stride + (int64_t)(h >= n_q ? h - n_q : h) * a.d;
+        x[0] = *(const piece_t*)(from + e0);
+        x[1] = *(const piece_t*)(from + e1);
+    };
+    piece_t next[2] = {};
+    load(head, next);
+    // Gains and biases of Q and K.
+    piece_t gain[NORM > 0 ? 2 : 1][2], bias[NORM == 2 ? 2 : 1][2];
     auto of_head = [&](piece_t (&to)[2], const void* from, float without) {
         if (from && real) {
             to[0] = *(const piece_t*)((const T*)from + e0);
@@ -128,52 +143,44 @@ void qk_norm_wide(cf_qk_norm_args_t a, WideQk p, int64_t row0) {
     };
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        of_head(gain[i], a.rows[i].gain, 1.0f);
-        of_head(bias[i], a.rows[i].bias, 0.0f);
+        if constexpr (NORM > 0) of_head(gain[i], a.rows[i].gain, 1.0f);
+        if constexpr (NORM == 2) of_head(bias[i], a.rows[i].bias, 0.0f);
     }
-    struct Item { int row, which, h; bool any; piece_t x[2]; };
-    const int items = n_rows * p.per_row, step = kThreads / p.lanes * gridDim.y;
-    auto load = [&](int item) {
-        Item it;
-        it.any = item < items && real;
-        it.row = fastdiv(min(item, items - 1), p.by_heads);
-        const int head = min(item, items - 1) - it.row * p.per_row;
-        it.which = head >= a.rows[0].heads;
-        it.h = head - (it.which ? a.rows[0].heads : 0);
-        const cf_qk_rows_t& rows = a.rows[it.which];
-        const T* const x = (const T*)rows.x + (t0 + it.row) * rows.stride + (int64_t)it.h * a.d;
-        it.x[0] = *(const piece_t*)(x + (it.any ? e0 : 0));
-        it.x[1] = *(const piece_t*)(x + (it.any ? e1 : 0));
-        return it;
-    };
-    int item = blockIdx.y * (kThreads / p.lanes) + tid / p.lanes;
-    Item next = load(item);
+    float2 cs[VEC];
     if (a.positions) {
         for (int i = tid; i < n_rows * (a.r / 2); i += kThreads) {
-            const int row = i / (a.r / 2), pair = i - row * (a.r / 2);
-            const float2 cs = turn_of(a, a.positions[t0 + row], pair);
-            ((float2*)&turns[row][pair % VEC / 2][pair / VEC])[pair & 1] = cs;
+            const int of = i / (a.r / 2), pair = i - of * (a.r / 2);
+            ((float2*)&turns[of][pair % VEC / 2][pair / VEC])[pair & 1] = turn_of(a, a.positions[t0 + of], pair);
         }
         __syncthreads();
+        if (turned0 && !skip)
+#pragma unroll
+            for (int q = 0; q < VEC / 2; q++) {
+                const f4_t x = turns[row][q][j];
+                cs[2 * q] = float2{x[0], x[1]};
+                cs[2 * q + 1] = float2{x[2], x[3]};
+            }
     }
-    for (; item < (items + kThreads / p.lanes - 1) / (kThreads / p.lanes) * (kThreads / p.lanes); item += step) {
-        const Item it = next;
-        next = load(item + step);
+    if (skip) return;
+    for (; head < heads; head += step) {
+        const bool is_k = head >= n_q;
         float u[2][VEC];
 #pragma unroll
         for (int k = 0; k < 2; k++)
 #pragma unroll
-            for (int e = 0; e < VEC; e++) u[k][e] = it.any ? (float)it.x[k].e[e] : 0.0f;
-        if (a.norm) {
-            if (a.norm == 2) {
+            for (int e = 0; e < VEC; e++) u[k][e] = (float)next[k].e[e];       // zeros where there is no piece
+        load(head + step, next);
+        if constexpr (NORM > 0) {
+            if constexpr (NORM == 2) {
                 float sum = 0.0f;
 #pragma unroll
                 for (int e = 0; e < VEC; e++) sum += u[0][e] + u[1][e];
-                const float mean = head_sum(sum, p.lanes) / (float)a.d;
+                sum = head_sum(sum, p.lanes);                  // by all lanes
+                const float mean = real ? sum / (float)a.d : 0.0f;
 #pragma unroll
                 for (int k = 0; k < 2; k++)
 #pragma unroll
-                    for (int e = 0; e < VEC; e++) u[k][e] = it.any ? u[k][e] - mean : 0.0f;
+                    for (int e = 0; e < VEC; e++) u[k][e] -= mean;
             }
             float sum = 0.0f;
 #pragma unroll
@@ -182,22 +189,12 @@ void qk_norm_wide(cf_qk_norm_args_t a, WideQk p, int64_t row0) {
 #pragma unroll
             for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int e = 0; e < VEC; e++)
-                    u[k][e] = u[k][e] * scale * (float)(it.which ? gain[1][k].e[e] : gain[0][k].e[e]);
-            if (a.norm == 2)
-#pragma unroll
-                for (int k = 0; k < 2; k++)
-#pragma unroll
-                    for (int e = 0; e < VEC; e++) u[k][e] += (float)(it.which ? bias[1][k].e[e] : bias[0][k].e[e]);
+                for (int e = 0; e < VEC; e++) {
+                    u[k][e] = u[k][e] * scale * (float)(is_k ? gain[1][k].e[e] : gain[0][k].e[e]);
+                    if constexpr (NORM == 2) u[k][e] += (float)(is_k ? bias[1][k].e[e] : bias[0][k].e[e]);
+                }
         }
         if (a.positions && turned0) {
-            float2 cs[VEC];
-#pragma unroll
-            for (int q = 0; q < VEC / 2; q++) {
-                const f4_t x = turns[it.row][q][j];
-                cs[2 * q] = float2{x[0], x[1]};
-                cs[2 * q + 1] = float2{x[2], x[3]};
-            }
             auto turn = [](float& x, float& y, float2 c) {
                 const float v = x;
                 x = v * c.x - y * c.y;
@@ -214,9 +211,9 @@ void qk_norm_wide(cf_qk_norm_args_t a, WideQk p, int64_t row0) {
                     for (int e = 0; e < VEC; e += 2) turn(u[1][e], u[1][e + 1], cs[VEC / 2 + e / 2]);
             }
         }
-        if (!it.any || (a.positions && a.positions[t0 + it.row] < 0)) continue;
-        const cf_qk_rows_t& rows = a.rows[it.which];
-        T* const y = (T*)rows.y + (t0 + it.row) * rows.out_stride + (int64_t)it.h * a.d;
+        if (!real) continue;
+        const cf_qk_rows_t& rows = a.rows[is_k];
+        T* const y = (T*)rows.y + t * rows.out_stride + (int64_t)(is_k ? head - n_q : head) * a.d;
         piece_t out[2];
 #pragma unroll
         for (int k = 0; k < 2; k++)
@@ -246,16 +243,19 @@ int launch_qk_wide(const cf_qk_norm_args_t& a, hipStream_t st) {
     WideQk p;
     p.lanes = 1;
     while (2 * VEC * p.lanes < a.d) p.lanes *= 2;
-    p.per_row = a.rows[0].heads + a.rows[1].heads;
-    p.by_heads = fastdiv_make(p.per_row);
+    const int heads = a.rows[0].heads + a.rows[1].heads;
     // Few rows: a workgroup for every 256 lanes' worth of heads.
     const bool few = a.T < 1024;
     p.rows = few ? 1 : kRows;
-    const int64_t parts = few ? ((int64_t)p.per_row * p.lanes + kThreads - 1) / kThreads : 1;
+    p.at_once = kThreads / p.lanes / p.rows;
+    const int parts = few ? (heads + p.at_once - 1) / p.at_once : 1;
     constexpr int64_t kMost = 1 << 22;             // workgroups of a launch: a grid has less than 2^32 threads
     for (int64_t t0 = 0; t0 < a.T; t0 += kMost * p.rows) {
         const int64_t n = (a.T - t0 + p.rows - 1) / p.rows;
-        hipLaunchKernelGGL(qk_norm_wide<T>, dim3((unsigned)(n < kMost ? n : kMost), (unsigned)parts), dim3(kThreads), 0, st, a, p, t0);
+        const dim3 grid((unsigned)(n < kMost ? n : kMost), (unsigned)parts), block(kThreads);
+        if (a.norm == 0) hipLaunchKernelGGL((qk_norm_wide<T, 0>), grid, block, 0, st, a, p, t0);
+        else if (a.norm == 1) hipLaunchKernelGGL((qk_norm_wide<T, 1>), grid, block, 0, st, a, p, t0);
+        else hipLaunchKernelGGL((qk_norm_wide<T, 2>), grid, block, 0, st, a, p, t0);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return (int)e;
     }
