@@ -227,7 +227,7 @@ int launch_store(const cf_page_store_q8_args_t& a, hipStream_t st) {
     // run of its own (8 heads of 128 fp16, us with 1, 4, 8 and 16 rows: 256 sequences of one row 6.0, 6.2, 9.8
     // and 17.1; 840 rows of 3 sequences, blocks of 32, 8.8, 5.9, 6.4 and 6.4; 2048 rows of 2 23.9, 9.5, 6.6
     // and 6.4; 8192 rows of 4 49.1, 19.9, 13.3 and 11.8).
-    const int R = a.T < 1024 ? 4 : a.T < 4096 ? 8 : 16;
+    const int R = a.T < 1536 ? 4 : a.T < 4096 ? 8 : 16;
     const unsigned parts = (unsigned)((2 * (int64_t)a.H_kv + kStoreWaves - 1) / kStoreWaves);
     constexpr int64_t kMost = 1 << 23;             // rows of a launch: a grid has less than 2^32 threads
     for (int64_t t0 = 0; t0 < a.T; t0 += kMost * R) {

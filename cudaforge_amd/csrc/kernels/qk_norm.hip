@@ -78,7 +78,8 @@ void qk_norm_any(cf_qk_norm_args_t a) {
 // head.  A lane's pieces hold both values of its pairs: with `halves` pieces j and j + r / 2 values,
 // else neighbours; lane j has pairs VEC j .. + VEC - 1 either way.  It stays on one row and goes over
 // its heads, so that it keeps their cosines and sines, which the workgroup works out once per row.
-// HBM bounds it. ----
+// HBM bounds it: 8192 rows of 40 heads of 128 fp16, 168 MB, 28.2 us (5.9 TB/s), of 1001 FP32 rows of 24
+// heads of 64 6.9 us; 16 rows take 7.0 us, 5 of them the kernel's. ----
 constexpr int kThreads = 256;
 template <typename T> struct alignas(16) Piece { T e[16 / sizeof(T)]; };
 
@@ -100,7 +101,7 @@ __device__ __forceinline__ float head_sum(float x, int lanes) {
 }
 
 constexpr int kRows = 4;
-template <typename T, int NORM>
+template <typename T, int NORM, bool PAST>
 __global__ __launch_bounds__(kThreads)
 void qk_norm_wide(cf_qk_norm_args_t a, WideQk p, int64_t row0) {
     constexpr int VEC = 16 / sizeof(T);
@@ -219,10 +220,21 @@ void qk_norm_wide(cf_qk_norm_args_t a, WideQk p, int64_t row0) {
         for (int k = 0; k < 2; k++)
 #pragma unroll
             for (int e = 0; e < VEC; e++) out[k].e[e] = (T)u[k][e];
-        *(piece_t*)(y + e0) = out[0];
-        *(piece_t*)(y + e1) = out[1];
+        auto put = [](T* to, const piece_t& x) {
+            typedef uint32_t words_t __attribute__((ext_vector_type(4)));
+            if constexpr (PAST) __builtin_nontemporal_store(__builtin_bit_cast(words_t, x), (words_t*)to);
+            else *(piece_t*)to = x;
+        };
+        put(y + e0, out[0]);
+        put(y + e1, out[1]);
     }
 }
+
+// Results of more bytes than this are stored past the caches, which they would only sweep (rows of 40
+// heads of 128 fp16, us by themselves and with a copy of Q behind them that reads it: 4096 rows, 42 MB,
+// 16.0 and 33.0, through the caches 20.0 and 30.7; 8192 rows 29.7 and 63.3, and 40.8 and 65.5; 16384
+// rows 73 and 126, and 76 and 134).
+constexpr int64_t kPastBytes = 64 << 20;
 
 template <typename T>
 bool wide_ok(const cf_qk_norm_args_t& a) {
@@ -249,13 +261,15 @@ int launch_qk_wide(const cf_qk_norm_args_t& a, hipStream_t st) {
     p.rows = few ? 1 : kRows;
     p.at_once = kThreads / p.lanes / p.rows;
     const int parts = few ? (heads + p.at_once - 1) / p.at_once : 1;
+    const bool past = a.T * heads * a.d * (int64_t)sizeof(T) > kPastBytes;
     constexpr int64_t kMost = 1 << 22;             // workgroups of a launch: a grid has less than 2^32 threads
     for (int64_t t0 = 0; t0 < a.T; t0 += kMost * p.rows) {
         const int64_t n = (a.T - t0 + p.rows - 1) / p.rows;
         const dim3 grid((unsigned)(n < kMost ? n : kMost), (unsigned)parts), block(kThreads);
-        if (a.norm == 0) hipLaunchKernelGGL((qk_norm_wide<T, 0>), grid, block, 0, st, a, p, t0);
-        else if (a.norm == 1) hipLaunchKernelGGL((qk_norm_wide<T, 1>), grid, block, 0, st, a, p, t0);
-        else hipLaunchKernelGGL((qk_norm_wide<T, 2>), grid, block, 0, st, a, p, t0);
+        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, a, p, t0); };
+        if (a.norm == 0) past ? go(qk_norm_wide<T, 0, true>) : go(qk_norm_wide<T, 0, false>);
+        else if (a.norm == 1) past ? go(qk_norm_wide<T, 1, true>) : go(qk_norm_wide<T, 1, false>);
+        else past ? go(qk_norm_wide<T, 2, true>) : go(qk_norm_wide<T, 2, false>);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return (int)e;
     }

@@ -30,14 +30,15 @@ static int fill_turns(const qk_norm_rope_params_t* p, int64_t r, double* turns) 
         low = lo > 0.0L ? lo : 0.0L;
         high = hi < (long double)(r - 1) ? hi : (long double)(r - 1);
     }
-    const long double step = powl(base, -2.0L / (long double)r);
+    const long double step = powl(base, -2.0L / (long double)r), divided = p->scaling ? 1.0L / factor : 1.0L;
+    const long double range = p->scaling < 2 ? 0.0L : 1.0L / (p->scaling == 2 || high - low > 0.001L ? high - low : 0.001L);
     long double f = 1.0L / TWO_PI;
     for (int64_t i = 0; i < r / 2; i++, f *= step) {
         long double keep = p->scaling == 1 ? 0.0L : 1.0L;      /* share of f that is not divided */
-        if (p->scaling == 2) keep = (L * f - low) / (high - low);
-        if (p->scaling == 3) keep = 1.0L - ((long double)i - low) / (high - low > 0.001L ? high - low : 0.001L);
+        if (p->scaling == 2) keep = (L * f - low) * range;
+        if (p->scaling == 3) keep = 1.0L - ((long double)i - low) * range;
         keep = keep < 0.0L ? 0.0L : keep > 1.0L ? 1.0L : keep;
-        turns[i] = (double)(p->scaling == 0 ? f : f * (keep + (1.0L - keep) / factor));
+        turns[i] = (double)(p->scaling == 0 ? f : f * (keep + (1.0L - keep) * divided));
     }
     return 0;
 }
