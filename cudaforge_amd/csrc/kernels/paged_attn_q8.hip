@@ -1,6 +1,8 @@
 // paged_attn_q8.hip — attention of chunks of new tokens over a paged KV cache of 8-bit numbers
-// (gfx950).  The sums, rows and positions are those of paged_attn.hip; K and V are codes times the
-// power of two of their block.
+// (gfx950).  The sums, rows, positions and tiles are those of paged_attn.hip; K and V are codes times the
+// power of two of their block.  Times below are of one call among others on one MI355X; "n rows over m"
+// is n new tokens of a sequence of m positions in all, and heads are 32 of 128 over 8 KV heads and rows
+// fp16 where none are named.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -439,7 +441,11 @@ __device__ __forceinline__ void narrow_range8(const cf_paged_q8_args_t& a, const
 }
 
 // A wave per unit, the units of neighbouring KV heads in one workgroup: they read the same
-// cache rows at about the same time.
+// cache rows at about the same time.  HBM bounds it: 64 rows over 4096 each, 537 MB, 101 us (5.3 TB/s);
+// 16 rows over 1778 to 4096 positions, 114 MB, 29.2 us, 4 of them the merge's and 3 until the first
+// codes are there (launch, lengths, table, powers).  Two stages of a ring: with 3 or 4 the same 16 rows
+// take 30.0 and 32.7, as fewer workgroups fit a CU; a K part filled again before its V is used, 30.6; the
+// powers by DMA beside the first codes, 29.1, and 0.3 more where a wave has one or two blocks.
 template <int D> struct Heads8 {
     static constexpr int WAVES = 4, NS = 2;
     static constexpr int RING = Narrow8<D, NS>::RING;
@@ -476,7 +482,7 @@ void paged_heads8(cf_paged_q8_args_t a, PagedPlan pl, Q8Divs dv) {
 
 // Up to 16 rows by all waves of a workgroup: each takes a share of the unit's positions, and they
 // join their m, l and sums in LDS (WAVES rings at `lds`, one each).  True where rows that this wave
-// stored are spoilt.
+// stored are spoilt.  Latency bounds it: an FP32 row of 12 heads of 64 over 257 6.6 us, 16 rows over 512 8.8.
 template <typename T, int D, int TM, int WAVES>
 __device__ __forceinline__ bool narrow_unit8(const cf_paged_q8_args_t& a, const PagedPlan& pl, const Q8Divs& dv, uint8_t* lds,
                                              const Unit& un, int kvh, const Work& w) {
@@ -560,6 +566,10 @@ void paged_split8(cf_paged_q8_args_t a, PagedPlan pl, Q8Divs dv) {
 // V_{i-1}.  Turn i of waves 0 .. 3 takes phases 2 i (products) and 2 i + 1, of the others 2 i + 1 and
 // 2 i + 2.  Stage i, which turn i - 2 has left by the end of phase 2 i - 3, is written during the softmax
 // phases before it, 2 i - 1 of waves 0 .. 3 and 2 i - 2 of the others: two stages do.
+// NJ = 2: 2048 rows over 8192, 241 GFLOP in 244 to 254 us (950 to 985 TFLOP/s; a large library product
+// 1144, the same rows over an fp16 cache 254): softmax and products are side by side, and converting
+// adds 16 + 4 instructions a turn to the former's 300.  FP32 (NJ = 1, three products for one): 840 rows
+// of 16 heads of 64 over 300 to 1129 positions 28.2 us, 3 rounds of launch and latency among them.
 template <typename T, int D, int NJ> struct Wide8 {
     static constexpr int TM = 128 * NJ, BK = 64, NS = 2;
     static constexpr int TILE = BK * D, STAGE = 2 * TILE;    // 16-bit numbers
@@ -711,7 +721,7 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
 
         // Fragment x of a turn: x < 2 UT is V^T (32-key step x / UT, dims 16 (x % UT)), the rest K
         // (key tile, then chunk).  They are read kAhead fragments before their products, in
-        // exactly this order.
+        // exactly this order (2048 rows over 8192: 254 us, 8 ahead, which spills, 257).
         constexpr int kAhead = 6, kV = 2 * UT, kAll = kV + 4 * NF;
         auto products = [&](int i, auto first_c, auto last_c) {   // fragments first .. last - 1
             constexpr int first = decltype(first_c)::value, last = decltype(last_c)::value;
@@ -869,14 +879,16 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
     return again_all;
 }
 
-constexpr int kNarrowCost8 = 4;              // blocks of tiles of up to 16 rows that cost a wide tile's one
+// Blocks of tiles of up to 16 rows that cost a wide tile's one (31 decode rows beside 4 chunks of 230 to 517
+// rows: 93 us; with 2 118, with 8 97).
+constexpr int kNarrowCost8 = 4;
 template <typename T, int D, int NJ>
 __global__ __launch_bounds__(512, 2)
 void paged_wide8(cf_paged_q8_args_t a, PagedPlan pl, Q8Divs dv) {
     using W = Wide8<T, D, NJ>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[W::LDS];
     __shared__ int kept[3 * 64];
-    const Geometry<W::TM, 64, kNarrowCost8> geo(a.at, pl, kept);
+    const Geometry<W::TM, 64, kNarrowCost8, true, true> geo(a.at, pl, kept);
     if (geo.lists_cut_tiles()) return;
     for (int unit = (int)blockIdx.x;; unit += pl.step) {
         const int id = fastdiv(unit, pl.by_kv), kvh = unit - id * a.at.H_kv;
@@ -921,7 +933,16 @@ struct Plan8 {
     size_t bytes;         // workspace
 };
 
+// paged_split8 for sequences of up to 1024 positions, which it finishes in one range, as long as its units,
+// a workgroup each, go in one round (us with paged_split8 and paged_heads8: 1 row over 512 7.3 and 10.5, 16
+// over 512 8.8 and 12.9, 32 over 1024 16.7 and 20.2).  Longer ones: 1 over 2048 14.5 and 11.1, 16 over 2048 17.3
+// and 20.1, 16 over 4096 40.9 and 32.2; where one of 16 is that long, only what it takes alone counts.
 constexpr int64_t kSplitLen8 = 1024;
+// Tiles of 256 rows read a block's K and V once for twice the rows, but are twice as long a piece of work.
+// They pay where they fill three quarters of the chip by themselves (4 x 512 rows over 1024: 48 us, with 128
+// rows 58; 2 x 2048 over 4096 212 and 292; 1024 over 1024, half the chip, 44.6 and 32.1), and where long
+// ranges can be cut evenly (512 over 4608: 57 and 104; 4 x 230 over 2430 59.7 and 64; 700 over 1400, not cut,
+// 53.8 and 38.6).
 constexpr int64_t kLongLen8 = 2048;
 
 bool fast_ok8(const cf_paged_q8_args_t& q) {
@@ -953,24 +974,29 @@ Plan8 make_plan8(const cf_paged_attn_args_t& a) {
         p.form = units <= cus && a.max_len <= kSplitLen8 ? kSplit8 : kHeads8;
     } else {
         const int64_t units = (int64_t)a.T * G / 256 * a.H_kv;
-        const bool few_long = a.max_len > kLongLen8 && 2 * (int64_t)a.max_new >= a.T && units >= cus / 8;
+        const bool few_long = a.max_len > kLongLen8 && units >= cus / 8;
         p.form = f16 && (4 * units >= 3 * cus || few_long) ? kWide2x8 : kWide1x8;
     }
     const bool wide = p.form >= kWide1x8;
     const int64_t TM = !wide ? 16 : p.form == kWide2x8 ? 256 : 128;
     const int64_t BK = p.form == kHeads8 ? Narrow8<64>::BK : 64;
     const int64_t tiles = tiles_of(TM);
-    // Units in flight, by the LDS a workgroup takes.
+    // Units of a round: four waves of paged_heads8 a CU (d = 64: eight), though twice as many fit, as ranges
+    // are longer then and records fewer (16 rows over 4096: 32.3 us, with twice as many 33.9; 1 over 16384 17.2
+    // and 22.6).
     const int64_t per_cu = wide ? 1 : a.d == 128 ? 4 : 8;
     const int64_t fill = cus * per_cu > a.H_kv ? cus * per_cu / a.H_kv : 1;
     p.pl.fill = (int32_t)fill;
+    // What is not worth cutting: a merge and the records cost some 5 us, and fp16 wide tiles take 1.5 to 2.2 us
+    // a block (3 x 500 rows of 16 heads of 64 over 1200: 30.8 us, from 8 blocks on into ranges of 4 38.6; FP32
+    // chunks of 129 to 411 rows over 300 to 1129 the other way round, 33 and 28.2).
     p.pl.min_blocks = (int32_t)(wide ? f16 ? 12 : 4 : 64 / BK);
     p.pl.one_blocks = (int32_t)((wide ? f16 ? 1536 : 512 : 128) / BK);
     p.pl.max_records = (int32_t)(4 * fill + 8);
     const bool cut = !a.uncut && p.form != kSplit8 && (a.max_len + BK - 1) / BK > (wide ? kFewOne / BK : p.pl.one_blocks);
     if (!cut) p.pl.one_blocks = INT32_MAX;                    // nor is what is longer than max_len
     p.bytes = cut ? header_bytes(p.pl.max_records) + (size_t)p.pl.max_records * a.H_kv * (TM * (a.d + 2)) * sizeof(float) : 0;
-    int64_t units = (p.form == kHeads8 && cut && tiles <= fill ? fill : tiles + (cut ? 2 * fill : 0)) * a.H_kv;
+    int64_t units = (p.form == kHeads8 && cut && tiles <= fill ? 2 * fill : tiles + (cut ? 2 * fill : 0)) * a.H_kv;
     if (units > (1 << 22)) units = 1 << 22;
     p.wgs = (int)(p.form == kHeads8 ? (units + 3) / 4 : units);
     p.pl.step = p.form == kHeads8 ? 4 * p.wgs : p.wgs;

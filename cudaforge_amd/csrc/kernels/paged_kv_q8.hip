@@ -6,6 +6,9 @@
 // earlier call, then code = x * 2^(127 - p) to the nearest.  Where the power of a begun block grows,
 // its other codes are rounded to the new one: a division by a power of two, so no mantissa changes
 // but of numbers that leave the normal range.
+//
+// HBM bounds it: 8192 rows of 8 heads of 128 fp16, 50 MB, 11.8 us (4.3 TB/s); launch and latency few
+// rows: 16 rows 6.4 us, 3.7 of them the kernel's, 840 FP32 rows of 12 heads of 64 6.3.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -160,17 +160,19 @@ struct Geometry {
         inv_C = 1.0f / C;
         if (pl.one_blocks == INT32_MAX) one = INT32_MAX;
         if constexpr (COUNTS) {
-            // The shortest ranges of which there are no more than `fill`, if they are not much longer than
-            // an equal share (else a few long sequences would wait for ranges of their own).
+            // The shortest ranges that go in one round of `fill` units (narrow ones as parts of one), if they
+            // are not much longer than an equal share: else a few long sequences would wait for ranges
+            // of their own.
             if (!plans || a.B > 64 || t > fill) return;
-            const float share = fmaxf(wave_sum(cost(first)) / fill, (float)pl.min_blocks), was = C;
+            const float least = (float)(few ? kFewMin : pl.min_blocks), by_fill = 1.0f / fill, was = C;
+            const float share = fmaxf(wave_sum(cost(first)) * by_fill, least);
             C = ceilf(share);
-            for (int i = 0; i < 8; i++) {
-                inv_C = 1.0f / C;
-                const float units = wave_sum((float)(tiles(first) * ranges(first)));
+            for (int i = 0; i < 3 && C <= 1.5f * share + 1.0f; i++) {
+                inv_C = __builtin_amdgcn_rcpf(C);
+                const float own = (float)(tiles(first) * ranges(first));
+                const float units = wave_sum(narrow(first) ? fminf(cost(first) * inv_C, own) : own);
                 if (units <= fill) return;
-                C = fmaxf(C + 1.0f, ceilf(C * (units / fill)));
-                if (C > 1.5f * share + 1.0f) break;
+                C = fmaxf(C + 1.0f, ceilf(C * units * by_fill));
             }
             C = was;
             inv_C = 1.0f / C;
