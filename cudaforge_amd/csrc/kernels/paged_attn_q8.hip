@@ -39,7 +39,8 @@ __device__ __forceinline__ void plain_row_q8(const cf_paged_q8_args_t& a, const 
     const uint8_t* const k = (const uint8_t*)a.at.k + (int64_t)kvh * a.at.head_stride;
     const uint8_t* const v = (const uint8_t*)a.at.v + (int64_t)kvh * a.at.head_stride;
     const float c = a.at.scale * kLog2e;
-    float m = -INFINITY, l = 0.0f, acc[DIMS];
+    float m = -INFINITY, acc[DIMS];
+    LongSum l_run;
 #pragma unroll
     for (int i = 0; i < DIMS; i++) acc[i] = 0.0f;
 #pragma clang loop unroll(disable)
@@ -65,9 +66,13 @@ __device__ __forceinline__ void plain_row_q8(const cf_paged_q8_args_t& a, const 
         const float m_use = m_new == -INFINITY ? 0.0f : m_new;
         const float alpha = exp2f(m - m_use), p = exp2f(x - m_use);
         m = m_new;
-        l = l * alpha + wave_sum(p);
+        l_run.scale(alpha);
+        l_run.add(wave_sum(p));
+        // Codes are few different numbers, so that roundings of a long sum would lean one way: 64
+        // positions' by themselves first.
+        float part[DIMS];
 #pragma unroll
-        for (int i = 0; i < DIMS; i++) acc[i] *= alpha;
+        for (int i = 0; i < DIMS; i++) part[i] = 0.0f;
 #pragma clang loop unroll(disable)
         for (int j = 0; j < min(64, seen - k0); j++) {
             const float pj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(p), j));
@@ -78,9 +83,12 @@ __device__ __forceinline__ void plain_row_q8(const cf_paged_q8_args_t& a, const 
 #pragma unroll
             for (int i = 0; i < DIMS; i++)
                 if (lane + 64 * i < d)
-                    acc[i] = __builtin_fmaf(pj, codes_f32<false>(v[row + lane + 64 * i], power)[0], acc[i]);
+                    part[i] = __builtin_fmaf(pj, codes_f32<false>(v[row + lane + 64 * i], power)[0], part[i]);
         }
+#pragma unroll
+        for (int i = 0; i < DIMS; i++) acc[i] = __builtin_fmaf(acc[i], alpha, part[i]);
     }
+    const float l = l_run.sum();
     if (rec) {
         if (lane == 0) {
             rec[0] = m;
@@ -443,9 +451,8 @@ __device__ __forceinline__ void narrow_range8(const cf_paged_q8_args_t& a, const
 // A wave per unit, the units of neighbouring KV heads in one workgroup: they read the same
 // cache rows at about the same time.  HBM bounds it: 64 rows over 4096 each, 537 MB, 101 us (5.3 TB/s);
 // 16 rows over 1778 to 4096 positions, 114 MB, 29.2 us, 4 of them the merge's and 3 until the first
-// codes are there (launch, lengths, table, powers).  Two stages of a ring: with 3 or 4 the same 16 rows
-// take 30.0 and 32.7, as fewer workgroups fit a CU; a K part filled again before its V is used, 30.6; the
-// powers by DMA beside the first codes, 29.1, and 0.3 more where a wave has one or two blocks.
+// codes are there (launch, lengths, table, powers).  Two stages of a ring: with 3 the same 16 rows take
+// 30.0, with 4, which leave room for one workgroup a CU, 32.7.
 template <int D> struct Heads8 {
     static constexpr int WAVES = 4, NS = 2;
     static constexpr int RING = Narrow8<D, NS>::RING;
@@ -880,7 +887,7 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
 }
 
 // Blocks of tiles of up to 16 rows that cost a wide tile's one (31 decode rows beside 4 chunks of 230 to 517
-// rows: 93 us; with 2 118, with 8 97).
+// rows: 93 us; with 2 118).
 constexpr int kNarrowCost8 = 4;
 template <typename T, int D, int NJ>
 __global__ __launch_bounds__(512, 2)

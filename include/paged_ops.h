@@ -153,7 +153,7 @@ int mha_paged_attn_f16_cuda(const void* inputs[], void* outputs[], const operato
  * (255: NaN).  Layouts: K and V pages (num_pages, page_size, H_kv, d) bytes, K and V powers
  * (num_pages, page_size / B, H_kv) bytes; 1 + 1 / (B d) bytes a value.  The steps, tables, slots
  * and lengths are those above; kv_page_map serves both.  A power of two instead of any scale: taking
- * a larger one later changes no number's mantissa, and fp16 and bf16 hold the values exactly. */
+ * a larger one later leaves the numbers' mantissas alone, and fp16 and bf16 hold the values exactly. */
 
 typedef struct {
     int64_t num_tokens;    /* T */
@@ -194,10 +194,13 @@ typedef struct {
  *          K_powers, V_powers]
  * outputs [O (T, H_q, d)]
  * mha_paged_attn's rules, on the values that the bytes stand for; Q and O are of the operator's type.
- * f16: values are taken as fp16 (exact for what kv_page_store_q8_f16 stores; past its range infinite,
- * below it rounded); f32: as bf16, exact down to 2^-133.  d = 64 and 128 with blocks of a multiple of
- * 16 positions, 16-byte aligned pages, strides, Q and O, scale > 0 and at most 32768 sequences run on
- * the matrix cores, every other call on a plain kernel. */
+ * f16: values are taken as fp16, which is exact for what kv_page_store_q8_f16 stores; past fp16's range
+ * they may count as infinite.  f32: as bf16, exact but for values below 2^-126, with Q and the weights as
+ * sums of three bf16 numbers each, which are FP32's 24 bits (Q below 3.38e38).  A NaN V touches the rows
+ * that see it; rows that do not, though a later token of the same call does, are computed again by a slow
+ * loop.  d = 64 and 128 with blocks of a multiple of 16 positions, 16-byte aligned pointers (the powers'
+ * apart) and strides, scale > 0 and at most 32768 sequences run on the matrix cores, every other
+ * call on a plain kernel. */
 int mha_paged_attn_q8_f32_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
 int mha_paged_attn_q8_f16_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
 
