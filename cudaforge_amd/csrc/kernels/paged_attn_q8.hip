@@ -124,14 +124,18 @@ template <> struct Parts<float> {
     typedef __bf16 half_t;
     static constexpr int Q = 3, P = 3;
 };
-// x as the sum of N numbers of B, part by part into element e of `to`.
+// x and y as sums of N numbers of B, part by part into elements e and e + 1 of `to`.  Two by two, as the
+// converting instruction takes them (FP32 chunk below: 27.0 us, one at a time 28.3).
 template <int N, typename B, typename V>
-__device__ __forceinline__ void split_into(V (&to)[N], int e, float x) {
+__device__ __forceinline__ void split_into(V (&to)[N], int e, float x, float y) {
+    typedef B two_t __attribute__((ext_vector_type(2)));
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const B y = (B)x;
-        to[i][e] = y;
-        x -= (float)y;
+        const two_t b = __builtin_convertvector(f2_t{x, y}, two_t);
+        to[i][e] = b[0];
+        to[i][e + 1] = b[1];
+        x -= (float)b[0];
+        y -= (float)b[1];
     }
 }
 
@@ -354,9 +358,13 @@ __device__ __forceinline__ void narrow_range8(const cf_paged_q8_args_t& a, const
 #pragma unroll
     for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            if constexpr (QP == 1) qf[ks][0][e] = q[ks][e];
-            else split_into<QP, B>(qf[ks], e, (float)q[ks][e]);
+        for (int e = 0; e < 8; e += 2) {
+            if constexpr (QP == 1) {
+                qf[ks][0][e] = q[ks][e];
+                qf[ks][0][e + 1] = q[ks][e + 1];
+            } else {
+                split_into<QP, B>(qf[ks], e, q[ks][e], q[ks][e + 1]);
+            }
         }
     wait_lds_reads();                                         // what the ring held before
     static_for<NS - 1>([&](auto i) {
@@ -426,10 +434,12 @@ __device__ __forceinline__ void narrow_range8(const cf_paged_q8_args_t& a, const
 #pragma unroll
         for (int t = 0; t < NG; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], c, -m_use));
-                l_blk += p;
-                split_into<PP, B>(pf[t / 2], 4 * (t & 1) + i, p);
+            for (int i = 0; i < 4; i += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], c, -m_use));
+                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i + 1], c, -m_use));
+                l_blk += p0;
+                l_blk += p1;
+                split_into<PP, B>(pf[t / 2], 4 * (t & 1) + i, p0, p1);
             }
         l.add(l_blk);
 #pragma unroll
@@ -576,7 +586,7 @@ void paged_split8(cf_paged_q8_args_t a, PagedPlan pl, Q8Divs dv) {
 // NJ = 2: 2048 rows over 8192, 241 GFLOP in 244 to 254 us (950 to 985 TFLOP/s; a large library product
 // 1144, the same rows over an fp16 cache 254): softmax and products are side by side, and converting
 // adds 16 + 4 instructions a turn to the former's 300.  FP32 (NJ = 1, three products for one): 840 rows
-// of 16 heads of 64 over 300 to 1129 positions 28.2 us, 3 rounds of launch and latency among them.
+// of 16 heads of 64 over 300 to 1129 positions 27.0 us, 3 rounds of launch and latency among them.
 template <typename T, int D, int NJ> struct Wide8 {
     static constexpr int TM = 128 * NJ, BK = 64, NS = 2;
     static constexpr int TILE = BK * D, STAGE = 2 * TILE;    // 16-bit numbers
@@ -712,8 +722,10 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
                     qf[j][f][0] = *(const eight_t*)(q + 8 * ((4 * f + lq) ^ (lr & 7)));
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        split_into<QP, B>(qf[j][f], e, q[4 * ((8 * f + 2 * lq + e / 4) ^ (lr & 7)) + e % 4]);
+                    for (int e = 0; e < 8; e += 2) {
+                        const T* const x = q + 4 * ((8 * f + 2 * lq + e / 4) ^ (lr & 7)) + e % 4;
+                        split_into<QP, B>(qf[j][f], e, x[0], x[1]);
+                    }
                 }
             }
         }
@@ -820,10 +832,16 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
 #pragma unroll
                 for (int t = 0; t < 4; t++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][t][e], c, -m_use));
-                        if constexpr (!F16) l_blk += p;
-                        split_into<PP, B>(pf[j][t >> 1], (t & 1) * 4 + e, p);
+                    for (int e = 0; e < 4; e += 2) {
+                        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][t][e], c, -m_use));
+                        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][t][e + 1], c, -m_use));
+                        if constexpr (F16) {
+                            pf[j][t >> 1][0][(t & 1) * 4 + e] = (B)p0;
+                            pf[j][t >> 1][0][(t & 1) * 4 + e + 1] = (B)p1;
+                        } else {
+                            l_blk += p0 + p1;
+                            split_into<PP, B>(pf[j][t >> 1], (t & 1) * 4 + e, p0, p1);
+                        }
                     }
                 if constexpr (!F16) l_run[j].add(l_blk);
             }
@@ -996,7 +1014,7 @@ Plan8 make_plan8(const cf_paged_attn_args_t& a) {
     p.pl.fill = (int32_t)fill;
     // What is not worth cutting: a merge and the records cost some 5 us, and fp16 wide tiles take 1.5 to 2.2 us
     // a block (3 x 500 rows of 16 heads of 64 over 1200: 30.8 us, from 8 blocks on into ranges of 4 38.6; FP32
-    // chunks of 129 to 411 rows over 300 to 1129 the other way round, 33 and 28.2).
+    // chunks of 129 to 411 rows over 300 to 1129 the other way round, 37 and 27).
     p.pl.min_blocks = (int32_t)(wide ? f16 ? 12 : 4 : 64 / BK);
     p.pl.one_blocks = (int32_t)((wide ? f16 ? 1536 : 512 : 128) / BK);
     p.pl.max_records = (int32_t)(4 * fill + 8);
