@@ -8,7 +8,7 @@
 // but of numbers that leave the normal range.
 //
 // HBM bounds it: 8192 rows of 8 heads of 128 fp16, 50 MB, 11.8 us (4.3 TB/s); launch and latency few
-// rows: 16 rows 6.4 us, 3.7 of them the kernel's, 840 FP32 rows of 12 heads of 64 6.3.
+// rows: 16 rows 6.3 us a call, 3.8 of them the kernel's, 840 FP32 rows of 12 heads of 64 6.3 and 5.3.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -64,10 +64,10 @@ __device__ __forceinline__ float finite_size(float x) {
     return s < INFINITY ? s : 0.0f;
 }
 
-// A wave's run: rows t .. t + len - 1, whose slots the lanes first .. first + len - 1 hold.
+// A wave's run: rows t .. t + len - 1, whose slots the lanes 0 .. len - 1 hold.
 struct Run {
     int64_t t;
-    int first, len;
+    int len;
     uint8_t* cells;        // the block's first position
     int slot0;             // ... and its slot
 };
@@ -108,7 +108,7 @@ __device__ __forceinline__ void store_run(const cf_page_store_q8_args_t& a, cons
             }
     }
     const int need = power_for(wave_max(most));
-    const bool mine = lane >= run.first && lane < run.first + run.len;
+    const bool mine = lane < run.len;
     const bool begun = __builtin_amdgcn_ballot_w64(mine && slot == run.slot0) != 0;
     const int now = begun ? need : max(old, need);
     if (lane == 0) *power = (uint8_t)now;
@@ -143,7 +143,7 @@ __device__ __forceinline__ void store_run(const cf_page_store_q8_args_t& a, cons
     }
     // Where no code can pass 448 or the type's largest number, as almost always, one instruction does.
     const float limit = fminf(448.0f, ldexpf(kMostStored<T>, 127 - now)), over = power_bits(now);
-    auto place = [&](int r) { return run.cells + (int64_t)(__shfl(slot, run.first + min(r, run.len - 1)) - run.slot0) * a.row_stride; };
+    auto place = [&](int r) { return run.cells + (int64_t)(__shfl(slot, min(r, run.len - 1)) - run.slot0) * a.row_stride; };
     auto put = [&](int r, uint8_t* cell, const pack_t& x) {
         if (r >= run.len) return;
         if constexpr (WIDE) {
@@ -176,38 +176,39 @@ __device__ __forceinline__ void store_run(const cf_page_store_q8_args_t& a, cons
     }
 }
 
-// Workgroup (x, y): the runs that begin in rows R x .. R x + R - 1, of heads 4 y .. 4 y + 3 of K's
-// and V's, a wave each, whose lanes hold the slots of 64 rows.
-constexpr int kStoreWaves = 4;
+// Workgroup (x, y): of the runs that begin in its 64 rows every 2^log_per-th, of heads 4 y .. 4 y + 3 of
+// K's and V's, a wave each.  Which workgroup takes the first goes round with the rows: workgroups at a
+// distance of a power of two share an XCD, or a part of one, and so would a long sequence's runs (8192 rows
+// of 4, blocks of 64: 15.2 us, 29 without; 2048 of one 9.2 and 16.6).
+constexpr int kStoreWaves = 4, kStoreRows = 64;
 template <typename T, int VEC, int KEEP>
 __global__ __launch_bounds__(64 * kStoreWaves)
-void page_store_q8(cf_page_store_q8_args_t a, StoreDivs dv, int R, int64_t row0) {
+void page_store_q8(cf_page_store_q8_args_t a, StoreDivs dv, int log_per, int64_t row0) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int unit = (int)blockIdx.y * kStoreWaves + wave;
     if (unit >= 2 * a.H_kv) return;
     const int which = unit >= a.H_kv, h = unit - (which ? a.H_kv : 0);
-    const int64_t t0 = row0 + (int64_t)blockIdx.x * R;
-    const int slot = t0 + lane < a.T ? a.slots[t0 + lane] : -1;
-    const int last = t0 > 0 ? a.slots[t0 - 1] : -1;
+    const int part = (int)blockIdx.x >> log_per, sub = (int)blockIdx.x & ((1 << log_per) - 1);
+    const int64_t t0 = row0 + (int64_t)part * kStoreRows;
+    auto slot_at = [&](int64_t t) { return t >= 0 && t < a.T ? a.slots[t] : -1; };
+    const int slot = slot_at(t0 + lane), next = slot_at(t0 + kStoreRows + lane), last = slot_at(t0 - 1);
     auto block_of = [&](int s) { return (unsigned)s < (unsigned)a.num_slots ? fastdiv(s, dv.block) : -1; };
     const int block = block_of(slot);
     const int up = __shfl_up(block, 1), before = lane == 0 ? block_of(last) : up;
-    uint64_t heads = __builtin_amdgcn_ballot_w64(lane < R && block >= 0 && block != before);
+    const uint64_t all = __builtin_amdgcn_ballot_w64(block >= 0 && block != before);
+    const int rank = __builtin_popcountll(all & ((1ull << lane) - 1));
+    uint64_t heads = __builtin_amdgcn_ballot_w64((all >> lane & 1) && ((rank + part + (part >> 2) - sub) & ((1 << log_per) - 1)) == 0);
     const T* const rows = (const T*)(which ? a.v : a.k) + (int64_t)h * a.d;
     uint8_t* const pages = which ? a.v_pages : a.k_pages;
     uint8_t* const powers = which ? a.v_scales : a.k_scales;
     for (; heads; heads &= heads - 1) {
+        const int first = __builtin_ctzll(heads);
+        const int b = __builtin_amdgcn_readlane(block, first);
+        const int here = __shfl(slot, (first + lane) & 63), behind = __shfl(next, (first + lane) & 63);
+        const int its_slot = first + lane < 64 ? here : behind;
+        const uint64_t same = __builtin_amdgcn_ballot_w64(block_of(its_slot) == b);
         Run run;
-        run.first = __builtin_ctzll(heads);
-        const int b = __builtin_amdgcn_readlane(block, run.first);
-        run.t = t0 + run.first;
-        int its_slot = slot;
-        uint64_t same = __builtin_amdgcn_ballot_w64(block == b) >> run.first;
-        if (run.first + a.block > 64) {            // it may go on behind the 64
-            its_slot = run.t + lane < a.T ? a.slots[run.t + lane] : -1;
-            same = __builtin_amdgcn_ballot_w64(block_of(its_slot) == b);
-            run.first = 0;
-        }
+        run.t = t0 + first;
         run.len = ~same ? __builtin_ctzll(~same) : 64;
         run.slot0 = b * a.block;
         const int page = fastdiv(b, dv.blocks);
@@ -226,19 +227,21 @@ int launch_store(const cf_page_store_q8_args_t& a, hipStream_t st) {
     const int per_row = a.d / kWide;
     const bool wide = in % 16 == 0 && out % kWide == 0 && a.d % kWide == 0 && per_row <= 64 && (per_row & (per_row - 1)) == 0;
     const StoreDivs dv = {fastdiv_make(a.block), fastdiv_make(a.page_size / a.block)};
-    // Few rows of a workgroup cost launches of workgroups that find no run, many cost turns where each is a
-    // run of its own (8 heads of 128 fp16, us with 1, 4, 8 and 16 rows: 256 sequences of one row 6.0, 6.2, 9.8
-    // and 17.1; 840 rows of 3 sequences, blocks of 32, 8.8, 5.9, 6.4 and 6.4; 2048 rows of 2 23.9, 9.5, 6.6
-    // and 6.4; 8192 rows of 4 49.1, 19.9, 13.3 and 11.8).
-    const int R = a.T < 1536 ? 4 : a.T < 4096 ? 8 : 16;
     const unsigned parts = (unsigned)((2 * (int64_t)a.H_kv + kStoreWaves - 1) / kStoreWaves);
-    constexpr int64_t kMost = 1 << 23;             // rows of a launch: a grid has less than 2^32 threads
-    for (int64_t t0 = 0; t0 < a.T; t0 += kMost * R) {
-        const int64_t n = (a.T - t0 + R - 1) / R;
-        const dim3 grid((unsigned)(n < kMost ? n : kMost), parts), block(64 * kStoreWaves);
-        if (wide && a.block * per_row <= 8 * 64) hipLaunchKernelGGL((page_store_q8<T, kWide, 8>), grid, block, 0, st, a, dv, R, t0);
-        else if (wide) hipLaunchKernelGGL((page_store_q8<T, kWide, 16>), grid, block, 0, st, a, dv, R, t0);
-        else hipLaunchKernelGGL((page_store_q8<T, 1, 1>), grid, block, 0, st, a, dv, R, t0);
+    // Each run that a wave takes costs it 1 us, one after the other, and workgroups that find none a little
+    // too: for few rows a workgroup for each, for more as few as keep a thousand, at least two (8 heads of 128
+    // fp16, us of the kernel with at most 640, 1024 and 1536: 1024 sequences of one row 12.2, 9.8, 9.8; 1000
+    // rows of 2 sequences 5.0, 5.8, 5.8; 300 rows of one 4.9, 5.0, 5.5.  8192 rows of 4 with two 11.7, with
+    // four 13.0).
+    int log_per = 6;
+    while (log_per > 1 && ((int64_t)a.T * parts << log_per) > kStoreRows * 1024) log_per--;
+    constexpr int64_t kMost = 1 << 17;             // parts of 64 rows of a launch: a grid has less than 2^32 threads
+    for (int64_t t0 = 0; t0 < a.T; t0 += kMost * kStoreRows) {
+        const int64_t n = (a.T - t0 + kStoreRows - 1) / kStoreRows;
+        const dim3 grid((unsigned)((n < kMost ? n : kMost) << log_per), parts), block(64 * kStoreWaves);
+        if (wide && a.block * per_row <= 8 * 64) hipLaunchKernelGGL((page_store_q8<T, kWide, 8>), grid, block, 0, st, a, dv, log_per, t0);
+        else if (wide) hipLaunchKernelGGL((page_store_q8<T, kWide, 16>), grid, block, 0, st, a, dv, log_per, t0);
+        else hipLaunchKernelGGL((page_store_q8<T, 1, 1>), grid, block, 0, st, a, dv, log_per, t0);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return (int)e;
     }
