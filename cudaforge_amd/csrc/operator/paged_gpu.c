@@ -230,6 +230,11 @@ static int page_store_q8_op(int elem, const void* inputs[], void* outputs[], con
     if (cache_strides(p->page_stride, p->row_stride, p->head_stride, p->page_size, p->num_kv_heads, p->head_dim, &cs) != 0)
         return -1;
     if (p->num_tokens == 0) return 0;
+    /* Each array is written by waves of its own. */
+    for (int i = 0; i < 4; i++) {
+        for (int j = 0; j < i; j++) if (outputs[i] == outputs[j]) return -1;
+        for (int j = 0; j < 3; j++) if (outputs[i] == inputs[j]) return -1;
+    }
     cf_page_store_q8_args_t a;
     memset(&a, 0, sizeof(a));
     a.k = inputs[0];

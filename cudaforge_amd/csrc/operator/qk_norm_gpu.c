@@ -79,6 +79,8 @@ static int qk_norm_rope_op(int elem, const void* inputs[], void* outputs[], cons
         if (p->norm >= 1) x->gain = inputs[3 + i];
         if (p->norm == 2) x->bias = inputs[5 + i];
     }
+    /* Rows of Q and of K are written while others of both are still to be read. */
+    if (heads[0] && heads[1] && (outputs[0] == outputs[1] || outputs[0] == inputs[1] || outputs[1] == inputs[0])) return -1;
     if (p->rope_base > 0.0f) {
         if ((r & 1) || r > d || r > QK_ROPE_MAX_DIM || !inputs[2]) return -1;
         if (fill_turns(p, r, a.turns) != 0) return -1;

@@ -176,7 +176,8 @@ typedef struct {
  * rounding would pass the type's largest number, as 65504 to 65536, the one below is stored, so that
  * what is read back stays finite.  A row with an invalid slot is not stored.  Rows for one block follow
  * each other, in any order, as kv_page_map gives them, and each slot may be given once per
- * call: otherwise that block's numbers and powers mean nothing. */
+ * call: otherwise that block's numbers and powers mean nothing.  Seven arrays of their own (-1 where
+ * an output is another array). */
 int kv_page_store_q8_f32_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
 int kv_page_store_q8_f16_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
 

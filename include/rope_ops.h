@@ -89,8 +89,10 @@ typedef struct {
  * Without rotation positions may be NULL; with it a row of a negative position is left alone in both
  * outputs.  Gains are read with norm 1 and 2 and biases with norm 2 only; NULL stands for ones and
  * zeros (the slots have to be there).  An output may be its input (with one stride, else -1); other
- * overlaps are not allowed.  d = 64, 128, 256 and other sizes whose row is 2^k pairs of 16-byte pieces
- * take the wide kernel where every pointer and stride is a multiple of 16 bytes. */
+ * overlaps are not allowed (-1 where the other's input or output is named).  Where every pointer and
+ * stride is a multiple of 16 bytes, d one of 32 and at most 2048 bytes, and what turns together (r
+ * values, half of them with `halves`) one of 16 bytes, a row's pieces of 16 bytes go at once; other calls take a
+ * plain kernel. */
 int qk_norm_rope_f32_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
 int qk_norm_rope_f16_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
 

@@ -188,6 +188,16 @@ def test_store_refuses_missing_arrays(native, op):
     assert _call(native, op, [DP] * 3, [DP] * 4, cf.KvPageStoreQ8Params(**dict(STORE_OK, num_tokens=0))) == 0
 
 
+@pytest.mark.parametrize("op", STORES)
+def test_store_refuses_arrays_given_twice(native, op):
+    p, arrays = cf.KvPageStoreQ8Params(**STORE_OK), [DP + 64 * i for i in range(7)]
+    for i in range(3, 7):
+        for j in range(7):
+            if i != j:
+                names = [arrays[j] if k == i else x for k, x in enumerate(arrays)]
+                assert _call(native, op, names[:3], names[3:], p) == -1
+
+
 @pytest.mark.parametrize("change", [
     dict(batch_size=-1), dict(num_tokens=-1), dict(num_heads=0), dict(num_kv_heads=3), dict(head_dim=0), dict(head_dim=513),
     dict(page_size=0), dict(num_pages=0), dict(max_pages=0), dict(num_pages=1 << 27), dict(max_pages=1 << 27),

@@ -180,6 +180,13 @@ def test_refuses_missing_arrays(native, op):
                  cf.QkNormRopeParams(**dict(OK, num_tokens=0, num_heads=0, rope_base=0.0, rotary_dim=0))) == 0
 
 
+@pytest.mark.parametrize("op", OPS)
+def test_refuses_the_others_array(native, op):
+    ins, outs, p = [DP + 64 * i for i in range(7)], [DP + 1024, DP + 2048], cf.QkNormRopeParams(**OK)
+    for pair in ([outs[0], outs[0]], [ins[1], outs[1]], [outs[0], ins[0]], [ins[1], ins[0]]):
+        assert _call(native, op, ins, pair, p) == -1
+
+
 def test_layout(native):
     assert ctypes.sizeof(cf.QkNormRopeParams) == 112
     for op in OPS:
