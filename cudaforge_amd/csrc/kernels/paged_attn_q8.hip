@@ -912,7 +912,7 @@ __global__ __launch_bounds__(512, 2)
 void paged_wide8(cf_paged_q8_args_t a, PagedPlan pl, Q8Divs dv) {
     using W = Wide8<T, D, NJ>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[W::LDS];
-    __shared__ int kept[3 * 64];
+    __shared__ int kept[4 * 64];
     const Geometry<W::TM, 64, kNarrowCost8, true, true> geo(a.at, pl, kept);
     if (geo.lists_cut_tiles()) return;
     for (int unit = (int)blockIdx.x;; unit += pl.step) {

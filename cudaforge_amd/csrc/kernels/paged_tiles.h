@@ -90,7 +90,8 @@ struct Unit {
 
 // The tiles' geometry, one sequence per lane and 64 at a time.  TM rows per tile, BK
 // positions per key block; a tile of up to 16 rows costs 1 / NARROW of a full one's block.
-// CUTS: tiles may be cut.  COUNTS: ranges of few sequences are counted, so that they go in one round.
+// CUTS: tiles may be cut.  COUNTS: ranges of few sequences are counted, so that they go
+// in one round, and where that can't be those of wide tiles are ordered.
 template <int TM, int BK, int NARROW, bool CUTS = true, bool COUNTS = false>
 struct Geometry {
     const cf_paged_attn_args_t& a;
@@ -108,6 +109,7 @@ struct Geometry {
     // Sequences base + lane, base + 64 + lane, ..: the loads of four wait together (1024 sequences
     // of 128 positions: 154 us, one at a time 192).
     static constexpr int kAtOnce = 4;
+    static constexpr bool ORDERS = COUNTS && NARROW > 1;
     __device__ __forceinline__ void next_rows(int base, SeqRows (&s)[kAtOnce]) const {
 #pragma unroll
         for (int j = 0; j < kAtOnce; j++) s[j] = rows(base + 64 * j + lane);
@@ -160,23 +162,52 @@ struct Geometry {
         inv_C = 1.0f / C;
         if (pl.one_blocks == INT32_MAX) one = INT32_MAX;
         if constexpr (COUNTS) {
-            // The shortest ranges that go in one round of `fill` units (narrow ones as parts of one), if they
-            // are not much longer than an equal share: else a few long sequences would wait for ranges
-            // of their own.
-            if (!plans || a.B > 64 || t > fill) return;
-            const float least = (float)(few ? kFewMin : pl.min_blocks), by_fill = 1.0f / fill, was = C;
-            const float share = fmaxf(wave_sum(cost(first)) * by_fill, least);
-            C = ceilf(share);
-            for (int i = 0; i < 3 && C <= 1.5f * share + 1.0f; i++) {
-                inv_C = __builtin_amdgcn_rcpf(C);
-                const float own = (float)(tiles(first) * ranges(first));
-                const float units = wave_sum(narrow(first) ? fminf(cost(first) * inv_C, own) : own);
-                if (units <= fill) return;
-                C = fmaxf(C + 1.0f, ceilf(C * units * by_fill));
+            int one_round = 0;
+            if (plans && a.B <= 64 && t <= fill) one_round = count_ranges(few);
+            if constexpr (ORDERS) {
+                one_round &= __builtin_amdgcn_ballot_w64(narrow(first)) == 0;
+                int before = -1;
+                if (a.B <= 64 && !__builtin_amdgcn_readfirstlane(one_round)) before = in_order();
+                kept[192 + lane] = before;       // once: other waves, with the same values, may be ahead
             }
-            C = was;
-            inv_C = 1.0f / C;
         }
+    }
+    // COUNTS: the shortest ranges that go in one round of `fill` units (narrow ones as parts of one), if they
+    // are not much longer than an equal share: else a few long sequences would wait for ranges
+    // of their own.
+    __device__ __forceinline__ bool count_ranges(bool few) {
+        const float fill = (float)pl.fill;
+        const float least = (float)(few ? kFewMin : pl.min_blocks), by_fill = 1.0f / fill, was = C;
+        const float share = fmaxf(wave_sum(cost(first)) * by_fill, least);
+        C = ceilf(share);
+        for (int i = 0; i < 3 && C <= 1.5f * share + 1.0f; i++) {
+            inv_C = __builtin_amdgcn_rcpf(C);
+            const float own = (float)(tiles(first) * ranges(first));
+            const float units = wave_sum(narrow(first) ? fminf(cost(first) * inv_C, own) : own);
+            if (units <= fill) return true;
+            C = fmaxf(C + 1.0f, ceilf(C * units * by_fill));
+        }
+        C = was;
+        inv_C = 1.0f / C;
+        return false;
+    }
+    // ORDERS: what goes before each sequence's units, the longest ranges first.  Narrow tiles as if they took
+    // longer than they do, so that they are spread: all of them at once wait for memory, between wide
+    // ones they wait beside products (us of 31 decode rows with 4 chunks, of 40 with 3, of 56 with 8, and of
+    // the 4 chunks alone: 92.5, 58, 114, 77; with a quarter 100, 59, 116, 78, with half 92.5, 66, 114, 78; in the
+    // order of the sequences, what is less than half of C last, 92.5, 72, 122, 88).
+    static constexpr float kNarrowFirst = 1.0f / 3.0f;
+    __device__ __forceinline__ int in_order() const {
+        const int items = tiles(first) * ranges(first);
+        const float x = narrow(first) ? (float)blocks(first) * kNarrowFirst : (float)blocks(first);
+        const int key = (__float_as_int(x * __builtin_amdgcn_rcpf((float)ranges(first))) & ~63) | (63 - lane);
+        int before = 0;
+#pragma clang loop unroll(disable)
+        for (int j = 0; j < min(a.B, 64); j++) {
+            const int n = __builtin_amdgcn_readlane(items, j);
+            before += __builtin_amdgcn_readlane(key, j) > key ? n : 0;
+        }
+        return before;
     }
     // True for the workgroup behind the units', which lists the cut tiles.
     __device__ __forceinline__ bool lists_cut_tiles() const {
@@ -198,17 +229,19 @@ struct Geometry {
     // Unit u; false where there is none.
     __device__ __forceinline__ bool find(int u, Unit& out) const {
         int items0 = 0;
+        const int first_unit = ORDERS ? kept[192 + lane] : -1;
+        const bool ordered = ORDERS && __builtin_amdgcn_readfirstlane(first_unit) >= 0;
         // Wide tiles: the sequences with the long ranges first, so that short pieces fill the end
         // (35 sequences, 4 of them chunks: 108 us, in the order of the sequences 131).
         constexpr int CLASSES = NARROW > 1 ? 2 : 1;
-        for (int cls = 0; cls < CLASSES; cls++) {
+        for (int cls = 0; cls < (ordered ? 1 : CLASSES); cls++) {
             int records0 = 0;
             auto scan = [&](const SeqRows& s, int base) {
                 const int t = tiles(s), ns = ranges(s), rec = ns > 1 ? t * ns : 0;
                 const bool cut = __builtin_amdgcn_ballot_w64(ns > 1) != 0;
                 int items = t * ns;
-                if (CLASSES > 1 && (2.0f * (float)blocks(s) > C * (float)ns ? 0 : 1) != cls) items = 0;
-                const int before = items0 + wave_excl_sum(items, lane);
+                if (CLASSES > 1 && !ordered && (2.0f * (float)blocks(s) > C * (float)ns ? 0 : 1) != cls) items = 0;
+                const int before = ordered ? first_unit : items0 + wave_excl_sum(items, lane);
                 const int rec_before = records0 + (cut ? wave_excl_sum(rec, lane) : 0);
                 const unsigned long long hit = __ballot(before <= u && u < before + items);
                 if (!hit) {
