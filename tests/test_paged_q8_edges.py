@@ -289,6 +289,19 @@ def test_many_uneven_sequences(gpu, f16):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("H,H_kv", [(32, 32), (16, 2)])
+@pytest.mark.parametrize("B", [7, 64])
+def test_more_units_than_go_in_one_round(gpu, f16, H, H_kv, B):
+    """Up to 64 sequences of every kind, whose ranges the tiles take by their length: chunks of one tile and of
+    several, single rows, empty ones, equal lengths."""
+    new = [300, 1, 40, 0, 129, 1, 257] + [1, 1, 20, 0, 1, 33, 1] * 8 + [64]
+    past = [500, 900, 0, 300, 1500, 0, 2] + [200, 63, 64, 5, 200, 31, 700] * 8 + [0]
+    c = PagedQ8(new[:B], past[:B], H, H_kv, 64, 32, f16, seed=43)
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f16", [False, True])
 def test_store_again_changes_nothing(gpu, f16):
     """The same rows to the same slots once more: a power that has grown stays, and so do all bits."""
     s = Store(f16, 4, 64, 32, 16, 20, seed=21)
