@@ -583,10 +583,13 @@ void paged_split8(cf_paged_q8_args_t a, PagedPlan pl, Q8Divs dv) {
 // V_{i-1}.  Turn i of waves 0 .. 3 takes phases 2 i (products) and 2 i + 1, of the others 2 i + 1 and
 // 2 i + 2.  Stage i, which turn i - 2 has left by the end of phase 2 i - 3, is written during the softmax
 // phases before it, 2 i - 1 of waves 0 .. 3 and 2 i - 2 of the others: two stages do.
-// NJ = 2: 2048 rows over 8192, 241 GFLOP in 244 to 254 us (950 to 985 TFLOP/s; a large library product
-// 1144, the same rows over an fp16 cache 254): softmax and products are side by side, and converting
-// adds 16 + 4 instructions a turn to the former's 300.  FP32 (NJ = 1, three products for one): 840 rows
-// of 16 heads of 64 over 300 to 1129 positions 27.0 us, 3 rounds of launch and latency among them.
+// The weights of V in two fp16 parts (FP32 rows: three of bf16), so that their rounding leaves the result.  In
+// one part they cost half of the products with V, but the result is then off by 2.3e-4 of its size in the root
+// mean square over 8192 positions and 2.8e-4 over 742 to 2717, so 2.07e-4 in two, which is its own rounding,
+// and which rows that meets depends on how the whole batch is cut.
+// NJ = 2: 2048 rows over 8192, 241 GFLOP in 330 us (730 TFLOP/s; 361 and 1090 with the second product; a large
+// library product 1144; in one part 245 us): the products bound it.  FP32 (NJ = 1, three products for one): 840
+// rows of 16 heads of 64 over 300 to 1129 positions 27.0 us, 3 rounds of launch and latency among them.
 template <typename T, int D, int NJ> struct Wide8 {
     static constexpr int TM = 128 * NJ, BK = 64, NS = 2;
     static constexpr int TILE = BK * D, STAGE = 2 * TILE;    // 16-bit numbers
@@ -611,9 +614,8 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
     using B = typename Parts<T>::half_t;
     using C = Codes<B>;
     typedef typename C::eight_t eight_t;
-    constexpr bool F16 = sizeof(T) == 2;
     constexpr int BK = W::BK, TILE = W::TILE, STAGE = W::STAGE, UT = R::UT, NF = R::NF;
-    constexpr int QP = Parts<T>::Q, PP = F16 ? 1 : Parts<T>::P;
+    constexpr int QP = Parts<T>::Q, PP = Parts<T>::P;
     constexpr int QC = D * (int)sizeof(T) / 16, QR = 64 / QC, QE = 16 / (int)sizeof(T);
     constexpr int CB = D / 8;                                // codes of a lane
     const int lane = unit_lane(), lr = lane & 15, lq = lane >> 4;
@@ -623,14 +625,13 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
     const int wrow = 16 * NJ * wave;
     const bool active = wrow < w.n_rows;
     const int n = w.key1 > w.key0 ? (w.key1 - w.key0 + BK - 1) / BK : 0;
-    f4_t acc[NJ][UT], lsum[NJ];
-    LongSum l_run[F16 ? 1 : NJ];
+    f4_t acc[NJ][UT];
+    LongSum l_run[NJ];
     float m_run[NJ];
     int seen[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
         m_run[j] = -INFINITY;
-        lsum[j] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < UT; u++) acc[j][u] = f4_t{0.f, 0.f, 0.f, 0.f};
         seen[j] = min(w.base + fastdiv(w.R0 + min(wrow + 16 * j + lr, w.n_rows - 1), pl.by_group), un.s.len);
@@ -735,12 +736,10 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
 
         f4_t sc[NJ][4];
         eight_t pf[NJ][2][PP];
-        h8_t ones = {1, 1, 1, 1, 1, 1, 1, 1};
-        if constexpr (F16) asm volatile("" : "+v"(ones));     // kept in registers for the whole loop
 
         // Fragment x of a turn: x < 2 UT is V^T (32-key step x / UT, dims 16 (x % UT)), the rest K
         // (key tile, then chunk).  They are read kAhead fragments before their products, in
-        // exactly this order (2048 rows over 8192: 254 us, 8 ahead, which spills, 257).
+        // exactly this order (2048 rows over 8192: 329 us, 8 ahead 333).
         constexpr int kAhead = 6, kV = 2 * UT, kAll = kV + 4 * NF;
         auto products = [&](int i, auto first_c, auto last_c) {   // fragments first .. last - 1
             constexpr int first = decltype(first_c)::value, last = decltype(last_c)::value;
@@ -762,14 +761,8 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
                 constexpr int x = decltype(x_c)::value;
                 const eight_t f = frag[x % kAhead];
                 // O^T += V^T P^T: in 32-key step s2, k-slot e of lane group lq is key
-                // 32 s2 + 16 (e / 4) + 4 lq + e % 4, the lane's own scores.  fp16: p is rounded to fp16, the
-                // type of V and of the product, and l comes out of the matrix cores too, from the same
-                // rounded p that weights V.  FP32: p in three parts, small ones first.
+                // 32 s2 + 16 (e / 4) + 4 lq + e % 4, the lane's own scores.  p in its parts, small ones first.
                 if constexpr (x < kV) {
-                    if constexpr (F16 && x % UT == 0)
-#pragma unroll
-                        for (int j = 0; j < NJ; j++)
-                            lsum[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, __builtin_bit_cast(h8_t, pf[j][x / UT][0]), lsum[j], 0, 0, 0);
 #pragma unroll
                     for (int q = PP - 1; q >= 0; q--)
 #pragma unroll
@@ -822,8 +815,7 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
                 mloc = low_max<T>(max_xor32(max_xor16(mloc)), c);  // -inf if the row sees nothing here
                 float alpha;
                 if (move_max<T>(mloc, m_run[j], alpha)) {
-                    if constexpr (F16) lsum[j] *= alpha;
-                    else l_run[j].scale(alpha);
+                    l_run[j].scale(alpha);
 #pragma unroll
                     for (int u = 0; u < UT; u++) acc[j][u] *= alpha;
                 }
@@ -835,15 +827,10 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
                     for (int e = 0; e < 4; e += 2) {
                         const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][t][e], c, -m_use));
                         const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][t][e + 1], c, -m_use));
-                        if constexpr (F16) {
-                            pf[j][t >> 1][0][(t & 1) * 4 + e] = (B)p0;
-                            pf[j][t >> 1][0][(t & 1) * 4 + e + 1] = (B)p1;
-                        } else {
-                            l_blk += p0 + p1;
-                            split_into<PP, B>(pf[j][t >> 1], (t & 1) * 4 + e, p0, p1);
-                        }
+                        l_blk += p0 + p1;
+                        split_into<PP, B>(pf[j][t >> 1], (t & 1) * 4 + e, p0, p1);
                     }
-                if constexpr (!F16) l_run[j].add(l_blk);
+                l_run[j].add(l_blk);
             }
         };
         // Stage i into the ring, the codes of the next one on their way.
@@ -891,7 +878,7 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
         const int row = wrow + 16 * j + lr;
-        const float l = F16 ? lsum[j][0] : add_xor32(add_xor16(l_run[F16 ? 0 : j].sum()));
+        const float l = add_xor32(add_xor16(l_run[j].sum()));
         const uint32_t again = rows_of_16(row < w.n_rows && spoilt(acc[j], l));
         if (row < w.n_rows) {
             const RowOut out = row_out<T, D, W::TM>(a.at, pl, un, kvh, w, row, m_run[j], l, lq == 0);
@@ -905,7 +892,7 @@ __device__ __forceinline__ uint32_t wide8_unit(const cf_paged_q8_args_t& a, cons
 }
 
 // Blocks of tiles of up to 16 rows that cost a wide tile's one (31 decode rows beside 4 chunks of 230 to 517
-// rows: 93 us; with 2 118).
+// rows: 106 us, with 2 111; 56 beside 8 of 300 rows 126 and 119).
 constexpr int kNarrowCost8 = 4;
 template <typename T, int D, int NJ>
 __global__ __launch_bounds__(512, 2)
@@ -964,10 +951,10 @@ struct Plan8 {
 // and 20.1, 16 over 4096 40.9 and 32.2; where one of 16 is that long, only what it takes alone counts.
 constexpr int64_t kSplitLen8 = 1024;
 // Tiles of 256 rows read a block's K and V once for twice the rows, but are twice as long a piece of work.
-// They pay where they fill three quarters of the chip by themselves (4 x 512 rows over 1024: 48 us, with 128
-// rows 58; 2 x 2048 over 4096 212 and 292; 1024 over 1024, half the chip, 44.6 and 32.1), and where long
-// ranges can be cut evenly (512 over 4608: 57 and 104; 4 x 230 over 2430 59.7 and 64; 700 over 1400, not cut,
-// 53.8 and 38.6).
+// They pay where they fill three quarters of the chip by themselves (4 x 512 rows over 1024: 57 us, with 128
+// rows 63; 2 x 2048 over 4096 272 and 329; 1024 over 1024, half the chip, 53 and 35.5), and where long
+// ranges can be cut evenly (512 over 4608: 67 and 73; 4 x 230 over 2430 70.5 and 72.4; 700 over 1400, not cut,
+// 66 and 43.5).
 constexpr int64_t kLongLen8 = 2048;
 
 bool fast_ok8(const cf_paged_q8_args_t& q) {
@@ -1012,8 +999,8 @@ Plan8 make_plan8(const cf_paged_attn_args_t& a) {
     const int64_t per_cu = wide ? 1 : a.d == 128 ? 4 : 8;
     const int64_t fill = cus * per_cu > a.H_kv ? cus * per_cu / a.H_kv : 1;
     p.pl.fill = (int32_t)fill;
-    // What is not worth cutting: a merge and the records cost some 5 us, and fp16 wide tiles take 1.5 to 2.2 us
-    // a block (3 x 500 rows of 16 heads of 64 over 1200: 30.8 us, from 8 blocks on into ranges of 4 38.6; FP32
+    // What is not worth cutting: a merge and the records cost some 5 us, and fp16 wide tiles take 2 to 2.7 us
+    // a block (3 x 500 rows of 16 heads of 64 over 1200: 33.6 us, from 8 blocks on into ranges of 4 41.9; FP32
     // chunks of 129 to 411 rows over 300 to 1129 the other way round, 37 and 27).
     p.pl.min_blocks = (int32_t)(wide ? f16 ? 12 : 4 : 64 / BK);
     p.pl.one_blocks = (int32_t)((wide ? f16 ? 1536 : 512 : 128) / BK);

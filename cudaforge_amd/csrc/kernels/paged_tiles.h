@@ -193,9 +193,9 @@ struct Geometry {
     }
     // ORDERS: what goes before each sequence's units, the longest ranges first.  Narrow tiles as if they took
     // longer than they do, so that they are spread: all of them at once wait for memory, between wide
-    // ones they wait beside products (us of 31 decode rows with 4 chunks, of 40 with 3, of 56 with 8, and of
-    // the 4 chunks alone: 92.5, 58, 114, 77; with a quarter 100, 59, 116, 78, with half 92.5, 66, 114, 78; in the
-    // order of the sequences, what is less than half of C last, 92.5, 72, 122, 88).
+    // ones they wait beside products (us of 31 decode rows with 4 chunks, of 56 with 8, and of the 4 chunks
+    // alone: 106, 126, 87; with a quarter 108, 126, 87, with half 109, 127, 87; in the order of the
+    // sequences, what is less than half of C last, 111, 133, 95).
     static constexpr float kNarrowFirst = 1.0f / 3.0f;
     __device__ __forceinline__ int in_order() const {
         const int items = tiles(first) * ranges(first);

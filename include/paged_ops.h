@@ -196,8 +196,10 @@ typedef struct {
  * outputs [O (T, H_q, d)]
  * mha_paged_attn's rules, on the values that the bytes stand for; Q and O are of the operator's type.
  * f16: values are taken as fp16, which is exact for what kv_page_store_q8_f16 stores; past fp16's range
- * they may count as infinite.  f32: as bf16, exact but for values below 2^-126, with Q and the weights as
- * sums of three bf16 numbers each, which are FP32's 24 bits (Q below 3.38e38).  A NaN V touches the rows
+ * they may count as infinite.  The weights of V are sums of two fp16 numbers each, in every tile (other than
+ * mha_paged_attn's, whose tiles of more than 16 rows round them to one).  f32: as bf16, exact but for
+ * values below 2^-126, with Q and the weights as sums of three bf16 numbers each, which are FP32's 24 bits (Q
+ * below 3.38e38).  A NaN V touches the rows
  * that see it; rows that do not, though a later token of the same call does, are computed again by a slow
  * loop.  d = 64 and 128 with blocks of a multiple of 16 positions, 16-byte aligned pointers (the powers'
  * apart) and strides, scale > 0 and at most 32768 sequences run on the matrix cores, every other
