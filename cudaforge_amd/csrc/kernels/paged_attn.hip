@@ -1086,7 +1086,7 @@ void paged_any(cf_paged_attn_args_t a, FastDiv by_page) {
         const int t = (int)(unit / a.H_q), h = (int)(unit - (int64_t)t * a.H_q);
         int lo = 0, hi = a.B;                  // the last sequence that does not start behind t
         while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
+            const int mid = lo + ((hi - lo) >> 1);
             if (a.q_start[mid] <= t) lo = mid; else hi = mid;
         }
         const SeqRows s = seq_rows(a, lo);

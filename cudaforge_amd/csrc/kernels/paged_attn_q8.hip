@@ -928,7 +928,7 @@ void paged_any_q8(cf_paged_q8_args_t a, Q8Divs dv) {
         const int t = (int)(unit / a.at.H_q), h = (int)(unit - (int64_t)t * a.at.H_q);
         int lo = 0, hi = a.at.B;               // the last sequence that does not start behind t
         while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
+            const int mid = lo + ((hi - lo) >> 1);
             if (a.at.q_start[mid] <= t) lo = mid; else hi = mid;
         }
         const SeqRows s = seq_rows(a.at, lo);
