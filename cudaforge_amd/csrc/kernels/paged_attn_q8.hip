@@ -203,14 +203,22 @@ __device__ __forceinline__ uint4 zeros() {
     return uint4{z, z, z, z};
 }
 
-// Which of some V are NaN: bit 7 of the byte of each element of the lane's 16-byte chunk.
+// Which of some V are NaN: bit 7 of the byte of each element of the lane's 16-byte chunk; and whether numbers
+// among them are past the range of B, infinite on the matrix cores.
 struct Nans {
     uint32_t w[4] = {0, 0, 0, 0};
+    uint32_t past = 0;
     __device__ __forceinline__ bool any_but(const Nans& x) const {
         return ((w[0] & ~x.w[0]) | (w[1] & ~x.w[1]) | (w[2] & ~x.w[2]) | (w[3] & ~x.w[3])) != 0;
     }
 };
-template <int D>
+// The least code (without its sign) that is past the range of B at a power: values reach 2^16 (fp16) or 2^128
+// (bf16).  128: none.
+template <typename B> __device__ __forceinline__ int least_past(int power) {
+    const int e = (std::is_same<B, _Float16>::value ? 150 : 262) - power;      // exponent bits of that
+    return e > 15 ? 128 : e > 0 ? e << 3 : max(4 >> min(-e, 2), 1);
+}
+template <typename B, int D>
 __device__ __forceinline__ void find_nan(const cf_paged_q8_args_t& a, const Q8Divs& dv, int b, int kvh, int from, int to, Nans& found) {
     using R = Rows8<D>;
     const int lane = unit_lane(), sub = R::drow(lane);
@@ -221,15 +229,20 @@ __device__ __forceinline__ void find_nan(const cf_paged_q8_args_t& a, const Q8Di
     for (int p0 = from; p0 < to; p0 += 64) {
         const int key = min(p0 + lane, to - 1);
         const Cell cell = cell_of(a, dv, table, key);
-        const int all = cell.at >= 0 && a.v_scales[cell.power + kvh] == 255 ? 0x7f7f7f7f : 0;
+        const int power = cell.at >= 0 ? a.v_scales[cell.power + kvh] : 0;
 #pragma clang loop unroll(disable)
         for (int r = sub; r < 64; r += R::RPI) {
             const int64_t row = (int64_t)((uint64_t)(uint32_t)__shfl((int)(cell.at >> 32), r) << 32 | (uint32_t)__shfl((int)cell.at, r));
-            const uint32_t whole = (uint32_t)__shfl(all, r);
+            const int its_power = __shfl(power, r);
+            const uint32_t whole = its_power == 255 ? 0x7f7f7f7fu : 0u, to_past = (uint32_t)(128 - least_past<B>(its_power)) * 0x01010101u;
             const uint4 x = row < 0 ? uint4{} : *(const uint4*)(v + row);
             const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-            for (int i = 0; i < 4; i++) mine.w[i] |= (((w[i] | whole) & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+            for (int i = 0; i < 4; i++) {
+                const uint32_t nan = (((w[i] | whole) & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                mine.w[i] |= nan;
+                mine.past |= ((w[i] & 0x7f7f7f7fu) + to_past) & 0x80808080u & ~nan;
+            }
         }
     }
 #pragma unroll
@@ -238,15 +251,18 @@ __device__ __forceinline__ void find_nan(const cf_paged_q8_args_t& a, const Q8Di
         for (int step = R::CPR; step < 64; step *= 2) mine.w[i] |= __shfl_xor(mine.w[i], step);
         found.w[i] |= mine.w[i];
     }
+    found.past |= __builtin_amdgcn_ballot_w64(mine.past != 0) != 0;
 }
 
 // Rows row0 + bit of a unit (a bit of `rows` each), computed and stored by this wave, where a sum is NaN
-// while l is a number (spoilt).  An element is NaN where a V that its row sees is; where only V are
-// that it does not see, or none is (codes past fp16's range), the plain loop computes the row again.
+// while l is a number (spoilt).  An element is NaN where a V that its row sees is; where V are that it does
+// not see, or V past the range of the products' type are about (0 times those is NaN too), the plain
+// loop computes the row again.
 template <typename T, int D, int TM>
 __device__ __forceinline__ void mend_rows8(const cf_paged_q8_args_t& a, const PagedPlan& pl, const Q8Divs& dv, const Unit& un,
                                            int kvh, const Work& w, int row0, uint32_t rows) {
     using R = Rows8<D>;
+    using B = typename Parts<T>::half_t;
     const int lane = unit_lane();
     wait_vm<0>();                                             // what it stored is stored
     Nans seen;
@@ -255,13 +271,14 @@ __device__ __forceinline__ void mend_rows8(const cf_paged_q8_args_t& a, const Pa
         const int row = row0 + __builtin_ctz(rows);
         const RowAt at = row_at(pl, pl.G, kvh, w.R0 + row);
         const int sees = max(min(min(w.base + at.tok, un.s.len), w.key1), upto);     // rises with the rows
-        find_nan<D>(a, dv, un.b, kvh, upto, sees, seen);
+        find_nan<B, D>(a, dv, un.b, kvh, upto, sees, seen);
         upto = sees;
         Nans hidden;
-        find_nan<D>(a, dv, un.b, kvh, sees, w.key1, hidden);
+        find_nan<B, D>(a, dv, un.b, kvh, sees, w.key1, hidden);
         float* const rec = un.n_ranges > 1 ? record_of<TM, D>(a.at, pl, un, kvh) : nullptr;
         T* const o = (T*)a.at.o + ((int64_t)(un.s.row0 + at.tok) * a.at.H_q + at.h) * D;
-        if (__builtin_amdgcn_ballot_w64(hidden.any_but(seen)) || !__builtin_amdgcn_ballot_w64(seen.any_but(Nans{}))) {
+        if (seen.past | hidden.past || __builtin_amdgcn_ballot_w64(hidden.any_but(seen)) ||
+            !__builtin_amdgcn_ballot_w64(seen.any_but(Nans{}))) {
             plain_row_q8<T, D / 64>(a, dv, un.s, un.b, at.tok, at.h, D, w.key0, w.key1, rec ? rec + row : nullptr, TM,
                                     rec + 2 * TM + row * D);
             continue;
