@@ -46,13 +46,13 @@ __device__ __forceinline__ void plain_row_q8(const cf_paged_q8_args_t& a, const 
 #pragma clang loop unroll(disable)
     for (uint32_t at0 = (uint32_t)key0; at0 < (uint32_t)max(seen, 0); at0 += 64) {    // unsigned: up to 2^31 positions
         const int k0 = (int)at0, key = k0 + lane;
-        int64_t at = 0;
+        int64_t at = -1;
         int vpower = 0;
         float x = -INFINITY;
         if (key < seen) {
             const Cell cell = cell_of(a, dv, table, key);
-            if (cell.at >= 0) {
-                at = cell.at;
+            at = cell.at;
+            if (at >= 0) {
                 vpower = a.v_scales[cell.power + kvh];
                 const float kpower = power_bits(a.k_scales[cell.power + kvh]);
                 float dot = 0.0f;
@@ -62,7 +62,9 @@ __device__ __forceinline__ void plain_row_q8(const cf_paged_q8_args_t& a, const 
             }
         }
         const float m_new = fmaxf(m, wave_max(x));
-        if (m_new == -INFINITY && !__builtin_amdgcn_ballot_w64(x != x)) continue;
+        // Positions that count, whatever they weigh: a NaN V touches the row from any of them.
+        const uint64_t counts = __builtin_amdgcn_ballot_w64(key < seen && at >= 0);
+        if (!counts) continue;
         const float m_use = m_new == -INFINITY ? 0.0f : m_new;
         const float alpha = exp2f(m - m_use), p = exp2f(x - m_use);
         m = m_new;
@@ -75,15 +77,17 @@ __device__ __forceinline__ void plain_row_q8(const cf_paged_q8_args_t& a, const 
         for (int i = 0; i < DIMS; i++) part[i] = 0.0f;
 #pragma clang loop unroll(disable)
         for (int j = 0; j < min(64, seen - k0); j++) {
+            if (!(counts >> j & 1)) continue;  // not attended: its V may hold anything
             const float pj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(p), j));
-            if (pj == 0.0f) continue;          // not attended: its V may hold anything
             const int64_t row = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(at >> 32), j) << 32) |
                                           (uint32_t)__builtin_amdgcn_readlane((int)at, j));
             const float power = power_bits(__builtin_amdgcn_readlane(vpower, j));
 #pragma unroll
             for (int i = 0; i < DIMS; i++)
-                if (lane + 64 * i < d)
-                    part[i] = __builtin_fmaf(pj, codes_f32<false>(v[row + lane + 64 * i], power)[0], part[i]);
+                if (lane + 64 * i < d) {
+                    const float y = codes_f32<false>(v[row + lane + 64 * i], power)[0];
+                    part[i] = __builtin_fmaf(pj, pj == 0.0f && y == y ? 0.0f : y, part[i]);
+                }
         }
 #pragma unroll
         for (int i = 0; i < DIMS; i++) acc[i] = __builtin_fmaf(acc[i], alpha, part[i]);
