@@ -1,7 +1,7 @@
 // paged_kv_q8.hip — the write of new K and V rows into pages of 8-bit numbers (gfx950).
 //
-// Rows of one block (block positions of a page, one KV head) follow each other in a call: a run.  A
-// wave takes a run of one head of K or V: the largest finite size A of it, the power p = the least
+// Rows of one block (block positions of a page, one KV head) stand together in a call, within 64 rows and with
+// nothing between them but rows that are not stored: a run.  A wave takes a run of one head of K or V: the largest finite size A of it, the power p = the least
 // with A <= 448 * 2^(p - 127), or the block's own where that is larger and the block was begun by an
 // earlier call, then code = x * 2^(127 - p) to the nearest.  Where the power of a begun block grows,
 // its other codes are rounded to the new one: a division by a power of two, so no mantissa changes
@@ -64,17 +64,19 @@ __device__ __forceinline__ float finite_size(float x) {
     return s < INFINITY ? s : 0.0f;
 }
 
-// A wave's run: rows t .. t + len - 1, whose slots the lanes 0 .. len - 1 hold.
+// A wave's run of len rows, whose slots the lanes 0 .. len - 1 hold: rows t .. t + len - 1, or with HOLES
+// t + `off` of those lanes.
 struct Run {
     int64_t t;
     int len;
+    int off;
     uint8_t* cells;        // the block's first position
     int slot0;             // ... and its slot
 };
 
 // VEC elements of 16 bytes a lane, d / VEC = 2^k lanes a row, KEEP steps of rows in registers; VEC = 1:
 // any shape, all lanes on one row.
-template <typename T, int VEC, int KEEP>
+template <typename T, int VEC, int KEEP, bool HOLES>
 __device__ __forceinline__ void store_run(const cf_page_store_q8_args_t& a, const Run& run, int slot, const T* rows,
                                           uint8_t* power) {
     constexpr bool WIDE = VEC > 1;
@@ -83,29 +85,37 @@ __device__ __forceinline__ void store_run(const cf_page_store_q8_args_t& a, cons
     const int sub = WIDE ? lane / per_row : 0, e0 = (lane % per_row) * VEC, step_e = WIDE ? a.d : 64;
     typedef Pack<T, VEC> pack_t;
     const int old = *power;
-    auto load = [&](int r, int e) { return *(const pack_t*)(rows + (run.t + min(r, run.len - 1)) * a.kv_stride + e); };
+    auto row_at = [&](int r) {                     // (by all lanes)
+        const int i = min(r, run.len - 1);
+        return rows + (run.t + (HOLES ? __shfl(run.off, i) : i)) * a.kv_stride;
+    };
+    auto load = [&](const T* row, int e) { return *(const pack_t*)(row + e); };
     pack_t kept[KEEP];
     float most = 0.0f;
     bool finite = true;
     if constexpr (WIDE) {
 #pragma unroll
         for (int s = 0; s < KEEP; s++)
-            if (s * at_once < run.len) kept[s] = load(s * at_once + sub, e0);
+            if (s * at_once < run.len) kept[s] = load(row_at(s * at_once + sub), e0);
 #pragma unroll
         for (int s = 0; s < KEEP; s++)
             if (s * at_once < run.len) most = fmaxf(most, largest(kept[s], finite));
     }
-    for (int r = WIDE ? KEEP * at_once : 0; r < run.len; r += at_once)
-        for (int e = e0; e < a.d; e += step_e) most = fmaxf(most, largest(load(r + sub, e), finite));
+    for (int r = WIDE ? KEEP * at_once : 0; r < run.len; r += at_once) {
+        const T* const row = row_at(r + sub);
+        for (int e = e0; e < a.d; e += step_e) most = fmaxf(most, largest(load(row, e), finite));
+    }
     finite = !__builtin_amdgcn_ballot_w64(!finite);
     if (!finite) {                                 // once more, without what is infinite or NaN
         most = 0.0f;
-        for (int r = 0; r < run.len; r += at_once)
+        for (int r = 0; r < run.len; r += at_once) {
+            const T* const row = row_at(r + sub);
             for (int e = e0; e < a.d; e += step_e) {
-                const pack_t x = load(r + sub, e);
+                const pack_t x = load(row, e);
 #pragma unroll
                 for (int i = 0; i < VEC; i++) most = fmaxf(most, finite_size((float)x.e[i]));
             }
+        }
     }
     const int need = power_for(wave_max(most));
     const bool mine = lane < run.len;
@@ -172,7 +182,8 @@ __device__ __forceinline__ void store_run(const cf_page_store_q8_args_t& a, cons
             if (s * at_once < run.len) put(s * at_once + sub, place(s * at_once + sub) + e0, kept[s]);
     for (int r = WIDE ? KEEP * at_once : 0; r < run.len; r += at_once) {
         uint8_t* const cell = place(r + sub);      // (by all lanes)
-        for (int e = e0; e < a.d; e += step_e) put(r + sub, cell + e, load(r + sub, e));
+        const T* const row = row_at(r + sub);
+        for (int e = e0; e < a.d; e += step_e) put(r + sub, cell + e, load(row, e));
     }
 }
 
@@ -191,30 +202,57 @@ void page_store_q8(cf_page_store_q8_args_t a, StoreDivs dv, int log_per, int64_t
     const int part = (int)blockIdx.x >> log_per, sub = (int)blockIdx.x & ((1 << log_per) - 1);
     const int64_t t0 = row0 + (int64_t)part * kStoreRows;
     auto slot_at = [&](int64_t t) { return t >= 0 && t < a.T ? a.slots[t] : -1; };
-    const int slot = slot_at(t0 + lane), next = slot_at(t0 + kStoreRows + lane), last = slot_at(t0 - 1);
+    const int slot = slot_at(t0 + lane), next = slot_at(t0 + kStoreRows + lane), last = slot_at(t0 - kStoreRows + lane);
     auto block_of = [&](int s) { return (unsigned)s < (unsigned)a.num_slots ? fastdiv(s, dv.block) : -1; };
-    const int block = block_of(slot);
-    const int up = __shfl_up(block, 1), before = lane == 0 ? block_of(last) : up;
+    const int block = block_of(slot), last_block = block_of(last);
+    // The block of the stored row before this one, of those less than 64 rows before it.
+    const uint64_t lower = (1ull << lane) - 1, stored = __builtin_amdgcn_ballot_w64(block >= 0) & lower;
+    const uint64_t last_stored = __builtin_amdgcn_ballot_w64(last_block >= 0);
+    const int last_lane = last_stored ? 63 - __builtin_clzll(last_stored) : 0;
+    const int up = __shfl(block, stored ? 63 - __builtin_clzll(stored) : 0);
+    const int before = stored ? up : last_lane > lane ? __builtin_amdgcn_readlane(last_block, last_lane) : -1;
     const uint64_t all = __builtin_amdgcn_ballot_w64(block >= 0 && block != before);
-    const int rank = __builtin_popcountll(all & ((1ull << lane) - 1));
+    const int rank = __builtin_popcountll(all & lower);
     uint64_t heads = __builtin_amdgcn_ballot_w64((all >> lane & 1) && ((rank + part + (part >> 2) - sub) & ((1 << log_per) - 1)) == 0);
     const T* const rows = (const T*)(which ? a.v : a.k) + (int64_t)h * a.d;
     uint8_t* const pages = which ? a.v_pages : a.k_pages;
     uint8_t* const powers = which ? a.v_scales : a.k_scales;
-    for (; heads; heads &= heads - 1) {
-        const int first = __builtin_ctzll(heads);
+    // The run that begins at lane `first`: its rows, a bit each of the 64 from there, and this lane's slot among them.
+    auto find = [&](int first, Run& run, int& its_slot, uint8_t*& power) {
         const int b = __builtin_amdgcn_readlane(block, first);
         const int here = __shfl(slot, (first + lane) & 63), behind = __shfl(next, (first + lane) & 63);
-        const int its_slot = first + lane < 64 ? here : behind;
-        const uint64_t same = __builtin_amdgcn_ballot_w64(block_of(its_slot) == b);
-        Run run;
+        its_slot = first + lane < 64 ? here : behind;
+        const int its_block = block_of(its_slot);
+        const uint64_t others = __builtin_amdgcn_ballot_w64(its_block >= 0 && its_block != b);
+        const uint64_t its_rows = __builtin_amdgcn_ballot_w64(its_block == b) & ((others & -others) - 1);   // before another block's
         run.t = t0 + first;
-        run.len = ~same ? __builtin_ctzll(~same) : 64;
+        run.len = __builtin_popcountll(its_rows);
         run.slot0 = b * a.block;
         const int page = fastdiv(b, dv.blocks);
         run.cells = pages + (int64_t)page * a.page_stride + (int64_t)(run.slot0 - page * a.page_size) * a.row_stride +
                     (int64_t)h * a.head_stride;
-        store_run<T, VEC, KEEP>(a, run, its_slot, rows, powers + (int64_t)b * a.H_kv + h);
+        power = powers + (int64_t)b * a.H_kv + h;
+        return its_rows;
+    };
+    uint64_t with_holes = 0;
+    for (; heads; heads &= heads - 1) {
+        Run run;
+        int its_slot;
+        uint8_t* power;
+        const uint64_t its_rows = find(__builtin_ctzll(heads), run, its_slot, power);
+        if (its_rows & (its_rows + 1)) with_holes |= heads & -heads;
+        else store_run<T, VEC, KEEP, false>(a, run, its_slot, rows, power);
+    }
+    for (; with_holes; with_holes &= with_holes - 1) {        // rare: few registers
+        Run run;
+        int its_slot;
+        uint8_t* power;
+        const uint64_t its_rows = find(__builtin_ctzll(with_holes), run, its_slot, power);
+        // Its rows to the lanes 0 .. len - 1, the others behind them.
+        const int among = __builtin_popcountll(its_rows & lower);
+        const int to = its_rows >> lane & 1 ? among : run.len + lane - among;
+        run.off = __builtin_amdgcn_ds_permute(4 * to, lane);
+        store_run<T, VEC, 1, true>(a, run, __shfl(its_slot, run.off), rows, power);
     }
 }
 

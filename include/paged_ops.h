@@ -174,8 +174,9 @@ typedef struct {
  * positions but the new ones) is divided by as much: exact but for numbers that come below 2^-6 of
  * the power.  Values are rounded to nearest, ties to even; infinite and NaN ones become NaN.  Where a
  * rounding would pass the type's largest number, as 65504 to 65536, the one below is stored, so that
- * what is read back stays finite.  A row with an invalid slot is not stored.  Rows for one block follow
- * each other, in any order, as kv_page_map gives them, and each slot may be given once per
+ * what is read back stays finite.  A row with an invalid slot is not stored.  Rows for one block stand
+ * together, as kv_page_map gives them: in any order, the first and the last of them less than 64 rows apart, and
+ * between them no other row but such as are not stored; and each slot may be given once per
  * call: otherwise that block's numbers and powers mean nothing.  Seven arrays of their own (-1 where
  * an output is another array). */
 int kv_page_store_q8_f32_cuda(const void* inputs[], void* outputs[], const operator_params_t* params, stream_t* stream);
