@@ -13,6 +13,8 @@ import ctypes
 import numpy as np
 import pytest
 
+import cudaforge_amd as cf
+from helpers import dev
 from test_paged import ref_attn
 from test_paged_q8 import PagedQ8
 
@@ -65,3 +67,86 @@ def test_weights_are_not_rounded_to_fp16(gpu, H, H_kv, d, new, past, rows):
     c = PagedQ8(new, past, H, H_kv, d, 16, True, seed=51)
     assert tile_rows(gpu, c, max(new)) == rows
     check_tight(c, c.run(max_new=max(new)))
+
+
+# Fewer rows than fill the chip over a long context, whose ranges are cut, and more over a short one; rows of chunks
+# that end inside a wave's share, single rows, none.
+BIG = [(32, 8, 128, [200, 1, 58, 0, 3], [2300, 900, 0, 40, 2044]), (64, 16, 64, [131, 1, 5], [2200, 31, 700]),
+       (64, 8, 64, [513, 1, 300], [60, 900, 0]), (32, 8, 128, [1540, 20], [5, 560])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,H_kv,d,new,past", BIG)
+def test_tiles_of_256_rows(gpu, H, H_kv, d, new, past):
+    """Hints that are right, absent and wrong; Q as a part of a projection, K and V of a page in one tensor."""
+    c = PagedQ8(new, past, H, H_kv, d, 16, True, seed=52)
+    assert tile_rows(gpu, c, max(new)) == 256 and tile_rows(gpu, c, 0) == 256
+    check_tight(c, c.run(max_new=max(new)))
+    check_tight(c, c.run(max_len=1))                     # in one range; which tiles goes by the rows alone
+    wide = np.full((c.T, (H + 2 * H_kv) * d), 9.0, c.dt)
+    wide[:, :H * d] = c.q.reshape(c.T, -1)
+    both = np.full((c.n_pages, 16, 2, H_kv, d), 0x7f, np.uint8)
+    both[:, :, 0], both[:, :, 1] = c.codes
+    kv = dev(both)
+    bufs = [dev(wide), kv, kv.ptr + H_kv * d] + c.bufs()[3:]
+    check_tight(c, c.run(bufs, q_stride=(H + 2 * H_kv) * d, page_stride=32 * H_kv * d, row_stride=2 * H_kv * d))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_tiles_of_256_rows_with_missing_pages(gpu, d):
+    c = PagedQ8([260, 2, 30], [2300, 500, 100], 32, 8, d, 16, True, seed=53)
+    c.table[0, [0, 5, 6, 100, 159]] = [-1, c.n_pages, 2 ** 31 - 1, -2 ** 31, -3]
+    c.table[0, 20:60] = -1                               # whole blocks and, cut, whole ranges
+    c.table[2, :] = -1
+    assert tile_rows(gpu, c) == 256
+    for hint in (0, 1):
+        got = c.run(max_len=hint)
+        check_tight(c, got)
+        assert (got[262:292] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_tiles_of_256_rows_with_nan(gpu, d):
+    """NaN V among the cached, in a new token, and of a whole block's power; a K in one head; rows that do not
+    see them keep theirs."""
+    new, past = [260, 40], [2300, 500]
+    c = PagedQ8(new, past, 32, 8, d, 16, True, seed=54)
+    at = lambda b, pos: (c.table[b, pos // 16], pos % 16)
+    nan = np.zeros(c.q.shape, bool)
+    r = [np.arange(c.start[b], c.start[b + 1]) for b in range(2)]
+    c.codes[1][at(0, 77)][:, 3] = 0x7f                   # seen by all
+    nan[r[0], :, 3] = True
+    for k in (70, 130, 259):                             # in different waves' rows and tiles
+        c.codes[1][at(0, past[0] + k)][:, 5 + k % 7] = 0xff
+        nan[r[0][k:], :, 5 + k % 7] = True
+    c.powers[1][c.table[1, 3], 0, 2] = 255               # a block of V in KV head 2
+    nan[r[1], 8:12] = True
+    c.codes[0][at(0, past[0] + 200)][6, 9] = 0x7f        # a K in KV head 6
+    nan[r[0][200:], 24:28] = True
+    assert tile_rows(gpu, c) == 256
+    clean = PagedQ8(new, past, 32, 8, d, 16, True, seed=54)
+    for hint in (0, 1):
+        got = c.run(max_len=hint)
+        assert (np.isnan(got) == nan).all()
+        base = clean.run(max_len=hint)
+        got[nan] = base[nan]
+        check_tight(clean, got)
+
+
+@pytest.mark.gpu
+def test_tiles_of_256_rows_without_a_workspace(gpu):
+    c = PagedQ8([260, 1, 20], [2300, 900, 3], 32, 8, 128, 16, True, seed=55)
+    assert tile_rows(gpu, c) == 256
+    st = cf.Stream()
+    o = dev(np.full(c.q.shape, 7.0, c.dt))
+    bufs = c.bufs()
+    gpu.gpu_inject_alloc_failures(1000)
+    try:
+        rc = cf.call_op(c.op, bufs, [o], c.params(), st)
+    finally:
+        gpu.gpu_inject_alloc_failures(0)
+    assert rc == 0
+    st.synchronize()
+    check_tight(c, o.download())
