@@ -51,3 +51,30 @@ def test_a_row_behind_2_to_the_30_sequences(gpu, q8):
         x.free()
     # p = 1 and l = 1: the value itself.
     assert (got == want).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q8", [False, True])
+def test_more_rows_than_a_round_takes(gpu, q8):
+    """2^24 rows of a head are a round of the plain kernels' workgroups; each of these is a sequence of one
+    position."""
+    T, H, d, P, n_pages = 2 ** 22 + 3, 4, 4, 16, 1000
+    rng = np.random.default_rng(3)
+    page = (np.arange(T) * 7 % n_pages).astype(np.int32)
+    q = dev(np.ones((T, H, d), np.float16))
+    o = cf.DeviceBuffer(2 * T * H * d, np.float16, (T, H, d))
+    index = [dev(page.reshape(T, 1)), dev(np.ones(T, np.int32)), dev(np.arange(T + 1, dtype=np.int32))]
+    common = dict(batch_size=T, num_tokens=T, num_heads=H, num_kv_heads=2, head_dim=d, scale=0.5, page_size=P,
+                  num_pages=n_pages, max_pages=1)
+    if q8:
+        c = rng.integers(0, 100, (n_pages, P, 2, d))
+        v = np.where(c > 7, (8 + c % 8) * 2.0 ** (c // 8 - 10.0), c * 2.0 ** -9)
+        codes, powers = dev(c.astype(np.uint8)), dev(np.full((n_pages, 1, 2), 127, np.uint8))
+        assert cf.call_op("mha_paged_attn_q8_f16_cuda", [q, codes, codes] + index + [powers, powers], [o],
+                          cf.MhaPagedQ8Params(**common)) == 0
+    else:
+        v = rng.standard_normal((n_pages, P, 2, d)).astype(np.float16)
+        kv = dev(v)
+        assert cf.call_op("mha_paged_attn_f16_cuda", [q, kv, kv] + index, [o], cf.MhaPagedParams(**common)) == 0
+    want = np.repeat(v[:, 0], 2, 1).astype(np.float16)
+    assert (o.download() == want[page]).all()

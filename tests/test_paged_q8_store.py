@@ -1,10 +1,12 @@
-"""The 8-bit store where rows that are not stored stand among those of a block, bit by bit against
-test_paged_q8.py's oracle (GPU)."""
+"""The 8-bit store where rows that are not stored stand among those of a block, and on more rows than one launch
+takes, bit by bit against test_paged_q8.py's oracle (GPU)."""
 
 import numpy as np
 import pytest
 
-from test_paged_q8 import Store
+import cudaforge_amd as cf
+from helpers import dev
+from test_paged_q8 import Store, encode, power_for
 
 
 @pytest.mark.gpu
@@ -38,3 +40,27 @@ def test_skipped_rows_inside_a_block(gpu, f16, H, d, P, block):
                 own.insert(int(s.rng.integers(0, len(own) + 1)), none[int(s.rng.integers(0, 4))])
             slots += own + [-1] * int(s.rng.integers(0, 3)) * 40 * int(b % 5 == 0)
         call(slots)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("d,block", [(2, 1), (16, 1), (16, 4)])
+def test_more_rows_than_a_launch_takes(gpu, f16, d, block):
+    """2^23 rows are a launch's.  Blocks of rows that repeat after 997 go to slots in another order: every code
+    and every power, and nothing behind the last."""
+    n, t = 2 ** 23 // block + 5, "f16" if f16 else "f32"
+    rng = np.random.default_rng(73)
+    base = (rng.standard_normal((997, block, d)) * np.exp2(rng.integers(-9, 9, (997, block, 1)))).astype(np.float16 if f16 else np.float32)
+    power = power_for(np.abs(base.astype(np.float64)).max((1, 2)))
+    code = encode(base.astype(np.float64) * 2.0 ** (127.0 - power)[:, None, None])
+    at, to = np.arange(n) % 997, rng.permutation(n)
+    slots = (to[:, None] * block + np.arange(block)).astype(np.int32)
+    ins = [dev(base[at]), dev(base[::-1][at]), dev(slots)]
+    pages = [dev(np.full((n + 3, block, 1, d), 0x55, np.uint8)) for _ in range(2)]
+    powers = [dev(np.full((n + 3, 1, 1), 9, np.uint8)) for _ in range(2)]
+    p = cf.KvPageStoreQ8Params(num_tokens=n * block, num_kv_heads=1, head_dim=d, page_size=block, num_pages=n + 3, block_size=block)
+    assert cf.call_op("kv_page_store_q8_%s_cuda" % t, ins, pages + powers, p) == 0
+    for x, y, c, e in zip(pages, powers, (code, code[::-1]), (power, power[::-1])):
+        x, y = x.download().reshape(n + 3, block, d), y.download().reshape(-1)
+        assert (y[to] == e[at]).all() and (y[n:] == 9).all()
+        assert (x[to] == c[at]).all() and (x[n:] == 0x55).all()
