@@ -115,7 +115,7 @@ __device__ __forceinline__ void plain_row_q8(const cf_paged_q8_args_t& a, const 
 // Codes go to LDS as they are and become 16-bit operands on their way to the matrix cores, one
 // instruction for two, the power of their block with them: exact, so nothing is scaled afterwards.
 // fp16 rows go with fp16 codes.  FP32 rows go with bf16 codes, and Q and the weights of V as sums of
-// three bf16 numbers, whose 24 bits are FP32's own: three products for one, at 8 times the FP32
+// three bf16 numbers, whose 24 bits are FP32's own: three products for one, at 16 times the FP32
 // MFMA's rate.
 
 // T rows: what the matrix cores take, and in how many parts Q and the weights.

@@ -7,8 +7,8 @@
 // its other codes are rounded to the new one: a division by a power of two, so no mantissa changes
 // but of numbers that leave the normal range.
 //
-// HBM bounds it: 8192 rows of 8 heads of 128 fp16, 50 MB, 11.8 us (4.3 TB/s); launch and latency few
-// rows: 16 rows 6.3 us a call, 3.8 of them the kernel's, 840 FP32 rows of 12 heads of 64 6.3 and 5.3.
+// HBM bounds it: 8192 rows of 8 heads of 128 fp16, 50 MB, 11.9 us (4.2 TB/s); launch and latency few
+// rows: 16 rows 6.4 us a call, 3.8 of them the kernel's, 840 FP32 rows of 12 heads of 64 6.4 and 5.6.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -174,7 +174,8 @@ struct Geometry {
     }
     // COUNTS: the shortest ranges that go in one round of `fill` units (narrow ones as parts of one), if they
     // are not much longer than an equal share: else a few long sequences would wait for ranges
-    // of their own.
+    // of their own.  For up to 64 sequences, one per lane (64 decode rows over 2000 in 8 bits 55 us,
+    // uncounted 69, 65 uncounted 63; 64 over 500, one of them over 32000, 34 and 41, 65 37).
     __device__ __forceinline__ bool count_ranges(bool few) {
         const float fill = (float)pl.fill;
         const float least = (float)(few ? kFewMin : pl.min_blocks), by_fill = 1.0f / fill, was = C;

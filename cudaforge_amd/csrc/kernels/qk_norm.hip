@@ -79,7 +79,7 @@ void qk_norm_any(cf_qk_norm_args_t a) {
 // else neighbours; lane j has pairs VEC j .. + VEC - 1 either way.  It stays on one row and goes over
 // its heads, so that it keeps their cosines and sines, which the workgroup works out once per row.
 // HBM bounds it: 8192 rows of 40 heads of 128 fp16, 168 MB, 28.2 us (5.9 TB/s), of 1001 FP32 rows of 24
-// heads of 64 6.9 us; 16 rows take 7.0 us, 5 of them the kernel's. ----
+// heads of 64 7.0 us; 16 rows take 7.1 us, 4.3 of them the kernel's. ----
 constexpr int kThreads = 256;
 template <typename T> struct alignas(16) Piece { T e[16 / sizeof(T)]; };
 
@@ -256,7 +256,10 @@ int launch_qk_wide(const cf_qk_norm_args_t& a, hipStream_t st) {
     p.lanes = 1;
     while (2 * VEC * p.lanes < a.d) p.lanes *= 2;
     const int heads = a.rows[0].heads + a.rows[1].heads;
-    // Few rows: a workgroup for every 256 lanes' worth of heads.
+    // Few rows: a workgroup for every 256 lanes' worth of heads, else one for four rows (us with the former and
+    // with the latter: 40 heads of 128 fp16, 512 rows 7.1 and 7.8, 1001 9.6 and 9.2, 2048 16.3 and 11.8; 24 of 64
+    // fp16 or FP32, up to 1500 rows 7.0 and 7.1, 4096 FP32 ones 11.2 and 10.1.  40 of 128 FP32, which the
+    // rule does not go by, are faster with the former throughout: 512 rows 7.0 and 12.0, 4096 27.3 and 31.0).
     const bool few = a.T < 1024;
     p.rows = few ? 1 : kRows;
     p.at_once = kThreads / p.lanes / p.rows;
