@@ -78,16 +78,24 @@ __device__ __forceinline__ void plain_row_q8(const cf_paged_q8_args_t& a, const 
 #pragma clang loop unroll(disable)
         for (int j = 0; j < min(64, seen - k0); j++) {
             if (!(counts >> j & 1)) continue;  // not attended: its V may hold anything
-            const float pj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(p), j));
+            const int pbits = __builtin_amdgcn_readlane(__float_as_int(p), j);
+            const float pj = __int_as_float(pbits);
             const int64_t row = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(at >> 32), j) << 32) |
                                           (uint32_t)__builtin_amdgcn_readlane((int)at, j));
             const float power = power_bits(__builtin_amdgcn_readlane(vpower, j));
+            if (pbits == 0) {                  // of weight 0: NaN only
+#pragma unroll
+                for (int i = 0; i < DIMS; i++)
+                    if (lane + 64 * i < d) {
+                        const float y = codes_f32<false>(v[row + lane + 64 * i], power)[0];
+                        if (y != y) part[i] = y;
+                    }
+                continue;
+            }
 #pragma unroll
             for (int i = 0; i < DIMS; i++)
-                if (lane + 64 * i < d) {
-                    const float y = codes_f32<false>(v[row + lane + 64 * i], power)[0];
-                    part[i] = __builtin_fmaf(pj, pj == 0.0f && y == y ? 0.0f : y, part[i]);
-                }
+                if (lane + 64 * i < d)
+                    part[i] = __builtin_fmaf(pj, codes_f32<false>(v[row + lane + 64 * i], power)[0], part[i]);
         }
 #pragma unroll
         for (int i = 0; i < DIMS; i++) acc[i] = __builtin_fmaf(acc[i], alpha, part[i]);
